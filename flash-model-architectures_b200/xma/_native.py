@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_int32, c_int64, c_void_p
+from ctypes import c_float, c_int32, c_int64, c_void_p
 
 import torch
 
@@ -18,6 +18,7 @@ LIB_PATH = os.environ.get("XMA_B200_LIB") or os.path.join(_PKG_ROOT, "libxma_b20
 
 XMA_BLOCK_M = 128
 XMA_BLOCK_N = 256
+NORM_PARTIALS = 148
 EPI_STORE, EPI_SWIGLU, EPI_SWIGLU_BWD, EPI_STORE_F32, EPI_ADD_F32 = 0, 1, 2, 3, 4
 GEMM_NT, GEMM_NN = 0, 1
 
@@ -56,6 +57,11 @@ _SIGNATURES = {
     "xma_swiglu_backward": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_void_p, c_void_p, c_void_p]),
     "xma_pack_sequence": (c_int32, [c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int32, c_void_p, c_void_p]),
     "xma_unpack_sequence": (c_int32, [c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int32, c_void_p, c_void_p]),
+    "xma_norm_workspace_floats": (c_int64, [c_int64, c_int64]),
+    "xma_norm_forward": (
+        c_int32, [c_void_p] * 5 + [c_int32] * 4 + [c_int64, c_int64, c_float, c_float] + [c_void_p] * 5),
+    "xma_norm_backward": (
+        c_int32, [c_void_p] * 7 + [c_int32] * 4 + [c_int64, c_int64, c_float] + [c_void_p] * 10),
     "xma_ipc_get_handle": (c_int32, [c_void_p, ctypes.c_char_p]),
     "xma_ipc_open_handle": (c_int32, [ctypes.c_char_p, ctypes.POINTER(c_void_p)]),
     "xma_ipc_close_handle": (c_int32, [c_void_p]),
@@ -148,6 +154,12 @@ def index_workspace_elems(n: int, num_experts: int) -> int:
     seg_len = -(-(-(-max(n, 1) // segs)) // 32) * 32
     segs = -(-n // seg_len) if n > 0 else 1
     return 2 * segs * num_experts + 64
+
+
+def norm_workspace_floats(rows: int, hidden: int) -> int:
+    """float32 elements of workspace xma_norm_backward needs (xma_norm_workspace_floats, kept in Python for
+    the same reason as index_workspace_elems)."""
+    return 3 * NORM_PARTIALS * hidden + 4 * rows
 
 
 _status_words: dict[int, torch.Tensor] = {}

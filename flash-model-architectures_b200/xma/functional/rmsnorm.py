@@ -1,0 +1,170 @@
+"""rmsnorm and fused_residual_add_rmsnorm, the functionals of those names in the reference
+(xma/functional/__init__.py:5-16), extended to the norm after a block, the block's gate and the scale of
+its residual add; one kernel forward and one (plus a small sum) backward."""
+
+from __future__ import annotations
+
+import torch
+
+from .. import _native as N
+from ..accelerator import KernelBackend, require_cuda_backend
+
+GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_FULL = 0, 1, 2, 3
+_MAX_HIDDEN = 1 << 24
+
+
+class _Norm(torch.autograd.Function):
+    """x [rows, H] and, unless it is None, residual [rows, H]; returns y, or (y, stream) with a residual."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, post_weight, gate, gate_mode: int, eps: float, multiplier: float):
+        from ..ops import norm_forward_cuda
+
+        x = x.contiguous()
+        residual = None if residual is None else residual.contiguous()
+        weight = None if weight is None else weight.contiguous()
+        post_weight = None if post_weight is None else post_weight.contiguous()
+        gate = None if gate is None else gate.contiguous()
+        rows = x.size(0)
+        y = torch.empty_like(x)
+        stream = None if residual is None else torch.empty_like(residual)
+        saving = any(ctx.needs_input_grad)
+        rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if saving else None
+        rstd_post = torch.empty(rows, dtype=torch.float32, device=x.device) if saving and post_weight is not None else None
+        norm_forward_cuda(x, residual, weight, post_weight, gate, gate_mode, eps, multiplier, stream, y, rstd, rstd_post)
+        if saving:
+            branch = x if post_weight is not None or gate is not None else None  # a plain residual add needs no input
+            ctx.save_for_backward(x if residual is None else stream, branch, weight, post_weight, gate, rstd, rstd_post)
+            ctx.dtype, ctx.alone = x.dtype, residual is None
+            ctx.gate_mode, ctx.multiplier = gate_mode, multiplier
+        ctx.set_materialize_grads(False)
+        return y if residual is None else (y, stream)
+
+    @staticmethod
+    def backward(ctx, dy, d_stream=None):
+        from ..ops import norm_backward_cuda
+
+        stream, x, weight, post_weight, gate, rstd, rstd_post = ctx.saved_tensors
+        dy = None if dy is None else dy.contiguous()
+        d_stream = None if d_stream is None else d_stream.contiguous()
+        want_x, want_residual, want_weight, want_post, want_gate = ctx.needs_input_grad[:5]
+        empty = stream.numel() == 0
+
+        # The norm alone differentiates with respect to its "stream", x. A plain residual add in one type
+        # gives x and the residual the same gradient: one tensor.
+        shared = not ctx.alone and x is None and ctx.multiplier == 1.0 and stream.dtype == ctx.dtype
+        want_stream = want_x if ctx.alone else want_residual or (shared and want_x)
+        d_residual = torch.empty_like(stream) if want_stream else None
+        dx = None
+        if want_x and not ctx.alone and not shared:
+            dx = torch.empty(stream.shape, dtype=ctx.dtype, device=stream.device)
+        new = torch.zeros_like if empty else torch.empty_like
+        d_weight = new(weight) if want_weight and weight is not None else None
+        d_post = new(post_weight) if want_post and post_weight is not None else None
+        d_gate = new(gate) if want_gate and gate is not None else None
+        if not empty:
+            workspace = torch.empty(N.norm_workspace_floats(*stream.shape), dtype=torch.float32, device=stream.device)
+            norm_backward_cuda(
+                dy, d_stream, stream, x, weight, post_weight, gate, ctx.gate_mode, ctx.dtype, ctx.multiplier, rstd,
+                rstd_post, dx, d_residual, d_gate, d_weight, d_post, workspace)
+        if ctx.alone:
+            return d_residual, None, d_weight, None, None, None, None, None
+        if shared:
+            dx = d_residual if want_x else None
+            d_residual = d_residual if want_residual else None
+        return dx, d_residual, d_weight, d_post, d_gate, None, None, None
+
+
+def _check_rows(x: torch.Tensor) -> None:
+    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError(f"x should be bfloat16, float16 or float32, got {x.dtype}")
+    if x.dim() < 1 or not 1 <= x.size(-1) <= _MAX_HIDDEN:
+        raise ValueError(f"x should have a last dimension of 1 to {_MAX_HIDDEN} elements, got shape {tuple(x.shape)}")
+
+
+def _check_parameter(name: str, t: torch.Tensor | None, x: torch.Tensor) -> None:
+    if t is None:
+        return
+    if t.shape != x.shape[-1:]:
+        raise ValueError(f"{name} should have shape {tuple(x.shape[-1:])}, got {tuple(t.shape)}")
+    if t.dtype not in (x.dtype, torch.float32):
+        raise ValueError(f"{name} should be {x.dtype} or float32, got {t.dtype}")
+    if t.device != x.device:
+        raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+
+
+def _eps(eps: float | None, x: torch.Tensor) -> float:
+    eps = torch.finfo(x.dtype).eps if eps is None else float(eps)
+    if not eps >= 0:
+        raise ValueError(f"eps should not be negative, got {eps}")
+    return eps
+
+
+def rmsnorm(
+    x: torch.Tensor, weight: torch.Tensor | None, eps: float | None = None, *, kernel_backend: KernelBackend | None = None
+) -> torch.Tensor:
+    """`weight * x / sqrt(mean(x^2, -1) + eps)`, computed in float32 and rounded once to the dtype of `x`.
+
+    `weight` is `[H]` in the dtype of `x` or in float32, or None (ones). `eps=None` takes the machine epsilon of
+    the dtype of `x`."""
+    require_cuda_backend(kernel_backend)
+    _check_rows(x)
+    _check_parameter("weight", weight, x)
+    y = _Norm.apply(x.reshape(-1, x.size(-1)), None, weight, None, None, GATE_NONE, _eps(eps, x), 1.0)
+    return y.view(x.shape)
+
+
+def fused_residual_add_rmsnorm(
+    x: torch.Tensor,
+    residual: torch.Tensor,
+    weight: torch.Tensor | None,
+    eps: float | None = None,
+    multiplier: float | None = None,
+    *,
+    post_weight: torch.Tensor | None = None,
+    gate: torch.Tensor | None = None,
+    kernel_backend: KernelBackend | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Joins the output `x` of a block to the residual stream and norms the result for the next block:
+
+        u = x if post_weight is None else rmsnorm(x, post_weight, eps)
+        stream = residual + multiplier * gate * u
+        y = rmsnorm(stream, weight, eps)
+
+    and returns `(y, stream)`. All of it runs in float32; `y` is taken before `stream` is rounded.
+
+    `residual` (and with it `stream`) has the shape of `x` and its dtype or float32. `gate` is `[H]` (a
+    parameter), one factor per token (the shape of `x` with a last dimension of 1) or has the shape of `x`; a
+    gate that is not `[H]` has the dtype of `x`, the parameters that or float32. `weight=None` norms without a
+    weight, `multiplier=None` is 1, `eps=None` the machine epsilon of the dtype of `x`."""
+    require_cuda_backend(kernel_backend)
+    _check_rows(x)
+    if residual.shape != x.shape:
+        raise ValueError(f"residual should have the shape of x, {tuple(x.shape)}, got {tuple(residual.shape)}")
+    if residual.dtype not in (x.dtype, torch.float32):
+        raise ValueError(f"residual should be {x.dtype} or float32, got {residual.dtype}")
+    if residual.device != x.device:
+        raise ValueError(f"residual is on {residual.device}, x on {x.device}")
+    _check_parameter("weight", weight, x)
+    _check_parameter("post_weight", post_weight, x)
+    hidden = x.size(-1)
+    gate_mode = GATE_NONE
+    if gate is not None:
+        if gate.shape == x.shape and gate.dtype == x.dtype:
+            gate_mode, gate_rows = GATE_FULL, gate.reshape(-1, hidden)
+        elif gate.shape == x.shape[-1:]:
+            _check_parameter("gate", gate, x)
+            gate_mode, gate_rows = GATE_CHANNEL, gate
+        elif gate.shape == x.shape[:-1] + (1,):
+            gate_mode, gate_rows = GATE_TOKEN, gate.reshape(-1)
+        else:
+            raise ValueError(
+                f"gate should have shape {(hidden,)}, {tuple(x.shape[:-1]) + (1,)} or {tuple(x.shape)}, got {tuple(gate.shape)}")
+        if gate_mode != GATE_CHANNEL and gate.dtype != x.dtype:
+            raise ValueError(f"a gate of every token should be {x.dtype}, got {gate.dtype}")
+        if gate.device != x.device:
+            raise ValueError(f"gate is on {gate.device}, x on {x.device}")
+    y, stream = _Norm.apply(
+        x.reshape(-1, hidden), residual.reshape(-1, hidden), weight, post_weight, None if gate is None else gate_rows,
+        gate_mode, _eps(eps, x), 1.0 if multiplier is None else float(multiplier))
+    return y.view(x.shape), stream.view(x.shape)

@@ -302,3 +302,44 @@ def pack_unpack_sequence_cuda(
         N.ptr(x), N.ptr(cu_seqlens), int(cu_seqlens.dtype == torch.int64), batch, seq, row_bytes,
         int(padding_side == "left"), N.ptr(output),
     )
+
+
+def _f32_params(weight: torch.Tensor | None, post_weight: torch.Tensor | None, gate: torch.Tensor | None) -> int:
+    return sum(bit for bit, t in ((1, weight), (2, post_weight), (4, gate)) if t is not None and t.dtype == torch.float32)
+
+
+@xma_op(mutates_args={"stream_out", "y", "rstd", "rstd_post"})
+def norm_forward_cuda(
+    x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor | None, post_weight: torch.Tensor | None,
+    gate: torch.Tensor | None, gate_mode: int, eps: float, multiplier: float, stream_out: torch.Tensor | None,
+    y: torch.Tensor, rstd: torch.Tensor | None, rstd_post: torch.Tensor | None
+) -> None:
+    """stream_out = residual + multiplier * gate * norm(x; post_weight), y = norm(stream_out; weight); see
+    xma_norm_forward in include/xma_b200.h."""
+    assert x.is_contiguous() and (residual is None or residual.is_contiguous())
+    rows, hidden = x.shape
+    stream_dtype = x.dtype if residual is None else residual.dtype
+    _launch("xma_norm_forward", x,
+        N.ptr(x), N.ptr(residual), N.ptr(weight), N.ptr(post_weight), N.ptr(gate), gate_mode, N.dtype_code(x.dtype),
+        N.dtype_code(stream_dtype), _f32_params(weight, post_weight, gate), rows, hidden, eps, multiplier,
+        N.ptr(stream_out), N.ptr(y), N.ptr(rstd), N.ptr(rstd_post),
+    )
+
+
+@xma_op(mutates_args={"dx", "d_residual", "d_gate", "d_weight", "d_post_weight", "workspace"})
+def norm_backward_cuda(
+    dy: torch.Tensor | None, d_stream: torch.Tensor | None, stream: torch.Tensor, x: torch.Tensor | None,
+    weight: torch.Tensor | None, post_weight: torch.Tensor | None, gate: torch.Tensor | None, gate_mode: int,
+    dtype: torch.dtype, multiplier: float, rstd: torch.Tensor, rstd_post: torch.Tensor | None, dx: torch.Tensor | None,
+    d_residual: torch.Tensor | None, d_gate: torch.Tensor | None, d_weight: torch.Tensor | None,
+    d_post_weight: torch.Tensor | None, workspace: torch.Tensor
+) -> None:
+    """Gradients of norm_forward_cuda's inputs; see xma_norm_backward in include/xma_b200.h."""
+    assert stream.is_contiguous() and all(t is None or t.is_contiguous() for t in (dy, d_stream, x, gate))
+    rows, hidden = stream.shape
+    _launch("xma_norm_backward", stream,
+        N.ptr(dy), N.ptr(d_stream), N.ptr(stream), N.ptr(x), N.ptr(weight), N.ptr(post_weight), N.ptr(gate), gate_mode,
+        N.dtype_code(dtype), N.dtype_code(stream.dtype), _f32_params(weight, post_weight, gate), rows, hidden,
+        multiplier, N.ptr(rstd), N.ptr(rstd_post), N.ptr(dx), N.ptr(d_residual), N.ptr(d_gate), N.ptr(d_weight),
+        N.ptr(d_post_weight), N.ptr(workspace), N.ptr(N.status_word(stream.device)),
+    )

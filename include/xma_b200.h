@@ -373,6 +373,39 @@ int xma_pack_sequence(const void* x, const void* cu_seqlens, int32_t cu_is_int64
 int xma_unpack_sequence(const void* x, const void* cu_seqlens, int32_t cu_is_int64, int64_t batch, int64_t seq,
                         int64_t row_bytes, int32_t pad_left, void* out, void* stream);
 
+/*
+ * Root-mean-square norms before and after a block, fused with the block's gate and the residual add. Per
+ * row of `hidden` elements, in float32:
+ *   u = post_weight * x / rms(x)   (u = x when post_weight is NULL),   rms(v) = sqrt(mean(v^2) + eps)
+ *   stream_out = residual + multiplier * gate * u
+ *   y = weight * stream_out / rms(stream_out)   (taken before stream_out is rounded; weight NULL: ones)
+ * With residual NULL: y = weight * x / rms(x) alone (post_weight, gate NULL; stream_out unused).
+ *   dtype         x, gate [rows] / [rows, hidden], y          stream_dtype   residual, stream_out: `dtype` or float32
+ *   gate_mode     0 none, 1 [hidden] (a parameter), 2 [rows], 3 [rows, hidden]
+ *   f32_params    bit 0 weight, bit 1 post_weight, bit 2 a [hidden] gate is float32 (else `dtype`)
+ *   rstd, rstd_post   float32 [rows], 1 / rms of the stream and of x, kept for the backward pass; may be NULL
+ * Any row length up to 2^24 and any element alignment; rows of a multiple of 8 elements with 16-byte
+ * aligned bases take wide accesses.
+ *
+ * xma_norm_backward: from dy (gradient of y) and d_stream (gradient of stream_out), either of which may be
+ * NULL (zero), to d_residual, dx, d_gate, d_weight, d_post_weight; each output may be NULL. stream_saved is
+ * stream_out (x for the norm alone, whose gradient is then d_residual); x is needed with a post norm or a
+ * gate only. Gradients of parameters have the parameters' types and are summed over the rows in a fixed
+ * order through `workspace`: xma_norm_workspace_floats(rows, hidden) floats, 16-byte aligned, contents
+ * irrelevant before and after. rows == 0 writes nothing. Code 401 or 402 goes to *status when a wait for
+ * the kernel's own copies runs out.
+ */
+#define XMA_NORM_PARTIALS 148
+int64_t xma_norm_workspace_floats(int64_t rows, int64_t hidden);
+int xma_norm_forward(const void* x, const void* residual, const void* weight, const void* post_weight, const void* gate,
+                     int32_t gate_mode, int32_t dtype, int32_t stream_dtype, int32_t f32_params, int64_t rows, int64_t hidden,
+                     float eps, float multiplier, void* stream_out, void* y, float* rstd, float* rstd_post, void* stream);
+int xma_norm_backward(const void* dy, const void* d_stream, const void* stream_saved, const void* x, const void* weight,
+                      const void* post_weight, const void* gate, int32_t gate_mode, int32_t dtype, int32_t stream_dtype,
+                      int32_t f32_params, int64_t rows, int64_t hidden, float multiplier, const float* rstd,
+                      const float* rstd_post, void* dx, void* d_residual, void* d_gate, void* d_weight, void* d_post_weight,
+                      float* workspace, int32_t* status, void* stream);
+
 /* Maps another process's device allocation into this process for the CURRENT device, with peer access
  * enabled: handle64 is that allocation's 64-byte cudaIpcMemHandle_t. Host-side call, no stream. */
 int xma_ipc_open_handle(const void* handle64, void** device_ptr);
