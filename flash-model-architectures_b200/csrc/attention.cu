@@ -1,0 +1,1307 @@
+// Causal attention over a packed token stream, forward and backward, on sm_100a tensor cores.
+//
+// The stream holds sequences one after another (cu_seqlens); a query attends to the keys of its own
+// sequence up to its own position. Query head h reads key/value head h / (heads / kv_heads). With
+// s_ij = scale q_i . k_j, p_ij = exp(s_ij - lse_i), lse_i = log sum_{j <= i} exp(s_ij):
+//   o_i  = sum_j p_ij v_j
+//   dv_j = sum_i p_ij do_i,  ds_ij = p_ij (do_i . v_j - delta_i),  delta_i = o_i . do_i
+//   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i    (dk, dv also over the head's group)
+//
+// Tiles are 128 x 128 scores; a head is kD = 64 or 128 wide in shared memory (narrower heads are padded
+// with zeros by the tensor-map bounds). Scores, statistics and all sums are float32 in tensor memory or
+// registers; p and ds are rounded to the inputs' type where they become operands of the second product.
+//
+//   plan      one small launch: the list of row blocks of all sequences, longest work first, and zeros
+//             for the rows that no sequence owns
+//   forward   persistent CTAs, two 128-row query tiles each: while one tile's softmax runs, the tensor
+//             core works for the other. p overwrites s in tensor memory and is the A operand of p v
+//   dkdv      a 128-row key tile per work item, all query tiles and heads that see it; s^T and dp^T
+//             are computed transposed so that p^T and ds^T are A operands from tensor memory
+//   dq        a 128-row query tile per work item over its key tiles
+// dk, dv and dq are each summed by one CTA in a fixed order: no atomics, the same bits every time. That
+// costs two of seven products (s and dp are computed twice).
+//
+// Rows beyond a sequence's end inside a tile belong to other sequences: their scores are masked by
+// selection, and where a masked (zero) probability would multiply such a row, the row is zeroed in shared
+// memory first, so that not even a NaN crosses over. Every wait is bounded, as in the grouped GEMM.
+#include <mutex>
+#include <type_traits>
+
+#include "common.cuh"
+#include "ptx.cuh"
+
+namespace xma {
+namespace attn {
+
+using namespace ptx;
+
+constexpr int kTile = 128;            // query or key rows of a tile
+constexpr int kThreads = 384;         // load warp, MMA warp, two idle, two groups of four compute warps
+constexpr int kTmemCols = 512;
+constexpr float kRescaleLog2 = 8.f;   // the accumulator is rescaled when a row's maximum grew by more than 2^8
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanBuckets = 1024;
+constexpr int kMaxHeads = 4096;
+
+// One block of rows of one sequence.
+struct Block {
+    int start;  // first token of the sequence
+    int len;    // its tokens
+    int index;  // block number inside the sequence
+    int pad;    // first entry of the sequence in the padded row statistics
+};
+
+struct Params {
+    const Block* blocks;
+    const int32_t* num_blocks;
+    int heads, kv_heads, group, dim;
+    int64_t pad_rows;  // entries of the padded row statistics per head
+    float scale, scale_log2;
+    void* out;         // forward: o
+    float* lse;        // [heads][pad_rows], log2 units; may be NULL in the forward pass
+    const float* delta;
+    void* dq;
+    void* dk;
+    void* dv;
+    const uint32_t* absmax;  // backward, fp16: bit patterns of max |do| and max |v|
+    int32_t* status;
+    int ab_format;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Plan
+// ---------------------------------------------------------------------------------------------
+
+// Sequence b of cu_seqlens, clamped into the stream whatever the array holds.
+template <typename IntT>
+__device__ __forceinline__ void sequence(const IntT* cu, int64_t b, int64_t total, int* start, int* len) {
+    const int64_t s = min(max(static_cast<int64_t>(cu[b]), int64_t(0)), total);
+    const int64_t e = min(max(static_cast<int64_t>(cu[b + 1]), s), total);
+    *start = static_cast<int>(s);
+    *len = static_cast<int>(e - s);
+}
+__device__ __forceinline__ int pad_offset(int start, int64_t b) { return static_cast<int>((start / kTile + b) * kTile); }
+
+struct ZeroRows {
+    void* base;
+    int64_t row_bytes;  // a multiple of 16
+};
+
+// Block 0 (and 1, for the second list) writes a list; the others zero the rows before the first and after
+// the last sequence. A list holds every block of `block_rows` rows of every sequence, by falling work:
+// kFromEnd = false: a block's index (keys before it), true: the number of blocks after it.
+template <typename IntT>
+__global__ void __launch_bounds__(kPlanThreads)
+plan_kernel(const IntT* __restrict__ cu, int64_t batch, int64_t total, int block_rows, int64_t capacity, Block* list0, int32_t* count0,
+            Block* list1, int32_t* count1, uint32_t* absmax, ZeroRows z0, ZeroRows z1, ZeroRows z2, int num_lists) {
+    if (static_cast<int>(blockIdx.x) >= num_lists) {
+        const int64_t first = min(max(static_cast<int64_t>(cu[0]), int64_t(0)), total);
+        const int64_t last = min(max(static_cast<int64_t>(cu[batch]), first), total);
+        const int64_t tail = total - last, rows = first + tail;
+        const int64_t at = static_cast<int64_t>(blockIdx.x - num_lists) * blockDim.x + threadIdx.x;
+        const int64_t step = static_cast<int64_t>(gridDim.x - num_lists) * blockDim.x;
+        const ZeroRows zs[3] = {z0, z1, z2};
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            if (zs[i].base == nullptr) continue;
+            const int64_t per_row = zs[i].row_bytes / 16;
+            for (int64_t c = at; c < rows * per_row; c += step) {
+                const int64_t r = c / per_row;
+                const int64_t row = r < first ? r : last + (r - first);
+                reinterpret_cast<uint4*>(zs[i].base)[row * per_row + (c - r * per_row)] = make_uint4(0, 0, 0, 0);
+            }
+        }
+        return;
+    }
+    const bool from_end = blockIdx.x == 1;
+    Block* list = from_end ? list1 : list0;
+    __shared__ int bucket[kPlanBuckets];
+    __shared__ int warp_sum[32];
+    for (int i = threadIdx.x; i < kPlanBuckets; i += blockDim.x) bucket[i] = 0;
+    if (threadIdx.x < 2 && absmax != nullptr && !from_end) absmax[threadIdx.x] = 0;
+    __syncthreads();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int64_t b = warp; b < batch; b += kPlanThreads / 32) {
+        int start, len;
+        sequence(cu, b, total, &start, &len);
+        const int n = (len + block_rows - 1) / block_rows;
+        for (int i = lane; i < n; i += 32) atomicAdd(&bucket[min(from_end ? n - 1 - i : i, kPlanBuckets - 1)], 1);
+    }
+    __syncthreads();
+    // thread t takes bucket kPlanBuckets - 1 - t: an exclusive prefix sum from the largest work down
+    const int mine = kPlanBuckets - 1 - static_cast<int>(threadIdx.x);
+    const int value = bucket[mine];
+    int incl = value;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, incl, off);
+        if (lane >= off) incl += o;
+    }
+    if (lane == 31) warp_sum[warp] = incl;
+    __syncthreads();
+    if (warp == 0) {
+        int v = warp_sum[lane];
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, v, off);
+            if (lane >= off) v += o;
+        }
+        warp_sum[lane] = v;
+    }
+    __syncthreads();
+    bucket[mine] = incl - value + (warp > 0 ? warp_sum[warp - 1] : 0);
+    // Sequences that overlap (not a valid cu_seqlens) could be more than the list holds: the rest is dropped.
+    if (threadIdx.x == 0) *(from_end ? count1 : count0) = static_cast<int>(min(static_cast<int64_t>(warp_sum[31]), capacity));
+    __syncthreads();
+    for (int64_t b = warp; b < batch; b += kPlanThreads / 32) {
+        int start, len;
+        sequence(cu, b, total, &start, &len);
+        const int n = (len + block_rows - 1) / block_rows;
+        for (int i = lane; i < n; i += 32) {
+            // the order inside a bucket is not fixed; it decides who computes a block, not what
+            const int at = atomicAdd(&bucket[min(from_end ? n - 1 - i : i, kPlanBuckets - 1)], 1);
+            if (at < capacity) list[at] = Block{start, len, i, pad_offset(start, b)};
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Shared device pieces
+// ---------------------------------------------------------------------------------------------
+
+// A [128, kD] tile of one head from a [tokens, heads, dim] tensor: kD / 64 boxes of 128 rows x 64 columns
+// (128-byte swizzle), 16 KB each.
+template <int kD>
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, uint32_t bar, int head, int row) {
+#pragma unroll
+    for (int c = 0; c < kD / 64; ++c) tma_load_3d_cta1(dst + c * (kTile * 128), map, bar, c * 64, head, row);
+}
+
+// Rows [first, 128) of a tile become zeros (a warp's work); the tile's rows are 128 bytes per box.
+template <int kD>
+__device__ __forceinline__ void zero_tile_rows(uint32_t tile, int first, int lane) {
+    const int chunks = (kTile - first) * 8;
+#pragma unroll
+    for (int c = 0; c < kD / 64; ++c)
+        for (int i = lane; i < chunks; i += 32)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + c * (kTile * 128) + first * 128 + i * 16), "r"(0) : "memory");
+}
+
+// Operand with the reduction along the head dimension (rows of a tile are rows or columns of the product).
+__device__ __forceinline__ uint64_t desc_k_major(uint32_t tile, int kk) {
+    return make_smem_desc(tile + (kk >> 2) * (kTile * 128) + (kk & 3) * 32, 0, 1024);
+}
+// Operand with the reduction along the tile's rows (the head dimension is a dimension of the product).
+__device__ __forceinline__ uint64_t desc_row_major(uint32_t tile, int kk) {
+    return make_smem_desc(tile + kk * 2048, kTile * 128, 1024);
+}
+
+// D[128, 128] = A B^T over the head dimension.
+template <int kD>
+__device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a_tile, uint32_t b_tile, uint32_t idesc) {
+#pragma unroll
+    for (int kk = 0; kk < kD / 16; ++kk)
+        umma_ss_cta1(d, desc_k_major(a_tile, kk), desc_k_major(b_tile, kk), idesc, kk != 0 ? 1u : 0u);
+}
+// D[128, kD] (+)= A B over 128 rows of B; A in tensor memory, its second half of the rows `second` columns on.
+__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t second, uint32_t b_tile, uint32_t idesc, bool accumulate) {
+#pragma unroll
+    for (int kk = 0; kk < kTile / 16; ++kk)
+        umma_ts_cta1(d, a + (kk >> 2) * second + (kk & 3) * 8, desc_row_major(b_tile, kk), idesc, (accumulate || kk != 0) ? 1u : 0u);
+}
+
+// 16-byte pieces of one row of kD float32 values in tensor memory, scaled and rounded, to global memory.
+template <typename T, int kD>
+__device__ __forceinline__ void store_row(uint32_t taddr, T* dst, int dim, float scale, bool valid) {
+#pragma unroll
+    for (int c = 0; c < kD / 32; ++c) {
+        uint32_t r[32];
+        tmem_ld32(taddr + c * 32, r);
+        tmem_ld_wait();
+        tmem_tie32(r);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (valid && c * 32 + q * 8 < dim) {
+                uint4 v;
+                v.x = pack2<T>(__uint_as_float(r[q * 8]) * scale, __uint_as_float(r[q * 8 + 1]) * scale);
+                v.y = pack2<T>(__uint_as_float(r[q * 8 + 2]) * scale, __uint_as_float(r[q * 8 + 3]) * scale);
+                v.z = pack2<T>(__uint_as_float(r[q * 8 + 4]) * scale, __uint_as_float(r[q * 8 + 5]) * scale);
+                v.w = pack2<T>(__uint_as_float(r[q * 8 + 6]) * scale, __uint_as_float(r[q * 8 + 7]) * scale);
+                *reinterpret_cast<uint4*>(dst + c * 32 + q * 8) = v;
+            }
+        }
+    }
+}
+
+struct Ring {
+    int stage = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void next(int stages) {
+        if (++stage == stages) {
+            stage = 0;
+            phase ^= 1u;
+        }
+    }
+};
+
+// ---------------------------------------------------------------------------------------------
+// Forward
+// ---------------------------------------------------------------------------------------------
+
+template <int kD>
+struct Forward {
+    static constexpr uint32_t kTileBytes = kTile * kD * 2;
+    static constexpr int kStages = kD == 128 ? 5 : 8;
+    static constexpr uint32_t kSmem = 1024 + (2 + kStages) * kTileBytes + 256;
+    static constexpr uint32_t kO = 256;  // tensor memory: s of the two tiles at 0 and 128, o at 256 and 256 + kD
+};
+
+// Work item: 256 query rows (two tiles) of one head. Tile t's last key tile is its diagonal.
+template <typename T, int kD>
+__global__ void __launch_bounds__(kThreads, 1)
+forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+               const __grid_constant__ CUtensorMap map_v, const Params p) {
+    using F = Forward<kD>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t q_tile = base, ring = base + 2 * F::kTileBytes;
+    constexpr uint32_t kBars = (2 + F::kStages) * F::kTileBytes;
+    const uint32_t bars = base + kBars;
+    const uint32_t full = bars, empty = bars + 64;
+    const uint32_t q_full = bars + 128, q_empty = bars + 144, s_full = bars + 160, p_ready = bars + 176, o_full = bars + 192;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + kBars + 208);
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + kBars + 212);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < F::kStages; ++i) {
+            mbar_init(full + 8 * i, 1);
+            mbar_init(empty + 8 * i, 1);
+        }
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(q_full + 8 * t, 1);
+            mbar_init(q_empty + 8 * t, 1);
+            mbar_init(s_full + 8 * t, 1);
+            mbar_init(p_ready + 8 * t, 4);  // the four warps of a tile
+            mbar_init(o_full + 8 * t, 1);
+        }
+        *abort_flag = 0;
+        fence_barrier_init();
+        prefetch_tmap(&map_q);
+        prefetch_tmap(&map_k);
+        prefetch_tmap(&map_v);
+    }
+    if (warp == 1) {
+        tmem_alloc(bars + 212, kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int64_t items = static_cast<int64_t>(*p.num_blocks) * p.heads;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            Ring kv;
+            uint32_t q_phase[2] = {1u, 1u};
+            bool ok = true;
+            for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x) {
+                const Block b = p.blocks[it / p.heads];
+                const int head = static_cast<int>(it % p.heads), kv_head = head / p.group;
+                const int row0 = b.index * 2 * kTile;
+                const int tiles = b.len > row0 + kTile ? 2 : 1;
+                const int n = b.index * 2 + tiles;
+                for (int t = 0; ok && t < tiles; ++t) {
+                    ok = mbar_wait(q_empty + 8 * t, q_phase[t], abort_flag, p.status, 501);
+                    if (!ok) break;
+                    q_phase[t] ^= 1u;
+                    mbar_expect_tx(q_full + 8 * t, F::kTileBytes);
+                    load_tile<kD>(q_tile + t * F::kTileBytes, &map_q, q_full + 8 * t, head, b.start + row0 + t * kTile);
+                }
+                for (int j = 0; ok && j < 2 * n; ++j) {  // k of tile 0, v of tile 0, k of tile 1, ...
+                    ok = mbar_wait(empty + 8 * kv.stage, kv.phase ^ 1u, abort_flag, p.status, 502);
+                    if (!ok) break;
+                    mbar_expect_tx(full + 8 * kv.stage, F::kTileBytes);
+                    load_tile<kD>(ring + kv.stage * F::kTileBytes, (j & 1) ? &map_v : &map_k, full + 8 * kv.stage, kv_head,
+                                  b.start + (j >> 1) * kTile);
+                    kv.next(F::kStages);
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        const uint32_t idesc_s = make_idesc(kTile, kTile, false, false, p.ab_format);
+        const uint32_t idesc_o = make_idesc(kTile, kD, false, true, p.ab_format);
+        Ring kv;
+        uint32_t q_phase[2] = {0u, 0u}, p_phase[2] = {0u, 0u};
+        bool ok = true;
+        for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x) {
+            const Block b = p.blocks[it / p.heads];
+            const int row0 = b.index * 2 * kTile;
+            const int tiles = b.len > row0 + kTile ? 2 : 1;
+            const int n = b.index * 2 + tiles;              // key tiles of the last query tile
+            const int first = b.index * 2 + 1;              // key tiles of query tile 0
+            // s of key tile 0
+            ok = mbar_wait(full + 8 * kv.stage, kv.phase, abort_flag, p.status, 503);
+            for (int t = 0; ok && t < tiles; ++t) {
+                ok = mbar_wait(q_full + 8 * t, q_phase[t], abort_flag, p.status, 504);
+                if (!ok) break;
+                q_phase[t] ^= 1u;
+                tc_fence_after();
+                if (lane == 0) {
+                    mma_scores<kD>(tmem + t * kTile, q_tile + t * F::kTileBytes, ring + kv.stage * F::kTileBytes, idesc_s);
+                    umma_commit_cta1(s_full + 8 * t);
+                    if (first + t == 1) umma_commit_cta1(q_empty + 8 * t);
+                }
+                __syncwarp();
+            }
+            if (!ok) break;
+            if (lane == 0) umma_commit_cta1(empty + 8 * kv.stage);
+            kv.next(F::kStages);
+            for (int j = 0; ok && j < n; ++j) {
+                const uint32_t v_tile = ring + kv.stage * F::kTileBytes;
+                const uint32_t v_empty = empty + 8 * kv.stage;
+                ok = mbar_wait(full + 8 * kv.stage, kv.phase, abort_flag, p.status, 505);
+                if (!ok) break;
+                kv.next(F::kStages);
+                const int valid = b.len - j * kTile;
+                if (valid < kTile) {  // rows of other sequences
+                    zero_tile_rows<kD>(v_tile, valid, lane);
+                    fence_proxy_async();
+                    __syncwarp();
+                }
+                const uint32_t k_tile = ring + kv.stage * F::kTileBytes;
+                const uint32_t k_empty = empty + 8 * kv.stage;
+                const bool more = j + 1 < n;
+                if (more) ok = mbar_wait(full + 8 * kv.stage, kv.phase, abort_flag, p.status, 506);
+                for (int t = 0; ok && t < tiles; ++t) {
+                    const int count = first + t;
+                    if (j >= count) continue;
+                    ok = mbar_wait(p_ready + 8 * t, p_phase[t], abort_flag, p.status, 507);
+                    if (!ok) break;
+                    p_phase[t] ^= 1u;
+                    tc_fence_after();
+                    if (lane == 0) {
+                        mma_rows(tmem + F::kO + t * kD, tmem + t * kTile, 32, v_tile, idesc_o, j != 0);
+                        if (j + 1 < count) {
+                            // overwrites p, which the product just issued reads: the pipe runs them in order
+                            mma_scores<kD>(tmem + t * kTile, q_tile + t * F::kTileBytes, k_tile, idesc_s);
+                            umma_commit_cta1(s_full + 8 * t);
+                            if (j + 2 == count) umma_commit_cta1(q_empty + 8 * t);
+                        } else {
+                            umma_commit_cta1(o_full + 8 * t);
+                        }
+                    }
+                    __syncwarp();
+                }
+                if (!ok) break;
+                if (lane == 0) {
+                    umma_commit_cta1(v_empty);
+                    if (more) umma_commit_cta1(k_empty);
+                }
+                __syncwarp();
+                if (more) kv.next(F::kStages);
+            }
+        }
+    } else if (warp >= 4) {
+        const int t = (warp >> 2) - 1;               // query tile of this group
+        const int row = (warp & 3) * 32 + lane;      // its row, and the tensor-memory lane
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t s_addr = tmem + lanes + t * kTile, o_addr = tmem + lanes + F::kO + t * kD;
+        uint32_t s_phase = 0, o_phase = 0;
+        bool ok = true;
+        for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x) {
+            const Block b = p.blocks[it / p.heads];
+            const int head = static_cast<int>(it % p.heads);
+            const int row0 = b.index * 2 * kTile;
+            if (t == 1 && b.len <= row0 + kTile) continue;
+            const int count = b.index * 2 + 1 + t;
+            float m = -INFINITY, l = 0.f;  // running maximum (log2 units) that p refers to, and sum of p
+            for (int j = 0; j < count; ++j) {
+                ok = mbar_wait(s_full + 8 * t, s_phase, abort_flag, p.status, 508);
+                if (!ok) break;
+                s_phase ^= 1u;
+                tc_fence_after();
+                uint32_t s[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, s[c]);
+                tmem_ld_wait();
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_tie32(s[c]);
+                if (j == count - 1) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (c * 32 + i > row) s[c][i] = 0xff800000u;  // -inf
+                }
+                float top[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    top[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+                    for (int i = 1; i < 32; ++i) top[c] = fmaxf(top[c], __uint_as_float(s[c][i]));
+                }
+                const float tile_max = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
+                if (j == 0) {
+                    m = tile_max;
+                } else {
+                    // The sum stays exact whatever m is, as long as p does not overflow: the accumulator is
+                    // touched only when a maximum grew by 2^8, which after the first tiles hardly happens.
+                    const bool grow = tile_max - m > kRescaleLog2;
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float factor = grow ? ex2(m - tile_max) : 1.f;
+                        if (grow) m = tile_max;
+                        l *= factor;
+#pragma unroll
+                        for (int c = 0; c < kD / 32; ++c) {
+                            uint32_t o[32];
+                            tmem_ld32(o_addr + c * 32, o);
+                            tmem_ld_wait();
+                            tmem_tie32(o);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+                            tmem_st32(o_addr + c * 32, o);
+                        }
+                    }
+                }
+                const float neg_m = m == -INFINITY ? 0.f : -m;  // a row with no finite score so far
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t packed[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int c = h * 2 + (i >> 4), e = (i & 15) * 2;
+                        const float a = ex2(fmaf(__uint_as_float(s[c][e]), p.scale_log2, neg_m));
+                        const float d = ex2(fmaf(__uint_as_float(s[c][e + 1]), p.scale_log2, neg_m));
+                        sum[i & 1] += a;
+                        sum[2 + (i & 1)] += d;
+                        packed[i] = pack2<T>(a, d);
+                    }
+                    tmem_st32(s_addr + h * 32, packed);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_ready + 8 * t);
+            }
+            if (!ok) break;
+            ok = mbar_wait(o_full + 8 * t, o_phase, abort_flag, p.status, 509);
+            if (!ok) break;
+            o_phase ^= 1u;
+            tc_fence_after();
+            const int r = row0 + t * kTile + row;
+            const bool valid = r < b.len;
+            T* dst = static_cast<T*>(p.out) + (static_cast<int64_t>(b.start + r) * p.heads + head) * p.dim;
+            store_row<T, kD>(o_addr, dst, p.dim, 1.f / l, valid);
+            if (p.lse != nullptr && valid) p.lse[head * p.pad_rows + b.pad + r] = m + lg2(l);
+            tc_fence_before();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, kTmemCols);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Backward
+// ---------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ float absmax_value(uint32_t bits) {
+    const float v = __uint_as_float(bits);
+    return v <= 65504.f ? v : 65504.f;  // also when it is infinite or NaN
+}
+// Factor (a power of two) that ds carries while it is rounded to T. bf16 has float32's range: 1. fp16 has
+// not: |ds| is at most 2 dim max|do| max|v|, and that bound is put at 2^15, just below the largest fp16, so
+// that what gradients without loss scaling are made of does not fall under its smallest.
+template <typename T>
+__device__ __forceinline__ float ds_factor(const Params& p) { return 1.f; }
+template <>
+__device__ __forceinline__ float ds_factor<__half>(const Params& p) {
+    const float bound = 2.f * static_cast<float>(p.dim) * absmax_value(p.absmax[0]) * absmax_value(p.absmax[1]);
+    if (!(bound > 0.f)) return 1.f;
+    return exp2f(static_cast<float>(min(max(14 - ilogbf(bound), -100), 100)));
+}
+
+// delta_i = o_i . do_i for every owned row and head, one warp per row and head; for fp16 also max |do| and
+// max |v| (over bit patterns, whose order does not depend on that of the atomics).
+template <typename T, typename IntT>
+__global__ void __launch_bounds__(256)
+delta_kernel(const T* __restrict__ o, const T* __restrict__ d_o, const T* __restrict__ v, int64_t v_token, int64_t v_head,
+             const IntT* __restrict__ cu, int64_t batch, int64_t total, float* __restrict__ delta, uint32_t* absmax, const Params p) {
+    constexpr bool kHalf = std::is_same<T, __half>::value;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t most_do = 0, most_v = 0;
+    for (int64_t row = blockIdx.x; row < total; row += gridDim.x) {
+        // last sequence that starts at or before the row
+        int64_t lo = 0, hi = batch - 1;
+        while (lo < hi) {
+            const int64_t mid = (lo + hi + 1) >> 1;
+            if (static_cast<int64_t>(cu[mid]) <= row) lo = mid; else hi = mid - 1;
+        }
+        int start, len;
+        sequence(cu, lo, total, &start, &len);
+        if (row < start || row >= static_cast<int64_t>(start) + len) continue;  // nobody's row
+        const int64_t at = pad_offset(start, lo) + (row - start);
+        for (int h = warp; h < p.heads; h += 8) {
+            const int64_t off = (row * p.heads + h) * p.dim;
+            float sum = 0.f;
+            for (int c = lane * 4; c < p.dim; c += 128) {
+                const uint2 a = *reinterpret_cast<const uint2*>(o + off + c), b = *reinterpret_cast<const uint2*>(d_o + off + c);
+                const float2 a0 = unpack2<T>(a.x), a1 = unpack2<T>(a.y), b0 = unpack2<T>(b.x), b1 = unpack2<T>(b.y);
+                sum += a0.x * b0.x + a0.y * b0.y + a1.x * b1.x + a1.y * b1.y;
+                if (kHalf) most_do = max(most_do, __float_as_uint(fmaxf(fmaxf(fabsf(b0.x), fabsf(b0.y)), fmaxf(fabsf(b1.x), fabsf(b1.y)))));
+            }
+#pragma unroll
+            for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+            if (lane == 0) delta[h * p.pad_rows + at] = sum;
+        }
+        if (kHalf) {
+            for (int h = warp; h < p.kv_heads; h += 8)
+                for (int c = lane * 4; c < p.dim; c += 128) {
+                    const uint2 a = *reinterpret_cast<const uint2*>(v + row * v_token + h * v_head + c);
+                    const float2 a0 = unpack2<T>(a.x), a1 = unpack2<T>(a.y);
+                    most_v = max(most_v, __float_as_uint(fmaxf(fmaxf(fabsf(a0.x), fabsf(a0.y)), fmaxf(fabsf(a1.x), fabsf(a1.y)))));
+                }
+        }
+    }
+    if (kHalf) {
+        most_do = __reduce_max_sync(0xffffffffu, most_do);
+        most_v = __reduce_max_sync(0xffffffffu, most_v);
+        if (lane == 0) {
+            atomicMax(&absmax[0], most_do);
+            atomicMax(&absmax[1], most_v);
+        }
+    }
+}
+
+template <int kD>
+struct Backward {
+    static_assert(kD == 64 || kD == 128, "tile widths");
+    static constexpr uint32_t kTileBytes = kTile * kD * 2;
+    static constexpr int kStages = kD == 128 ? 2 : 4;
+    static constexpr uint32_t kStageBytes = 2 * kTileBytes;
+    static constexpr uint32_t kStats = 2 * kTile * 4;  // lse and delta of a query tile
+    static constexpr uint32_t kBars = 2 * kTileBytes + kStages * (kStageBytes + kStats);
+    static constexpr uint32_t kSmem = 1024 + kBars + 256;
+};
+
+// Work item: 128 key rows of one key/value head, all query tiles at or after them of the group's heads.
+// Tensor memory: s^T at 0, dp^T at 128, dv at 256, dk at 256 + kD. Each group of four compute warps takes 64
+// of the 128 query columns; p^T (and ds^T) of a half lies at the start of that half's columns.
+template <typename T, int kD>
+__global__ void __launch_bounds__(kThreads, 1)
+dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+            const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, const Params p) {
+    using B = Backward<kD>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t k_tile = base, v_tile = base + B::kTileBytes, ring = base + 2 * B::kTileBytes;
+    constexpr uint32_t kStatsAt = 2 * B::kTileBytes + B::kStages * B::kStageBytes;
+    const uint32_t bars = base + B::kBars;
+    const uint32_t full = bars, empty = bars + 32, kv_full = bars + 64, kv_empty = bars + 72, s_full = bars + 80, dp_full = bars + 88,
+                   p_ready = bars + 96, ds_ready = bars + 104, done = bars + 112;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + B::kBars + 128);
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + B::kBars + 132);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < B::kStages; ++i) {
+            mbar_init(full + 8 * i, 1);
+            mbar_init(empty + 8 * i, 1 + 8);  // the MMAs that read the stage, and the warps that read its statistics
+        }
+        mbar_init(kv_full, 1);
+        mbar_init(kv_empty, 1);
+        mbar_init(s_full, 1);
+        mbar_init(dp_full, 1);
+        mbar_init(p_ready, 8);
+        mbar_init(ds_ready, 8);
+        mbar_init(done, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+        prefetch_tmap(&map_q);
+        prefetch_tmap(&map_k);
+        prefetch_tmap(&map_v);
+        prefetch_tmap(&map_do);
+    }
+    if (warp == 1) {
+        tmem_alloc(bars + 132, kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t tm_s = tmem, tm_dp = tmem + kTile, tm_dv = tmem + 2 * kTile, tm_dk = tm_dv + kD;
+    const int64_t items = static_cast<int64_t>(*p.num_blocks) * p.kv_heads;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            Ring r;
+            uint32_t kv_phase = 1u;
+            bool ok = true;
+            for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x) {
+                const Block b = p.blocks[it / p.kv_heads];
+                const int kv_head = static_cast<int>(it % p.kv_heads);
+                const int n = (b.len + kTile - 1) / kTile;
+                ok = mbar_wait(kv_empty, kv_phase, abort_flag, p.status, 511);
+                if (!ok) break;
+                kv_phase ^= 1u;
+                mbar_expect_tx(kv_full, 2 * B::kTileBytes);
+                load_tile<kD>(k_tile, &map_k, kv_full, kv_head, b.start + b.index * kTile);
+                load_tile<kD>(v_tile, &map_v, kv_full, kv_head, b.start + b.index * kTile);
+                for (int g = 0; ok && g < p.group; ++g) {
+                    const int head = kv_head * p.group + g;
+                    for (int i = b.index; ok && i < n; ++i) {
+                        ok = mbar_wait(empty + 8 * r.stage, r.phase ^ 1u, abort_flag, p.status, 512);
+                        if (!ok) break;
+                        const uint32_t bar = full + 8 * r.stage, dst = ring + r.stage * B::kStageBytes;
+                        mbar_expect_tx(bar, B::kStageBytes + B::kStats);
+                        load_tile<kD>(dst, &map_q, bar, head, b.start + i * kTile);
+                        load_tile<kD>(dst + B::kTileBytes, &map_do, bar, head, b.start + i * kTile);
+                        const int64_t at = head * p.pad_rows + b.pad + i * kTile;
+                        const uint32_t stats = base + kStatsAt + r.stage * B::kStats;
+                        bulk_load(stats, p.lse + at, kTile * 4, bar);
+                        bulk_load(stats + kTile * 4, p.delta + at, kTile * 4, bar);
+                        r.next(B::kStages);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        const uint32_t idesc_s = make_idesc(kTile, kTile, false, false, p.ab_format);
+        const uint32_t idesc_d = make_idesc(kTile, kD, false, true, p.ab_format);
+        Ring r;
+        uint32_t kv_phase = 0, p_phase = 0, ds_phase = 0;
+        bool ok = true;
+        for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x) {
+            const Block b = p.blocks[it / p.kv_heads];
+            const int n = (b.len + kTile - 1) / kTile;
+            const int per_head = n - b.index, steps = per_head * p.group;
+            ok = mbar_wait(kv_full, kv_phase, abort_flag, p.status, 513);
+            if (!ok) break;
+            kv_phase ^= 1u;
+            for (int st = -1; ok && st < steps; ++st) {
+                // dv += p^T do and s^T of the next step; then dk += ds^T q and dp^T of the next step
+                const bool more = st + 1 < steps;
+                const uint32_t cur = ring + r.stage * B::kStageBytes;
+                const uint32_t cur_empty = empty + 8 * r.stage;
+                Ring ahead = r;
+                if (st >= 0) ahead.next(B::kStages);
+                const uint32_t nxt = ring + ahead.stage * B::kStageBytes;
+                if (more) {
+                    ok = mbar_wait(full + 8 * ahead.stage, ahead.phase, abort_flag, p.status, 514);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const int valid = b.len - (b.index + (st + 1) % per_head) * kTile;
+                    if (valid < kTile) {  // query rows of other sequences
+                        zero_tile_rows<kD>(nxt, valid, lane);
+                        zero_tile_rows<kD>(nxt + B::kTileBytes, valid, lane);
+                        fence_proxy_async();
+                        __syncwarp();
+                    }
+                }
+                if (st >= 0) {
+                    ok = mbar_wait(p_ready, p_phase, abort_flag, p.status, 515);
+                    if (!ok) break;
+                    p_phase ^= 1u;
+                    tc_fence_after();
+                }
+                if (lane == 0) {
+                    if (st >= 0) mma_rows(tm_dv, tm_s, 64, cur + B::kTileBytes, idesc_d, st > 0);
+                    if (more) {
+                        mma_scores<kD>(tm_s, k_tile, nxt, idesc_s);
+                        umma_commit_cta1(s_full);
+                    }
+                }
+                __syncwarp();
+                if (st >= 0) {
+                    ok = mbar_wait(ds_ready, ds_phase, abort_flag, p.status, 516);
+                    if (!ok) break;
+                    ds_phase ^= 1u;
+                    tc_fence_after();
+                }
+                if (lane == 0) {
+                    if (st >= 0) {
+                        mma_rows(tm_dk, tm_dp, 64, cur, idesc_d, st > 0);
+                        umma_commit_cta1(cur_empty);
+                    }
+                    if (more) {
+                        mma_scores<kD>(tm_dp, v_tile, nxt + B::kTileBytes, idesc_s);
+                        umma_commit_cta1(dp_full);
+                    } else {
+                        umma_commit_cta1(done);
+                        umma_commit_cta1(kv_empty);
+                    }
+                }
+                __syncwarp();
+                r = ahead;
+            }
+        }
+    } else if (warp >= 4) {
+        const int half = (warp >> 2) - 1;          // query columns 64 half .. 64 half + 63
+        const int row = (warp & 3) * 32 + lane;    // key row
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t s_addr = tm_s + lanes + half * 64, dp_addr = tm_dp + lanes + half * 64;
+        const float factor = ds_factor<T>(p);
+        Ring r;
+        uint32_t s_phase = 0, dp_phase = 0, done_phase = 0;
+        bool ok = true;
+        for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x) {
+            const Block b = p.blocks[it / p.kv_heads];
+            const int kv_head = static_cast<int>(it % p.kv_heads);
+            const int n = (b.len + kTile - 1) / kTile;
+            for (int g = 0; ok && g < p.group; ++g) {
+                for (int i = b.index; ok && i < n; ++i) {
+                    ok = mbar_wait(full + 8 * r.stage, r.phase, abort_flag, p.status, 517);
+                    if (!ok) break;
+                    const float4* lse = reinterpret_cast<const float4*>(gen + kStatsAt + r.stage * B::kStats + half * 256);
+                    const float4* delta = lse + kTile / 4;
+                    ok = mbar_wait(s_full, s_phase, abort_flag, p.status, 518);
+                    if (!ok) break;
+                    s_phase ^= 1u;
+                    tc_fence_after();
+                    const int last = b.len - i * kTile - half * 64;        // columns from here on are no queries
+                    const int from = i == b.index ? row - half * 64 : 0;   // columns before are not causal
+                    const bool edge = last < 64 || i == b.index;
+                    float pr[64];
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t s[32];
+                        tmem_ld32(s_addr + c * 32, s);
+                        tmem_ld_wait();
+                        tmem_tie32(s);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const float4 f = lse[c * 8 + e];
+                            pr[c * 32 + e * 4] = ex2(fmaf(__uint_as_float(s[e * 4]), p.scale_log2, -f.x));
+                            pr[c * 32 + e * 4 + 1] = ex2(fmaf(__uint_as_float(s[e * 4 + 1]), p.scale_log2, -f.y));
+                            pr[c * 32 + e * 4 + 2] = ex2(fmaf(__uint_as_float(s[e * 4 + 2]), p.scale_log2, -f.z));
+                            pr[c * 32 + e * 4 + 3] = ex2(fmaf(__uint_as_float(s[e * 4 + 3]), p.scale_log2, -f.w));
+                        }
+                    }
+                    if (edge) {
+#pragma unroll
+                        for (int c = 0; c < 64; ++c)
+                            if (c < from || c >= last) pr[c] = 0.f;
+                    }
+                    uint32_t packed[32];
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) packed[c] = pack2<T>(pr[2 * c], pr[2 * c + 1]);
+                    tmem_st32(s_addr, packed);
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_ready);
+
+                    ok = mbar_wait(dp_full, dp_phase, abort_flag, p.status, 519);
+                    if (!ok) break;
+                    dp_phase ^= 1u;
+                    tc_fence_after();
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t d[32];
+                        tmem_ld32(dp_addr + c * 32, d);
+                        tmem_ld_wait();
+                        tmem_tie32(d);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const float4 f = delta[c * 8 + e];
+                            const float sub[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                const int at = c * 32 + e * 4 + q;
+                                pr[at] *= (__uint_as_float(d[e * 4 + q]) - sub[q]) * factor;
+                            }
+                        }
+                    }
+                    if (edge) {
+#pragma unroll
+                        for (int c = 0; c < 64; ++c)
+                            if (c < from || c >= last) pr[c] = 0.f;  // delta of such a column is no number to rely on
+                    }
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) packed[c] = pack2<T>(pr[2 * c], pr[2 * c + 1]);
+                    tmem_st32(dp_addr, packed);
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(ds_ready);
+                        mbar_arrive(empty + 8 * r.stage);
+                    }
+                    r.next(B::kStages);
+                }
+            }
+            if (!ok) break;
+            ok = mbar_wait(done, done_phase, abort_flag, p.status, 520);
+            if (!ok) break;
+            done_phase ^= 1u;
+            tc_fence_after();
+            const int key = b.index * kTile + row;
+            const int64_t at = (static_cast<int64_t>(b.start + key) * p.kv_heads + kv_head) * p.dim;
+            if (half == 0) store_row<T, kD>(tm_dv + lanes, static_cast<T*>(p.dv) + at, p.dim, 1.f, key < b.len);
+            else store_row<T, kD>(tm_dk + lanes, static_cast<T*>(p.dk) + at, p.dim, p.scale / factor, key < b.len);
+            tc_fence_before();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, kTmemCols);
+    }
+}
+
+// Work item: 128 query rows of one head over their key tiles. Tensor memory: s at 0 and 128 (two buffers),
+// dp (then ds) at 256, dq at 384. The compute groups take 64 key columns each.
+template <typename T, int kD>
+__global__ void __launch_bounds__(kThreads, 1)
+dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, const Params p) {
+    using B = Backward<kD>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t q_tile = base, do_tile = base + B::kTileBytes, ring = base + 2 * B::kTileBytes;
+    const uint32_t bars = base + B::kBars;
+    const uint32_t full = bars, empty = bars + 32, q_full = bars + 64, q_empty = bars + 72, s_full = bars + 80, dp_full = bars + 96,
+                   ds_ready = bars + 104, done = bars + 112;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + B::kBars + 128);
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + B::kBars + 132);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < B::kStages; ++i) {
+            mbar_init(full + 8 * i, 1);
+            mbar_init(empty + 8 * i, 1);
+        }
+        mbar_init(q_full, 1);
+        mbar_init(q_empty, 1);
+        mbar_init(s_full, 1);
+        mbar_init(s_full + 8, 1);
+        mbar_init(dp_full, 1);
+        mbar_init(ds_ready, 8);
+        mbar_init(done, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+        prefetch_tmap(&map_q);
+        prefetch_tmap(&map_k);
+        prefetch_tmap(&map_v);
+        prefetch_tmap(&map_do);
+    }
+    if (warp == 1) {
+        tmem_alloc(bars + 132, kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t tm_dp = tmem + 2 * kTile, tm_dq = tmem + 3 * kTile;
+    const int64_t items = static_cast<int64_t>(*p.num_blocks) * p.heads;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            Ring r;
+            uint32_t q_phase = 1u;
+            bool ok = true;
+            for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x) {
+                const Block b = p.blocks[it / p.heads];
+                const int head = static_cast<int>(it % p.heads), kv_head = head / p.group;
+                ok = mbar_wait(q_empty, q_phase, abort_flag, p.status, 521);
+                if (!ok) break;
+                q_phase ^= 1u;
+                mbar_expect_tx(q_full, 2 * B::kTileBytes);
+                load_tile<kD>(q_tile, &map_q, q_full, head, b.start + b.index * kTile);
+                load_tile<kD>(do_tile, &map_do, q_full, head, b.start + b.index * kTile);
+                for (int j = 0; ok && j <= b.index; ++j) {
+                    ok = mbar_wait(empty + 8 * r.stage, r.phase ^ 1u, abort_flag, p.status, 522);
+                    if (!ok) break;
+                    const uint32_t bar = full + 8 * r.stage, dst = ring + r.stage * B::kStageBytes;
+                    mbar_expect_tx(bar, B::kStageBytes);
+                    load_tile<kD>(dst, &map_k, bar, kv_head, b.start + j * kTile);
+                    load_tile<kD>(dst + B::kTileBytes, &map_v, bar, kv_head, b.start + j * kTile);
+                    r.next(B::kStages);
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        const uint32_t idesc_s = make_idesc(kTile, kTile, false, false, p.ab_format);
+        const uint32_t idesc_d = make_idesc(kTile, kD, false, true, p.ab_format);
+        Ring r;
+        uint32_t q_phase = 0, ds_phase = 0, buf = 0;
+        bool ok = true;
+        for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x) {
+            const Block b = p.blocks[it / p.heads];
+            ok = mbar_wait(q_full, q_phase, abort_flag, p.status, 523);
+            if (!ok) break;
+            q_phase ^= 1u;
+            for (int j = -1; ok && j <= b.index; ++j) {
+                // s of the next step; then dq += ds k and dp of the next step
+                const bool more = j < b.index;
+                const uint32_t cur = ring + r.stage * B::kStageBytes;
+                const uint32_t cur_empty = empty + 8 * r.stage;
+                Ring ahead = r;
+                if (j >= 0) ahead.next(B::kStages);
+                const uint32_t nxt = ring + ahead.stage * B::kStageBytes;
+                if (more) {
+                    ok = mbar_wait(full + 8 * ahead.stage, ahead.phase, abort_flag, p.status, 524);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const int valid = b.len - (j + 1) * kTile;
+                    if (valid < kTile) {  // key rows of other sequences
+                        zero_tile_rows<kD>(nxt, valid, lane);
+                        fence_proxy_async();
+                        __syncwarp();
+                    }
+                    if (lane == 0) {
+                        // the step before last has read this buffer (its ds was waited for)
+                        mma_scores<kD>(tmem + buf * kTile, q_tile, nxt, idesc_s);
+                        umma_commit_cta1(s_full + 8 * buf);
+                    }
+                    __syncwarp();
+                    buf ^= 1u;
+                }
+                if (j >= 0) {
+                    ok = mbar_wait(ds_ready, ds_phase, abort_flag, p.status, 525);
+                    if (!ok) break;
+                    ds_phase ^= 1u;
+                    tc_fence_after();
+                }
+                if (lane == 0) {
+                    if (j >= 0) {
+                        mma_rows(tm_dq, tm_dp, 64, cur, idesc_d, j > 0);
+                        umma_commit_cta1(cur_empty);
+                    }
+                    if (more) {
+                        mma_scores<kD>(tm_dp, do_tile, nxt + B::kTileBytes, idesc_s);
+                        umma_commit_cta1(dp_full);
+                    } else {
+                        umma_commit_cta1(done);
+                        umma_commit_cta1(q_empty);
+                    }
+                }
+                __syncwarp();
+                r = ahead;
+            }
+        }
+    } else if (warp >= 4) {
+        const int half = (warp >> 2) - 1;          // key columns 64 half .. 64 half + 63
+        const int row = (warp & 3) * 32 + lane;    // query row
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t dp_addr = tm_dp + lanes + half * 64;
+        const float factor = ds_factor<T>(p);
+        uint32_t s_phase[2] = {0u, 0u}, dp_phase = 0, done_phase = 0, buf = 0;
+        bool ok = true;
+        for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x) {
+            const Block b = p.blocks[it / p.heads];
+            const int head = static_cast<int>(it % p.heads);
+            const int query = b.index * kTile + row;
+            const bool valid = query < b.len;
+            const int64_t stat = head * p.pad_rows + b.pad + query;
+            const float neg_lse = valid ? -p.lse[stat] : 0.f;
+            const float delta = valid ? p.delta[stat] : 0.f;
+            for (int j = 0; ok && j <= b.index; ++j) {
+                ok = mbar_wait(s_full + 8 * buf, s_phase[buf], abort_flag, p.status, 526);
+                if (!ok) break;
+                s_phase[buf] ^= 1u;
+                tc_fence_after();
+                const uint32_t s_addr = tmem + lanes + buf * kTile + half * 64;
+                buf ^= 1u;
+                float pr[64];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t s[32];
+                    tmem_ld32(s_addr + c * 32, s);
+                    tmem_ld_wait();
+                    tmem_tie32(s);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) pr[c * 32 + i] = ex2(fmaf(__uint_as_float(s[i]), p.scale_log2, neg_lse));
+                }
+                ok = mbar_wait(dp_full, dp_phase, abort_flag, p.status, 527);
+                if (!ok) break;
+                dp_phase ^= 1u;
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t d[32];
+                    tmem_ld32(dp_addr + c * 32, d);
+                    tmem_ld_wait();
+                    tmem_tie32(d);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) pr[c * 32 + i] *= (__uint_as_float(d[i]) - delta) * factor;
+                }
+                if (j == b.index) {
+#pragma unroll
+                    for (int c = 0; c < 64; ++c)
+                        if (half * 64 + c > row) pr[c] = 0.f;
+                }
+                uint32_t packed[32];
+#pragma unroll
+                for (int c = 0; c < 32; ++c) packed[c] = pack2<T>(pr[2 * c], pr[2 * c + 1]);
+                tmem_st32(dp_addr, packed);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(ds_ready);
+            }
+            if (!ok) break;
+            ok = mbar_wait(done, done_phase, abort_flag, p.status, 528);
+            if (!ok) break;
+            done_phase ^= 1u;
+            tc_fence_after();
+            if (half == 0) {
+                T* dst = static_cast<T*>(p.dq) + (static_cast<int64_t>(b.start + query) * p.heads + head) * p.dim;
+                store_row<T, kD>(tm_dq + lanes, dst, p.dim, p.scale / factor, valid);
+            }
+            tc_fence_before();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, kTmemCols);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------------------------
+
+// Shared-memory attribute of a kernel, set once per device.
+template <auto kKernel>
+static bool prepare_kernel(uint32_t smem) {
+    constexpr int kMaxDevices = 64;
+    static bool set[kMaxDevices];
+    static std::mutex mu;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return false;
+    std::lock_guard<std::mutex> lock(mu);
+    if (!set[dev]) {
+        if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) {
+            cudaGetLastError();
+            return false;
+        }
+        set[dev] = true;
+    }
+    return true;
+}
+
+// [tokens, heads, dim] with token and head strides in elements; boxes of 128 tokens x 64 columns of a head.
+static bool stream_map(CUtensorMap* map, int dtype, const void* base, int64_t total, int heads, int dim, int64_t token_stride,
+                       int64_t head_stride) {
+    const uint64_t dims[3] = {static_cast<uint64_t>(dim), static_cast<uint64_t>(heads), static_cast<uint64_t>(total)};
+    const uint64_t strides[2] = {static_cast<uint64_t>(head_stride) * 2, static_cast<uint64_t>(token_stride) * 2};
+    const uint32_t box[3] = {64, 1, static_cast<uint32_t>(kTile)};
+    return make_tmap(map, dtype, base, 3, dims, strides, box);
+}
+
+static int64_t list_capacity(int64_t total, int64_t batch, int block_rows) { return total / block_rows + batch; }
+
+struct Workspace {  // counts and maxima, then up to two lists
+    int32_t* counts;
+    uint32_t* absmax;
+    Block* list0;
+    Block* list1;
+};
+static Workspace split_workspace(void* base, int64_t total, int64_t batch) {
+    Workspace w;
+    w.counts = static_cast<int32_t*>(base);
+    w.absmax = reinterpret_cast<uint32_t*>(w.counts + 2);
+    w.list0 = reinterpret_cast<Block*>(w.counts + 4);
+    w.list1 = w.list0 + list_capacity(total, batch, kTile);
+    return w;
+}
+
+static int launch_plan(const void* cu, int cu_is_int64, int64_t batch, int64_t total, int block_rows, const Workspace& w, int lists,
+                       ZeroRows z0, ZeroRows z1, ZeroRows z2, cudaStream_t stream) {
+    constexpr int kZeroBlocks = 32;
+    const int64_t capacity = list_capacity(total, batch, block_rows);
+    uint32_t* absmax = lists == 2 ? w.absmax : nullptr;
+    if (cu_is_int64)
+        plan_kernel<int64_t><<<lists + kZeroBlocks, kPlanThreads, 0, stream>>>(
+            static_cast<const int64_t*>(cu), batch, total, block_rows, capacity, w.list0, w.counts, w.list1, w.counts + 1, absmax, z0, z1, z2, lists);
+    else
+        plan_kernel<int32_t><<<lists + kZeroBlocks, kPlanThreads, 0, stream>>>(
+            static_cast<const int32_t*>(cu), batch, total, block_rows, capacity, w.list0, w.counts, w.list1, w.counts + 1, absmax, z0, z1, z2, lists);
+    return launch_status();
+}
+
+struct Call {
+    const void *q, *k, *v;
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+    int dtype;
+    const void* cu;
+    int cu_is_int64;
+    int64_t batch, total;
+    int heads, kv_heads, dim;
+    float scale;
+    void* workspace;
+    int32_t* status;
+    cudaStream_t stream;
+};
+
+static int check_call(const Call& c) {
+    if (c.dtype != kDtypeBF16 && c.dtype != kDtypeF16) return XMA_ERR_UNSUPPORTED;
+    if (c.batch < 0 || c.total < 0 || c.heads <= 0 || c.kv_heads <= 0 || c.dim <= 0) return XMA_ERR_BAD_ARG;
+    if (c.dim % 8 != 0 || c.dim > 128 || c.heads % c.kv_heads != 0 || c.heads > kMaxHeads) return XMA_ERR_UNSUPPORTED;
+    if (c.total > (int64_t(1) << 30) || c.batch > (int64_t(1) << 20)) return XMA_ERR_UNSUPPORTED;
+    if (!(c.scale > 0.f) || !(c.scale <= 3.4e38f)) return XMA_ERR_BAD_ARG;
+    if (c.total == 0) return XMA_OK;
+    if (!c.q || !c.k || !c.v || !c.cu || !c.workspace) return XMA_ERR_BAD_ARG;
+    if (!aligned16(c.q) || !aligned16(c.k) || !aligned16(c.v) || !aligned16(c.workspace)) return XMA_ERR_BAD_ARG;
+    const int64_t strides[6] = {c.q_token, c.q_head, c.k_token, c.k_head, c.v_token, c.v_head};
+    for (int i = 0; i < 6; ++i)
+        if (strides[i] <= 0 || strides[i] % 8 != 0 || strides[i] >= (int64_t(1) << 39)) return XMA_ERR_BAD_ARG;
+    return XMA_OK;
+}
+
+static Params common_params(const Call& c) {
+    Params p{};
+    p.heads = c.heads, p.kv_heads = c.kv_heads, p.group = c.heads / c.kv_heads, p.dim = c.dim;
+    p.pad_rows = (c.total / kTile + c.batch + 1) * kTile;
+    p.scale = c.scale;
+    p.scale_log2 = c.scale * 1.4426950408889634f;  // log2(e): exp(scale s) = 2^(scale_log2 s)
+    p.status = c.status;
+    p.ab_format = c.dtype == kDtypeBF16 ? 1 : 0;
+    return p;
+}
+
+static unsigned grid_for(int64_t items) {
+    const int64_t sms = sm_count();
+    return static_cast<unsigned>(items < sms ? (items < 1 ? 1 : items) : sms);
+}
+
+template <typename T, int kD>
+static int run_forward(const Call& c, void* out, float* lse) {
+    CUtensorMap mq, mk, mv;
+    if (!stream_map(&mq, c.dtype, c.q, c.total, c.heads, c.dim, c.q_token, c.q_head) ||
+        !stream_map(&mk, c.dtype, c.k, c.total, c.kv_heads, c.dim, c.k_token, c.k_head) ||
+        !stream_map(&mv, c.dtype, c.v, c.total, c.kv_heads, c.dim, c.v_token, c.v_head))
+        return XMA_ERR_DRIVER;
+    if (!prepare_kernel<forward_kernel<T, kD>>(Forward<kD>::kSmem)) return XMA_ERR_LAUNCH;
+    const Workspace w = split_workspace(c.workspace, c.total, c.batch);
+    const ZeroRows zo{out, static_cast<int64_t>(c.heads) * c.dim * 2}, none{nullptr, 0};
+    const int status = launch_plan(c.cu, c.cu_is_int64, c.batch, c.total, 2 * kTile, w, 1, zo, none, none, c.stream);
+    if (status != XMA_OK) return status;
+    Params p = common_params(c);
+    p.blocks = w.list0, p.num_blocks = w.counts, p.out = out, p.lse = lse;
+    const unsigned grid = grid_for(list_capacity(c.total, c.batch, 2 * kTile) * c.heads);
+    forward_kernel<T, kD><<<grid, kThreads, Forward<kD>::kSmem, c.stream>>>(mq, mk, mv, p);
+    return launch_status();
+}
+
+template <typename T, int kD>
+static int run_backward(const Call& c, const void* out, const void* d_out, const float* lse, float* delta, void* dq, void* dk, void* dv) {
+    CUtensorMap mq, mk, mv, mdo;
+    const int64_t o_token = static_cast<int64_t>(c.heads) * c.dim;
+    if (!stream_map(&mq, c.dtype, c.q, c.total, c.heads, c.dim, c.q_token, c.q_head) ||
+        !stream_map(&mk, c.dtype, c.k, c.total, c.kv_heads, c.dim, c.k_token, c.k_head) ||
+        !stream_map(&mv, c.dtype, c.v, c.total, c.kv_heads, c.dim, c.v_token, c.v_head) ||
+        !stream_map(&mdo, c.dtype, d_out, c.total, c.heads, c.dim, o_token, c.dim))
+        return XMA_ERR_DRIVER;
+    if (!prepare_kernel<dkdv_kernel<T, kD>>(Backward<kD>::kSmem) || !prepare_kernel<dq_kernel<T, kD>>(Backward<kD>::kSmem))
+        return XMA_ERR_LAUNCH;
+    const Workspace w = split_workspace(c.workspace, c.total, c.batch);
+    const int64_t row_q = o_token * 2, row_kv = static_cast<int64_t>(c.kv_heads) * c.dim * 2;
+    int status = launch_plan(c.cu, c.cu_is_int64, c.batch, c.total, kTile, w, 2, ZeroRows{dq, row_q}, ZeroRows{dk, row_kv},
+                             ZeroRows{dv, row_kv}, c.stream);
+    if (status != XMA_OK || c.batch == 0) return status;
+    Params p = common_params(c);
+    p.lse = const_cast<float*>(lse), p.delta = delta, p.dq = dq, p.dk = dk, p.dv = dv, p.absmax = w.absmax;
+    const int64_t most = static_cast<int64_t>(sm_count()) * 8;
+    const unsigned rows = static_cast<unsigned>(c.total < most ? c.total : most);
+    if (c.cu_is_int64)
+        delta_kernel<T, int64_t><<<rows, 256, 0, c.stream>>>(
+            static_cast<const T*>(out), static_cast<const T*>(d_out), static_cast<const T*>(c.v), c.v_token, c.v_head,
+            static_cast<const int64_t*>(c.cu), c.batch, c.total, delta, w.absmax, p);
+    else
+        delta_kernel<T, int32_t><<<rows, 256, 0, c.stream>>>(
+            static_cast<const T*>(out), static_cast<const T*>(d_out), static_cast<const T*>(c.v), c.v_token, c.v_head,
+            static_cast<const int32_t*>(c.cu), c.batch, c.total, delta, w.absmax, p);
+    status = launch_status();
+    if (status != XMA_OK) return status;
+    const int64_t blocks = list_capacity(c.total, c.batch, kTile);
+    p.blocks = w.list1, p.num_blocks = w.counts + 1;
+    dkdv_kernel<T, kD><<<grid_for(blocks * c.kv_heads), kThreads, Backward<kD>::kSmem, c.stream>>>(mq, mk, mv, mdo, p);
+    status = launch_status();
+    if (status != XMA_OK) return status;
+    p.blocks = w.list0, p.num_blocks = w.counts;
+    dq_kernel<T, kD><<<grid_for(blocks * c.heads), kThreads, Backward<kD>::kSmem, c.stream>>>(mq, mk, mv, mdo, p);
+    return launch_status();
+}
+
+}  // namespace attn
+}  // namespace xma
+
+extern "C" {
+
+int64_t xma_attention_workspace_bytes(int64_t total, int64_t batch) {
+    if (total < 0 || batch < 0) return 0;
+    return 16 + 2 * static_cast<int64_t>(sizeof(xma::attn::Block)) * xma::attn::list_capacity(total, batch, xma::attn::kTile);
+}
+
+int64_t xma_attention_stat_rows(int64_t total, int64_t batch) {
+    return total < 0 || batch < 0 ? 0 : (total / xma::attn::kTile + batch + 1) * xma::attn::kTile;
+}
+
+int xma_attention_forward(const void* q, const void* k, const void* v, int64_t q_token, int64_t q_head, int64_t k_token,
+                          int64_t k_head, int64_t v_token, int64_t v_head, int32_t dtype, const void* cu_seqlens,
+                          int32_t cu_is_int64, int64_t batch, int64_t total, int32_t heads, int32_t kv_heads, int32_t dim,
+                          float scale, void* out, float* lse, void* workspace, int32_t* status, void* stream) {
+    using namespace xma;
+    using namespace xma::attn;
+    const Call c{q, k, v, q_token, q_head, k_token, k_head, v_token, v_head, dtype, cu_seqlens, cu_is_int64, batch, total,
+                 heads, kv_heads, dim, scale, workspace, status, static_cast<cudaStream_t>(stream)};
+    const int rc = check_call(c);
+    if (rc != XMA_OK || total == 0) return rc;
+    if (!out || !aligned16(out)) return XMA_ERR_BAD_ARG;
+    if (dtype == kDtypeBF16) return dim <= 64 ? run_forward<__nv_bfloat16, 64>(c, out, lse) : run_forward<__nv_bfloat16, 128>(c, out, lse);
+    return dim <= 64 ? run_forward<__half, 64>(c, out, lse) : run_forward<__half, 128>(c, out, lse);
+}
+
+int xma_attention_backward(const void* q, const void* k, const void* v, int64_t q_token, int64_t q_head, int64_t k_token,
+                           int64_t k_head, int64_t v_token, int64_t v_head, int32_t dtype, const void* cu_seqlens,
+                           int32_t cu_is_int64, int64_t batch, int64_t total, int32_t heads, int32_t kv_heads, int32_t dim,
+                           float scale, const void* out, const void* d_out, const float* lse, float* delta, void* dq, void* dk,
+                           void* dv, void* workspace, int32_t* status, void* stream) {
+    using namespace xma;
+    using namespace xma::attn;
+    const Call c{q, k, v, q_token, q_head, k_token, k_head, v_token, v_head, dtype, cu_seqlens, cu_is_int64, batch, total,
+                 heads, kv_heads, dim, scale, workspace, status, static_cast<cudaStream_t>(stream)};
+    const int rc = check_call(c);
+    if (rc != XMA_OK || total == 0) return rc;
+    const void* need[] = {out, d_out, lse, delta, dq, dk, dv};
+    for (int i = 0; i < 7; ++i)
+        if (need[i] == nullptr || !aligned16(need[i])) return XMA_ERR_BAD_ARG;
+    if (dtype == kDtypeBF16)
+        return dim <= 64 ? run_backward<__nv_bfloat16, 64>(c, out, d_out, lse, delta, dq, dk, dv)
+                         : run_backward<__nv_bfloat16, 128>(c, out, d_out, lse, delta, dq, dk, dv);
+    return dim <= 64 ? run_backward<__half, 64>(c, out, d_out, lse, delta, dq, dk, dv)
+                     : run_backward<__half, 128>(c, out, d_out, lse, delta, dq, dk, dv);
+}
+
+}  // extern "C"

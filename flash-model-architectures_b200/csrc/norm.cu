@@ -336,12 +336,6 @@ __device__ __forceinline__ RowScale row_scale(const Params& p, const float (&sum
     return r;
 }
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
-                 : "memory");
-}
-
 // Shared-memory layout of the ring kernel: parameters, reduction scratch and barriers, then the stages.
 struct RingLayout {
     int slots;            // rows a CTA works on at once

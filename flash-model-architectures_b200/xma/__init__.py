@@ -9,8 +9,8 @@ import torch
 
 from ._native import check_status
 from .accelerator import Accelerator, KernelBackend
-from .functional import (continuous_count, fused_residual_add_rmsnorm, pack_sequence, rmsnorm, swiglu, swiglu_packed,
-                         unpack_sequence)
+from .functional import (attention_packed, continuous_count, fused_residual_add_rmsnorm, pack_sequence, rmsnorm, swiglu,
+                         swiglu_packed, unpack_sequence)
 from .layers import Experts, MoE
 
 

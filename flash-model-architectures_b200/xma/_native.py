@@ -62,6 +62,14 @@ _SIGNATURES = {
         c_int32, [c_void_p] * 5 + [c_int32] * 4 + [c_int64, c_int64, c_float, c_float] + [c_void_p] * 5),
     "xma_norm_backward": (
         c_int32, [c_void_p] * 7 + [c_int32] * 4 + [c_int64, c_int64, c_float] + [c_void_p] * 10),
+    "xma_attention_workspace_bytes": (c_int64, [c_int64, c_int64]),
+    "xma_attention_stat_rows": (c_int64, [c_int64, c_int64]),
+    "xma_attention_forward": (
+        c_int32, [c_void_p] * 3 + [c_int64] * 6 + [c_int32, c_void_p, c_int32, c_int64, c_int64] + [c_int32] * 3
+        + [c_float] + [c_void_p] * 5),
+    "xma_attention_backward": (
+        c_int32, [c_void_p] * 3 + [c_int64] * 6 + [c_int32, c_void_p, c_int32, c_int64, c_int64] + [c_int32] * 3
+        + [c_float] + [c_void_p] * 10),
     "xma_ipc_get_handle": (c_int32, [c_void_p, ctypes.c_char_p]),
     "xma_ipc_open_handle": (c_int32, [ctypes.c_char_p, ctypes.POINTER(c_void_p)]),
     "xma_ipc_close_handle": (c_int32, [c_void_p]),
@@ -160,6 +168,17 @@ def norm_workspace_floats(rows: int, hidden: int) -> int:
     """float32 elements of workspace xma_norm_backward needs (xma_norm_workspace_floats, kept in Python for
     the same reason as index_workspace_elems)."""
     return 3 * NORM_PARTIALS * hidden + 4 * rows
+
+
+def attention_workspace_bytes(total: int, batch: int) -> int:
+    """Bytes of workspace the attention entry points need (xma_attention_workspace_bytes, kept in Python for
+    the same reason as index_workspace_elems)."""
+    return 16 + 32 * (total // 128 + batch)
+
+
+def attention_stat_rows(total: int, batch: int) -> int:
+    """Row statistics per head: every sequence starts on a multiple of 128 (xma_attention_stat_rows)."""
+    return (total // 128 + batch + 1) * 128
 
 
 _status_words: dict[int, torch.Tensor] = {}

@@ -21,6 +21,10 @@ def _kernels_per_call(name: str, args: tuple) -> int:
     launch up to the size the library reports (xma_moe_index_small_limit, at most 256 experts) and
     five launches beyond (csrc/routing.cu:launch_index_build)."""
     global _index_small_limit
+    if name in ("xma_attention_forward", "xma_norm_backward"):  # a plan and the kernel; the kernel and the sums of its partials
+        return 2
+    if name == "xma_attention_backward":  # plan, row sums, dk and dv, dq
+        return 4
     if name == "xma_moe_index_build":
         if _index_small_limit is None:
             _index_small_limit = int(N.lib().xma_moe_index_small_limit())
@@ -33,10 +37,14 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _entry_points: dict = {}
 
 
-def _launch(name: str, anchor: torch.Tensor, *args) -> None:
-    """Calls one C-ABI entry point on `anchor`'s device and current stream; raises on a non-zero status."""
+def _require_cuda(anchor: torch.Tensor) -> None:
     if not anchor.is_cuda:
         raise RuntimeError("libxma_b200 runs on CUDA tensors only (sm_100a); there is no CPU path")
+
+
+def _launch(name: str, anchor: torch.Tensor, *args) -> None:
+    """Calls one C-ABI entry point on `anchor`'s device and current stream; raises on a non-zero status."""
+    _require_cuda(anchor)
     fn = _entry_points.get(name)
     if fn is None:
         fn = _entry_points[name] = getattr(N.lib(), name)
@@ -342,4 +350,48 @@ def norm_backward_cuda(
         N.dtype_code(dtype), N.dtype_code(stream.dtype), _f32_params(weight, post_weight, gate), rows, hidden,
         multiplier, N.ptr(rstd), N.ptr(rstd_post), N.ptr(dx), N.ptr(d_residual), N.ptr(d_gate), N.ptr(d_weight),
         N.ptr(d_post_weight), N.ptr(workspace), N.ptr(N.status_word(stream.device)),
+    )
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """`t`, or a contiguous copy when its first element is not on a 16-byte boundary."""
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _attention_args(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, softmax_scale: float) -> tuple:
+    _require_cuda(q)
+    total, heads, dim = q.shape
+    kv_heads = k.size(1)
+    # a single head has no stride of its own: any valid one will do
+    strides = [s for t in (q, k, v) for s in (t.stride(0) if total > 1 else t.size(1) * dim, t.stride(1) if t.size(1) > 1 else dim)]
+    return (N.ptr(q), N.ptr(k), N.ptr(v), *strides, N.dtype_code(q.dtype), N.ptr(cu_seqlens), int(cu_seqlens.dtype == torch.int64),
+            cu_seqlens.numel() - 1, total, heads, kv_heads, dim, softmax_scale)
+
+
+@xma_op(mutates_args={"out", "lse", "workspace"})
+def attention_packed_forward_cuda(
+    q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, softmax_scale: float, out: torch.Tensor,
+    lse: torch.Tensor | None, workspace: torch.Tensor
+) -> None:
+    """Causal attention over a packed stream; see xma_attention_forward in include/xma_b200.h."""
+    assert out.is_contiguous() and cu_seqlens.is_contiguous()
+    q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    _launch("xma_attention_forward", q,
+        *_attention_args(q, k, v, cu_seqlens, softmax_scale), N.ptr(out), N.ptr(lse), N.ptr(workspace),
+        N.ptr(N.status_word(q.device)),
+    )
+
+
+@xma_op(mutates_args={"delta", "dq", "dk", "dv", "workspace"})
+def attention_packed_backward_cuda(
+    q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, softmax_scale: float, out: torch.Tensor,
+    d_out: torch.Tensor, lse: torch.Tensor, delta: torch.Tensor, dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor,
+    workspace: torch.Tensor
+) -> None:
+    """Gradients of attention_packed_forward_cuda; see xma_attention_backward in include/xma_b200.h."""
+    assert all(t.is_contiguous() for t in (out, d_out, lse, delta, dq, dk, dv, cu_seqlens))
+    q, k, v, d_out = _aligned(q), _aligned(k), _aligned(v), _aligned(d_out)
+    _launch("xma_attention_backward", q,
+        *_attention_args(q, k, v, cu_seqlens, softmax_scale), N.ptr(out), N.ptr(d_out), N.ptr(lse), N.ptr(delta), N.ptr(dq),
+        N.ptr(dk), N.ptr(dv), N.ptr(workspace), N.ptr(N.status_word(q.device)),
     )

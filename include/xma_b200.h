@@ -406,6 +406,33 @@ int xma_norm_backward(const void* dy, const void* d_stream, const void* stream_s
                       const float* rstd_post, void* dx, void* d_residual, void* d_gate, void* d_weight, void* d_post_weight,
                       float* workspace, int32_t* status, void* stream);
 
+/*
+ * Causal attention over a packed token stream: sequence b owns tokens cu_seqlens[b] .. cu_seqlens[b+1]-1
+ * (int32 or int64 [batch + 1], ascending), each token attends to the tokens of its sequence up to itself.
+ *   q [total, heads, dim], k, v [total, kv_heads, dim] of `dtype` (bf16 or fp16); *_token and *_head are their
+ *   strides in elements (multiples of 8, bases 16-byte aligned); out, d_out, dq [total, heads, dim] and dk, dv
+ *   [total, kv_heads, dim] are contiguous. heads is a multiple of kv_heads (query head h reads kv head
+ *   h / (heads / kv_heads)), dim a multiple of 8 up to 128, scale positive.
+ *   lse   float32 [heads, xma_attention_stat_rows(total, batch)], 16-byte aligned: the rows' log-sum-exp (base
+ *         2), written by the forward pass for the backward pass; NULL when there is none
+ *   delta float32, the same size, scratch of the backward pass
+ *   workspace  xma_attention_workspace_bytes(total, batch) bytes, 16-byte aligned, contents irrelevant
+ * Tokens that no sequence owns (before cu_seqlens[0], from cu_seqlens[batch] on) get zeros in every output and
+ * are read by nothing else. Entries of cu_seqlens outside [0, total] or out of order give meaningless values
+ * but touch no memory outside the operands. A code 501-528 goes to *status when a device-side wait runs out.
+ */
+int64_t xma_attention_workspace_bytes(int64_t total, int64_t batch);
+int64_t xma_attention_stat_rows(int64_t total, int64_t batch);
+int xma_attention_forward(const void* q, const void* k, const void* v, int64_t q_token, int64_t q_head, int64_t k_token,
+                          int64_t k_head, int64_t v_token, int64_t v_head, int32_t dtype, const void* cu_seqlens,
+                          int32_t cu_is_int64, int64_t batch, int64_t total, int32_t heads, int32_t kv_heads, int32_t dim,
+                          float scale, void* out, float* lse, void* workspace, int32_t* status, void* stream);
+int xma_attention_backward(const void* q, const void* k, const void* v, int64_t q_token, int64_t q_head, int64_t k_token,
+                           int64_t k_head, int64_t v_token, int64_t v_head, int32_t dtype, const void* cu_seqlens,
+                           int32_t cu_is_int64, int64_t batch, int64_t total, int32_t heads, int32_t kv_heads, int32_t dim,
+                           float scale, const void* out, const void* d_out, const float* lse, float* delta, void* dq, void* dk,
+                           void* dv, void* workspace, int32_t* status, void* stream);
+
 /* Maps another process's device allocation into this process for the CURRENT device, with peer access
  * enabled: handle64 is that allocation's 64-byte cudaIpcMemHandle_t. Host-side call, no stream. */
 int xma_ipc_open_handle(const void* handle64, void** device_ptr);

@@ -1,0 +1,352 @@
+"""attention_packed on the GPU against its formula in 64 bits.
+
+Bounds. With u the half step of the inputs' type: p is rounded once (u relative) where it meets v, so
+|o - exact| <= u |o| + u sum_j p_ij |v_j| + e sum_j p_ij |v_j|, where e collects what is done in float32: scores are
+sums of D products (D 2^-24 sum |q||k| scale, an absolute error of the exponent, the same in nominator and sum), ex2
+(2 steps) and the sums over keys. The backward pass adds, per ds, the rounding of ds and that of delta (taken from the
+rounded o: u sum_d |o||do|)."""
+
+import math
+
+import pytest
+import torch
+
+import xma
+from block_reference import F32, assert_within, half_step
+from gpu_helpers import assert_status_clean
+
+pytestmark = pytest.mark.gpu
+
+
+def offsets(lengths, first=0, dtype=torch.int32):
+    return torch.tensor([first] + lengths, dtype=torch.int64).cumsum(0).to(dtype).cuda()
+
+
+def make(lengths, heads, kv_heads, dim, dtype, behind=0, before=0, seed=0, q_scale=1.5):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    total = before + sum(lengths) + behind
+    n = lambda h, s: (torch.randn(total, h, dim, device="cuda", generator=g) * s).to(dtype)
+    return n(heads, q_scale), n(kv_heads, 1.0), n(kv_heads, 1.0), n(heads, 0.05)
+
+
+def reference(q, k, v, do, lengths, before=0, scale=None):
+    """Per output (value, bound) in float64; rows of no sequence are zeros with a bound of zero."""
+    u = half_step(q.dtype)
+    T, H, D = q.shape
+    G = H // k.size(1)
+    scale = scale or 1 / math.sqrt(D)
+    out = {n: (torch.zeros(t.shape, dtype=torch.float64, device=q.device), torch.zeros(t.shape, dtype=torch.float64, device=q.device))
+           for n, t in (("o", q), ("dq", q), ("dk", k), ("dv", v))}
+    at = before
+    for L in lengths:
+        r = slice(at, at + L)
+        at += L
+        if L == 0:
+            continue
+        for h in range(H):
+            qq, kk, vv, dd = (t.double() for t in (q[r, h], k[r, h // G], v[r, h // G], do[r, h]))
+            mask = torch.ones(L, L, dtype=torch.bool, device=q.device).tril()
+            s = (qq @ kk.t() * scale).masked_fill(~mask, -math.inf)
+            p = torch.softmax(s, -1)
+            o = p @ vv
+            # float32: D products a score, their rounding is an absolute error of the exponent; row sums of L terms
+            es = ((D + 8) * F32 * (qq.abs() @ kk.abs().t()) * scale).masked_fill(~mask, 0)
+            # p's own relative error: exponent, ex2 (2^-22), argument (|s - m| 2^-23, at most 2^-16 for |s| <= 128), sum
+            ep = es + es.max(-1, keepdim=True).values + 2 ** -16 + (L / 8 + 64) * F32
+            bo = u * o.abs() + (p * (ep + u)) @ vv.abs() + 64 * F32 * (p @ vv.abs())
+            out["o"][0][r, h], out["o"][1][r, h] = o, bo
+            delta = (o * dd).sum(-1, keepdim=True)
+            e_delta = (bo * dd.abs()).sum(-1, keepdim=True) + D * F32 * (o.abs() * dd.abs()).sum(-1, keepdim=True)
+            dp = dd @ vv.t()
+            e_dp = D * F32 * (dd.abs() @ vv.abs().t())
+            ds = p * (dp - delta)
+            e_ds = p * (e_dp + e_delta) + ds.abs() * (ep + u + 4 * F32)
+            acc = (L * G + 64) * F32
+            bq = scale * (e_ds @ kk.abs() + acc * (ds.abs() @ kk.abs()))
+            bk = scale * (e_ds.t() @ qq.abs() + acc * (ds.abs().t() @ qq.abs()))
+            bv = (p * (ep + u + acc)).t() @ dd.abs()
+            dq, dk, dv = scale * ds @ kk, scale * ds.t() @ qq, p.t() @ dd
+            out["dq"][0][r, h], out["dq"][1][r, h] = dq, bq
+            for name, val, b in (("dk", dk, bk), ("dv", dv, bv)):
+                out[name][0][r, h // G] += val
+                out[name][1][r, h // G] += b
+    tiny = torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps
+    for n in ("dq", "dk", "dv"):
+        val, b = out[n]
+        out[n] = (val, b + u * (val.abs() + b))
+    # a subnormal result steps evenly; zeros of unowned rows are exact
+    return {n: (val, torch.where(b > 0, b + tiny, b)) for n, (val, b) in out.items()}
+
+
+def run(q, k, v, do, cu, scale=None):
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = xma.attention_packed(*leaves, cu, softmax_scale=scale)
+    return dict(zip(("o", "dq", "dk", "dv"), (o.detach(), *torch.autograd.grad(o, leaves, do))))
+
+
+def check(lengths, heads, kv_heads, dim, dtype, behind=0, before=0, seed=0, q_scale=1.5, scale=None, int64=False):
+    q, k, v, do = make(lengths, heads, kv_heads, dim, dtype, behind, before, seed, q_scale)
+    cu = offsets(lengths, before, torch.int64 if int64 else torch.int32)
+    got = run(q, k, v, do, cu, scale)
+    assert_status_clean(q.device)
+    ref = reference(q, k, v, do, lengths, before, scale)
+    for name, value in got.items():
+        assert value.dtype == dtype and value.is_contiguous()
+        assert_within(name, value, *ref[name])
+    with torch.no_grad():
+        assert torch.equal(xma.attention_packed(q, k, v, cu, softmax_scale=scale), got["o"])
+    return got
+
+
+LENGTHS = [[1], [2], [127], [128], [129], [255, 1, 0, 257], [0, 0, 5], [300, 77, 512, 1, 1, 130], [1025], [64] * 9, [640, 384]]
+
+
+def test_first_one_tile():
+    """The smallest case, forward only."""
+    q, k, v, do = make([128], 1, 1, 64, torch.bfloat16)
+    with torch.no_grad():
+        o = xma.attention_packed(q, k, v, offsets([128]))
+    assert_status_clean(q.device)
+    assert_within("o", o, *reference(q, k, v, do, [128])["o"])
+
+
+@pytest.mark.parametrize("lengths", LENGTHS, ids=str)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_lengths(lengths, dim):
+    check(lengths, 2, 1, dim, torch.bfloat16)
+    check(lengths, 2, 2, dim, torch.float16, seed=1)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (4, 4), (8, 2), (5, 1), (12, 3)])
+def test_heads(heads, kv_heads):
+    check([200, 33], heads, kv_heads, 128, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dim", [8, 16, 24, 40, 56, 72, 80, 96, 104, 112, 120])
+def test_head_dims(dim):
+    check([150, 270], 4, 2, dim, torch.bfloat16)
+    check([150, 270], 2, 2, dim, torch.float16)
+
+
+def test_long():
+    check([2300, 1], 2, 1, 128, torch.bfloat16)
+    check([3001], 1, 1, 64, torch.float16)
+
+
+@pytest.mark.parametrize("q_scale", [0.0, 1e-3, 20.0])
+def test_sharp_and_flat(q_scale):
+    """Rows that look at one key alone (the running maximum keeps growing) and rows that look at all alike."""
+    check([700], 2, 1, 64, torch.bfloat16, q_scale=q_scale)
+
+
+def test_growing_scores():
+    """Scores rise along the keys by far more than 2^8 a tile: the accumulator is rescaled in every tile."""
+    L, D = 900, 64
+    q, k, v, do = make([L], 2, 2, D, torch.bfloat16)
+    ramp = torch.linspace(0, 60, L, device="cuda")[:, None].to(torch.bfloat16)
+    q[..., 0], k[..., 0] = 8.0, ramp
+    got, ref = run(q, k, v, do, offsets([L])), reference(q, k, v, do, [L])
+    for name, value in got.items():
+        assert_within(name, value, *ref[name])
+
+
+def test_softmax_scale_and_int64_offsets():
+    check([100, 60], 2, 1, 64, torch.bfloat16, scale=0.3, int64=True)
+
+
+@pytest.mark.parametrize("before,behind", [(0, 70), (13, 0), (130, 500)])
+def test_rows_of_no_sequence(before, behind):
+    """They get zeros, and NaNs in them (in inputs and upstream gradient) reach no row of a sequence."""
+    lengths = [77, 128, 200]
+    clean = check(lengths, 4, 2, 64, torch.bfloat16, behind, before)
+    q, k, v, do = make(lengths, 4, 2, 64, torch.bfloat16, behind, before)
+    for t in (q, k, v, do):
+        t[:before] = math.nan
+        t[before + sum(lengths):] = math.inf
+    got = run(q, k, v, do, offsets(lengths, before))
+    for name in got:
+        assert torch.equal(got[name], clean[name])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_no_leak_between_sequences(dtype):
+    """A sequence of NaN and infinity changes no bit of its neighbours, outputs and gradients."""
+    lengths = [100, 60, 300, 41]
+    q, k, v, do = make(lengths, 4, 2, 128, dtype)
+    if dtype == torch.float16:  # the factor ds is rounded with comes from the largest values: keep those
+        v[0, 0, 0], do[0, 0, 0] = 60000.0, 60000.0
+    clean = run(q, k, v, do, offsets(lengths))
+    bad = slice(160, 460)
+    for t in (q, k, v, do):
+        t[bad, :, ::2] = math.nan
+        t[bad, :, 1::2] = math.inf
+    got = run(q, k, v, do, offsets(lengths))
+    for name in got:
+        assert torch.equal(got[name][:160], clean[name][:160]) and torch.equal(got[name][460:], clean[name][460:])
+        assert not got[name][bad].isfinite().all()
+
+
+def test_strided_views():
+    """Slices of one projection, heads first, a misaligned slice: the same bits as contiguous copies."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    T, H, K, D = 333, 4, 2, 64
+    cu = offsets([133, 200])
+    qkv = torch.randn(T, H + 2 * K, D, device="cuda", generator=g).to(torch.bfloat16)
+    heads_first = torch.randn(H + 2 * K, T, D, device="cuda", generator=g).to(torch.bfloat16).transpose(0, 1)
+    odd = torch.randn(T, H + 2 * K, D + 3, device="cuda", generator=g).to(torch.bfloat16)[..., 1: D + 1]
+    do = torch.randn(T, H, D, device="cuda", generator=g).to(torch.bfloat16)
+    for t in (qkv, heads_first, odd):
+        views = t[:, :H], t[:, H: H + K], t[:, H + K:]
+        a = run(*views, do, cu)
+        b = run(*(x.contiguous() for x in views), do, cu)
+        c = run(*views, do.transpose(0, 1).contiguous().transpose(0, 1), cu)
+        for name in a:
+            assert torch.equal(a[name], b[name]) and torch.equal(a[name], c[name])
+    flat = torch.randn(T * H * D + 1, device="cuda", generator=g).to(torch.bfloat16)[1:].view(T, H, D)  # 2 bytes off
+    for name, value in run(flat, flat, flat, flat, cu).items():
+        assert torch.equal(value, run(flat.clone(), flat.clone(), flat.clone(), flat.clone(), cu)[name])
+    one = torch.randn(T, 1, D, device="cuda", generator=g).to(torch.bfloat16)
+    shared = one.expand(T, H, D)  # a head shared by expansion: its gradient is the sum over the heads
+    leaf = one.clone().requires_grad_()
+    o = xma.attention_packed(qkv[:, :H], leaf.expand(T, H, D), shared, cu)
+    (d_one,) = torch.autograd.grad(o, leaf, do)
+    d_all = run(qkv[:, :H], shared, shared, do, cu)["dk"]
+    assert torch.equal(d_one, d_all.sum(1, keepdim=True))
+
+
+def test_gradients_in_small_numbers_fp16():
+    """Upstream gradients as small as a mean over many tokens makes them, where fp16 has few steps left."""
+    q, k, v, do = make([500], 2, 1, 64, torch.float16)
+    do = (do * 2.0 ** -6).to(torch.float16)
+    got, ref = run(q, k, v, do, offsets([500])), reference(q, k, v, do, [500])
+    for name, value in got.items():
+        assert_within(name, value, *ref[name])
+
+
+def test_large_values_fp16():
+    """Values near the largest fp16: products overflow fp16, not the result."""
+    q, k, v, do = make([300], 2, 1, 64, torch.float16, q_scale=1.0)
+    v = (v * 8000).clamp(-60000, 60000)
+    do = (do * 0.01).to(torch.float16)
+    got, ref = run(q, k, v, do, offsets([300])), reference(q, k, v, do, [300])
+    for name, value in got.items():
+        want, bound = ref[name]
+        assert_within(name, value, want, bound)
+
+
+def test_gradient_against_differences():
+    """Directional derivatives: o is rounded to bf16 (2^-9 each, random over 64 000 values), a step moves the scores by
+    about h: the difference quotient is off by the roundings' sum over 2h and h^2."""
+    L, H, D = 250, 2, 128
+    q, k, v, do = make([L], H, H, D, torch.bfloat16)
+    got = run(q, k, v, do, offsets([L]))
+
+    def loss(q, k, v):
+        with torch.no_grad():
+            return (xma.attention_packed(q, k, v, offsets([L])).double() * do.double()).sum().item()
+
+    for i, name in enumerate(("dq", "dk", "dv")):
+        direction = torch.sign(got[name]).to(torch.bfloat16)  # along the gradient's signs the slope is its 1-norm
+        h = 2.0 ** -4
+        up, down = [q, k, v], [q, k, v]
+        up[i], down[i] = up[i] + h * direction, down[i] - h * direction
+        step = (up[i].double() - down[i].double())
+        want = (got[name].double() * step).sum().item()
+        assert abs(loss(*up) - loss(*down) - want) <= 0.05 * abs(want), name
+
+
+def test_same_results_every_time_and_on_a_side_stream():
+    lengths = [700, 1, 300, 129]
+    q, k, v, do = make(lengths, 8, 2, 128, torch.bfloat16)
+    cu = offsets(lengths)
+    first = run(q, k, v, do, cu)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = run(q, k, v, do, cu)
+    torch.cuda.current_stream().wait_stream(side)
+    for name in first:
+        assert torch.equal(first[name], again[name])
+
+
+def test_two_calls_at_once():
+    """Two streams, each with its own workspace."""
+    a, b = make([900], 4, 4, 64, torch.bfloat16), make([400, 500], 4, 4, 64, torch.bfloat16, seed=2)
+    cu_a, cu_b = offsets([900]), offsets([400, 500])
+    want_a, want_b = run(*a, cu_a), run(*b, cu_b)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s, args, cu in zip(streams, (a, b), (cu_a, cu_b)):
+        with torch.cuda.stream(s):
+            got.append(run(*args, cu))
+    torch.cuda.synchronize()
+    for g, w in zip(got, (want_a, want_b)):
+        for name in w:
+            assert torch.equal(g[name], w[name])
+
+
+def test_captured_step():
+    """Forward and backward in a CUDA graph, replayed on other values and other sequence lengths."""
+    lengths = [200, 56, 144]
+    q, k, v, do = make(lengths, 4, 2, 64, torch.bfloat16)
+    cu = offsets(lengths)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+
+    def step():
+        o = xma.attention_packed(*leaves, cu)
+        return [o, *torch.autograd.grad(o, leaves, do)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    new = make([1], 4, 2, 64, torch.bfloat16, behind=399, seed=8)
+    with torch.no_grad():
+        for old, n in zip((q, k, v, do), new):
+            old.copy_(n)
+        cu.copy_(offsets([1, 390, 3]))
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(captured, step()):
+        assert torch.equal(a, b)
+    assert (captured[0][394:] == 0).all()
+
+
+def test_compiled():
+    lengths = [100, 28]
+    q, k, v, do = make(lengths, 4, 2, 64, torch.bfloat16)
+    cu = offsets(lengths)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    f = torch.compile(lambda *a: xma.attention_packed(*a), fullgraph=True)
+    o = f(*leaves, cu)
+    want = run(*(t.detach() for t in leaves), do, cu)
+    assert torch.equal(o, want["o"])
+    for a, name in zip(torch.autograd.grad(o, leaves, do), ("dq", "dk", "dv")):
+        assert torch.equal(a, want[name])
+
+
+def test_nothing_to_do():
+    for shape_k, cu in (((0, 2, 64), offsets([])), ((0, 2, 64), offsets([0, 0])), ((5, 2, 64), offsets([])), ((5, 2, 64), offsets([0, 0]))):
+        q = torch.randn(shape_k[0], 4, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+        k = torch.randn(shape_k, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+        o = xma.attention_packed(q, k, k, cu)
+        dq, dk = torch.autograd.grad(o, (q, k), torch.ones_like(o))
+        assert o.shape == q.shape and (o == 0).all() and (dq == 0).all() and (dk == 0).all()
+    torch.cuda.synchronize()
+
+
+def test_offsets_outside_the_stream_touch_nothing():
+    """Not a valid cu_seqlens: the values are meaningless, nothing faults and the neighbours of the operands keep."""
+    T, H, D = 300, 2, 64
+    q, k, v, do = make([T], H, H, D, torch.bfloat16)
+    guard = torch.full((T + 512, H, D), 7.0, device="cuda", dtype=torch.bfloat16)
+    for values in ([0, 10 ** 6], [-50, 100, 300], [200, 100, 300], [0, 300, 0, 300, 0, 300]):
+        run(q, k, v, do, torch.tensor(values, dtype=torch.int32, device="cuda"))
+    torch.cuda.synchronize()
+    assert_status_clean(q.device)
+    assert (guard == 7.0).all()

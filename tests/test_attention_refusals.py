@@ -1,0 +1,65 @@
+"""What attention_packed refuses, on the host."""
+
+import pytest
+import torch
+
+import xma
+
+
+def t(*shape, dtype=torch.bfloat16):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+CU = torch.tensor([0, 4], dtype=torch.int32)
+
+
+@pytest.mark.parametrize("q,k,v,cu,options,match", [
+    (t(4, 64), t(4, 2, 64), t(4, 2, 64), CU, {}, "q should be \\[tokens"),
+    (t(4, 2, 64), t(4, 64), t(4, 64), CU, {}, "k should be \\[tokens"),
+    (t(4, 2, 64, dtype=torch.float32), t(4, 2, 64), t(4, 2, 64), CU, {}, "bfloat16 or float16"),
+    (t(4, 2, 64), t(4, 2, 64, dtype=torch.float16), t(4, 2, 64), CU, {}, "like q"),
+    (t(4, 2, 64), t(4, 2, 64), t(4, 1, 64), CU, {}, "same shape"),
+    (t(4, 2, 64), t(5, 2, 64), t(5, 2, 64), CU, {}, "k and v should be"),
+    (t(4, 2, 64), t(4, 2, 32), t(4, 2, 32), CU, {}, "k and v should be"),
+    (t(4, 2, 60), t(4, 2, 60), t(4, 2, 60), CU, {}, "head_dim"),
+    (t(4, 2, 136), t(4, 2, 136), t(4, 2, 136), CU, {}, "head_dim"),
+    (t(4, 2, 0), t(4, 2, 0), t(4, 2, 0), CU, {}, "head_dim"),
+    (t(4, 3, 64), t(4, 2, 64), t(4, 2, 64), CU, {}, "multiple of kv_heads"),
+    (t(4, 2, 64), t(4, 0, 64), t(4, 0, 64), CU, {}, "multiple of kv_heads"),
+    (t(4, 0, 64), t(4, 1, 64), t(4, 1, 64), CU, {}, "multiple of kv_heads"),
+    (t(4, 2, 64), t(4, 2, 64), t(4, 2, 64), CU.float(), {}, "cu_seqlens"),
+    (t(4, 2, 64), t(4, 2, 64), t(4, 2, 64), CU[None], {}, "cu_seqlens"),
+    (t(4, 2, 64), t(4, 2, 64), t(4, 2, 64), CU[:0], {}, "cu_seqlens"),
+    (t(4, 2, 64), t(4, 2, 64), t(4, 2, 64), CU.to("meta"), {}, "cu_seqlens is on"),
+    (t(4, 2, 64), t(4, 2, 64), t(4, 2, 64), CU, {"softmax_scale": 0.0}, "softmax_scale"),
+    (t(4, 2, 64), t(4, 2, 64), t(4, 2, 64), CU, {"softmax_scale": -1.0}, "softmax_scale"),
+    (t(4, 2, 64), t(4, 2, 64), t(4, 2, 64), CU, {"softmax_scale": float("inf")}, "softmax_scale"),
+    (t(4, 2, 64), t(4, 2, 64), t(4, 2, 64), CU, {"kernel_backend": xma.KernelBackend.torch}, "kernel_backend"),
+])
+def test_refused(q, k, v, cu, options, match):
+    with pytest.raises(ValueError, match=match):
+        xma.attention_packed(q, k, v, cu, **options)
+
+
+def test_no_cpu_path():
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        xma.attention_packed(t(4, 2, 64), t(4, 2, 64), t(4, 2, 64), CU)
+
+
+def test_c_entry_refuses():
+    from xma import _native as N
+
+    lib, a = N.lib(), 1 << 20
+    def forward(q=a, k=a, v=a, strides=(128, 64) * 3, dt=0, cu=a, batch=1, total=4, heads=2, kv=2, dim=64, scale=0.1, out=a, ws=a):
+        return lib.xma_attention_forward(q, k, v, *strides, dt, cu, 0, batch, total, heads, kv, dim, scale, out, None, ws, None, None)
+
+    assert forward(total=0) == 0
+    assert forward(q=None) == 1 and forward(out=None) == 1 and forward(ws=None) == 1 and forward(cu=None) == 1
+    assert forward(q=a + 2) == 1 and forward(out=a + 8) == 1 and forward(batch=-1) == 1 and forward(total=-1) == 1
+    assert forward(strides=(128, 64, 128, 60, 128, 64)) == 1 and forward(strides=(0, 64) * 3) == 1
+    assert forward(scale=0.0) == 1 and forward(scale=float("nan")) == 1
+    assert forward(dt=2) == 2 and forward(dim=20) == 2 and forward(dim=136) == 2 and forward(heads=3) == 2
+    assert forward(batch=1 << 21) == 2 and forward(total=1 << 31) == 2
+    for total, batch in ((0, 0), (1, 1), (127, 3), (128, 1), (100000, 77)):
+        assert lib.xma_attention_workspace_bytes(total, batch) == N.attention_workspace_bytes(total, batch)
+        assert lib.xma_attention_stat_rows(total, batch) == N.attention_stat_rows(total, batch)
