@@ -39,6 +39,9 @@ constexpr int kTile = 128;            // query or key rows of a tile
 constexpr int kThreads = 384;         // load warp, MMA warp, two idle, two groups of four compute warps
 constexpr int kTmemCols = 512;
 constexpr float kRescaleLog2 = 8.f;   // the accumulator is rescaled when a row's maximum grew by more than 2^8
+constexpr int kPolyEvery = 4;         // every fourth pair of a softmax row takes ex2_poly
+constexpr int kControlRegs = 88;      // registers of the load and MMA warps' group and of the compute groups:
+constexpr int kComputeRegs = 208;     // 128 * 88 + 256 * 208 = 384 * 168
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanBuckets = 1024;
 constexpr int kMaxHeads = 4096;
@@ -72,6 +75,34 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// 2^x for a pair on the FMA pipe (the ex2 unit does 16 a cycle and SM, which is what a softmax would wait
+// for): with n the integer nearest to x and f = x - n, 2^f is a polynomial (minimax for the relative error on
+// [-1/2, 1/2], found by exchange: 2^-13.7 of degree 3 for bf16, which rounds at 2^-9, and 2^-18.5 of degree
+// 4 for fp16, which rounds at 2^-12) and n is added to its exponent. Arguments below -126 give 2^-126.
+template <typename T>
+__device__ __forceinline__ f32x2 ex2_poly(f32x2 x2) {
+    float x, y;
+    split_f32x2(x2, x, y);
+    x2 = make_f32x2(fmaxf(x, -126.f), fmaxf(y, -126.f));
+    constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it leaves the nearest integer in the low bits
+    const f32x2 t = add_f32x2(x2, make_f32x2(kRound, kRound));
+    const f32x2 f = add_f32x2(x2, mul_f32x2(add_f32x2(t, make_f32x2(-kRound, -kRound)), make_f32x2(-1.f, -1.f)));
+    f32x2 r;
+    if (std::is_same<T, __half>::value) {
+        r = fma_f32x2(make_f32x2(0.009570102207362652f, 0.009570102207362652f), f, make_f32x2(0.05591785907745361f, 0.05591785907745361f));
+        r = fma_f32x2(r, f, make_f32x2(0.240247443318367f, 0.240247443318367f));
+        r = fma_f32x2(r, f, make_f32x2(0.6931217908859253f, 0.6931217908859253f));
+        r = fma_f32x2(r, f, make_f32x2(0.9999992847442627f, 0.9999992847442627f));
+    } else {
+        r = fma_f32x2(make_f32x2(0.0551716685295105f, 0.0551716685295105f), f, make_f32x2(0.2426111251115799f, 0.2426111251115799f));
+        r = fma_f32x2(r, f, make_f32x2(0.6932609677314758f, 0.6932609677314758f));
+        r = fma_f32x2(r, f, make_f32x2(0.9999280571937561f, 0.9999280571937561f));
+    }
+    float a, b, na, nb;
+    split_f32x2(r, a, b);
+    split_f32x2(t, na, nb);
+    return make_f32x2(__int_as_float(__float_as_int(a) + (__float_as_int(na) << 23)), __int_as_float(__float_as_int(b) + (__float_as_int(nb) << 23)));
 }
 __device__ __forceinline__ float lg2(float x) {
     float y;
@@ -214,10 +245,12 @@ __device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a_tile, uint32_t
     for (int kk = 0; kk < kD / 16; ++kk)
         umma_ss_cta1(d, desc_k_major(a_tile, kk), desc_k_major(b_tile, kk), idesc, kk != 0 ? 1u : 0u);
 }
-// D[128, kD] (+)= A B over 128 rows of B; A in tensor memory, its second half of the rows `second` columns on.
+// D[128, kD] (+)= A B over rows 16 kFirst .. 16 kLast - 1 of B; A in tensor memory, the part for the upper 64
+// rows `second` columns on.
+template <int kFirst = 0, int kLast = kTile / 16>
 __device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t second, uint32_t b_tile, uint32_t idesc, bool accumulate) {
 #pragma unroll
-    for (int kk = 0; kk < kTile / 16; ++kk)
+    for (int kk = kFirst; kk < kLast; ++kk)
         umma_ts_cta1(d, a + (kk >> 2) * second + (kk & 3) * 8, desc_row_major(b_tile, kk), idesc, (accumulate || kk != 0) ? 1u : 0u);
 }
 
@@ -242,6 +275,12 @@ __device__ __forceinline__ void store_row(uint32_t taddr, T* dst, int dim, float
             }
         }
     }
+}
+
+// The item a CTA takes in its turn-th turn: items lie by falling work, so every other turn runs backwards
+// through the CTAs, which evens out what one CTA gets.
+__device__ __forceinline__ int64_t work_item(int64_t turn) {
+    return turn * gridDim.x + ((turn & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
 }
 
 struct Ring {
@@ -280,9 +319,10 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     constexpr uint32_t kBars = (2 + F::kStages) * F::kTileBytes;
     const uint32_t bars = base + kBars;
     const uint32_t full = bars, empty = bars + 64;
-    const uint32_t q_full = bars + 128, q_empty = bars + 144, s_full = bars + 160, p_ready = bars + 176, o_full = bars + 192;
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + kBars + 208);
-    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + kBars + 212);
+    const uint32_t q_full = bars + 128, q_empty = bars + 144, s_full = bars + 160, o_full = bars + 176;
+    const uint32_t p_ready = bars + 192;  // [tile][half of the keys]
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + kBars + 224);
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + kBars + 228);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -294,7 +334,8 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             mbar_init(q_full + 8 * t, 1);
             mbar_init(q_empty + 8 * t, 1);
             mbar_init(s_full + 8 * t, 1);
-            mbar_init(p_ready + 8 * t, 4);  // the four warps of a tile
+            mbar_init(p_ready + 16 * t, 4);  // the four warps of a tile
+            mbar_init(p_ready + 16 * t + 8, 4);
             mbar_init(o_full + 8 * t, 1);
         }
         *abort_flag = 0;
@@ -304,7 +345,7 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         prefetch_tmap(&map_v);
     }
     if (warp == 1) {
-        tmem_alloc(bars + 212, kTmemCols);
+        tmem_alloc(bars + 228, kTmemCols);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -313,12 +354,13 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     const uint32_t tmem = *tmem_slot;
     const int64_t items = static_cast<int64_t>(*p.num_blocks) * p.heads;
 
+    if (warp < 4) regs_shrink<kControlRegs>();  // in a branch of its own: the compute branch keeps its budget
     if (warp == 0) {
         if (lane == 0) {
             Ring kv;
             uint32_t q_phase[2] = {1u, 1u};
             bool ok = true;
-            for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x) {
+            for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
                 const Block b = p.blocks[it / p.heads];
                 const int head = static_cast<int>(it % p.heads), kv_head = head / p.group;
                 const int row0 = b.index * 2 * kTile;
@@ -348,7 +390,7 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         Ring kv;
         uint32_t q_phase[2] = {0u, 0u}, p_phase[2] = {0u, 0u};
         bool ok = true;
-        for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x) {
+        for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
             const Block b = p.blocks[it / p.heads];
             const int row0 = b.index * 2 * kTile;
             const int tiles = b.len > row0 + kTile ? 2 : 1;
@@ -390,12 +432,17 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 for (int t = 0; ok && t < tiles; ++t) {
                     const int count = first + t;
                     if (j >= count) continue;
-                    ok = mbar_wait(p_ready + 8 * t, p_phase[t], abort_flag, p.status, 507);
+                    ok = mbar_wait(p_ready + 16 * t, p_phase[t], abort_flag, p.status, 507);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (lane == 0) mma_rows<0, 4>(tmem + F::kO + t * kD, tmem + t * kTile, 32, v_tile, idesc_o, j != 0);
+                    __syncwarp();
+                    ok = mbar_wait(p_ready + 16 * t + 8, p_phase[t], abort_flag, p.status, 510);
                     if (!ok) break;
                     p_phase[t] ^= 1u;
                     tc_fence_after();
                     if (lane == 0) {
-                        mma_rows(tmem + F::kO + t * kD, tmem + t * kTile, 32, v_tile, idesc_o, j != 0);
+                        mma_rows<4, 8>(tmem + F::kO + t * kD, tmem + t * kTile, 32, v_tile, idesc_o, true);
                         if (j + 1 < count) {
                             // overwrites p, which the product just issued reads: the pipe runs them in order
                             mma_scores<kD>(tmem + t * kTile, q_tile + t * F::kTileBytes, k_tile, idesc_s);
@@ -417,13 +464,14 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             }
         }
     } else if (warp >= 4) {
+        regs_grow<kComputeRegs>();
         const int t = (warp >> 2) - 1;               // query tile of this group
         const int row = (warp & 3) * 32 + lane;      // its row, and the tensor-memory lane
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_addr = tmem + lanes + t * kTile, o_addr = tmem + lanes + F::kO + t * kD;
         uint32_t s_phase = 0, o_phase = 0;
         bool ok = true;
-        for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x) {
+        for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
             const Block b = p.blocks[it / p.heads];
             const int head = static_cast<int>(it % p.heads);
             const int row0 = b.index * 2 * kTile;
@@ -479,26 +527,37 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                     }
                 }
                 const float neg_m = m == -INFINITY ? 0.f : -m;  // a row with no finite score so far
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                const f32x2 scale2 = make_f32x2(p.scale_log2, p.scale_log2), neg_m2 = make_f32x2(neg_m, neg_m);
+                f32x2 sum[2] = {make_f32x2(0.f, 0.f), make_f32x2(0.f, 0.f)};
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int h = 0; h < 2; ++h) {  // p of 64 keys at a time: their product starts while the others are computed
                     uint32_t packed[32];
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         const int c = h * 2 + (i >> 4), e = (i & 15) * 2;
-                        const float a = ex2(fmaf(__uint_as_float(s[c][e]), p.scale_log2, neg_m));
-                        const float d = ex2(fmaf(__uint_as_float(s[c][e + 1]), p.scale_log2, neg_m));
-                        sum[i & 1] += a;
-                        sum[2 + (i & 1)] += d;
+                        f32x2 x = fma_f32x2(make_f32x2(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])), scale2, neg_m2);
+                        float a, d;
+                        if (i % kPolyEvery == kPolyEvery - 1) {
+                            x = ex2_poly<T>(x);
+                            split_f32x2(x, a, d);
+                        } else {
+                            split_f32x2(x, a, d);
+                            a = ex2(a);
+                            d = ex2(d);
+                            x = make_f32x2(a, d);
+                        }
+                        sum[i & 1] = add_f32x2(sum[i & 1], x);
                         packed[i] = pack2<T>(a, d);
                     }
                     tmem_st32(s_addr + h * 32, packed);
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_ready + 16 * t + 8 * h);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_ready + 8 * t);
+                float part[2];
+                split_f32x2(add_f32x2(sum[0], sum[1]), part[0], part[1]);
+                l += part[0] + part[1];
             }
             if (!ok) break;
             ok = mbar_wait(o_full + 8 * t, o_phase, abort_flag, p.status, 509);
@@ -659,7 +718,7 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
             Ring r;
             uint32_t kv_phase = 1u;
             bool ok = true;
-            for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x) {
+            for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
                 const Block b = p.blocks[it / p.kv_heads];
                 const int kv_head = static_cast<int>(it % p.kv_heads);
                 const int n = (b.len + kTile - 1) / kTile;
@@ -694,7 +753,7 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         Ring r;
         uint32_t kv_phase = 0, p_phase = 0, ds_phase = 0;
         bool ok = true;
-        for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x) {
+        for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
             const Block b = p.blocks[it / p.kv_heads];
             const int n = (b.len + kTile - 1) / kTile;
             const int per_head = n - b.index, steps = per_head * p.group;
@@ -767,7 +826,7 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         Ring r;
         uint32_t s_phase = 0, dp_phase = 0, done_phase = 0;
         bool ok = true;
-        for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x) {
+        for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
             const Block b = p.blocks[it / p.kv_heads];
             const int kv_head = static_cast<int>(it % p.kv_heads);
             const int n = (b.len + kTile - 1) / kTile;
@@ -926,7 +985,7 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
             Ring r;
             uint32_t q_phase = 1u;
             bool ok = true;
-            for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x) {
+            for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
                 const Block b = p.blocks[it / p.heads];
                 const int head = static_cast<int>(it % p.heads), kv_head = head / p.group;
                 ok = mbar_wait(q_empty, q_phase, abort_flag, p.status, 521);
@@ -953,7 +1012,7 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
         Ring r;
         uint32_t q_phase = 0, ds_phase = 0, buf = 0;
         bool ok = true;
-        for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x) {
+        for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
             const Block b = p.blocks[it / p.heads];
             ok = mbar_wait(q_full, q_phase, abort_flag, p.status, 523);
             if (!ok) break;
@@ -1015,7 +1074,7 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
         const float factor = ds_factor<T>(p);
         uint32_t s_phase[2] = {0u, 0u}, dp_phase = 0, done_phase = 0, buf = 0;
         bool ok = true;
-        for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x) {
+        for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
             const Block b = p.blocks[it / p.heads];
             const int head = static_cast<int>(it % p.heads);
             const int query = b.index * kTile + row;
