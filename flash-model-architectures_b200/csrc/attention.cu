@@ -39,7 +39,6 @@ constexpr int kTile = 128;            // query or key rows of a tile
 constexpr int kThreads = 384;         // load warp, MMA warp, two idle, two groups of four compute warps
 constexpr int kTmemCols = 512;
 constexpr float kRescaleLog2 = 8.f;   // the accumulator is rescaled when a row's maximum grew by more than 2^8
-constexpr int kPolyEvery = 4;         // every fourth pair of a softmax row takes ex2_poly
 constexpr int kControlRegs = 88;      // registers of the load and MMA warps' group and of the compute groups:
 constexpr int kComputeRegs = 208;     // 128 * 88 + 256 * 208 = 384 * 168
 constexpr int kPlanThreads = 1024;
@@ -75,34 +74,6 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
-}
-// 2^x for a pair on the FMA pipe (the ex2 unit does 16 a cycle and SM, which is what a softmax would wait
-// for): with n the integer nearest to x and f = x - n, 2^f is a polynomial (minimax for the relative error on
-// [-1/2, 1/2], found by exchange: 2^-13.7 of degree 3 for bf16, which rounds at 2^-9, and 2^-18.5 of degree
-// 4 for fp16, which rounds at 2^-12) and n is added to its exponent. Arguments below -126 give 2^-126.
-template <typename T>
-__device__ __forceinline__ f32x2 ex2_poly(f32x2 x2) {
-    float x, y;
-    split_f32x2(x2, x, y);
-    x2 = make_f32x2(fmaxf(x, -126.f), fmaxf(y, -126.f));
-    constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it leaves the nearest integer in the low bits
-    const f32x2 t = add_f32x2(x2, make_f32x2(kRound, kRound));
-    const f32x2 f = add_f32x2(x2, mul_f32x2(add_f32x2(t, make_f32x2(-kRound, -kRound)), make_f32x2(-1.f, -1.f)));
-    f32x2 r;
-    if (std::is_same<T, __half>::value) {
-        r = fma_f32x2(make_f32x2(0.009570102207362652f, 0.009570102207362652f), f, make_f32x2(0.05591785907745361f, 0.05591785907745361f));
-        r = fma_f32x2(r, f, make_f32x2(0.240247443318367f, 0.240247443318367f));
-        r = fma_f32x2(r, f, make_f32x2(0.6931217908859253f, 0.6931217908859253f));
-        r = fma_f32x2(r, f, make_f32x2(0.9999992847442627f, 0.9999992847442627f));
-    } else {
-        r = fma_f32x2(make_f32x2(0.0551716685295105f, 0.0551716685295105f), f, make_f32x2(0.2426111251115799f, 0.2426111251115799f));
-        r = fma_f32x2(r, f, make_f32x2(0.6932609677314758f, 0.6932609677314758f));
-        r = fma_f32x2(r, f, make_f32x2(0.9999280571937561f, 0.9999280571937561f));
-    }
-    float a, b, na, nb;
-    split_f32x2(r, a, b);
-    split_f32x2(t, na, nb);
-    return make_f32x2(__int_as_float(__float_as_int(a) + (__float_as_int(na) << 23)), __int_as_float(__float_as_int(b) + (__float_as_int(nb) << 23)));
 }
 __device__ __forceinline__ float lg2(float x) {
     float y;
@@ -211,6 +182,12 @@ plan_kernel(const IntT* __restrict__ cu, int64_t batch, int64_t total, int block
 // Shared device pieces
 // ---------------------------------------------------------------------------------------------
 
+// A list entry, read by a converged warp and known to be the same in all of it.
+__device__ __forceinline__ Block load_block(const Block* at) {
+    const int4 v = __ldg(reinterpret_cast<const int4*>(at));
+    return Block{warp_uniform(v.x), warp_uniform(v.y), warp_uniform(v.z), warp_uniform(v.w)};
+}
+
 // A [128, kD] tile of one head from a [tokens, heads, dim] tensor: kD / 64 boxes of 128 rows x 64 columns
 // (128-byte swizzle), 16 KB each.
 template <int kD>
@@ -229,29 +206,29 @@ __device__ __forceinline__ void zero_tile_rows(uint32_t tile, int first, int lan
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + c * (kTile * 128) + first * 128 + i * 16), "r"(0) : "memory");
 }
 
-// Operand with the reduction along the head dimension (rows of a tile are rows or columns of the product).
-__device__ __forceinline__ uint64_t desc_k_major(uint32_t tile, int kk) {
-    return make_smem_desc(tile + (kk >> 2) * (kTile * 128) + (kk & 3) * 32, 0, 1024);
-}
+// Operand with the reduction along the head dimension (a tile's rows are rows or columns of the product),
+// and its step kk of 16 elements.
+__device__ __forceinline__ uint64_t desc_k_major(uint32_t tile) { return make_smem_desc(tile, 0, 1024); }
+__device__ __forceinline__ constexpr uint64_t k_step(int kk) { return ((kk >> 2) * (kTile * 128) + (kk & 3) * 32) >> 4; }
 // Operand with the reduction along the tile's rows (the head dimension is a dimension of the product).
-__device__ __forceinline__ uint64_t desc_row_major(uint32_t tile, int kk) {
-    return make_smem_desc(tile + kk * 2048, kTile * 128, 1024);
-}
+__device__ __forceinline__ uint64_t desc_row_major(uint32_t tile) { return make_smem_desc(tile, kTile * 128, 1024); }
+__device__ __forceinline__ constexpr uint64_t row_step(int kk) { return (kk * 2048) >> 4; }
 
 // D[128, 128] = A B^T over the head dimension.
 template <int kD>
 __device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a_tile, uint32_t b_tile, uint32_t idesc) {
+    const uint64_t a = desc_k_major(a_tile), b = desc_k_major(b_tile);
 #pragma unroll
-    for (int kk = 0; kk < kD / 16; ++kk)
-        umma_ss_cta1(d, desc_k_major(a_tile, kk), desc_k_major(b_tile, kk), idesc, kk != 0 ? 1u : 0u);
+    for (int kk = 0; kk < kD / 16; ++kk) umma_ss_cta1(d, a + k_step(kk), b + k_step(kk), idesc, kk != 0 ? 1u : 0u);
 }
 // D[128, kD] (+)= A B over rows 16 kFirst .. 16 kLast - 1 of B; A in tensor memory, the part for the upper 64
 // rows `second` columns on.
 template <int kFirst = 0, int kLast = kTile / 16>
 __device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t second, uint32_t b_tile, uint32_t idesc, bool accumulate) {
+    const uint64_t b = desc_row_major(b_tile);
 #pragma unroll
     for (int kk = kFirst; kk < kLast; ++kk)
-        umma_ts_cta1(d, a + (kk >> 2) * second + (kk & 3) * 8, desc_row_major(b_tile, kk), idesc, (accumulate || kk != 0) ? 1u : 0u);
+        umma_ts_cta1(d, a + (kk >> 2) * second + (kk & 3) * 8, b + row_step(kk), idesc, (accumulate || kk != 0) ? 1u : 0u);
 }
 
 // 16-byte pieces of one row of kD float32 values in tensor memory, scaled and rounded, to global memory.
@@ -324,7 +301,7 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + kBars + 224);
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + kBars + 228);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < F::kStages; ++i) {
             mbar_init(full + 8 * i, 1);
@@ -351,8 +328,8 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
-    const int64_t items = static_cast<int64_t>(*p.num_blocks) * p.heads;
+    const uint32_t tmem = warp_uniform(*tmem_slot);
+    const int64_t items = static_cast<int64_t>(warp_uniform(*p.num_blocks)) * p.heads;
 
     if (warp < 4) regs_shrink<kControlRegs>();  // in a branch of its own: the compute branch keeps its budget
     if (warp == 0) {
@@ -391,19 +368,19 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         uint32_t q_phase[2] = {0u, 0u}, p_phase[2] = {0u, 0u};
         bool ok = true;
         for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
-            const Block b = p.blocks[it / p.heads];
+            const Block b = load_block(p.blocks + it / p.heads);
             const int row0 = b.index * 2 * kTile;
             const int tiles = b.len > row0 + kTile ? 2 : 1;
             const int n = b.index * 2 + tiles;              // key tiles of the last query tile
             const int first = b.index * 2 + 1;              // key tiles of query tile 0
             // s of key tile 0
-            ok = mbar_wait(full + 8 * kv.stage, kv.phase, abort_flag, p.status, 503);
+            ok = mbar_wait_warp(full + 8 * kv.stage, kv.phase, abort_flag, p.status, 503);
             for (int t = 0; ok && t < tiles; ++t) {
-                ok = mbar_wait(q_full + 8 * t, q_phase[t], abort_flag, p.status, 504);
+                ok = mbar_wait_warp(q_full + 8 * t, q_phase[t], abort_flag, p.status, 504);
                 if (!ok) break;
                 q_phase[t] ^= 1u;
                 tc_fence_after();
-                if (lane == 0) {
+                if (elect_one()) {
                     mma_scores<kD>(tmem + t * kTile, q_tile + t * F::kTileBytes, ring + kv.stage * F::kTileBytes, idesc_s);
                     umma_commit_cta1(s_full + 8 * t);
                     if (first + t == 1) umma_commit_cta1(q_empty + 8 * t);
@@ -411,12 +388,12 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 __syncwarp();
             }
             if (!ok) break;
-            if (lane == 0) umma_commit_cta1(empty + 8 * kv.stage);
+            if (elect_one()) umma_commit_cta1(empty + 8 * kv.stage);
             kv.next(F::kStages);
             for (int j = 0; ok && j < n; ++j) {
                 const uint32_t v_tile = ring + kv.stage * F::kTileBytes;
                 const uint32_t v_empty = empty + 8 * kv.stage;
-                ok = mbar_wait(full + 8 * kv.stage, kv.phase, abort_flag, p.status, 505);
+                ok = mbar_wait_warp(full + 8 * kv.stage, kv.phase, abort_flag, p.status, 505);
                 if (!ok) break;
                 kv.next(F::kStages);
                 const int valid = b.len - j * kTile;
@@ -428,20 +405,20 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 const uint32_t k_tile = ring + kv.stage * F::kTileBytes;
                 const uint32_t k_empty = empty + 8 * kv.stage;
                 const bool more = j + 1 < n;
-                if (more) ok = mbar_wait(full + 8 * kv.stage, kv.phase, abort_flag, p.status, 506);
+                if (more) ok = mbar_wait_warp(full + 8 * kv.stage, kv.phase, abort_flag, p.status, 506);
                 for (int t = 0; ok && t < tiles; ++t) {
                     const int count = first + t;
                     if (j >= count) continue;
-                    ok = mbar_wait(p_ready + 16 * t, p_phase[t], abort_flag, p.status, 507);
+                    ok = mbar_wait_warp(p_ready + 16 * t, p_phase[t], abort_flag, p.status, 507);
                     if (!ok) break;
                     tc_fence_after();
-                    if (lane == 0) mma_rows<0, 4>(tmem + F::kO + t * kD, tmem + t * kTile, 32, v_tile, idesc_o, j != 0);
+                    if (elect_one()) mma_rows<0, 4>(tmem + F::kO + t * kD, tmem + t * kTile, 32, v_tile, idesc_o, j != 0);
                     __syncwarp();
-                    ok = mbar_wait(p_ready + 16 * t + 8, p_phase[t], abort_flag, p.status, 510);
+                    ok = mbar_wait_warp(p_ready + 16 * t + 8, p_phase[t], abort_flag, p.status, 510);
                     if (!ok) break;
                     p_phase[t] ^= 1u;
                     tc_fence_after();
-                    if (lane == 0) {
+                    if (elect_one()) {
                         mma_rows<4, 8>(tmem + F::kO + t * kD, tmem + t * kTile, 32, v_tile, idesc_o, true);
                         if (j + 1 < count) {
                             // overwrites p, which the product just issued reads: the pipe runs them in order
@@ -455,7 +432,7 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                     __syncwarp();
                 }
                 if (!ok) break;
-                if (lane == 0) {
+                if (elect_one()) {
                     umma_commit_cta1(v_empty);
                     if (more) umma_commit_cta1(k_empty);
                 }
@@ -535,18 +512,12 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         const int c = h * 2 + (i >> 4), e = (i & 15) * 2;
-                        f32x2 x = fma_f32x2(make_f32x2(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])), scale2, neg_m2);
+                        const f32x2 x = fma_f32x2(make_f32x2(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])), scale2, neg_m2);
                         float a, d;
-                        if (i % kPolyEvery == kPolyEvery - 1) {
-                            x = ex2_poly<T>(x);
-                            split_f32x2(x, a, d);
-                        } else {
-                            split_f32x2(x, a, d);
-                            a = ex2(a);
-                            d = ex2(d);
-                            x = make_f32x2(a, d);
-                        }
-                        sum[i & 1] = add_f32x2(sum[i & 1], x);
+                        split_f32x2(x, a, d);
+                        a = ex2(a);
+                        d = ex2(d);
+                        sum[i & 1] = add_f32x2(sum[i & 1], make_f32x2(a, d));
                         packed[i] = pack2<T>(a, d);
                     }
                     tmem_st32(s_addr + h * 32, packed);
@@ -682,7 +653,7 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + B::kBars + 128);
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + B::kBars + 132);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < B::kStages; ++i) {
             mbar_init(full + 8 * i, 1);
@@ -709,9 +680,9 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = warp_uniform(*tmem_slot);
     const uint32_t tm_s = tmem, tm_dp = tmem + kTile, tm_dv = tmem + 2 * kTile, tm_dk = tm_dv + kD;
-    const int64_t items = static_cast<int64_t>(*p.num_blocks) * p.kv_heads;
+    const int64_t items = static_cast<int64_t>(warp_uniform(*p.num_blocks)) * p.kv_heads;
 
     if (warp == 0) {
         if (lane == 0) {
@@ -754,10 +725,10 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         uint32_t kv_phase = 0, p_phase = 0, ds_phase = 0;
         bool ok = true;
         for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
-            const Block b = p.blocks[it / p.kv_heads];
+            const Block b = load_block(p.blocks + it / p.kv_heads);
             const int n = (b.len + kTile - 1) / kTile;
             const int per_head = n - b.index, steps = per_head * p.group;
-            ok = mbar_wait(kv_full, kv_phase, abort_flag, p.status, 513);
+            ok = mbar_wait_warp(kv_full, kv_phase, abort_flag, p.status, 513);
             if (!ok) break;
             kv_phase ^= 1u;
             for (int st = -1; ok && st < steps; ++st) {
@@ -769,7 +740,7 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
                 if (st >= 0) ahead.next(B::kStages);
                 const uint32_t nxt = ring + ahead.stage * B::kStageBytes;
                 if (more) {
-                    ok = mbar_wait(full + 8 * ahead.stage, ahead.phase, abort_flag, p.status, 514);
+                    ok = mbar_wait_warp(full + 8 * ahead.stage, ahead.phase, abort_flag, p.status, 514);
                     if (!ok) break;
                     tc_fence_after();
                     const int valid = b.len - (b.index + (st + 1) % per_head) * kTile;
@@ -781,12 +752,12 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
                     }
                 }
                 if (st >= 0) {
-                    ok = mbar_wait(p_ready, p_phase, abort_flag, p.status, 515);
+                    ok = mbar_wait_warp(p_ready, p_phase, abort_flag, p.status, 515);
                     if (!ok) break;
                     p_phase ^= 1u;
                     tc_fence_after();
                 }
-                if (lane == 0) {
+                if (elect_one()) {
                     if (st >= 0) mma_rows(tm_dv, tm_s, 64, cur + B::kTileBytes, idesc_d, st > 0);
                     if (more) {
                         mma_scores<kD>(tm_s, k_tile, nxt, idesc_s);
@@ -795,12 +766,12 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
                 }
                 __syncwarp();
                 if (st >= 0) {
-                    ok = mbar_wait(ds_ready, ds_phase, abort_flag, p.status, 516);
+                    ok = mbar_wait_warp(ds_ready, ds_phase, abort_flag, p.status, 516);
                     if (!ok) break;
                     ds_phase ^= 1u;
                     tc_fence_after();
                 }
-                if (lane == 0) {
+                if (elect_one()) {
                     if (st >= 0) {
                         mma_rows(tm_dk, tm_dp, 64, cur, idesc_d, st > 0);
                         umma_commit_cta1(cur_empty);
@@ -949,7 +920,7 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + B::kBars + 128);
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + B::kBars + 132);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < B::kStages; ++i) {
             mbar_init(full + 8 * i, 1);
@@ -976,9 +947,9 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = warp_uniform(*tmem_slot);
     const uint32_t tm_dp = tmem + 2 * kTile, tm_dq = tmem + 3 * kTile;
-    const int64_t items = static_cast<int64_t>(*p.num_blocks) * p.heads;
+    const int64_t items = static_cast<int64_t>(warp_uniform(*p.num_blocks)) * p.heads;
 
     if (warp == 0) {
         if (lane == 0) {
@@ -1013,8 +984,8 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
         uint32_t q_phase = 0, ds_phase = 0, buf = 0;
         bool ok = true;
         for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
-            const Block b = p.blocks[it / p.heads];
-            ok = mbar_wait(q_full, q_phase, abort_flag, p.status, 523);
+            const Block b = load_block(p.blocks + it / p.heads);
+            ok = mbar_wait_warp(q_full, q_phase, abort_flag, p.status, 523);
             if (!ok) break;
             q_phase ^= 1u;
             for (int j = -1; ok && j <= b.index; ++j) {
@@ -1026,7 +997,7 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
                 if (j >= 0) ahead.next(B::kStages);
                 const uint32_t nxt = ring + ahead.stage * B::kStageBytes;
                 if (more) {
-                    ok = mbar_wait(full + 8 * ahead.stage, ahead.phase, abort_flag, p.status, 524);
+                    ok = mbar_wait_warp(full + 8 * ahead.stage, ahead.phase, abort_flag, p.status, 524);
                     if (!ok) break;
                     tc_fence_after();
                     const int valid = b.len - (j + 1) * kTile;
@@ -1035,7 +1006,7 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
                         fence_proxy_async();
                         __syncwarp();
                     }
-                    if (lane == 0) {
+                    if (elect_one()) {
                         // the step before last has read this buffer (its ds was waited for)
                         mma_scores<kD>(tmem + buf * kTile, q_tile, nxt, idesc_s);
                         umma_commit_cta1(s_full + 8 * buf);
@@ -1044,12 +1015,12 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
                     buf ^= 1u;
                 }
                 if (j >= 0) {
-                    ok = mbar_wait(ds_ready, ds_phase, abort_flag, p.status, 525);
+                    ok = mbar_wait_warp(ds_ready, ds_phase, abort_flag, p.status, 525);
                     if (!ok) break;
                     ds_phase ^= 1u;
                     tc_fence_after();
                 }
-                if (lane == 0) {
+                if (elect_one()) {
                     if (j >= 0) {
                         mma_rows(tm_dq, tm_dp, 64, cur, idesc_d, j > 0);
                         umma_commit_cta1(cur_empty);

@@ -197,6 +197,24 @@ __host__ __device__ constexpr uint32_t make_idesc(int m, int n, bool a_mn_major,
            (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+// One lane of a converged warp. Unlike a comparison of lane numbers it leaves the code it guards in the
+// warp-uniform form, so that tcgen05 operands are computed in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r));
+    return r != 0;
+}
+// Lane 0's value, known to the compiler to be the same in the whole warp.
+__device__ __forceinline__ int warp_uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+// mbar_wait by a converged warp, with one answer for all of it.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status, int code) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code));
+}
+
 // ---- one-CTA forms (no cluster) ----
 
 // Untiled copy of `bytes` (a multiple of 16, both addresses 16-byte aligned) into shared memory.
