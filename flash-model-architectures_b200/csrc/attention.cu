@@ -623,49 +623,87 @@ delta_kernel(const T* __restrict__ o, const T* __restrict__ d_o, const T* __rest
     }
 }
 
+// Shared memory of the two backward kernels: two resident tiles, a ring of three tiles whose contents live
+// through a whole step (they are operands of its first and of its last product), and a ring of two for the
+// others. There is no room left for alignment slack: the kernels check that the base is aligned.
 template <int kD>
 struct Backward {
     static_assert(kD == 64 || kD == 128, "tile widths");
     static constexpr uint32_t kTileBytes = kTile * kD * 2;
-    static constexpr int kStages = kD == 128 ? 2 : 4;
-    static constexpr uint32_t kStageBytes = 2 * kTileBytes;
-    static constexpr uint32_t kStats = 2 * kTile * 4;  // lse and delta of a query tile
-    static constexpr uint32_t kBars = 2 * kTileBytes + kStages * (kStageBytes + kStats);
-    static constexpr uint32_t kSmem = 1024 + kBars + 256;
+    static constexpr int kLong = 3, kShort = 2;
+    static constexpr uint32_t kStats = 2 * kTile * 4;  // lse and delta of a query tile (dkdv), beside a short-ring tile
+    static constexpr uint32_t kLongAt = 2 * kTileBytes, kShortAt = kLongAt + kLong * kTileBytes;
+    static constexpr uint32_t kStatsAt = kShortAt + kShort * kTileBytes;
+    static constexpr uint32_t kBars = kStatsAt + kShort * kStats;
+    static constexpr uint32_t kSmem = kBars + 256;
+    static_assert(kSmem <= 227 * 1024, "shared memory");
 };
+
+__device__ __forceinline__ bool base_is_aligned(uint32_t base, int32_t* status) {
+    if ((base & 1023u) == 0) return true;
+    if (threadIdx.x == 0 && status != nullptr) atomicCAS(status, 0, 530);
+    return false;
+}
+
+// p (or ds) of 32 neighbouring columns to tensor memory, as 16 packed columns.
+template <typename T>
+__device__ __forceinline__ void store_packed32(uint32_t taddr, const float* v) {
+    uint32_t packed[16];
+#pragma unroll
+    for (int c = 0; c < 16; ++c) packed[c] = pack2<T>(v[2 * c], v[2 * c + 1]);
+    tmem_st16(taddr, packed);
+}
+// Half `part` of the product over 128 rows of B whose A operand store_packed32 wrote: columns 32 part .. 32
+// part + 31 of each compute group's 64.
+__device__ __forceinline__ void mma_rows_part(int part, uint32_t d, uint32_t a, uint32_t b_tile, uint32_t idesc, bool accumulate) {
+    const uint64_t b = desc_row_major(b_tile);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int kk = (i >> 1) * 4 + part * 2 + (i & 1);
+        umma_ts_cta1(d, a + (kk >> 2) * 64 + (kk & 3) * 8, b + row_step(kk), idesc, (accumulate || part != 0 || i != 0) ? 1u : 0u);
+    }
+}
 
 // Work item: 128 key rows of one key/value head, all query tiles at or after them of the group's heads.
 // Tensor memory: s^T at 0, dp^T at 128, dv at 256, dk at 256 + kD. Each group of four compute warps takes 64
-// of the 128 query columns; p^T (and ds^T) of a half lies at the start of that half's columns.
+// of the 128 query columns; p^T (and ds^T) of a half lies at the start of that half's columns. One MMA warp
+// issues dv += p^T do and the next s^T, the other dk += ds^T q and the next dp^T: each pair shares a region of
+// tensor memory, and while one warp waits for the compute warps the other's products run.
 template <typename T, int kD>
 __global__ void __launch_bounds__(kThreads, 1)
 dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
             const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, const Params p) {
     using B = Backward<kD>;
-    extern __shared__ uint8_t smem_raw[];
-    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
-    const uint32_t k_tile = base, v_tile = base + B::kTileBytes, ring = base + 2 * B::kTileBytes;
-    constexpr uint32_t kStatsAt = 2 * B::kTileBytes + B::kStages * B::kStageBytes;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const uint32_t base = smem_u32(smem_raw);
+    if (!base_is_aligned(base, p.status)) return;
+    uint8_t* gen = smem_raw;
+    const uint32_t k_tile = base, v_tile = base + B::kTileBytes, q_ring = base + B::kLongAt, do_ring = base + B::kShortAt;
     const uint32_t bars = base + B::kBars;
-    const uint32_t full = bars, empty = bars + 32, kv_full = bars + 64, kv_empty = bars + 72, s_full = bars + 80, dp_full = bars + 88,
-                   p_ready = bars + 96, ds_ready = bars + 104, done = bars + 112;
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + B::kBars + 128);
-    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + B::kBars + 132);
+    const uint32_t q_full = bars, q_empty = bars + 24, do_full = bars + 48, do_empty = bars + 64, kv_full = bars + 80, kv_empty = bars + 88,
+                   s_full = bars + 96, dp_full = bars + 104, p_ready = bars + 112, ds_ready = bars + 128, done = bars + 144;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + B::kBars + 160);
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + B::kBars + 164);
 
     const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < B::kStages; ++i) {
-            mbar_init(full + 8 * i, 1);
-            mbar_init(empty + 8 * i, 1 + 8);  // the MMAs that read the stage, and the warps that read its statistics
+        for (int i = 0; i < B::kLong; ++i) {
+            mbar_init(q_full + 8 * i, 1);
+            mbar_init(q_empty + 8 * i, 1);
+        }
+        for (int i = 0; i < B::kShort; ++i) {
+            mbar_init(do_full + 8 * i, 1);
+            mbar_init(do_empty + 8 * i, 2);  // both MMA warps; the second's commit follows the reads of the statistics
         }
         mbar_init(kv_full, 1);
         mbar_init(kv_empty, 1);
         mbar_init(s_full, 1);
         mbar_init(dp_full, 1);
-        mbar_init(p_ready, 8);
-        mbar_init(ds_ready, 8);
-        mbar_init(done, 1);
+        for (int h = 0; h < 2; ++h) {
+            mbar_init(p_ready + 8 * h, 8);
+            mbar_init(ds_ready + 8 * h, 8);
+        }
+        mbar_init(done, 2);
         *abort_flag = 0;
         fence_barrier_init();
         prefetch_tmap(&map_q);
@@ -674,7 +712,7 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         prefetch_tmap(&map_do);
     }
     if (warp == 1) {
-        tmem_alloc(bars + 132, kTmemCols);
+        tmem_alloc(bars + 164, kTmemCols);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -685,8 +723,9 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
     const int64_t items = static_cast<int64_t>(warp_uniform(*p.num_blocks)) * p.kv_heads;
 
     if (warp == 0) {
+        // k, v and the query tiles
         if (lane == 0) {
-            Ring r;
+            Ring q;
             uint32_t kv_phase = 1u;
             bool ok = true;
             for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
@@ -700,29 +739,51 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
                 load_tile<kD>(k_tile, &map_k, kv_full, kv_head, b.start + b.index * kTile);
                 load_tile<kD>(v_tile, &map_v, kv_full, kv_head, b.start + b.index * kTile);
                 for (int g = 0; ok && g < p.group; ++g) {
+                    for (int i = b.index; ok && i < n; ++i) {
+                        ok = mbar_wait(q_empty + 8 * q.stage, q.phase ^ 1u, abort_flag, p.status, 512);
+                        if (!ok) break;
+                        mbar_expect_tx(q_full + 8 * q.stage, B::kTileBytes);
+                        load_tile<kD>(q_ring + q.stage * B::kTileBytes, &map_q, q_full + 8 * q.stage, kv_head * p.group + g,
+                                      b.start + i * kTile);
+                        q.next(B::kLong);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 3) {
+        // do tiles with the rows' statistics
+        if (lane == 0) {
+            Ring d;
+            bool ok = true;
+            for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
+                const Block b = p.blocks[it / p.kv_heads];
+                const int kv_head = static_cast<int>(it % p.kv_heads);
+                const int n = (b.len + kTile - 1) / kTile;
+                for (int g = 0; ok && g < p.group; ++g) {
                     const int head = kv_head * p.group + g;
                     for (int i = b.index; ok && i < n; ++i) {
-                        ok = mbar_wait(empty + 8 * r.stage, r.phase ^ 1u, abort_flag, p.status, 512);
+                        ok = mbar_wait(do_empty + 8 * d.stage, d.phase ^ 1u, abort_flag, p.status, 531);
                         if (!ok) break;
-                        const uint32_t bar = full + 8 * r.stage, dst = ring + r.stage * B::kStageBytes;
-                        mbar_expect_tx(bar, B::kStageBytes + B::kStats);
-                        load_tile<kD>(dst, &map_q, bar, head, b.start + i * kTile);
-                        load_tile<kD>(dst + B::kTileBytes, &map_do, bar, head, b.start + i * kTile);
+                        const uint32_t bar = do_full + 8 * d.stage;
+                        mbar_expect_tx(bar, B::kTileBytes + B::kStats);
+                        load_tile<kD>(do_ring + d.stage * B::kTileBytes, &map_do, bar, head, b.start + i * kTile);
                         const int64_t at = head * p.pad_rows + b.pad + i * kTile;
-                        const uint32_t stats = base + kStatsAt + r.stage * B::kStats;
+                        const uint32_t stats = base + B::kStatsAt + d.stage * B::kStats;
                         bulk_load(stats, p.lse + at, kTile * 4, bar);
                         bulk_load(stats + kTile * 4, p.delta + at, kTile * 4, bar);
-                        r.next(B::kStages);
+                        d.next(B::kShort);
                     }
                 }
             }
         }
         __syncwarp();
     } else if (warp == 1) {
+        // s^T = k q^T, dv += p^T do
         const uint32_t idesc_s = make_idesc(kTile, kTile, false, false, p.ab_format);
         const uint32_t idesc_d = make_idesc(kTile, kD, false, true, p.ab_format);
-        Ring r;
-        uint32_t kv_phase = 0, p_phase = 0, ds_phase = 0;
+        Ring q, d;
+        uint32_t kv_phase = 0, p_phase = 0;
         bool ok = true;
         for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
             const Block b = load_block(p.blocks + it / p.kv_heads);
@@ -731,53 +792,107 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
             ok = mbar_wait_warp(kv_full, kv_phase, abort_flag, p.status, 513);
             if (!ok) break;
             kv_phase ^= 1u;
-            for (int st = -1; ok && st < steps; ++st) {
-                // dv += p^T do and s^T of the next step; then dk += ds^T q and dp^T of the next step
+            ok = mbar_wait_warp(q_full + 8 * q.stage, q.phase, abort_flag, p.status, 514);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+                mma_scores<kD>(tm_s, k_tile, q_ring + q.stage * B::kTileBytes, idesc_s);
+                umma_commit_cta1(s_full);
+            }
+            __syncwarp();
+            q.next(B::kLong);
+            int i = b.index;
+            for (int st = 0; st < steps; ++st) {
                 const bool more = st + 1 < steps;
-                const uint32_t cur = ring + r.stage * B::kStageBytes;
-                const uint32_t cur_empty = empty + 8 * r.stage;
-                Ring ahead = r;
-                if (st >= 0) ahead.next(B::kStages);
-                const uint32_t nxt = ring + ahead.stage * B::kStageBytes;
-                if (more) {
-                    ok = mbar_wait_warp(full + 8 * ahead.stage, ahead.phase, abort_flag, p.status, 514);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const int valid = b.len - (b.index + (st + 1) % per_head) * kTile;
-                    if (valid < kTile) {  // query rows of other sequences
-                        zero_tile_rows<kD>(nxt, valid, lane);
-                        zero_tile_rows<kD>(nxt + B::kTileBytes, valid, lane);
-                        fence_proxy_async();
-                        __syncwarp();
-                    }
+                const uint32_t do_tile = do_ring + d.stage * B::kTileBytes, next_q = q_ring + q.stage * B::kTileBytes;
+                ok = mbar_wait_warp(do_full + 8 * d.stage, d.phase, abort_flag, p.status, 532);
+                if (ok && more) ok = mbar_wait_warp(q_full + 8 * q.stage, q.phase, abort_flag, p.status, 533);
+                if (!ok) break;
+                const int valid = b.len - i * kTile;
+                if (valid < kTile) {  // rows of other sequences, which p = 0 would meet
+                    zero_tile_rows<kD>(do_tile, valid, lane);
+                    fence_proxy_async();
+                    __syncwarp();
                 }
-                if (st >= 0) {
-                    ok = mbar_wait_warp(p_ready, p_phase, abort_flag, p.status, 515);
-                    if (!ok) break;
-                    p_phase ^= 1u;
-                    tc_fence_after();
-                }
+                i = i + 1 < n ? i + 1 : b.index;
+                ok = mbar_wait_warp(p_ready, p_phase, abort_flag, p.status, 515);
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) mma_rows_part(0, tm_dv, tm_s, do_tile, idesc_d, st > 0);
+                __syncwarp();
+                ok = mbar_wait_warp(p_ready + 8, p_phase, abort_flag, p.status, 534);
+                if (!ok) break;
+                p_phase ^= 1u;
+                tc_fence_after();
                 if (elect_one()) {
-                    if (st >= 0) mma_rows(tm_dv, tm_s, 64, cur + B::kTileBytes, idesc_d, st > 0);
+                    mma_rows_part(1, tm_dv, tm_s, do_tile, idesc_d, true);
                     if (more) {
-                        mma_scores<kD>(tm_s, k_tile, nxt, idesc_s);
+                        mma_scores<kD>(tm_s, k_tile, next_q, idesc_s);
                         umma_commit_cta1(s_full);
+                    } else {
+                        umma_commit_cta1(done);
                     }
+                    umma_commit_cta1(do_empty + 8 * d.stage);
                 }
                 __syncwarp();
-                if (st >= 0) {
-                    ok = mbar_wait_warp(ds_ready, ds_phase, abort_flag, p.status, 516);
-                    if (!ok) break;
-                    ds_phase ^= 1u;
-                    tc_fence_after();
+                d.next(B::kShort);
+                if (more) q.next(B::kLong);
+            }
+        }
+    } else if (warp == 2) {
+        // dp^T = v do^T, dk += ds^T q
+        const uint32_t idesc_s = make_idesc(kTile, kTile, false, false, p.ab_format);
+        const uint32_t idesc_d = make_idesc(kTile, kD, false, true, p.ab_format);
+        Ring q, d;
+        uint32_t kv_phase = 0, ds_phase = 0;
+        bool ok = true;
+        for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
+            const Block b = load_block(p.blocks + it / p.kv_heads);
+            const int n = (b.len + kTile - 1) / kTile;
+            const int per_head = n - b.index, steps = per_head * p.group;
+            ok = mbar_wait_warp(kv_full, kv_phase, abort_flag, p.status, 535);
+            if (!ok) break;
+            kv_phase ^= 1u;
+            ok = mbar_wait_warp(do_full + 8 * d.stage, d.phase, abort_flag, p.status, 536);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+                mma_scores<kD>(tm_dp, v_tile, do_ring + d.stage * B::kTileBytes, idesc_s);
+                umma_commit_cta1(dp_full);
+            }
+            __syncwarp();
+            int i = b.index;
+            for (int st = 0; st < steps; ++st) {
+                const bool more = st + 1 < steps;
+                const uint32_t q_tile = q_ring + q.stage * B::kTileBytes;
+                const uint32_t this_empty = do_empty + 8 * d.stage;
+                d.next(B::kShort);
+                const uint32_t next_do = do_ring + d.stage * B::kTileBytes;
+                ok = mbar_wait_warp(q_full + 8 * q.stage, q.phase, abort_flag, p.status, 537);
+                if (ok && more) ok = mbar_wait_warp(do_full + 8 * d.stage, d.phase, abort_flag, p.status, 538);
+                if (!ok) break;
+                ok = mbar_wait_warp(ds_ready, ds_phase, abort_flag, p.status, 516);
+                if (!ok) break;
+                const int valid = b.len - i * kTile;
+                if (valid < kTile) {  // rows of other sequences, which ds = 0 would meet; s^T has read the tile by now
+                    zero_tile_rows<kD>(q_tile, valid, lane);
+                    fence_proxy_async();
+                    __syncwarp();
                 }
+                i = i + 1 < n ? i + 1 : b.index;
+                tc_fence_after();
+                if (elect_one()) mma_rows_part(0, tm_dk, tm_dp, q_tile, idesc_d, st > 0);
+                __syncwarp();
+                ok = mbar_wait_warp(ds_ready + 8, ds_phase, abort_flag, p.status, 539);
+                if (!ok) break;
+                ds_phase ^= 1u;
+                tc_fence_after();
                 if (elect_one()) {
-                    if (st >= 0) {
-                        mma_rows(tm_dk, tm_dp, 64, cur, idesc_d, st > 0);
-                        umma_commit_cta1(cur_empty);
-                    }
+                    mma_rows_part(1, tm_dk, tm_dp, q_tile, idesc_d, true);
+                    umma_commit_cta1(q_empty + 8 * q.stage);
+                    umma_commit_cta1(this_empty);
                     if (more) {
-                        mma_scores<kD>(tm_dp, v_tile, nxt + B::kTileBytes, idesc_s);
+                        mma_scores<kD>(tm_dp, v_tile, next_do, idesc_s);
                         umma_commit_cta1(dp_full);
                     } else {
                         umma_commit_cta1(done);
@@ -785,16 +900,16 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
                     }
                 }
                 __syncwarp();
-                r = ahead;
+                q.next(B::kLong);
             }
         }
-    } else if (warp >= 4) {
+    } else {
         const int half = (warp >> 2) - 1;          // query columns 64 half .. 64 half + 63
         const int row = (warp & 3) * 32 + lane;    // key row
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_addr = tm_s + lanes + half * 64, dp_addr = tm_dp + lanes + half * 64;
         const float factor = ds_factor<T>(p);
-        Ring r;
+        Ring d;
         uint32_t s_phase = 0, dp_phase = 0, done_phase = 0;
         bool ok = true;
         for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
@@ -803,9 +918,9 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
             const int n = (b.len + kTile - 1) / kTile;
             for (int g = 0; ok && g < p.group; ++g) {
                 for (int i = b.index; ok && i < n; ++i) {
-                    ok = mbar_wait(full + 8 * r.stage, r.phase, abort_flag, p.status, 517);
+                    ok = mbar_wait(do_full + 8 * d.stage, d.phase, abort_flag, p.status, 517);
                     if (!ok) break;
-                    const float4* lse = reinterpret_cast<const float4*>(gen + kStatsAt + r.stage * B::kStats + half * 256);
+                    const float4* lse = reinterpret_cast<const float4*>(gen + B::kStatsAt + d.stage * B::kStats + half * 256);
                     const float4* delta = lse + kTile / 4;
                     ok = mbar_wait(s_full, s_phase, abort_flag, p.status, 518);
                     if (!ok) break;
@@ -829,20 +944,17 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
                             pr[c * 32 + e * 4 + 2] = ex2(fmaf(__uint_as_float(s[e * 4 + 2]), p.scale_log2, -f.z));
                             pr[c * 32 + e * 4 + 3] = ex2(fmaf(__uint_as_float(s[e * 4 + 3]), p.scale_log2, -f.w));
                         }
-                    }
-                    if (edge) {
+                        if (edge) {
 #pragma unroll
-                        for (int c = 0; c < 64; ++c)
-                            if (c < from || c >= last) pr[c] = 0.f;
+                            for (int e = 0; e < 32; ++e)
+                                if (c * 32 + e < from || c * 32 + e >= last) pr[c * 32 + e] = 0.f;
+                        }
+                        store_packed32<T>(s_addr + c * 16, pr + c * 32);
+                        tmem_st_wait();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(p_ready + 8 * c);
                     }
-                    uint32_t packed[32];
-#pragma unroll
-                    for (int c = 0; c < 32; ++c) packed[c] = pack2<T>(pr[2 * c], pr[2 * c + 1]);
-                    tmem_st32(s_addr, packed);
-                    tmem_st_wait();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(p_ready);
 
                     ok = mbar_wait(dp_full, dp_phase, abort_flag, p.status, 519);
                     if (!ok) break;
@@ -850,37 +962,29 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
                     tc_fence_after();
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        uint32_t d[32];
-                        tmem_ld32(dp_addr + c * 32, d);
+                        uint32_t dp[32];
+                        tmem_ld32(dp_addr + c * 32, dp);
                         tmem_ld_wait();
-                        tmem_tie32(d);
+                        tmem_tie32(dp);
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             const float4 f = delta[c * 8 + e];
                             const float sub[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
-                            for (int q = 0; q < 4; ++q) {
-                                const int at = c * 32 + e * 4 + q;
-                                pr[at] *= (__uint_as_float(d[e * 4 + q]) - sub[q]) * factor;
-                            }
+                            for (int q = 0; q < 4; ++q) pr[c * 32 + e * 4 + q] *= (__uint_as_float(dp[e * 4 + q]) - sub[q]) * factor;
                         }
-                    }
-                    if (edge) {
+                        if (edge) {
 #pragma unroll
-                        for (int c = 0; c < 64; ++c)
-                            if (c < from || c >= last) pr[c] = 0.f;  // delta of such a column is no number to rely on
+                            for (int e = 0; e < 32; ++e)  // delta of such a column is no number to rely on
+                                if (c * 32 + e < from || c * 32 + e >= last) pr[c * 32 + e] = 0.f;
+                        }
+                        store_packed32<T>(dp_addr + c * 16, pr + c * 32);
+                        tmem_st_wait();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(ds_ready + 8 * c);
                     }
-#pragma unroll
-                    for (int c = 0; c < 32; ++c) packed[c] = pack2<T>(pr[2 * c], pr[2 * c + 1]);
-                    tmem_st32(dp_addr, packed);
-                    tmem_st_wait();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive(ds_ready);
-                        mbar_arrive(empty + 8 * r.stage);
-                    }
-                    r.next(B::kStages);
+                    d.next(B::kShort);
                 }
             }
             if (!ok) break;
@@ -904,34 +1008,40 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
 }
 
 // Work item: 128 query rows of one head over their key tiles. Tensor memory: s at 0 and 128 (two buffers),
-// dp (then ds) at 256, dq at 384. The compute groups take 64 key columns each.
+// dp (then ds) at 256, dq at 384. The compute groups take 64 key columns each. One MMA warp issues s ahead, the
+// other dq += ds k and the next dp.
 template <typename T, int kD>
 __global__ void __launch_bounds__(kThreads, 1)
 dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
           const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, const Params p) {
     using B = Backward<kD>;
-    extern __shared__ uint8_t smem_raw[];
-    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
-    const uint32_t q_tile = base, do_tile = base + B::kTileBytes, ring = base + 2 * B::kTileBytes;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const uint32_t base = smem_u32(smem_raw);
+    if (!base_is_aligned(base, p.status)) return;
+    uint8_t* gen = smem_raw;
+    const uint32_t q_tile = base, do_tile = base + B::kTileBytes, k_ring = base + B::kLongAt, v_ring = base + B::kShortAt;
     const uint32_t bars = base + B::kBars;
-    const uint32_t full = bars, empty = bars + 32, q_full = bars + 64, q_empty = bars + 72, s_full = bars + 80, dp_full = bars + 96,
-                   ds_ready = bars + 104, done = bars + 112;
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + B::kBars + 128);
-    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + B::kBars + 132);
+    const uint32_t k_full = bars, k_empty = bars + 24, v_full = bars + 48, v_empty = bars + 64, q_full = bars + 80, q_empty = bars + 88,
+                   s_full = bars + 96, s_free = bars + 112, dp_full = bars + 128, ds_ready = bars + 136, done = bars + 152;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + B::kBars + 160);
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + B::kBars + 164);
 
     const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < B::kStages; ++i) {
-            mbar_init(full + 8 * i, 1);
-            mbar_init(empty + 8 * i, 1);
+        for (int i = 0; i < B::kLong; ++i) {
+            mbar_init(k_full + 8 * i, 1);
+            mbar_init(k_empty + 8 * i, 1);
+        }
+        for (int i = 0; i < B::kShort; ++i) {
+            mbar_init(v_full + 8 * i, 1);
+            mbar_init(v_empty + 8 * i, 1);
+            mbar_init(s_full + 8 * i, 1);
+            mbar_init(s_free + 8 * i, 8);
+            mbar_init(ds_ready + 8 * i, 8);
         }
         mbar_init(q_full, 1);
         mbar_init(q_empty, 1);
-        mbar_init(s_full, 1);
-        mbar_init(s_full + 8, 1);
         mbar_init(dp_full, 1);
-        mbar_init(ds_ready, 8);
         mbar_init(done, 1);
         *abort_flag = 0;
         fence_barrier_init();
@@ -941,7 +1051,7 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
         prefetch_tmap(&map_do);
     }
     if (warp == 1) {
-        tmem_alloc(bars + 132, kTmemCols);
+        tmem_alloc(bars + 164, kTmemCols);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -952,8 +1062,9 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
     const int64_t items = static_cast<int64_t>(warp_uniform(*p.num_blocks)) * p.heads;
 
     if (warp == 0) {
+        // q, do and the key tiles
         if (lane == 0) {
-            Ring r;
+            Ring k;
             uint32_t q_phase = 1u;
             bool ok = true;
             for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
@@ -966,84 +1077,124 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
                 load_tile<kD>(q_tile, &map_q, q_full, head, b.start + b.index * kTile);
                 load_tile<kD>(do_tile, &map_do, q_full, head, b.start + b.index * kTile);
                 for (int j = 0; ok && j <= b.index; ++j) {
-                    ok = mbar_wait(empty + 8 * r.stage, r.phase ^ 1u, abort_flag, p.status, 522);
+                    ok = mbar_wait(k_empty + 8 * k.stage, k.phase ^ 1u, abort_flag, p.status, 522);
                     if (!ok) break;
-                    const uint32_t bar = full + 8 * r.stage, dst = ring + r.stage * B::kStageBytes;
-                    mbar_expect_tx(bar, B::kStageBytes);
-                    load_tile<kD>(dst, &map_k, bar, kv_head, b.start + j * kTile);
-                    load_tile<kD>(dst + B::kTileBytes, &map_v, bar, kv_head, b.start + j * kTile);
-                    r.next(B::kStages);
+                    mbar_expect_tx(k_full + 8 * k.stage, B::kTileBytes);
+                    load_tile<kD>(k_ring + k.stage * B::kTileBytes, &map_k, k_full + 8 * k.stage, kv_head, b.start + j * kTile);
+                    k.next(B::kLong);
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 3) {
+        // value tiles
+        if (lane == 0) {
+            Ring v;
+            bool ok = true;
+            for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
+                const Block b = p.blocks[it / p.heads];
+                const int kv_head = static_cast<int>(it % p.heads) / p.group;
+                for (int j = 0; ok && j <= b.index; ++j) {
+                    ok = mbar_wait(v_empty + 8 * v.stage, v.phase ^ 1u, abort_flag, p.status, 541);
+                    if (!ok) break;
+                    mbar_expect_tx(v_full + 8 * v.stage, B::kTileBytes);
+                    load_tile<kD>(v_ring + v.stage * B::kTileBytes, &map_v, v_full + 8 * v.stage, kv_head, b.start + j * kTile);
+                    v.next(B::kShort);
                 }
             }
         }
         __syncwarp();
     } else if (warp == 1) {
+        // s = q k^T, up to two tiles ahead of what the compute warps have read
         const uint32_t idesc_s = make_idesc(kTile, kTile, false, false, p.ab_format);
-        const uint32_t idesc_d = make_idesc(kTile, kD, false, true, p.ab_format);
-        Ring r;
-        uint32_t q_phase = 0, ds_phase = 0, buf = 0;
+        Ring k, buf;
+        uint32_t q_phase = 0;
         bool ok = true;
         for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
             const Block b = load_block(p.blocks + it / p.heads);
             ok = mbar_wait_warp(q_full, q_phase, abort_flag, p.status, 523);
             if (!ok) break;
             q_phase ^= 1u;
-            for (int j = -1; ok && j <= b.index; ++j) {
-                // s of the next step; then dq += ds k and dp of the next step
-                const bool more = j < b.index;
-                const uint32_t cur = ring + r.stage * B::kStageBytes;
-                const uint32_t cur_empty = empty + 8 * r.stage;
-                Ring ahead = r;
-                if (j >= 0) ahead.next(B::kStages);
-                const uint32_t nxt = ring + ahead.stage * B::kStageBytes;
-                if (more) {
-                    ok = mbar_wait_warp(full + 8 * ahead.stage, ahead.phase, abort_flag, p.status, 524);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const int valid = b.len - (j + 1) * kTile;
-                    if (valid < kTile) {  // key rows of other sequences
-                        zero_tile_rows<kD>(nxt, valid, lane);
-                        fence_proxy_async();
-                        __syncwarp();
-                    }
-                    if (elect_one()) {
-                        // the step before last has read this buffer (its ds was waited for)
-                        mma_scores<kD>(tmem + buf * kTile, q_tile, nxt, idesc_s);
-                        umma_commit_cta1(s_full + 8 * buf);
-                    }
-                    __syncwarp();
-                    buf ^= 1u;
-                }
-                if (j >= 0) {
-                    ok = mbar_wait_warp(ds_ready, ds_phase, abort_flag, p.status, 525);
-                    if (!ok) break;
-                    ds_phase ^= 1u;
-                    tc_fence_after();
-                }
+            for (int j = 0; j <= b.index; ++j) {
+                ok = mbar_wait_warp(k_full + 8 * k.stage, k.phase, abort_flag, p.status, 524);
+                if (ok) ok = mbar_wait_warp(s_free + 8 * buf.stage, buf.phase ^ 1u, abort_flag, p.status, 542);
+                if (!ok) break;
+                tc_fence_after();
                 if (elect_one()) {
-                    if (j >= 0) {
-                        mma_rows(tm_dq, tm_dp, 64, cur, idesc_d, j > 0);
-                        umma_commit_cta1(cur_empty);
-                    }
+                    mma_scores<kD>(tmem + buf.stage * kTile, q_tile, k_ring + k.stage * B::kTileBytes, idesc_s);
+                    umma_commit_cta1(s_full + 8 * buf.stage);
+                }
+                __syncwarp();
+                k.next(B::kLong);
+                buf.next(2);
+            }
+        }
+    } else if (warp == 2) {
+        // dp = do v^T, dq += ds k
+        const uint32_t idesc_s = make_idesc(kTile, kTile, false, false, p.ab_format);
+        const uint32_t idesc_d = make_idesc(kTile, kD, false, true, p.ab_format);
+        Ring k, v;
+        uint32_t q_phase = 0, ds_phase = 0;
+        bool ok = true;
+        for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
+            const Block b = load_block(p.blocks + it / p.heads);
+            ok = mbar_wait_warp(q_full, q_phase, abort_flag, p.status, 543);
+            if (ok) ok = mbar_wait_warp(v_full + 8 * v.stage, v.phase, abort_flag, p.status, 544);
+            if (!ok) break;
+            q_phase ^= 1u;
+            tc_fence_after();
+            if (elect_one()) {
+                mma_scores<kD>(tm_dp, do_tile, v_ring + v.stage * B::kTileBytes, idesc_s);
+                umma_commit_cta1(dp_full);
+                umma_commit_cta1(v_empty + 8 * v.stage);
+            }
+            __syncwarp();
+            v.next(B::kShort);
+            for (int j = 0; j <= b.index; ++j) {
+                const bool more = j < b.index;
+                const uint32_t k_tile = k_ring + k.stage * B::kTileBytes;
+                ok = mbar_wait_warp(k_full + 8 * k.stage, k.phase, abort_flag, p.status, 545);
+                if (ok && more) ok = mbar_wait_warp(v_full + 8 * v.stage, v.phase, abort_flag, p.status, 546);
+                if (ok) ok = mbar_wait_warp(ds_ready, ds_phase, abort_flag, p.status, 525);
+                if (!ok) break;
+                const int valid = b.len - j * kTile;
+                if (valid < kTile) {  // rows of other sequences, which ds = 0 would meet; s has read the tile by now
+                    zero_tile_rows<kD>(k_tile, valid, lane);
+                    fence_proxy_async();
+                    __syncwarp();
+                }
+                tc_fence_after();
+                if (elect_one()) mma_rows_part(0, tm_dq, tm_dp, k_tile, idesc_d, j > 0);
+                __syncwarp();
+                ok = mbar_wait_warp(ds_ready + 8, ds_phase, abort_flag, p.status, 547);
+                if (!ok) break;
+                ds_phase ^= 1u;
+                tc_fence_after();
+                if (elect_one()) {
+                    mma_rows_part(1, tm_dq, tm_dp, k_tile, idesc_d, true);
+                    umma_commit_cta1(k_empty + 8 * k.stage);
                     if (more) {
-                        mma_scores<kD>(tm_dp, do_tile, nxt + B::kTileBytes, idesc_s);
+                        mma_scores<kD>(tm_dp, do_tile, v_ring + v.stage * B::kTileBytes, idesc_s);
                         umma_commit_cta1(dp_full);
+                        umma_commit_cta1(v_empty + 8 * v.stage);
                     } else {
                         umma_commit_cta1(done);
-                        umma_commit_cta1(q_empty);
+                        umma_commit_cta1(q_empty);  // every s has been read: ds of the last one is here
                     }
                 }
                 __syncwarp();
-                r = ahead;
+                k.next(B::kLong);
+                if (more) v.next(B::kShort);
             }
         }
-    } else if (warp >= 4) {
+    } else {
         const int half = (warp >> 2) - 1;          // key columns 64 half .. 64 half + 63
         const int row = (warp & 3) * 32 + lane;    // query row
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t dp_addr = tm_dp + lanes + half * 64;
         const float factor = ds_factor<T>(p);
-        uint32_t s_phase[2] = {0u, 0u}, dp_phase = 0, done_phase = 0, buf = 0;
+        Ring buf;
+        uint32_t dp_phase = 0, done_phase = 0;
         bool ok = true;
         for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
             const Block b = p.blocks[it / p.heads];
@@ -1053,49 +1204,47 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
             const int64_t stat = head * p.pad_rows + b.pad + query;
             const float neg_lse = valid ? -p.lse[stat] : 0.f;
             const float delta = valid ? p.delta[stat] : 0.f;
-            for (int j = 0; ok && j <= b.index; ++j) {
-                ok = mbar_wait(s_full + 8 * buf, s_phase[buf], abort_flag, p.status, 526);
+            for (int j = 0; j <= b.index; ++j) {
+                ok = mbar_wait(s_full + 8 * buf.stage, buf.phase, abort_flag, p.status, 526);
                 if (!ok) break;
-                s_phase[buf] ^= 1u;
                 tc_fence_after();
-                const uint32_t s_addr = tmem + lanes + buf * kTile + half * 64;
-                buf ^= 1u;
+                const uint32_t s_addr = tmem + lanes + buf.stage * kTile + half * 64;
+                uint32_t s[2][32];
+                tmem_ld32(s_addr, s[0]);
+                tmem_ld32(s_addr + 32, s[1]);
+                tmem_ld_wait();
+                tmem_tie32(s[0]);
+                tmem_tie32(s[1]);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_free + 8 * buf.stage);
+                buf.next(2);
                 float pr[64];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t s[32];
-                    tmem_ld32(s_addr + c * 32, s);
-                    tmem_ld_wait();
-                    tmem_tie32(s);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) pr[c * 32 + i] = ex2(fmaf(__uint_as_float(s[i]), p.scale_log2, neg_lse));
-                }
+                for (int c = 0; c < 64; ++c) pr[c] = ex2(fmaf(__uint_as_float(s[c >> 5][c & 31]), p.scale_log2, neg_lse));
                 ok = mbar_wait(dp_full, dp_phase, abort_flag, p.status, 527);
                 if (!ok) break;
                 dp_phase ^= 1u;
                 tc_fence_after();
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    uint32_t d[32];
-                    tmem_ld32(dp_addr + c * 32, d);
+                    uint32_t dp[32];
+                    tmem_ld32(dp_addr + c * 32, dp);
                     tmem_ld_wait();
-                    tmem_tie32(d);
+                    tmem_tie32(dp);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) pr[c * 32 + i] *= (__uint_as_float(d[i]) - delta) * factor;
+                    for (int i = 0; i < 32; ++i) pr[c * 32 + i] *= (__uint_as_float(dp[i]) - delta) * factor;
+                    if (j == b.index) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (half * 64 + c * 32 + i > row) pr[c * 32 + i] = 0.f;
+                    }
+                    store_packed32<T>(dp_addr + c * 16, pr + c * 32);
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(ds_ready + 8 * c);
                 }
-                if (j == b.index) {
-#pragma unroll
-                    for (int c = 0; c < 64; ++c)
-                        if (half * 64 + c > row) pr[c] = 0.f;
-                }
-                uint32_t packed[32];
-#pragma unroll
-                for (int c = 0; c < 32; ++c) packed[c] = pack2<T>(pr[2 * c], pr[2 * c + 1]);
-                tmem_st32(dp_addr, packed);
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(ds_ready);
             }
             if (!ok) break;
             ok = mbar_wait(done, done_phase, abort_flag, p.status, 528);
