@@ -57,6 +57,7 @@ struct Params {
     const Block* blocks;
     const int32_t* num_blocks;
     int heads, kv_heads, group, dim;
+    int dim_steps;     // ceil(dim / 16): what the products see of a head, zeros up to there
     int64_t pad_rows;  // entries of the padded row statistics per head
     float scale, scale_log2;
     void* out;         // forward: o
@@ -214,14 +215,15 @@ __device__ __forceinline__ constexpr uint64_t k_step(int kk) { return ((kk >> 2)
 __device__ __forceinline__ uint64_t desc_row_major(uint32_t tile) { return make_smem_desc(tile, kTile * 128, 1024); }
 __device__ __forceinline__ constexpr uint64_t row_step(int kk) { return (kk * 2048) >> 4; }
 
-// D[128, 128] = A B^T over the head dimension.
+// D[128, 128] = A B^T over the head dimension, `steps` times 16 of it.
 template <int kD>
-__device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a_tile, uint32_t b_tile, uint32_t idesc) {
+__device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a_tile, uint32_t b_tile, uint32_t idesc, int steps) {
     const uint64_t a = desc_k_major(a_tile), b = desc_k_major(b_tile);
 #pragma unroll
-    for (int kk = 0; kk < kD / 16; ++kk) umma_ss_cta1(d, a + k_step(kk), b + k_step(kk), idesc, kk != 0 ? 1u : 0u);
+    for (int kk = 0; kk < kD / 16; ++kk)
+        if (kk < steps) umma_ss_cta1(d, a + k_step(kk), b + k_step(kk), idesc, kk != 0 ? 1u : 0u);
 }
-// D[128, kD] (+)= A B over rows 16 kFirst .. 16 kLast - 1 of B; A in tensor memory, the part for the upper 64
+// D[128, head] (+)= A B over rows 16 kFirst .. 16 kLast - 1 of B; A in tensor memory, the part for the upper 64
 // rows `second` columns on.
 template <int kFirst = 0, int kLast = kTile / 16>
 __device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t second, uint32_t b_tile, uint32_t idesc, bool accumulate) {
@@ -363,7 +365,7 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         __syncwarp();
     } else if (warp == 1) {
         const uint32_t idesc_s = make_idesc(kTile, kTile, false, false, p.ab_format);
-        const uint32_t idesc_o = make_idesc(kTile, kD, false, true, p.ab_format);
+        const uint32_t idesc_o = make_idesc(kTile, p.dim_steps * 16, false, true, p.ab_format);
         Ring kv;
         uint32_t q_phase[2] = {0u, 0u}, p_phase[2] = {0u, 0u};
         bool ok = true;
@@ -381,7 +383,7 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 q_phase[t] ^= 1u;
                 tc_fence_after();
                 if (elect_one()) {
-                    mma_scores<kD>(tmem + t * kTile, q_tile + t * F::kTileBytes, ring + kv.stage * F::kTileBytes, idesc_s);
+                    mma_scores<kD>(tmem + t * kTile, q_tile + t * F::kTileBytes, ring + kv.stage * F::kTileBytes, idesc_s, p.dim_steps);
                     umma_commit_cta1(s_full + 8 * t);
                     if (first + t == 1) umma_commit_cta1(q_empty + 8 * t);
                 }
@@ -422,7 +424,7 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                         mma_rows<4, 8>(tmem + F::kO + t * kD, tmem + t * kTile, 32, v_tile, idesc_o, true);
                         if (j + 1 < count) {
                             // overwrites p, which the product just issued reads: the pipe runs them in order
-                            mma_scores<kD>(tmem + t * kTile, q_tile + t * F::kTileBytes, k_tile, idesc_s);
+                            mma_scores<kD>(tmem + t * kTile, q_tile + t * F::kTileBytes, k_tile, idesc_s, p.dim_steps);
                             umma_commit_cta1(s_full + 8 * t);
                             if (j + 2 == count) umma_commit_cta1(q_empty + 8 * t);
                         } else {
@@ -571,55 +573,83 @@ __device__ __forceinline__ float ds_factor<__half>(const Params& p) {
     return exp2f(static_cast<float>(min(max(14 - ilogbf(bound), -100), 100)));
 }
 
-// delta_i = o_i . do_i for every owned row and head, one warp per row and head; for fp16 also max |do| and
-// max |v| (over bit patterns, whose order does not depend on that of the atomics).
-template <typename T, typename IntT>
+// delta_i = o_i . do_i for every owned row and head; for fp16 also max |do| and max |v| (over bit patterns, whose
+// order does not depend on that of the atomics). A CTA takes kDeltaRows rows at a time: it looks their sequences up
+// once, then groups of kD / 8 lanes take one head of one row each, 16 bytes a lane.
+constexpr int kDeltaRows = 16;
+template <typename T, int kD, typename IntT>
 __global__ void __launch_bounds__(256)
 delta_kernel(const T* __restrict__ o, const T* __restrict__ d_o, const T* __restrict__ v, int64_t v_token, int64_t v_head,
              const IntT* __restrict__ cu, int64_t batch, int64_t total, float* __restrict__ delta, uint32_t* absmax, const Params p) {
     constexpr bool kHalf = std::is_same<T, __half>::value;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int kLanes = kD / 8;
+    __shared__ int at[kDeltaRows];  // entry in the row statistics, -1 for nobody's row
+    __shared__ uint32_t most[2];
+    if (threadIdx.x < 2) most[threadIdx.x] = 0;
+    const int sub = threadIdx.x % kLanes, slot = threadIdx.x / kLanes;
+    const bool in_head = sub * 8 < p.dim;
     uint32_t most_do = 0, most_v = 0;
-    for (int64_t row = blockIdx.x; row < total; row += gridDim.x) {
-        // last sequence that starts at or before the row
-        int64_t lo = 0, hi = batch - 1;
-        while (lo < hi) {
-            const int64_t mid = (lo + hi + 1) >> 1;
-            if (static_cast<int64_t>(cu[mid]) <= row) lo = mid; else hi = mid - 1;
+    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * kDeltaRows; row0 < total; row0 += static_cast<int64_t>(gridDim.x) * kDeltaRows) {
+        __syncthreads();
+        if (threadIdx.x < kDeltaRows) {
+            const int64_t row = row0 + threadIdx.x;
+            // last sequence that starts at or before the row
+            int64_t lo = 0, hi = batch - 1;
+            while (lo < hi) {
+                const int64_t mid = (lo + hi + 1) >> 1;
+                if (static_cast<int64_t>(cu[mid]) <= row) lo = mid; else hi = mid - 1;
+            }
+            int start, len;
+            sequence(cu, lo, total, &start, &len);
+            const bool owned = row >= start && row < static_cast<int64_t>(start) + len;
+            at[threadIdx.x] = owned ? pad_offset(start, lo) + static_cast<int>(row - start) : -1;
         }
-        int start, len;
-        sequence(cu, lo, total, &start, &len);
-        if (row < start || row >= static_cast<int64_t>(start) + len) continue;  // nobody's row
-        const int64_t at = pad_offset(start, lo) + (row - start);
-        for (int h = warp; h < p.heads; h += 8) {
-            const int64_t off = (row * p.heads + h) * p.dim;
+        __syncthreads();
+        const int pairs = kDeltaRows * p.heads;
+#pragma unroll 4
+        for (int i = slot; i < pairs; i += 256 / kLanes) {  // whole warps stay together: a warp holds 32 / kLanes pairs
+            const int r = i / p.heads, h = i - r * p.heads;
+            const int where = at[r];
             float sum = 0.f;
-            for (int c = lane * 4; c < p.dim; c += 128) {
-                const uint2 a = *reinterpret_cast<const uint2*>(o + off + c), b = *reinterpret_cast<const uint2*>(d_o + off + c);
-                const float2 a0 = unpack2<T>(a.x), a1 = unpack2<T>(a.y), b0 = unpack2<T>(b.x), b1 = unpack2<T>(b.y);
-                sum += a0.x * b0.x + a0.y * b0.y + a1.x * b1.x + a1.y * b1.y;
-                if (kHalf) most_do = max(most_do, __float_as_uint(fmaxf(fmaxf(fabsf(b0.x), fabsf(b0.y)), fmaxf(fabsf(b1.x), fabsf(b1.y)))));
+            if (where >= 0 && in_head) {
+                const int64_t off = ((row0 + r) * p.heads + h) * p.dim + sub * 8;
+                const uint4 a = __ldg(reinterpret_cast<const uint4*>(o + off)), b = __ldg(reinterpret_cast<const uint4*>(d_o + off));
+                const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float2 x = unpack2<T>(aw[q]), y = unpack2<T>(bw[q]);
+                    sum += x.x * y.x + x.y * y.y;
+                    if (kHalf) most_do = max(most_do, __float_as_uint(fmaxf(fabsf(y.x), fabsf(y.y))));
+                }
             }
 #pragma unroll
-            for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-            if (lane == 0) delta[h * p.pad_rows + at] = sum;
+            for (int w = kLanes / 2; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+            if (where >= 0 && sub == 0) delta[h * p.pad_rows + where] = sum;
         }
         if (kHalf) {
-            for (int h = warp; h < p.kv_heads; h += 8)
-                for (int c = lane * 4; c < p.dim; c += 128) {
-                    const uint2 a = *reinterpret_cast<const uint2*>(v + row * v_token + h * v_head + c);
-                    const float2 a0 = unpack2<T>(a.x), a1 = unpack2<T>(a.y);
-                    most_v = max(most_v, __float_as_uint(fmaxf(fmaxf(fabsf(a0.x), fabsf(a0.y)), fmaxf(fabsf(a1.x), fabsf(a1.y)))));
+            const int kv_pairs = kDeltaRows * p.kv_heads;
+            for (int i = slot; i < kv_pairs; i += 256 / kLanes) {
+                const int r = i / p.kv_heads, h = i - r * p.kv_heads;
+                if (at[r] < 0 || !in_head) continue;
+                const uint4 a = __ldg(reinterpret_cast<const uint4*>(v + (row0 + r) * v_token + h * v_head + sub * 8));
+                const uint32_t aw[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float2 x = unpack2<T>(aw[q]);
+                    most_v = max(most_v, __float_as_uint(fmaxf(fabsf(x.x), fabsf(x.y))));
                 }
+            }
         }
     }
     if (kHalf) {
         most_do = __reduce_max_sync(0xffffffffu, most_do);
         most_v = __reduce_max_sync(0xffffffffu, most_v);
-        if (lane == 0) {
-            atomicMax(&absmax[0], most_do);
-            atomicMax(&absmax[1], most_v);
+        if ((threadIdx.x & 31) == 0) {
+            atomicMax(&most[0], most_do);
+            atomicMax(&most[1], most_v);
         }
+        __syncthreads();
+        if (threadIdx.x < 2) atomicMax(&absmax[threadIdx.x], most[threadIdx.x]);
     }
 }
 
@@ -781,7 +811,7 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
     } else if (warp == 1) {
         // s^T = k q^T, dv += p^T do
         const uint32_t idesc_s = make_idesc(kTile, kTile, false, false, p.ab_format);
-        const uint32_t idesc_d = make_idesc(kTile, kD, false, true, p.ab_format);
+        const uint32_t idesc_d = make_idesc(kTile, p.dim_steps * 16, false, true, p.ab_format);
         Ring q, d;
         uint32_t kv_phase = 0, p_phase = 0;
         bool ok = true;
@@ -796,7 +826,7 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
             if (!ok) break;
             tc_fence_after();
             if (elect_one()) {
-                mma_scores<kD>(tm_s, k_tile, q_ring + q.stage * B::kTileBytes, idesc_s);
+                mma_scores<kD>(tm_s, k_tile, q_ring + q.stage * B::kTileBytes, idesc_s, p.dim_steps);
                 umma_commit_cta1(s_full);
             }
             __syncwarp();
@@ -827,7 +857,7 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
                 if (elect_one()) {
                     mma_rows_part(1, tm_dv, tm_s, do_tile, idesc_d, true);
                     if (more) {
-                        mma_scores<kD>(tm_s, k_tile, next_q, idesc_s);
+                        mma_scores<kD>(tm_s, k_tile, next_q, idesc_s, p.dim_steps);
                         umma_commit_cta1(s_full);
                     } else {
                         umma_commit_cta1(done);
@@ -842,7 +872,7 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
     } else if (warp == 2) {
         // dp^T = v do^T, dk += ds^T q
         const uint32_t idesc_s = make_idesc(kTile, kTile, false, false, p.ab_format);
-        const uint32_t idesc_d = make_idesc(kTile, kD, false, true, p.ab_format);
+        const uint32_t idesc_d = make_idesc(kTile, p.dim_steps * 16, false, true, p.ab_format);
         Ring q, d;
         uint32_t kv_phase = 0, ds_phase = 0;
         bool ok = true;
@@ -857,7 +887,7 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
             if (!ok) break;
             tc_fence_after();
             if (elect_one()) {
-                mma_scores<kD>(tm_dp, v_tile, do_ring + d.stage * B::kTileBytes, idesc_s);
+                mma_scores<kD>(tm_dp, v_tile, do_ring + d.stage * B::kTileBytes, idesc_s, p.dim_steps);
                 umma_commit_cta1(dp_full);
             }
             __syncwarp();
@@ -892,7 +922,7 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
                     umma_commit_cta1(q_empty + 8 * q.stage);
                     umma_commit_cta1(this_empty);
                     if (more) {
-                        mma_scores<kD>(tm_dp, v_tile, next_do, idesc_s);
+                        mma_scores<kD>(tm_dp, v_tile, next_do, idesc_s, p.dim_steps);
                         umma_commit_cta1(dp_full);
                     } else {
                         umma_commit_cta1(done);
@@ -1121,7 +1151,7 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
                 if (!ok) break;
                 tc_fence_after();
                 if (elect_one()) {
-                    mma_scores<kD>(tmem + buf.stage * kTile, q_tile, k_ring + k.stage * B::kTileBytes, idesc_s);
+                    mma_scores<kD>(tmem + buf.stage * kTile, q_tile, k_ring + k.stage * B::kTileBytes, idesc_s, p.dim_steps);
                     umma_commit_cta1(s_full + 8 * buf.stage);
                 }
                 __syncwarp();
@@ -1132,7 +1162,7 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
     } else if (warp == 2) {
         // dp = do v^T, dq += ds k
         const uint32_t idesc_s = make_idesc(kTile, kTile, false, false, p.ab_format);
-        const uint32_t idesc_d = make_idesc(kTile, kD, false, true, p.ab_format);
+        const uint32_t idesc_d = make_idesc(kTile, p.dim_steps * 16, false, true, p.ab_format);
         Ring k, v;
         uint32_t q_phase = 0, ds_phase = 0;
         bool ok = true;
@@ -1144,7 +1174,7 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
             q_phase ^= 1u;
             tc_fence_after();
             if (elect_one()) {
-                mma_scores<kD>(tm_dp, do_tile, v_ring + v.stage * B::kTileBytes, idesc_s);
+                mma_scores<kD>(tm_dp, do_tile, v_ring + v.stage * B::kTileBytes, idesc_s, p.dim_steps);
                 umma_commit_cta1(dp_full);
                 umma_commit_cta1(v_empty + 8 * v.stage);
             }
@@ -1174,7 +1204,7 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
                     mma_rows_part(1, tm_dq, tm_dp, k_tile, idesc_d, true);
                     umma_commit_cta1(k_empty + 8 * k.stage);
                     if (more) {
-                        mma_scores<kD>(tm_dp, do_tile, v_ring + v.stage * B::kTileBytes, idesc_s);
+                        mma_scores<kD>(tm_dp, do_tile, v_ring + v.stage * B::kTileBytes, idesc_s, p.dim_steps);
                         umma_commit_cta1(dp_full);
                         umma_commit_cta1(v_empty + 8 * v.stage);
                     } else {
@@ -1361,6 +1391,7 @@ static int check_call(const Call& c) {
 static Params common_params(const Call& c) {
     Params p{};
     p.heads = c.heads, p.kv_heads = c.kv_heads, p.group = c.heads / c.kv_heads, p.dim = c.dim;
+    p.dim_steps = static_cast<int>(ceil_div(c.dim, 16));
     p.pad_rows = (c.total / kTile + c.batch + 1) * kTile;
     p.scale = c.scale;
     p.scale_log2 = c.scale * 1.4426950408889634f;  // log2(e): exp(scale s) = 2^(scale_log2 s)
@@ -1411,14 +1442,14 @@ static int run_backward(const Call& c, const void* out, const void* d_out, const
     if (status != XMA_OK || c.batch == 0) return status;
     Params p = common_params(c);
     p.lse = const_cast<float*>(lse), p.delta = delta, p.dq = dq, p.dk = dk, p.dv = dv, p.absmax = w.absmax;
-    const int64_t most = static_cast<int64_t>(sm_count()) * 8;
-    const unsigned rows = static_cast<unsigned>(c.total < most ? c.total : most);
+    const int64_t chunks = ceil_div(c.total, kDeltaRows), most = static_cast<int64_t>(sm_count()) * 8;
+    const unsigned grid = static_cast<unsigned>(chunks < most ? chunks : most);
     if (c.cu_is_int64)
-        delta_kernel<T, int64_t><<<rows, 256, 0, c.stream>>>(
+        delta_kernel<T, kD, int64_t><<<grid, 256, 0, c.stream>>>(
             static_cast<const T*>(out), static_cast<const T*>(d_out), static_cast<const T*>(c.v), c.v_token, c.v_head,
             static_cast<const int64_t*>(c.cu), c.batch, c.total, delta, w.absmax, p);
     else
-        delta_kernel<T, int32_t><<<rows, 256, 0, c.stream>>>(
+        delta_kernel<T, kD, int32_t><<<grid, 256, 0, c.stream>>>(
             static_cast<const T*>(out), static_cast<const T*>(d_out), static_cast<const T*>(c.v), c.v_token, c.v_head,
             static_cast<const int32_t*>(c.cu), c.batch, c.total, delta, w.absmax, p);
     status = launch_status();

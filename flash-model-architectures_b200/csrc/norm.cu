@@ -30,13 +30,14 @@ constexpr int kGateChannel = 1;  // [H], a parameter
 constexpr int kGateToken = 2;    // [rows], one factor per row
 constexpr int kGateFull = 3;     // [rows, H]
 
-constexpr int kMaxThreads = 512;           // threads of a backward CTA that compute (a producer warp comes on top)
-constexpr int kForwardThreads = 256;
-constexpr int kForwardMaxHidden = 16384;   // longer rows are read once per pass
-constexpr int kRingMaxHidden = 8192;       // longer rows take the two-kernel backward
-constexpr int kPartials = XMA_NORM_PARTIALS;
+constexpr int kForwardThreads = 256;       // plain forward: threads of a CTA with short rows
+constexpr int kForwardMaxHidden = 16384;   // plain forward: longer rows are read once per pass
+constexpr int kRingThreads = 512;          // ring kernels: threads of a CTA, at most
+constexpr int kRingMaxHidden = 8192;
 constexpr uint32_t kRingSmem = 220 * 1024;
-constexpr int kMaxStages = 4;
+constexpr int kMaxStages = 6;
+constexpr int kRingMinChunks = 3;          // forward: chunks a CTA has to have for the ring to pay
+constexpr int kPartials = XMA_NORM_PARTIALS;
 
 struct Params {
     const void* x;
@@ -91,6 +92,35 @@ __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
     *reinterpret_cast<uint4*>(p) = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
 }
 
+// Eight elements as four pairs.
+__device__ __forceinline__ void load8(const float* p, f32x2 (&f)[4]) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    f[0] = make_f32x2(a.x, a.y), f[1] = make_f32x2(a.z, a.w), f[2] = make_f32x2(b.x, b.y), f[3] = make_f32x2(b.z, b.w);
+}
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, f32x2 (&f)[4]) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float2 t = unpack2<T>(w[j]);
+        f[j] = make_f32x2(t.x, t.y);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const f32x2 (&f)[4]) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) split_f32x2(f[j], v[2 * j], v[2 * j + 1]);
+    store8(p, v);
+}
+__device__ __forceinline__ f32x2 both(float v) { return make_f32x2(v, v); }
+__device__ __forceinline__ float total(f32x2 v) {
+    float a, b;
+    split_f32x2(v, a, b);
+    return a + b;
+}
+
 // Eight elements of a row: element j of vector `v` of thread `t` (of `group` threads) is column
 // column<kVec>(v, t, group, j). Vectorised rows give a thread eight neighbours (one or two 16-byte
 // accesses); others give neighbouring threads neighbouring elements, so that any row start and any
@@ -140,6 +170,19 @@ __device__ __forceinline__ void load_param(const void* p, bool f32, int v, int t
         load_cols<kVec>(static_cast<const float*>(p), v, t, group, hidden, f);
     } else {
         load_cols<kVec>(static_cast<const T*>(p), v, t, group, hidden, f);
+    }
+}
+
+// Eight neighbours of a parameter (ones where there is none).
+template <typename T>
+__device__ __forceinline__ void param8(const void* p, bool f32, int c, f32x2 (&f)[4]) {
+    if (p == nullptr) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = both(1.f);
+    } else if (f32) {
+        load8(static_cast<const float*>(p) + c, f);
+    } else {
+        load8(static_cast<const T*>(p) + c, f);
     }
 }
 
@@ -311,6 +354,252 @@ forward_long_kernel(const Params p) {
 }
 
 // ---------------------------------------------------------------------------------------------
+// Ring kernels: persistent CTAs whose rows come through shared memory
+// ---------------------------------------------------------------------------------------------
+
+// `slots` groups of `group` threads share a CTA; a thread keeps its columns (kVpt vectors of eight) and takes
+// kRows rows of every chunk of slots * kRows rows. Chunks are copied whole (bulk copies, one per tensor) into a
+// ring of stages, so what is in flight does not depend on registers and every row can be read twice. The
+// CTA's barriers, which a row sum needs anyway, also say when a stage is free: thread 0 refills it.
+struct RingLayout {
+    int slots, group, stages;
+    uint32_t stage_bytes;
+    uint32_t dy, d_stream, s, x, gate, residual;  // offsets inside a stage
+    uint32_t weight, post, channel_gate;          // offsets of the parameters' copies (rows of more than one vector a thread)
+    uint32_t ring;                                // offset of stage 0
+    uint32_t total;
+};
+constexpr uint32_t kRingHeader = 128 + 2 * 128 * 4;  // barriers and two scratches of 128 floats
+
+struct RingState {
+    uint32_t full;  // barriers
+    volatile int* abort_flag;
+    float* scratch;
+    int stage = 0;
+    uint32_t phase = 0, flip = 0;
+    __device__ __forceinline__ void next(int stages) {
+        if (++stage == stages) {
+            stage = 0;
+            phase ^= 1u;
+        }
+    }
+    // After a wait that ran out: the copies in flight land, or get the same time once more, before the CTA ends.
+    __device__ __forceinline__ void drain(int stages) const {
+        const uint64_t begin = global_timer_ns();
+        for (int i = 0; i < stages; ++i)
+            while (!mbar_try_wait(full + 8 * i, i < stage ? phase ^ 1u : phase) && global_timer_ns() - begin < kWaitLimitNs) {}
+    }
+};
+
+// Sums of kCount values (a power of two up to 8) over the group's threads, known to each of them; one CTA barrier.
+template <int kCount>
+__device__ __forceinline__ void ring_sum(float (&v)[kCount], RingState& st, int first_warp, int warps) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float* scratch = st.scratch + st.flip * 128;
+    st.flip ^= 1u;
+    // halve the values while lanes are added up: lane bits 16, 8, 4 come to select the value
+    int index = 0;
+    int off = 16;
+#pragma unroll
+    for (int n = kCount; n > 1; n >>= 1, off >>= 1) {
+        const bool upper = lane & off;
+#pragma unroll
+        for (int i = 0; i < n / 2; ++i) {
+            const float give = upper ? v[i] : v[i + n / 2], keep = upper ? v[i + n / 2] : v[i];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, give, off);
+        }
+        if (upper) index += n / 2;
+    }
+#pragma unroll
+    for (; off > 0; off >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], off);
+    if ((lane & (32 / kCount - 1)) == 0) scratch[warp * kCount + index] = v[0];
+    __syncthreads();
+    const int count = warps * kCount;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < (16 * kCount + 31) / 32; ++i) {
+        const int at = i * 32 + lane;
+        if (at < count) sum += scratch[first_warp * kCount + at];
+    }
+#pragma unroll
+    for (int o = 16; o >= kCount; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) v[i] = __shfl_sync(0xffffffffu, sum, i);
+}
+
+// One tensor's share of a chunk.
+__device__ __forceinline__ void ring_copy(uint32_t dst, const void* src, int64_t at, int64_t bytes, uint32_t bar) {
+    if (src != nullptr) bulk_load(dst, static_cast<const uint8_t*>(src) + at, static_cast<uint32_t>(bytes), bar);
+}
+__device__ __forceinline__ int64_t ring_bytes(const void* src, int64_t bytes) { return src != nullptr ? bytes : 0; }
+
+// The parameters' copies in shared memory, in their own types.
+template <typename T>
+__device__ __forceinline__ void copy_param(uint8_t* dst, const void* p, bool f32, int hidden) {
+    if (p == nullptr) return;
+    for (int c = threadIdx.x; c < hidden; c += blockDim.x) {
+        if (f32) reinterpret_cast<float*>(dst)[c] = static_cast<const float*>(p)[c];
+        else reinterpret_cast<T*>(dst)[c] = static_cast<const T*>(p)[c];
+    }
+}
+
+template <typename T, typename R, int kVpt, int kRows>
+__global__ void __launch_bounds__(kRingThreads, 1)
+forward_ring_kernel(const Params p, const RingLayout lay) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    RingState st;
+    st.full = smem_u32(smem);
+    st.abort_flag = reinterpret_cast<volatile int*>(smem + 64);
+    st.scratch = reinterpret_cast<float*>(smem + 128);
+    const int group = lay.group, warps = group >> 5;
+    const int slot = threadIdx.x / group, t = threadIdx.x - slot * group;
+    const int first_warp = slot * warps;
+    const int per_chunk = lay.slots * kRows;
+    const int64_t chunks = (p.rows + per_chunk - 1) / per_chunk;
+    const bool full_gate = p.gate_mode == kGateFull, channel_gate = p.gate_mode == kGateChannel;
+    const float inv_h = 1.f / static_cast<float>(p.hidden);
+    const void* gate_rows = full_gate ? p.gate : nullptr;
+
+    const auto load = [&](int64_t chunk, int stage) {
+        if (chunk >= chunks) return;
+        const int64_t row0 = chunk * per_chunk;
+        const int64_t count = min(static_cast<int64_t>(per_chunk), p.rows - row0) * p.hidden;
+        const uint32_t bar = st.full + 8 * stage, dst = smem_u32(smem) + lay.ring + stage * lay.stage_bytes;
+        const int64_t at = row0 * p.hidden, bt = count * static_cast<int64_t>(sizeof(T)), br = count * static_cast<int64_t>(sizeof(R));
+        mbar_expect_tx(bar, static_cast<uint32_t>(bt + ring_bytes(p.residual, br) + ring_bytes(gate_rows, bt)));
+        ring_copy(dst + lay.x, p.x, at * sizeof(T), bt, bar);
+        ring_copy(dst + lay.residual, p.residual, at * sizeof(R), br, bar);
+        ring_copy(dst + lay.gate, gate_rows, at * sizeof(T), bt, bar);
+    };
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < lay.stages; ++i) mbar_init(st.full + 8 * i, 1);
+        *st.abort_flag = 0;
+        fence_barrier_init();
+        for (int i = 0; i < lay.stages; ++i) load(blockIdx.x + static_cast<int64_t>(i) * gridDim.x, i);
+    }
+    // What a column is multiplied with: in registers for one vector a thread, else in shared memory.
+    f32x2 w_reg[4], c_reg[4];
+    if (kVpt == 1) {
+        const int c = t * 8;
+        if (c < p.hidden) {
+            param8<T>(p.weight, p.weight_f32, c, w_reg);
+            param8<T>(p.post, p.post_f32, c, c_reg);
+            if (channel_gate) {
+                f32x2 g[4];
+                param8<T>(p.gate, p.gate_f32, c, g);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) c_reg[j] = mul_f32x2(c_reg[j], g[j]);
+            }
+        }
+    } else {
+        copy_param<T>(smem + lay.weight, p.weight, p.weight_f32, p.hidden);
+        copy_param<T>(smem + lay.post, p.post, p.post_f32, p.hidden);
+        if (channel_gate) copy_param<T>(smem + lay.channel_gate, p.gate, p.gate_f32, p.hidden);
+    }
+    __syncthreads();
+
+    for (int64_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+        const int64_t row0 = chunk * per_chunk + slot * kRows;
+        if (!mbar_wait(st.full + 8 * st.stage, st.phase, st.abort_flag, p.status, 403)) {
+            st.drain(lay.stages);
+            break;
+        }
+        const uint8_t* stage = smem + lay.ring + st.stage * lay.stage_bytes;
+        f32x2 s[kRows][kVpt][4];
+        float sums[kRows], scale[kRows];
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+            const T* x = reinterpret_cast<const T*>(stage + lay.x) + (slot * kRows + r) * p.hidden;
+            f32x2 sum = both(0.f);
+#pragma unroll
+            for (int v = 0; v < kVpt; ++v) {
+                const int c = (v * group + t) * 8;
+                if (c < p.hidden) load8(x + c, s[r][v]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (c >= p.hidden) s[r][v][j] = both(0.f);
+                    sum = fma_f32x2(mul_f32x2(s[r][v][j], both(inv_h)), s[r][v][j], sum);
+                }
+            }
+            sums[r] = total(sum);
+            scale[r] = p.residual != nullptr && row0 + r < p.rows ? p.multiplier * token_gate<T>(p, row0 + r) : 1.f;
+        }
+        if (p.residual != nullptr) {
+            if (p.post != nullptr) {
+                ring_sum<kRows>(sums, st, first_warp, warps);
+#pragma unroll
+                for (int r = 0; r < kRows; ++r) {
+                    const float rp = rsqrtf(sums[r] + p.eps);
+                    scale[r] *= rp;
+                    if (t == 0 && p.rp != nullptr && row0 + r < p.rows) p.rp[row0 + r] = rp;
+                }
+            }
+#pragma unroll
+            for (int v = 0; v < kVpt; ++v) {
+                const int c = (v * group + t) * 8;
+                f32x2 f[4];
+                if (kVpt > 1 && c < p.hidden) {
+                    param8<T>(p.post ? smem + lay.post : nullptr, p.post_f32, c, f);
+                    if (channel_gate) {
+                        f32x2 g[4];
+                        param8<T>(smem + lay.channel_gate, p.gate_f32, c, g);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) f[j] = mul_f32x2(f[j], g[j]);
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < kRows; ++r) {
+                    if (c >= p.hidden) continue;
+                    const int off = (slot * kRows + r) * p.hidden + c;
+                    f32x2 res[4];
+                    load8(reinterpret_cast<const R*>(stage + lay.residual) + off, res);
+                    if (full_gate) {
+                        f32x2 g[4];
+                        load8(reinterpret_cast<const T*>(stage + lay.gate) + off, g);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) s[r][v][j] = mul_f32x2(s[r][v][j], g[j]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        s[r][v][j] = fma_f32x2(mul_f32x2(s[r][v][j], kVpt > 1 ? f[j] : c_reg[j]), both(scale[r]), res[j]);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) {
+                f32x2 sum = both(0.f);
+#pragma unroll
+                for (int v = 0; v < kVpt; ++v)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) sum = fma_f32x2(mul_f32x2(s[r][v][j], both(inv_h)), s[r][v][j], sum);
+                sums[r] = total(sum);
+            }
+        }
+        ring_sum<kRows>(sums, st, first_warp, warps);
+        // every thread has read the stage: it can take the chunk after the ones in flight
+        if (threadIdx.x == 0) load(chunk + static_cast<int64_t>(lay.stages) * gridDim.x, st.stage);
+        st.next(lay.stages);
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+            if (row0 + r >= p.rows) continue;
+            const float rs = rsqrtf(sums[r] + p.eps);
+            if (t == 0 && p.rs != nullptr) p.rs[row0 + r] = rs;
+            const int64_t base = (row0 + r) * p.hidden;
+#pragma unroll
+            for (int v = 0; v < kVpt; ++v) {
+                const int c = (v * group + t) * 8;
+                if (c >= p.hidden) continue;
+                if (p.residual != nullptr) store8(static_cast<R*>(p.s_out) + base + c, s[r][v]);
+                f32x2 f[4];
+                if (kVpt > 1) param8<T>(p.weight ? smem + lay.weight : nullptr, p.weight_f32, c, f);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) f[j] = mul_f32x2(mul_f32x2(s[r][v][j], both(rs)), kVpt > 1 ? f[j] : w_reg[j]);
+                store8(static_cast<T*>(p.y) + base + c, f);
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
 // Backward
 // ---------------------------------------------------------------------------------------------
 
@@ -331,300 +620,247 @@ __device__ __forceinline__ RowScale row_scale(const Params& p, const float (&sum
     r.k_s = rs * rs * sums[0] * inv_h;
     const float c_ds = rs * sums[1] - rs * r.k_s * sums[2] + sums[3];
     r.m = p.multiplier * token;
-    r.k_x = r.m * rp * c_ds * inv_h;
+    r.k_x = p.post != nullptr ? r.m * rp * c_ds * inv_h : 0.f;
     r.d_token_gate = p.multiplier * rp * c_ds;
     return r;
 }
 
-// Shared-memory layout of the ring kernel: parameters, reduction scratch and barriers, then the stages.
-struct RingLayout {
-    int slots;            // rows a CTA works on at once
-    int group;            // threads per row
-    int stages;
-    uint32_t stage_bytes;
-    uint32_t dy, d_stream, s, x, gate;  // offsets inside a stage
-    uint32_t post, channel_gate;        // offsets of the parameters (the weight's is 0)
-    uint32_t ring;                      // offset of stage 0
-    uint32_t total;
-};
-
-constexpr uint32_t kRingHeader = 1024;  // barriers and two reduction scratches of 16 warps x 4 floats
-
-// Persistent CTAs walk over the rows; a producer warp copies whole rows (bulk copies) into a ring of
-// stages ahead of the warps that compute, so the loads in flight do not depend on registers, and the
-// row's second pass reads shared memory. The gradients of the parameters stay in registers (a thread
-// keeps its columns) until the CTA's last row and leave as one partial row per CTA, summed in a fixed
-// order by sum_kernel.
-template <typename T, typename R, int kVpt>
-__global__ void __launch_bounds__(kMaxThreads + 32, 1)
+// The parameters' gradients stay in registers (a thread keeps its columns) until the CTA's last row and leave as
+// one partial row per CTA, summed in a fixed order by sum_kernel. kX: a post norm or a gate is there, so x is
+// read; kFull: the gate has the shape of x.
+template <typename T, typename R, int kVpt, int kRows, bool kX, bool kFull>
+__global__ void __launch_bounds__(kRingThreads, 1)
 backward_ring_kernel(const Params p, const RingLayout lay) {
+    constexpr int kSums = kX ? 4 : 1;
     extern __shared__ __align__(128) uint8_t smem[];
-    const uint32_t base_addr = smem_u32(smem);
-    const uint32_t full_bar = base_addr, empty_bar = base_addr + 64;
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + 128);
-    float* scratch = reinterpret_cast<float*>(smem + 256);  // [2][16 warps][4]
-    uint8_t* params_at = smem + kRingHeader;
-    uint8_t* ring = smem + lay.ring;
-    const int group = lay.group, slots = lay.slots;
-    const int compute_threads = group * slots;
-    const int64_t chunks = (p.rows + slots - 1) / slots;
-    const bool has_x = p.x != nullptr;
-
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < lay.stages; ++i) {
-            mbar_init(full_bar + 8 * i, 1);
-            mbar_init(empty_bar + 8 * i, compute_threads / 32);
-        }
-        *abort_flag = 0;
-        fence_barrier_init();
-    }
-    // parameters into shared memory, in their own type
-    for (int c = threadIdx.x; c < p.hidden; c += blockDim.x) {
-        if (p.weight != nullptr) {
-            if (p.weight_f32) reinterpret_cast<float*>(params_at)[c] = static_cast<const float*>(p.weight)[c];
-            else reinterpret_cast<T*>(params_at)[c] = static_cast<const T*>(p.weight)[c];
-        }
-        if (p.post != nullptr) {
-            if (p.post_f32) reinterpret_cast<float*>(params_at + lay.post)[c] = static_cast<const float*>(p.post)[c];
-            else reinterpret_cast<T*>(params_at + lay.post)[c] = static_cast<const T*>(p.post)[c];
-        }
-        if (p.gate_mode == kGateChannel) {
-            if (p.gate_f32) reinterpret_cast<float*>(params_at + lay.channel_gate)[c] = static_cast<const float*>(p.gate)[c];
-            else reinterpret_cast<T*>(params_at + lay.channel_gate)[c] = static_cast<const T*>(p.gate)[c];
-        }
-    }
-    __syncthreads();
-
-    if (threadIdx.x >= compute_threads) {
-        // ------------------------------ producer warp ------------------------------
-        if (threadIdx.x == compute_threads) {
-            int stage = 0;
-            uint32_t phase = 0;
-            bool ok = true;
-            for (int64_t ch = blockIdx.x; ok && ch < chunks; ch += gridDim.x) {
-                ok = mbar_wait(empty_bar + 8 * stage, phase ^ 1u, abort_flag, p.status, 401);
-                if (!ok) break;
-                const int64_t row0 = ch * slots;
-                const uint32_t count = static_cast<uint32_t>(min(static_cast<int64_t>(slots), p.rows - row0) * p.hidden);
-                const int64_t at = row0 * p.hidden;
-                const uint32_t dst = base_addr + lay.ring + stage * lay.stage_bytes;
-                const uint32_t bar = full_bar + 8 * stage;
-                const uint32_t bytes_t = count * sizeof(T), bytes_r = count * sizeof(R);
-                uint32_t expect = bytes_r;
-                if (p.dy != nullptr) expect += bytes_t;
-                if (p.d_stream != nullptr) expect += bytes_r;
-                if (has_x) expect += bytes_t;
-                if (p.gate_mode == kGateFull) expect += bytes_t;
-                mbar_expect_tx(bar, expect);
-                bulk_load(dst + lay.s, static_cast<const R*>(p.s) + at, bytes_r, bar);
-                if (p.dy != nullptr) bulk_load(dst + lay.dy, static_cast<const T*>(p.dy) + at, bytes_t, bar);
-                if (p.d_stream != nullptr) bulk_load(dst + lay.d_stream, static_cast<const R*>(p.d_stream) + at, bytes_r, bar);
-                if (has_x) bulk_load(dst + lay.x, static_cast<const T*>(p.x) + at, bytes_t, bar);
-                if (p.gate_mode == kGateFull) bulk_load(dst + lay.gate, static_cast<const T*>(p.gate) + at, bytes_t, bar);
-                if (++stage == lay.stages) {
-                    stage = 0;
-                    phase ^= 1u;
-                }
-            }
-            // Given up: the copies in flight land before the CTA ends (a stage's last load completed the
-            // phase before the one that the next load would).
-            for (int i = 0; !ok && i < lay.stages; ++i) {
-                const uint32_t last = i < stage ? phase : phase ^ 1u;
-                const uint64_t begin = global_timer_ns();
-                while (!mbar_try_wait(full_bar + 8 * i, last) && global_timer_ns() - begin < kWaitLimitNs) {}
-            }
-        }
-        __syncwarp();
-        __syncthreads();  // the one after the compute warps' loop
-        return;
-    }
-
-    // ------------------------------ compute warps ------------------------------
+    RingState st;
+    st.full = smem_u32(smem);
+    st.abort_flag = reinterpret_cast<volatile int*>(smem + 64);
+    st.scratch = reinterpret_cast<float*>(smem + 128);
+    const int group = lay.group, warps = group >> 5;
     const int slot = threadIdx.x / group, t = threadIdx.x - slot * group;
-    const int lane = threadIdx.x & 31;
-    float* my_scratch = scratch + slot * (group >> 5) * 4;
-    float acc_w[kVpt][8], acc_p[kVpt][8], acc_g[kVpt][8];
+    const int first_warp = slot * warps;
+    const int per_chunk = lay.slots * kRows;
+    const int64_t chunks = (p.rows + per_chunk - 1) / per_chunk;
+    const bool channel_gate = kX && p.gate_mode == kGateChannel;
+    const void* gate_rows = kFull ? p.gate : nullptr;
+
+    const auto load = [&](int64_t chunk, int stage) {
+        if (chunk >= chunks) return;
+        const int64_t row0 = chunk * per_chunk;
+        const int64_t count = min(static_cast<int64_t>(per_chunk), p.rows - row0) * p.hidden;
+        const uint32_t bar = st.full + 8 * stage, dst = smem_u32(smem) + lay.ring + stage * lay.stage_bytes;
+        const int64_t at = row0 * p.hidden, bt = count * static_cast<int64_t>(sizeof(T)), br = count * static_cast<int64_t>(sizeof(R));
+        mbar_expect_tx(bar, static_cast<uint32_t>(br + ring_bytes(p.dy, bt) + ring_bytes(p.d_stream, br) + ring_bytes(p.x, bt) +
+                                                  ring_bytes(gate_rows, bt)));
+        ring_copy(dst + lay.s, p.s, at * sizeof(R), br, bar);
+        ring_copy(dst + lay.dy, p.dy, at * sizeof(T), bt, bar);
+        ring_copy(dst + lay.d_stream, p.d_stream, at * sizeof(R), br, bar);
+        ring_copy(dst + lay.x, p.x, at * sizeof(T), bt, bar);
+        ring_copy(dst + lay.gate, gate_rows, at * sizeof(T), bt, bar);
+    };
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < lay.stages; ++i) mbar_init(st.full + 8 * i, 1);
+        *st.abort_flag = 0;
+        fence_barrier_init();
+        for (int i = 0; i < lay.stages; ++i) load(blockIdx.x + static_cast<int64_t>(i) * gridDim.x, i);
+    }
+    // Parameters: in registers for one vector a thread, else in shared memory.
+    f32x2 w_reg[4], post_reg[4], gate_reg[4];
+    if (kVpt == 1) {
+        const int c = t * 8;
+        if (c < p.hidden) {
+            param8<T>(p.weight, p.weight_f32, c, w_reg);
+            if (kX) param8<T>(p.post, p.post_f32, c, post_reg);
+            if (kX && !kFull) param8<T>(channel_gate ? p.gate : nullptr, p.gate_f32, c, gate_reg);
+        }
+    } else {
+        copy_param<T>(smem + lay.weight, p.weight, p.weight_f32, p.hidden);
+        copy_param<T>(smem + lay.post, p.post, p.post_f32, p.hidden);
+        if (channel_gate) copy_param<T>(smem + lay.channel_gate, p.gate, p.gate_f32, p.hidden);
+    }
+    const auto weight8 = [&](int c, f32x2 (&f)[4]) {
+        if (kVpt > 1) {
+            param8<T>(p.weight ? smem + lay.weight : nullptr, p.weight_f32, c, f);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[j] = w_reg[j];
+        }
+    };
+    const auto post8 = [&](int c, f32x2 (&f)[4]) {
+        if (kVpt > 1) {
+            param8<T>(p.post ? smem + lay.post : nullptr, p.post_f32, c, f);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[j] = post_reg[j];
+        }
+    };
+    const auto gate8 = [&](const T* gate_row, int c, f32x2 (&f)[4]) {
+        if (kFull) {
+            load8(gate_row + c, f);
+        } else if (kVpt > 1) {
+            param8<T>(channel_gate ? smem + lay.channel_gate : nullptr, p.gate_f32, c, f);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[j] = gate_reg[j];
+        }
+    };
+    f32x2 acc_w[kVpt][4], acc_p[kVpt][4], acc_g[kVpt][4];
 #pragma unroll
     for (int v = 0; v < kVpt; ++v)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc_w[v][j] = acc_p[v][j] = acc_g[v][j] = 0.f;
+        for (int j = 0; j < 4; ++j) acc_w[v][j] = acc_p[v][j] = acc_g[v][j] = both(0.f);
+    __syncthreads();
 
-    int stage = 0;
-    uint32_t phase = 0, flip = 0;
-    for (int64_t ch = blockIdx.x; ch < chunks; ch += gridDim.x) {
-        const int64_t row = ch * slots + slot;
-        const bool valid = row < p.rows;  // uniform in a row's group
-        float rs = 0.f, rp = 1.f, token = 1.f;
-        if (valid) {
-            rs = p.rs[row];
-            if (p.post != nullptr) rp = p.rp[row];
-            token = token_gate<T>(p, row);
+    int previous = -1;
+    for (int64_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+        const int64_t row0 = chunk * per_chunk + slot * kRows;
+        float rs[kRows], rp[kRows], token[kRows];
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+            const bool valid = row0 + r < p.rows;  // the same in the whole group
+            rs[r] = valid ? p.rs[row0 + r] : 0.f;
+            rp[r] = valid && kX && p.post != nullptr ? p.rp[row0 + r] : 1.f;
+            token[r] = valid && kX ? token_gate<T>(p, row0 + r) : 1.f;
         }
-        if (!mbar_wait(full_bar + 8 * stage, phase, abort_flag, p.status, 402)) break;
-        const uint8_t* st = ring + stage * lay.stage_bytes;
-        const int off = slot * p.hidden;
-        const T* dy = reinterpret_cast<const T*>(st + lay.dy) + off;
-        const R* dd = reinterpret_cast<const R*>(st + lay.d_stream) + off;
-        const R* sr = reinterpret_cast<const R*>(st + lay.s) + off;
-        const T* xr = reinterpret_cast<const T*>(st + lay.x) + off;
-        const T* gr = reinterpret_cast<const T*>(st + lay.gate) + off;
-
-        float sums[4] = {0.f, 0.f, 0.f, 0.f};
-        if (valid) {
+        if (!mbar_wait(st.full + 8 * st.stage, st.phase, st.abort_flag, p.status, 402)) {
+            st.drain(lay.stages);
+            break;
+        }
+        const uint8_t* stage = smem + lay.ring + st.stage * lay.stage_bytes;
+        float sums[kRows * kSums];
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+            const int off = (slot * kRows + r) * p.hidden;
+            f32x2 sum[kSums];
+#pragma unroll
+            for (int i = 0; i < kSums; ++i) sum[i] = both(0.f);
 #pragma unroll
             for (int v = 0; v < kVpt; ++v) {
                 const int c = (v * group + t) * 8;
                 if (c >= p.hidden) continue;
-                float a[8], s8[8];
-                load8(sr + c, s8);
+                f32x2 a[4], s8[4], f[4];
+                load8(reinterpret_cast<const R*>(stage + lay.s) + off + c, s8);
                 if (p.dy != nullptr) {
-                    float w[8];
-                    load8(dy + c, a);
-                    load_param<true, T>(p.weight ? params_at : nullptr, p.weight_f32, v, t, group, p.hidden, w);
+                    load8(reinterpret_cast<const T*>(stage + lay.dy) + off + c, a);
+                    weight8(c, f);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) a[j] *= w[j];
+                    for (int j = 0; j < 4; ++j) {
+                        a[j] = mul_f32x2(a[j], f[j]);
+                        sum[0] = fma_f32x2(a[j], s8[j], sum[0]);
+                    }
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) a[j] = 0.f;
+                    for (int j = 0; j < 4; ++j) a[j] = both(0.f);
                 }
+                if (kX) {
+                    f32x2 x8[4], g[4];
+                    load8(reinterpret_cast<const T*>(stage + lay.x) + off + c, x8);
+                    post8(c, f);
+                    gate8(reinterpret_cast<const T*>(stage + lay.gate) + off, c, g);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) sums[0] += a[j] * s8[j];
-                if (has_x) {
-                    float x8[8], f[8];
-                    load8(xr + c, x8);
-                    if (p.post != nullptr) {
-                        load_param<true, T>(params_at + lay.post, p.post_f32, v, t, group, p.hidden, f);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) x8[j] *= f[j];
-                    }
-                    if (p.gate_mode == kGateChannel || p.gate_mode == kGateFull) {
-                        if (p.gate_mode == kGateFull) load8(gr + c, f);
-                        else load_param<true, T>(params_at + lay.channel_gate, p.gate_f32, v, t, group, p.hidden, f);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) x8[j] *= f[j];
-                    }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        sums[1] += x8[j] * a[j];
-                        sums[2] += x8[j] * s8[j];
+                    for (int j = 0; j < 4; ++j) {
+                        x8[j] = mul_f32x2(x8[j], mul_f32x2(f[j], g[j]));
+                        sum[kSums > 1 ? 1 : 0] = fma_f32x2(x8[j], a[j], sum[kSums > 1 ? 1 : 0]);
+                        sum[kSums > 1 ? 2 : 0] = fma_f32x2(x8[j], s8[j], sum[kSums > 1 ? 2 : 0]);
                     }
                     if (p.d_stream != nullptr) {
-                        load8(dd + c, f);
+                        load8(reinterpret_cast<const R*>(stage + lay.d_stream) + off + c, f);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) sums[3] += x8[j] * f[j];
+                        for (int j = 0; j < 4; ++j) sum[kSums > 1 ? 3 : 0] = fma_f32x2(x8[j], f[j], sum[kSums > 1 ? 3 : 0]);
                     }
                 }
             }
+#pragma unroll
+            for (int i = 0; i < kSums; ++i) sums[r * kSums + i] = total(sum[i]);
         }
-        group_sum<4>(sums, my_scratch + flip * 64, t, group, 1 + slot);
-        flip ^= 1u;
-        const RowScale k = row_scale(p, sums, rs, rp, token);
-        if (valid) {
-            const int64_t base = row * p.hidden;
-            if (p.gate_mode == kGateToken && p.d_gate != nullptr && t == 0)
-                static_cast<T*>(p.d_gate)[row] = Elem<T>::from_float(k.d_token_gate);
+        ring_sum<kRows * kSums>(sums, st, first_warp, warps);
+        // every thread is done with the chunk before this one
+        if (threadIdx.x == 0 && previous >= 0) load(chunk + static_cast<int64_t>(lay.stages - 1) * gridDim.x, previous);
+        previous = st.stage;
+        st.next(lay.stages);
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+            if (row0 + r >= p.rows) continue;
+            float four[4] = {sums[r * kSums], 0.f, 0.f, 0.f};
+            if (kX) four[1] = sums[r * kSums + kSums - 3], four[2] = sums[r * kSums + kSums - 2], four[3] = sums[r * kSums + kSums - 1];
+            const RowScale k = row_scale(p, four, rs[r], rp[r], token[r]);
+            const int64_t base = (row0 + r) * p.hidden;
+            const int off = (slot * kRows + r) * p.hidden;
+            if (kX && !kFull && p.gate_mode == kGateToken && p.d_gate != nullptr && t == 0)
+                static_cast<T*>(p.d_gate)[row0 + r] = Elem<T>::from_float(k.d_token_gate);
 #pragma unroll
             for (int v = 0; v < kVpt; ++v) {
                 const int c = (v * group + t) * 8;
                 if (c >= p.hidden) continue;
-                float ds[8], s8[8], f[8];
-                load8(sr + c, s8);
-                if (p.dy != nullptr) {
-                    float d8[8];
-                    load8(dy + c, d8);
-                    load_param<true, T>(p.weight ? params_at : nullptr, p.weight_f32, v, t, group, p.hidden, f);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        acc_w[v][j] += d8[j] * (s8[j] * k.rs);
-                        ds[j] = k.rs * (d8[j] * f[j] - s8[j] * k.k_s);
-                    }
+                f32x2 ds[4], f[4];
+                if (p.d_stream != nullptr) {
+                    load8(reinterpret_cast<const R*>(stage + lay.d_stream) + off + c, ds);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) ds[j] = 0.f;
+                    for (int j = 0; j < 4; ++j) ds[j] = both(0.f);
                 }
-                if (p.d_stream != nullptr) {
-                    load8(dd + c, f);
+                if (p.dy != nullptr) {
+                    f32x2 d8[4], s8[4];
+                    load8(reinterpret_cast<const R*>(stage + lay.s) + off + c, s8);
+                    load8(reinterpret_cast<const T*>(stage + lay.dy) + off + c, d8);
+                    weight8(c, f);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) ds[j] += f[j];
+                    for (int j = 0; j < 4; ++j) {
+                        acc_w[v][j] = fma_f32x2(d8[j], mul_f32x2(s8[j], both(k.rs)), acc_w[v][j]);
+                        ds[j] = fma_f32x2(mul_f32x2(d8[j], f[j]), both(k.rs), fma_f32x2(s8[j], both(-k.rs * k.k_s), ds[j]));
+                    }
                 }
                 if (p.d_residual != nullptr) store8(static_cast<R*>(p.d_residual) + base + c, ds);
-                if (p.dx == nullptr && !has_x) continue;
-                float b[8];
+                f32x2 b[4];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) b[j] = k.m * ds[j];  // gradient of the gated branch, token gate in it
-                if (has_x) {
-                    float x8[8], u[8];
-                    load8(xr + c, x8);
+                for (int j = 0; j < 4; ++j) b[j] = mul_f32x2(ds[j], both(k.m));  // gradient of the gated branch, token gate in it
+                if (kX) {
+                    f32x2 hat[4], g[4];
+                    load8(reinterpret_cast<const T*>(stage + lay.x) + off + c, hat);
+                    post8(c, f);
+                    gate8(reinterpret_cast<const T*>(stage + lay.gate) + off, c, g);
+                    f32x2 dg[4];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) u[j] = x8[j] *= k.rp;
-                    if (p.post != nullptr) {
-                        load_param<true, T>(params_at + lay.post, p.post_f32, v, t, group, p.hidden, f);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) u[j] *= f[j];
+                    for (int j = 0; j < 4; ++j) {
+                        hat[j] = mul_f32x2(hat[j], both(k.rp));
+                        const f32x2 u = mul_f32x2(hat[j], f[j]);
+                        if (kFull) dg[j] = mul_f32x2(b[j], u);
+                        else acc_g[v][j] = fma_f32x2(b[j], u, acc_g[v][j]);
+                        b[j] = mul_f32x2(b[j], g[j]);
+                        acc_p[v][j] = fma_f32x2(b[j], hat[j], acc_p[v][j]);
+                        b[j] = fma_f32x2(mul_f32x2(b[j], f[j]), both(k.rp), mul_f32x2(hat[j], both(-k.rp * k.k_x)));
                     }
-                    if (p.gate_mode == kGateChannel || p.gate_mode == kGateFull) {
-                        float g[8];
-                        if (p.gate_mode == kGateFull) load8(gr + c, g);
-                        else load_param<true, T>(params_at + lay.channel_gate, p.gate_f32, v, t, group, p.hidden, g);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) u[j] *= b[j];  // d gate
-                        if (p.gate_mode == kGateFull) {
-                            if (p.d_gate != nullptr) store8(static_cast<T*>(p.d_gate) + base + c, u);
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) acc_g[v][j] += u[j];
-                        }
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) b[j] *= g[j];
-                    }
-                    if (p.post != nullptr) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            acc_p[v][j] += b[j] * x8[j];
-                            b[j] = k.rp * (b[j] * f[j] - x8[j] * k.k_x);
-                        }
-                    }
+                    if (kFull && p.d_gate != nullptr) store8(static_cast<T*>(p.d_gate) + base + c, dg);
                 }
                 if (p.dx != nullptr) store8(static_cast<T*>(p.dx) + base + c, b);
             }
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(empty_bar + 8 * stage);
-        if (++stage == lay.stages) {
-            stage = 0;
-            phase ^= 1u;
-        }
     }
-    __syncthreads();  // with the producer: every load has landed and been read, the ring is free
+    __syncthreads();  // every load has landed and been read: the ring is free
 
     // The slots' sums, added in slot order, leave as this CTA's partial rows.
-    float* buf = reinterpret_cast<float*>(ring);
+    float* buf = reinterpret_cast<float*>(smem + lay.ring);
     const bool want[3] = {p.want_weight, p.want_post, p.want_gate};
 #pragma unroll
     for (int which = 0; which < 3; ++which) {
         if (!want[which]) continue;
-        float(&acc)[kVpt][8] = which == 0 ? acc_w : which == 1 ? acc_p : acc_g;
+        f32x2(&acc)[kVpt][4] = which == 0 ? acc_w : which == 1 ? acc_p : acc_g;
         float* out = p.partials + (static_cast<int64_t>(which) * kPartials + blockIdx.x) * p.hidden;
-        if (slots == 1) {
-#pragma unroll
-            for (int v = 0; v < kVpt; ++v) {
-                const int c = (v * group + t) * 8;
-                if (c < p.hidden) store8(out + c, acc[v]);
-            }
-            continue;
-        }
+        float* mine = lay.slots == 1 ? out : buf + slot * p.hidden;
 #pragma unroll
         for (int v = 0; v < kVpt; ++v) {
             const int c = (v * group + t) * 8;
-            if (c < p.hidden) store8(buf + slot * p.hidden + c, acc[v]);
+            if (c < p.hidden) store8(mine + c, acc[v]);
         }
-        group_barrier(0, compute_threads);
-        for (int c = threadIdx.x; c < p.hidden; c += compute_threads) {
-            float total = 0.f;
-            for (int sl = 0; sl < slots; ++sl) total += buf[sl * p.hidden + c];
-            out[c] = total;
+        if (lay.slots == 1) continue;
+        __syncthreads();
+        for (int c = threadIdx.x; c < p.hidden; c += blockDim.x) {
+            float sum = 0.f;
+            for (int sl = 0; sl < lay.slots; ++sl) sum += buf[sl * p.hidden + c];
+            out[c] = sum;
         }
-        group_barrier(0, compute_threads);
+        __syncthreads();
     }
 }
 
@@ -733,8 +969,77 @@ sum_kernel(const Params p, int count, void* d_weight, void* d_post, void* d_gate
 // Host side
 // ---------------------------------------------------------------------------------------------
 
+// Threads, stages and offsets of a ring kernel; false when not `min_stages` stages of a chunk fit.
+template <typename T, typename R>
+static bool ring_layout(const Params& p, bool backward, int vpt, int rows, int min_stages, RingLayout* lay) {
+    const uint32_t h = static_cast<uint32_t>(p.hidden);
+    lay->group = static_cast<int>(ceil_div(ceil_div(h, 8 * vpt), 32) * 32);
+    if (lay->group > kRingThreads) return false;
+    const uint32_t row_t = h * sizeof(T), row_r = h * sizeof(R);
+    uint32_t at = kRingHeader;
+    const auto param = [&](bool there, bool f32) {
+        const uint32_t here = at;
+        if (vpt > 1 && there) at += h * (f32 ? 4u : static_cast<uint32_t>(sizeof(T)));
+        return here;
+    };
+    lay->weight = param(p.weight != nullptr, p.weight_f32);
+    lay->post = param(p.post != nullptr, p.post_f32);
+    lay->channel_gate = param(p.gate_mode == kGateChannel, p.gate_f32);
+    lay->ring = (at + 127u) & ~127u;
+    // halve the rows a CTA takes at once until enough stages fit
+    for (lay->slots = kRingThreads / lay->group;; lay->slots /= 2) {
+        const uint32_t n = static_cast<uint32_t>(lay->slots * rows);
+        uint32_t off = 0;
+        const auto tensor = [&](bool there, uint32_t row) {
+            const uint32_t here = off;
+            off += there ? n * row : 0;
+            return here;
+        };
+        lay->s = tensor(backward, row_r);
+        lay->dy = tensor(backward && p.dy != nullptr, row_t);
+        lay->d_stream = tensor(backward && p.d_stream != nullptr, row_r);
+        lay->x = tensor(p.x != nullptr, row_t);
+        lay->residual = tensor(!backward && p.residual != nullptr, row_r);
+        lay->gate = tensor(p.gate_mode == kGateFull, row_t);
+        lay->stage_bytes = (off + 127u) & ~127u;
+        lay->stages = static_cast<int>((kRingSmem - lay->ring) / lay->stage_bytes);
+        if (lay->stages >= min_stages || lay->slots == 1) break;
+    }
+    if (lay->stages < min_stages) return false;
+    if (lay->stages > kMaxStages) lay->stages = kMaxStages;
+    uint32_t ring = lay->stage_bytes * static_cast<uint32_t>(lay->stages);
+    const uint32_t reduce = backward && lay->slots > 1 ? static_cast<uint32_t>(lay->slots) * h * 4 : 0;
+    if (ring < reduce) ring = reduce;
+    lay->total = lay->ring + ring;
+    return lay->total <= kRingSmem;
+}
+
+// Launches a ring kernel on as many CTAs as there are chunks and SMs; *count says how many.
+template <typename Kernel>
+static int launch_ring(Kernel kernel, const Params& p, const RingLayout& lay, int rows, int* count, cudaStream_t stream) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kRingSmem)) != cudaSuccess) {
+        cudaGetLastError();
+        return XMA_ERR_LAUNCH;
+    }
+    int64_t grid = ceil_div(p.rows, lay.slots * rows);
+    const int64_t most = sm_count() < kPartials ? sm_count() : kPartials;
+    if (grid > most) grid = most;
+    *count = static_cast<int>(grid);
+    kernel<<<static_cast<unsigned>(grid), static_cast<unsigned>(lay.group * lay.slots), lay.total, stream>>>(p, lay);
+    return launch_status();
+}
+
 template <typename T, typename R>
 static int run_forward(const Params& p, bool vec, cudaStream_t stream) {
+    if (vec && p.hidden <= kRingMaxHidden) {
+        const int ring_vpt = p.hidden > 4096 ? 2 : 1, rows = ring_vpt == 1 ? 2 : 1;
+        RingLayout lay;
+        int count = 0;
+        if (ring_layout<T, R>(p, false, ring_vpt, rows, 2, &lay) &&
+            p.rows >= static_cast<int64_t>(kRingMinChunks) * sm_count() * lay.slots * rows)
+            return ring_vpt == 1 ? launch_ring(forward_ring_kernel<T, R, 1, 2>, p, lay, rows, &count, stream)
+                                 : launch_ring(forward_ring_kernel<T, R, 2, 1>, p, lay, rows, &count, stream);
+    }
     if (p.hidden > kForwardMaxHidden) {
         forward_long_kernel<T, R><<<static_cast<unsigned>(p.rows), 1024, 0, stream>>>(p);
         return launch_status();
@@ -754,65 +1059,20 @@ static int run_forward(const Params& p, bool vec, cudaStream_t stream) {
     return launch_status();
 }
 
-// Fills the ring's layout; false when not even one stage of one row fits.
-template <typename T, typename R>
-static bool ring_layout(const Params& p, int vpt, RingLayout* lay) {
-    const uint32_t h = static_cast<uint32_t>(p.hidden);
-    lay->group = static_cast<int>(ceil_div(ceil_div(h, 8 * vpt), 32) * 32);
-    if (lay->group > kMaxThreads) return false;
-    lay->slots = kMaxThreads / lay->group;
-    const uint32_t row_t = h * sizeof(T), row_r = h * sizeof(R);
-    uint32_t at = p.weight == nullptr ? 0 : h * (p.weight_f32 ? 4 : sizeof(T));
-    lay->post = at;
-    if (p.post != nullptr) at += h * (p.post_f32 ? 4 : sizeof(T));
-    lay->channel_gate = at;
-    if (p.gate_mode == kGateChannel) at += h * (p.gate_f32 ? 4 : sizeof(T));
-    lay->ring = (kRingHeader + at + 127u) & ~127u;
-    // halve the rows a CTA takes at once until two stages fit
-    for (;;) {
-        const uint32_t n = static_cast<uint32_t>(lay->slots);
-        uint32_t off = 0;
-        lay->s = off, off += n * row_r;
-        lay->dy = off, off += p.dy != nullptr ? n * row_t : 0;
-        lay->d_stream = off, off += p.d_stream != nullptr ? n * row_r : 0;
-        lay->x = off, off += p.x != nullptr ? n * row_t : 0;
-        lay->gate = off, off += p.gate_mode == kGateFull ? n * row_t : 0;
-        lay->stage_bytes = (off + 127u) & ~127u;
-        lay->stages = static_cast<int>((kRingSmem - lay->ring) / lay->stage_bytes);
-        if (lay->stages >= 2 || lay->slots == 1) break;
-        lay->slots /= 2;
-    }
-    if (lay->stages > kMaxStages) lay->stages = kMaxStages;
-    if (lay->stages < 1) return false;
-    uint32_t ring = lay->stage_bytes * static_cast<uint32_t>(lay->stages);
-    const uint32_t reduce = lay->slots > 1 ? static_cast<uint32_t>(lay->slots) * h * 4 : 0;
-    if (ring < reduce) ring = reduce;
-    lay->total = lay->ring + ring;
-    return lay->total <= kRingSmem;
-}
-
-template <typename T, typename R, int kVpt>
-static int launch_ring(const Params& p, const RingLayout& lay, int* count, cudaStream_t stream) {
-    auto kernel = backward_ring_kernel<T, R, kVpt>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kRingSmem)) != cudaSuccess) {
-        cudaGetLastError();
-        return XMA_ERR_LAUNCH;
-    }
-    int64_t grid = ceil_div(p.rows, lay.slots);
-    const int64_t most = sm_count() < kPartials ? sm_count() : kPartials;
-    if (grid > most) grid = most;
-    *count = static_cast<int>(grid);
-    kernel<<<static_cast<unsigned>(grid), static_cast<unsigned>(lay.group * lay.slots + 32), lay.total, stream>>>(p, lay);
-    return launch_status();
+template <typename T, typename R, int kVpt, int kRows>
+static int run_backward_ring(const Params& p, const RingLayout& lay, int* count, cudaStream_t stream) {
+    if (p.x == nullptr) return launch_ring(backward_ring_kernel<T, R, kVpt, kRows, false, false>, p, lay, kRows, count, stream);
+    if (p.gate_mode == kGateFull) return launch_ring(backward_ring_kernel<T, R, kVpt, kRows, true, true>, p, lay, kRows, count, stream);
+    return launch_ring(backward_ring_kernel<T, R, kVpt, kRows, true, false>, p, lay, kRows, count, stream);
 }
 
 template <typename T, typename R>
 static int run_backward(const Params& p, bool vec, void* d_weight, void* d_post, void* d_gate_channel, cudaStream_t stream) {
     int count = 0, status = XMA_OK;
-    const int vpt = p.hidden > 512 ? 2 : 1;
+    const int vpt = p.hidden > 4096 ? 2 : 1, rows = vpt == 1 ? 2 : 1;
     RingLayout lay;
-    if (vec && p.hidden <= kRingMaxHidden && ring_layout<T, R>(p, vpt, &lay)) {
-        status = vpt == 1 ? launch_ring<T, R, 1>(p, lay, &count, stream) : launch_ring<T, R, 2>(p, lay, &count, stream);
+    if (vec && p.hidden <= kRingMaxHidden && ring_layout<T, R>(p, true, vpt, rows, 2, &lay)) {
+        status = vpt == 1 ? run_backward_ring<T, R, 1, 2>(p, lay, &count, stream) : run_backward_ring<T, R, 2, 1>(p, lay, &count, stream);
     } else {
         backward_sums_kernel<T, R><<<static_cast<unsigned>(p.rows), 256, 0, stream>>>(p);
         status = launch_status();
@@ -853,7 +1113,8 @@ int64_t xma_norm_workspace_floats(int64_t rows, int64_t hidden) {
 
 int xma_norm_forward(const void* x, const void* residual, const void* weight, const void* post_weight, const void* gate,
                      int32_t gate_mode, int32_t dtype, int32_t stream_dtype, int32_t f32_params, int64_t rows, int64_t hidden,
-                     float eps, float multiplier, void* stream_out, void* y, float* rstd, float* rstd_post, void* stream) {
+                     float eps, float multiplier, void* stream_out, void* y, float* rstd, float* rstd_post, int32_t* status,
+                     void* stream) {
     using namespace xma;
     using namespace xma::norm;
     if (!size_ok(rows, hidden, gate_mode)) return XMA_ERR_BAD_ARG;
@@ -864,7 +1125,7 @@ int xma_norm_forward(const void* x, const void* residual, const void* weight, co
     p.x = x, p.residual = residual, p.weight = weight, p.post = post_weight, p.gate = gate, p.gate_mode = gate_mode;
     p.weight_f32 = f32_params & 1, p.post_f32 = f32_params & 2, p.gate_f32 = f32_params & 4;
     p.rows = rows, p.hidden = static_cast<int>(hidden), p.eps = eps, p.multiplier = multiplier;
-    p.s_out = stream_out, p.y = y, p.rs = rstd, p.rp = rstd_post;
+    p.s_out = stream_out, p.y = y, p.rs = rstd, p.rp = rstd_post, p.status = status;
     const bool vec = all_aligned(p);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == kDtypeBF16 && stream_dtype == kDtypeBF16) return run_forward<__nv_bfloat16, __nv_bfloat16>(p, vec, st);

@@ -59,7 +59,7 @@ _SIGNATURES = {
     "xma_unpack_sequence": (c_int32, [c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int32, c_void_p, c_void_p]),
     "xma_norm_workspace_floats": (c_int64, [c_int64, c_int64]),
     "xma_norm_forward": (
-        c_int32, [c_void_p] * 5 + [c_int32] * 4 + [c_int64, c_int64, c_float, c_float] + [c_void_p] * 5),
+        c_int32, [c_void_p] * 5 + [c_int32] * 4 + [c_int64, c_int64, c_float, c_float] + [c_void_p] * 6),
     "xma_norm_backward": (
         c_int32, [c_void_p] * 7 + [c_int32] * 4 + [c_int64, c_int64, c_float] + [c_void_p] * 10),
     "xma_attention_workspace_bytes": (c_int64, [c_int64, c_int64]),

@@ -324,13 +324,14 @@ def norm_forward_cuda(
 ) -> None:
     """stream_out = residual + multiplier * gate * norm(x; post_weight), y = norm(stream_out; weight); see
     xma_norm_forward in include/xma_b200.h."""
+    _require_cuda(x)
     assert x.is_contiguous() and (residual is None or residual.is_contiguous())
     rows, hidden = x.shape
     stream_dtype = x.dtype if residual is None else residual.dtype
     _launch("xma_norm_forward", x,
         N.ptr(x), N.ptr(residual), N.ptr(weight), N.ptr(post_weight), N.ptr(gate), gate_mode, N.dtype_code(x.dtype),
         N.dtype_code(stream_dtype), _f32_params(weight, post_weight, gate), rows, hidden, eps, multiplier,
-        N.ptr(stream_out), N.ptr(y), N.ptr(rstd), N.ptr(rstd_post),
+        N.ptr(stream_out), N.ptr(y), N.ptr(rstd), N.ptr(rstd_post), N.ptr(N.status_word(x.device)),
     )
 
 

@@ -392,14 +392,15 @@ int xma_unpack_sequence(const void* x, const void* cu_seqlens, int32_t cu_is_int
  * stream_out (x for the norm alone, whose gradient is then d_residual); x is needed with a post norm or a
  * gate only. Gradients of parameters have the parameters' types and are summed over the rows in a fixed
  * order through `workspace`: xma_norm_workspace_floats(rows, hidden) floats, 16-byte aligned, contents
- * irrelevant before and after. rows == 0 writes nothing. Code 401 or 402 goes to *status when a wait for
- * the kernel's own copies runs out.
+ * irrelevant before and after. rows == 0 writes nothing. Code 402 or 403 goes to *status when a wait for a
+ * kernel's own copies runs out.
  */
 #define XMA_NORM_PARTIALS 148
 int64_t xma_norm_workspace_floats(int64_t rows, int64_t hidden);
 int xma_norm_forward(const void* x, const void* residual, const void* weight, const void* post_weight, const void* gate,
                      int32_t gate_mode, int32_t dtype, int32_t stream_dtype, int32_t f32_params, int64_t rows, int64_t hidden,
-                     float eps, float multiplier, void* stream_out, void* y, float* rstd, float* rstd_post, void* stream);
+                     float eps, float multiplier, void* stream_out, void* y, float* rstd, float* rstd_post, int32_t* status,
+                     void* stream);
 int xma_norm_backward(const void* dy, const void* d_stream, const void* stream_saved, const void* x, const void* weight,
                       const void* post_weight, const void* gate, int32_t gate_mode, int32_t dtype, int32_t stream_dtype,
                       int32_t f32_params, int64_t rows, int64_t hidden, float multiplier, const float* rstd,

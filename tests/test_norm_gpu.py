@@ -246,3 +246,14 @@ def test_compiled():
         assert torch.equal(a, b)
     for a, b in zip(torch.autograd.grad(got, leaves, [t["dy"], t["dd"]]), torch.autograd.grad(want, leaves, [t["dy"], t["dd"]])):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows,hidden", [(2000, 4096), (1400, 6000), (9000, 320), (30000, 64), (1500, 8192), (891, 4104)])
+def test_many_rows(rows, hidden):
+    """Enough rows for every CTA to go several times round its ring, forward and backward."""
+    for types in TYPES:
+        check(make(rows, hidden, *types, "channel", True), 0.5)
+        check(make(rows, hidden, *types, "full", False), 1.0)
+        check(make(rows, hidden, types[0], None, "none", False), 1.0)
+    check(make(rows, hidden, torch.bfloat16, torch.bfloat16, "token", True, param_dtype=torch.float32), 0.5)
+    check(make(rows, hidden, torch.bfloat16, torch.float32, "none", False), 1.0)

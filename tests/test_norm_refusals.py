@@ -46,7 +46,7 @@ def test_c_entry_refuses():
 
     lib = N.lib()
     forward = lambda x=1 << 20, res=None, w=None, post=None, gate=None, mode=0, dt=0, sdt=0, rows=1, hidden=8, out=None, y=1 << 20: lib.xma_norm_forward(
-        x, res, w, post, gate, mode, dt, sdt, 0, rows, hidden, 1e-5, 1.0, out, y, None, None, None)
+        x, res, w, post, gate, mode, dt, sdt, 0, rows, hidden, 1e-5, 1.0, out, y, None, None, None, None)
     assert forward(rows=0) == 0
     assert forward(rows=-1) == 1 and forward(hidden=0) == 1 and forward(x=None) == 1 and forward(y=None) == 1
     assert forward(mode=4) == 1 and forward(mode=1) == 1 and forward(res=1 << 20) == 1
