@@ -18,28 +18,32 @@ _MAX_SEQUENCES = 1 << 20
 def _tiled(t: torch.Tensor) -> torch.Tensor:
     """`t` itself where the copy engine can read it in place (heads contiguous, other strides multiples of 16
     bytes), else a contiguous copy: slices of a fused projection are read where they are."""
-    strides = [t.stride(i) for i in (0, 1) if t.size(i) > 1]
-    return t if t.stride(2) == 1 and all(s > 0 and s % 8 == 0 for s in strides) else t.contiguous()
+    (tokens, heads, _), (token, head, inner) = t.shape, t.stride()
+    in_place = inner == 1 and (tokens <= 1 or (token > 0 and token % 8 == 0)) and (heads <= 1 or (head > 0 and head % 8 == 0))
+    return t if in_place else t.contiguous()
+
+
+def _forward(q, k, v, cu_seqlens, softmax_scale: float, saving: bool):
+    from ..ops import attention_packed_forward_cuda
+
+    q, k, v, cu_seqlens = _tiled(q), _tiled(k), _tiled(v), cu_seqlens.contiguous()
+    total, heads, _ = q.shape
+    batch = cu_seqlens.numel() - 1
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = None
+    if saving:
+        lse = torch.empty(heads, N.attention_stat_rows(total, batch), dtype=torch.float32, device=q.device)
+    workspace = torch.empty(N.attention_workspace_bytes(total, batch), dtype=torch.uint8, device=q.device)
+    attention_packed_forward_cuda(q, k, v, cu_seqlens, softmax_scale, out, lse, workspace)
+    return out, (q, k, v, cu_seqlens, out, lse)
 
 
 class _AttentionPacked(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_seqlens, softmax_scale: float):
-        from ..ops import attention_packed_forward_cuda
-
-        q, k, v, cu_seqlens = _tiled(q), _tiled(k), _tiled(v), cu_seqlens.contiguous()
-        total, heads, _ = q.shape
-        batch = cu_seqlens.numel() - 1
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        saving = any(ctx.needs_input_grad)
-        lse = None
-        if saving:
-            lse = torch.empty(heads, N.attention_stat_rows(total, batch), dtype=torch.float32, device=q.device)
-        workspace = torch.empty(N.attention_workspace_bytes(total, batch), dtype=torch.uint8, device=q.device)
-        attention_packed_forward_cuda(q, k, v, cu_seqlens, softmax_scale, out, lse, workspace)
-        if saving:
-            ctx.save_for_backward(q, k, v, cu_seqlens, out, lse)
-            ctx.softmax_scale = softmax_scale
+        out, saved = _forward(q, k, v, cu_seqlens, softmax_scale, True)
+        ctx.save_for_backward(*saved)
+        ctx.softmax_scale = softmax_scale
         return out
 
     @staticmethod
@@ -78,15 +82,16 @@ def attention_packed(
     that no sequence owns get zeros, in the output and in the gradients, and what they hold reaches nothing. Offsets are
     read on the device: values that are out of order or outside the stream give meaningless outputs, not an error."""
     require_cuda_backend(kernel_backend)
+    dtype, device = q.dtype, q.device
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"q should be bfloat16 or float16, got {dtype}")
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != 3:
             raise ValueError(f"{name} should be [tokens, heads, head_dim], got shape {tuple(t.shape)}")
-        if t.dtype not in (torch.bfloat16, torch.float16):
-            raise ValueError(f"{name} should be bfloat16 or float16, got {t.dtype}")
-        if t.dtype != q.dtype:
-            raise ValueError(f"{name} should be {q.dtype} like q, got {t.dtype}")
-        if t.device != q.device:
-            raise ValueError(f"{name} is on {t.device}, q on {q.device}")
+        if t.dtype != dtype:
+            raise ValueError(f"{name} should be {dtype} like q, got {t.dtype}")
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, q on {device}")
     total, heads, dim = q.shape
     if k.shape != v.shape:
         raise ValueError(f"k and v should have the same shape, got {tuple(k.shape)} and {tuple(v.shape)}")
@@ -99,11 +104,13 @@ def attention_packed(
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"cu_seqlens should be a 1-dimensional int32 or int64 tensor of at least one offset, got "
                          f"{cu_seqlens.dtype} {tuple(cu_seqlens.shape)}")
-    if cu_seqlens.device != q.device:
-        raise ValueError(f"cu_seqlens is on {cu_seqlens.device}, q on {q.device}")
+    if cu_seqlens.device != device:
+        raise ValueError(f"cu_seqlens is on {cu_seqlens.device}, q on {device}")
     if total > _MAX_TOKENS or cu_seqlens.numel() > _MAX_SEQUENCES:
         raise ValueError(f"at most {_MAX_TOKENS} tokens and {_MAX_SEQUENCES - 1} sequences are supported")
     scale = 1.0 / math.sqrt(dim) if softmax_scale is None else float(softmax_scale)
     if not 0.0 < scale < 1e30:
         raise ValueError(f"softmax_scale should be positive and finite, got {scale}")
-    return _AttentionPacked.apply(q, k, v, cu_seqlens, scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _AttentionPacked.apply(q, k, v, cu_seqlens, scale)
+    return _forward(q, k, v, cu_seqlens, scale, False)[0]

@@ -13,30 +13,35 @@ GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_FULL = 0, 1, 2, 3
 _MAX_HIDDEN = 1 << 24
 
 
+def _forward(x, residual, weight, post_weight, gate, gate_mode: int, eps: float, multiplier: float, saving: bool):
+    """(y, stream or None, contiguous inputs, row statistics): the forward launch."""
+    from ..ops import norm_forward_cuda
+
+    x, residual, weight, post_weight, gate = (
+        t if t is None or t.is_contiguous() else t.contiguous() for t in (x, residual, weight, post_weight, gate))
+    y = torch.empty_like(x)
+    stream = None if residual is None else torch.empty_like(residual)
+    rstd = rstd_post = None
+    if saving:
+        rows = x.numel() // x.size(-1)
+        rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
+        if post_weight is not None:
+            rstd_post = torch.empty(rows, dtype=torch.float32, device=x.device)
+    norm_forward_cuda(x, residual, weight, post_weight, gate, gate_mode, eps, multiplier, stream, y, rstd, rstd_post)
+    return y, stream, (x, weight, post_weight, gate), (rstd, rstd_post)
+
+
 class _Norm(torch.autograd.Function):
-    """x [rows, H] and, unless it is None, residual [rows, H]; returns y, or (y, stream) with a residual."""
+    """Rows of any leading shape; returns y, or (y, stream) with a residual."""
 
     @staticmethod
     def forward(ctx, x, residual, weight, post_weight, gate, gate_mode: int, eps: float, multiplier: float):
-        from ..ops import norm_forward_cuda
-
-        x = x.contiguous()
-        residual = None if residual is None else residual.contiguous()
-        weight = None if weight is None else weight.contiguous()
-        post_weight = None if post_weight is None else post_weight.contiguous()
-        gate = None if gate is None else gate.contiguous()
-        rows = x.size(0)
-        y = torch.empty_like(x)
-        stream = None if residual is None else torch.empty_like(residual)
-        saving = any(ctx.needs_input_grad)
-        rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if saving else None
-        rstd_post = torch.empty(rows, dtype=torch.float32, device=x.device) if saving and post_weight is not None else None
-        norm_forward_cuda(x, residual, weight, post_weight, gate, gate_mode, eps, multiplier, stream, y, rstd, rstd_post)
-        if saving:
-            branch = x if post_weight is not None or gate is not None else None  # a plain residual add needs no input
-            ctx.save_for_backward(x if residual is None else stream, branch, weight, post_weight, gate, rstd, rstd_post)
-            ctx.dtype, ctx.alone = x.dtype, residual is None
-            ctx.gate_mode, ctx.multiplier = gate_mode, multiplier
+        y, stream, (x, weight, post_weight, gate), (rstd, rstd_post) = _forward(
+            x, residual, weight, post_weight, gate, gate_mode, eps, multiplier, True)
+        branch = x if post_weight is not None or gate is not None else None  # a plain residual add needs no input
+        ctx.save_for_backward(x if residual is None else stream, branch, weight, post_weight, gate, rstd, rstd_post)
+        ctx.dtype, ctx.alone = x.dtype, residual is None
+        ctx.gate_mode, ctx.multiplier = gate_mode, multiplier
         ctx.set_materialize_grads(False)
         return y if residual is None else (y, stream)
 
@@ -57,13 +62,14 @@ class _Norm(torch.autograd.Function):
         d_residual = torch.empty_like(stream) if want_stream else None
         dx = None
         if want_x and not ctx.alone and not shared:
-            dx = torch.empty(stream.shape, dtype=ctx.dtype, device=stream.device)
+            dx = torch.empty_like(stream, dtype=ctx.dtype)
         new = torch.zeros_like if empty else torch.empty_like
         d_weight = new(weight) if want_weight and weight is not None else None
         d_post = new(post_weight) if want_post and post_weight is not None else None
         d_gate = new(gate) if want_gate and gate is not None else None
         if not empty:
-            workspace = torch.empty(N.norm_workspace_floats(*stream.shape), dtype=torch.float32, device=stream.device)
+            hidden = stream.size(-1)
+            workspace = torch.empty(N.norm_workspace_floats(stream.numel() // hidden, hidden), dtype=torch.float32, device=stream.device)
             norm_backward_cuda(
                 dy, d_stream, stream, x, weight, post_weight, gate, ctx.gate_mode, ctx.dtype, ctx.multiplier, rstd,
                 rstd_post, dx, d_residual, d_gate, d_weight, d_post, workspace)
@@ -73,6 +79,13 @@ class _Norm(torch.autograd.Function):
             dx = d_residual if want_x else None
             d_residual = d_residual if want_residual else None
         return dx, d_residual, d_weight, d_post, d_gate, None, None, None
+
+
+def _norm(x, residual, weight, post_weight, gate, gate_mode: int, eps: float, multiplier: float):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight, post_weight, gate)):
+        return _Norm.apply(x, residual, weight, post_weight, gate, gate_mode, eps, multiplier)
+    y, stream, _, _ = _forward(x, residual, weight, post_weight, gate, gate_mode, eps, multiplier, False)
+    return y if residual is None else (y, stream)
 
 
 def _check_rows(x: torch.Tensor) -> None:
@@ -85,7 +98,7 @@ def _check_rows(x: torch.Tensor) -> None:
 def _check_parameter(name: str, t: torch.Tensor | None, x: torch.Tensor) -> None:
     if t is None:
         return
-    if t.shape != x.shape[-1:]:
+    if t.dim() != 1 or t.size(0) != x.size(-1):
         raise ValueError(f"{name} should have shape {tuple(x.shape[-1:])}, got {tuple(t.shape)}")
     if t.dtype not in (x.dtype, torch.float32):
         raise ValueError(f"{name} should be {x.dtype} or float32, got {t.dtype}")
@@ -95,8 +108,8 @@ def _check_parameter(name: str, t: torch.Tensor | None, x: torch.Tensor) -> None
 
 def _eps(eps: float | None, x: torch.Tensor) -> float:
     eps = torch.finfo(x.dtype).eps if eps is None else float(eps)
-    if not eps >= 0:
-        raise ValueError(f"eps should not be negative, got {eps}")
+    if not 0 <= eps < float("inf"):
+        raise ValueError(f"eps should be finite and not negative, got {eps}")
     return eps
 
 
@@ -110,8 +123,7 @@ def rmsnorm(
     require_cuda_backend(kernel_backend)
     _check_rows(x)
     _check_parameter("weight", weight, x)
-    y = _Norm.apply(x.reshape(-1, x.size(-1)), None, weight, None, None, GATE_NONE, _eps(eps, x), 1.0)
-    return y.view(x.shape)
+    return _norm(x, None, weight, None, None, GATE_NONE, _eps(eps, x), 1.0)
 
 
 def fused_residual_add_rmsnorm(
@@ -147,24 +159,20 @@ def fused_residual_add_rmsnorm(
         raise ValueError(f"residual is on {residual.device}, x on {x.device}")
     _check_parameter("weight", weight, x)
     _check_parameter("post_weight", post_weight, x)
-    hidden = x.size(-1)
     gate_mode = GATE_NONE
     if gate is not None:
         if gate.shape == x.shape and gate.dtype == x.dtype:
-            gate_mode, gate_rows = GATE_FULL, gate.reshape(-1, hidden)
+            gate_mode = GATE_FULL
         elif gate.shape == x.shape[-1:]:
             _check_parameter("gate", gate, x)
-            gate_mode, gate_rows = GATE_CHANNEL, gate
+            gate_mode = GATE_CHANNEL
         elif gate.shape == x.shape[:-1] + (1,):
-            gate_mode, gate_rows = GATE_TOKEN, gate.reshape(-1)
+            gate_mode = GATE_TOKEN
         else:
             raise ValueError(
-                f"gate should have shape {(hidden,)}, {tuple(x.shape[:-1]) + (1,)} or {tuple(x.shape)}, got {tuple(gate.shape)}")
+                f"gate should have shape {tuple(x.shape[-1:])}, {tuple(x.shape[:-1]) + (1,)} or {tuple(x.shape)}, got {tuple(gate.shape)}")
         if gate_mode != GATE_CHANNEL and gate.dtype != x.dtype:
             raise ValueError(f"a gate of every token should be {x.dtype}, got {gate.dtype}")
         if gate.device != x.device:
             raise ValueError(f"gate is on {gate.device}, x on {x.device}")
-    y, stream = _Norm.apply(
-        x.reshape(-1, hidden), residual.reshape(-1, hidden), weight, post_weight, None if gate is None else gate_rows,
-        gate_mode, _eps(eps, x), 1.0 if multiplier is None else float(multiplier))
-    return y.view(x.shape), stream.view(x.shape)
+    return _norm(x, residual, weight, post_weight, gate, gate_mode, _eps(eps, x), 1.0 if multiplier is None else float(multiplier))

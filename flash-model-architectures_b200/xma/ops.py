@@ -34,6 +34,7 @@ def _kernels_per_call(name: str, args: tuple) -> int:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _entry_points: dict = {}
 
 
@@ -44,13 +45,14 @@ def _require_cuda(anchor: torch.Tensor) -> None:
 
 def _launch(name: str, anchor: torch.Tensor, *args) -> None:
     """Calls one C-ABI entry point on `anchor`'s device and current stream; raises on a non-zero status."""
-    _require_cuda(anchor)
+    index = anchor.get_device()
+    if index < 0:
+        _require_cuda(anchor)
     fn = _entry_points.get(name)
     if fn is None:
         fn = _entry_points[name] = getattr(N.lib(), name)
     profiler = N.profiler
-    index = anchor.device.index
-    if not profiler.enabled and _raw_stream is not None and index == torch.cuda.current_device():
+    if not profiler.enabled and _raw_stream is not None and index == _current_device():
         # The usual case (tensor on the current device, no profiling): no device guard and no stream
         # object, which keeps the host cost of a launch to the ctypes call itself.
         status = fn(*args, _raw_stream(index))
@@ -326,7 +328,8 @@ def norm_forward_cuda(
     xma_norm_forward in include/xma_b200.h."""
     _require_cuda(x)
     assert x.is_contiguous() and (residual is None or residual.is_contiguous())
-    rows, hidden = x.shape
+    hidden = x.size(-1)
+    rows = x.numel() // hidden
     stream_dtype = x.dtype if residual is None else residual.dtype
     _launch("xma_norm_forward", x,
         N.ptr(x), N.ptr(residual), N.ptr(weight), N.ptr(post_weight), N.ptr(gate), gate_mode, N.dtype_code(x.dtype),
@@ -345,7 +348,8 @@ def norm_backward_cuda(
 ) -> None:
     """Gradients of norm_forward_cuda's inputs; see xma_norm_backward in include/xma_b200.h."""
     assert stream.is_contiguous() and all(t is None or t.is_contiguous() for t in (dy, d_stream, x, gate))
-    rows, hidden = stream.shape
+    hidden = stream.size(-1)
+    rows = stream.numel() // hidden
     _launch("xma_norm_backward", stream,
         N.ptr(dy), N.ptr(d_stream), N.ptr(stream), N.ptr(x), N.ptr(weight), N.ptr(post_weight), N.ptr(gate), gate_mode,
         N.dtype_code(dtype), N.dtype_code(stream.dtype), _f32_params(weight, post_weight, gate), rows, hidden,
@@ -359,14 +363,18 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
+def _stride_args(t: torch.Tensor) -> tuple[int, int]:
+    """Token and head strides; a single token or head has no stride of its own: any valid one will do."""
+    (tokens, heads, dim), (token, head, _) = t.shape, t.stride()
+    return token if tokens > 1 else heads * dim, head if heads > 1 else dim
+
+
 def _attention_args(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, softmax_scale: float) -> tuple:
     _require_cuda(q)
     total, heads, dim = q.shape
-    kv_heads = k.size(1)
-    # a single head has no stride of its own: any valid one will do
-    strides = [s for t in (q, k, v) for s in (t.stride(0) if total > 1 else t.size(1) * dim, t.stride(1) if t.size(1) > 1 else dim)]
-    return (N.ptr(q), N.ptr(k), N.ptr(v), *strides, N.dtype_code(q.dtype), N.ptr(cu_seqlens), int(cu_seqlens.dtype == torch.int64),
-            cu_seqlens.numel() - 1, total, heads, kv_heads, dim, softmax_scale)
+    return (q.data_ptr(), k.data_ptr(), v.data_ptr(), *_stride_args(q), *_stride_args(k), *_stride_args(v), N.dtype_code(q.dtype),
+            cu_seqlens.data_ptr(), int(cu_seqlens.dtype == torch.int64), cu_seqlens.numel() - 1, total, heads, k.size(1), dim,
+            softmax_scale)
 
 
 @xma_op(mutates_args={"out", "lse", "workspace"})
