@@ -24,7 +24,6 @@
 // Rows beyond a sequence's end inside a tile belong to other sequences: their scores are masked by
 // selection, and where a masked (zero) probability would multiply such a row, the row is zeroed in shared
 // memory first, so that not even a NaN crosses over. Every wait is bounded, as in the grouped GEMM.
-#include <mutex>
 #include <type_traits>
 
 #include "common.cuh"
@@ -1300,25 +1299,6 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
 // Host side
 // ---------------------------------------------------------------------------------------------
 
-// Shared-memory attribute of a kernel, set once per device.
-template <auto kKernel>
-static bool prepare_kernel(uint32_t smem) {
-    constexpr int kMaxDevices = 64;
-    static bool set[kMaxDevices];
-    static std::mutex mu;
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return false;
-    std::lock_guard<std::mutex> lock(mu);
-    if (!set[dev]) {
-        if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) {
-            cudaGetLastError();
-            return false;
-        }
-        set[dev] = true;
-    }
-    return true;
-}
-
 // [tokens, heads, dim] with token and head strides in elements; boxes of 128 tokens x 64 columns of a head.
 static bool stream_map(CUtensorMap* map, int dtype, const void* base, int64_t total, int heads, int dim, int64_t token_stride,
                        int64_t head_stride) {
@@ -1412,7 +1392,7 @@ static int run_forward(const Call& c, void* out, float* lse) {
         !stream_map(&mk, c.dtype, c.k, c.total, c.kv_heads, c.dim, c.k_token, c.k_head) ||
         !stream_map(&mv, c.dtype, c.v, c.total, c.kv_heads, c.dim, c.v_token, c.v_head))
         return XMA_ERR_DRIVER;
-    if (!prepare_kernel<forward_kernel<T, kD>>(Forward<kD>::kSmem)) return XMA_ERR_LAUNCH;
+    if (!allow_smem<forward_kernel<T, kD>>(Forward<kD>::kSmem)) return XMA_ERR_LAUNCH;
     const Workspace w = split_workspace(c.workspace, c.total, c.batch);
     const ZeroRows zo{out, static_cast<int64_t>(c.heads) * c.dim * 2}, none{nullptr, 0};
     const int status = launch_plan(c.cu, c.cu_is_int64, c.batch, c.total, 2 * kTile, w, 1, zo, none, none, c.stream);
@@ -1433,7 +1413,7 @@ static int run_backward(const Call& c, const void* out, const void* d_out, const
         !stream_map(&mv, c.dtype, c.v, c.total, c.kv_heads, c.dim, c.v_token, c.v_head) ||
         !stream_map(&mdo, c.dtype, d_out, c.total, c.heads, c.dim, o_token, c.dim))
         return XMA_ERR_DRIVER;
-    if (!prepare_kernel<dkdv_kernel<T, kD>>(Backward<kD>::kSmem) || !prepare_kernel<dq_kernel<T, kD>>(Backward<kD>::kSmem))
+    if (!allow_smem<dkdv_kernel<T, kD>>(Backward<kD>::kSmem) || !allow_smem<dq_kernel<T, kD>>(Backward<kD>::kSmem))
         return XMA_ERR_LAUNCH;
     const Workspace w = split_workspace(c.workspace, c.total, c.batch);
     const int64_t row_q = o_token * 2, row_kv = static_cast<int64_t>(c.kv_heads) * c.dim * 2;

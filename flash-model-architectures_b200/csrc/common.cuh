@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "xma_b200.h"
 
 namespace xma {
@@ -27,6 +29,22 @@ int sm_count();
 
 // Launch-error check used after every kernel launch.
 inline int launch_status() { return cudaGetLastError() == cudaSuccess ? XMA_OK : XMA_ERR_LAUNCH; }
+
+// Lets a kernel use `bytes` of dynamic shared memory; asked of the runtime once per kernel and device.
+template <auto kKernel>
+bool allow_smem(uint32_t bytes) {
+    constexpr int kMaxDevices = 64;
+    static std::atomic<bool> set[kMaxDevices];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return false;
+    if (set[dev].load(std::memory_order_relaxed)) return true;
+    if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) != cudaSuccess) {
+        cudaGetLastError();
+        return false;
+    }
+    set[dev].store(true, std::memory_order_relaxed);
+    return true;
+}
 
 template <typename T>
 struct Elem;

@@ -1015,17 +1015,14 @@ static bool ring_layout(const Params& p, bool backward, int vpt, int rows, int m
 }
 
 // Launches a ring kernel on as many CTAs as there are chunks and SMs; *count says how many.
-template <typename Kernel>
-static int launch_ring(Kernel kernel, const Params& p, const RingLayout& lay, int rows, int* count, cudaStream_t stream) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kRingSmem)) != cudaSuccess) {
-        cudaGetLastError();
-        return XMA_ERR_LAUNCH;
-    }
+template <auto kKernel>
+static int launch_ring(const Params& p, const RingLayout& lay, int rows, int* count, cudaStream_t stream) {
+    if (!allow_smem<kKernel>(kRingSmem)) return XMA_ERR_LAUNCH;
     int64_t grid = ceil_div(p.rows, lay.slots * rows);
     const int64_t most = sm_count() < kPartials ? sm_count() : kPartials;
     if (grid > most) grid = most;
     *count = static_cast<int>(grid);
-    kernel<<<static_cast<unsigned>(grid), static_cast<unsigned>(lay.group * lay.slots), lay.total, stream>>>(p, lay);
+    kKernel<<<static_cast<unsigned>(grid), static_cast<unsigned>(lay.group * lay.slots), lay.total, stream>>>(p, lay);
     return launch_status();
 }
 
@@ -1037,8 +1034,8 @@ static int run_forward(const Params& p, bool vec, cudaStream_t stream) {
         int count = 0;
         if (ring_layout<T, R>(p, false, ring_vpt, rows, 2, &lay) &&
             p.rows >= static_cast<int64_t>(kRingMinChunks) * sm_count() * lay.slots * rows)
-            return ring_vpt == 1 ? launch_ring(forward_ring_kernel<T, R, 1, 2>, p, lay, rows, &count, stream)
-                                 : launch_ring(forward_ring_kernel<T, R, 2, 1>, p, lay, rows, &count, stream);
+            return ring_vpt == 1 ? launch_ring<forward_ring_kernel<T, R, 1, 2>>(p, lay, rows, &count, stream)
+                                 : launch_ring<forward_ring_kernel<T, R, 2, 1>>(p, lay, rows, &count, stream);
     }
     if (p.hidden > kForwardMaxHidden) {
         forward_long_kernel<T, R><<<static_cast<unsigned>(p.rows), 1024, 0, stream>>>(p);
@@ -1061,9 +1058,9 @@ static int run_forward(const Params& p, bool vec, cudaStream_t stream) {
 
 template <typename T, typename R, int kVpt, int kRows>
 static int run_backward_ring(const Params& p, const RingLayout& lay, int* count, cudaStream_t stream) {
-    if (p.x == nullptr) return launch_ring(backward_ring_kernel<T, R, kVpt, kRows, false, false>, p, lay, kRows, count, stream);
-    if (p.gate_mode == kGateFull) return launch_ring(backward_ring_kernel<T, R, kVpt, kRows, true, true>, p, lay, kRows, count, stream);
-    return launch_ring(backward_ring_kernel<T, R, kVpt, kRows, true, false>, p, lay, kRows, count, stream);
+    if (p.x == nullptr) return launch_ring<backward_ring_kernel<T, R, kVpt, kRows, false, false>>(p, lay, kRows, count, stream);
+    if (p.gate_mode == kGateFull) return launch_ring<backward_ring_kernel<T, R, kVpt, kRows, true, true>>(p, lay, kRows, count, stream);
+    return launch_ring<backward_ring_kernel<T, R, kVpt, kRows, true, false>>(p, lay, kRows, count, stream);
 }
 
 template <typename T, typename R>
