@@ -709,8 +709,8 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
     uint8_t* gen = smem_raw;
     const uint32_t k_tile = base, v_tile = base + B::kTileBytes, q_ring = base + B::kLongAt, do_ring = base + B::kShortAt;
     const uint32_t bars = base + B::kBars;
-    const uint32_t q_full = bars, q_empty = bars + 24, do_full = bars + 48, do_empty = bars + 64, kv_full = bars + 80, kv_empty = bars + 88,
-                   s_full = bars + 96, dp_full = bars + 104, p_ready = bars + 112, ds_ready = bars + 128, done = bars + 144;
+    const uint32_t q_full = bars, q_empty = bars + 24, do_full = bars + 48, do_empty = bars + 64, k_full = bars + 80, k_empty = bars + 88,
+                   s_full = bars + 96, dp_full = bars + 104, p_ready = bars + 112, ds_ready = bars + 128, done = bars + 144, v_full = bars + 168, v_empty = bars + 176;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + B::kBars + 160);
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + B::kBars + 164);
 
@@ -724,8 +724,10 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
             mbar_init(do_full + 8 * i, 1);
             mbar_init(do_empty + 8 * i, 2);  // both MMA warps; the second's commit follows the reads of the statistics
         }
-        mbar_init(kv_full, 1);
-        mbar_init(kv_empty, 1);
+        mbar_init(k_full, 1);
+        mbar_init(k_empty, 1);
+        mbar_init(v_full, 1);
+        mbar_init(v_empty, 1);
         mbar_init(s_full, 1);
         mbar_init(dp_full, 1);
         for (int h = 0; h < 2; ++h) {
@@ -752,21 +754,20 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
     const int64_t items = static_cast<int64_t>(warp_uniform(*p.num_blocks)) * p.kv_heads;
 
     if (warp == 0) {
-        // k, v and the query tiles
+        // k and the query tiles
         if (lane == 0) {
             Ring q;
-            uint32_t kv_phase = 1u;
+            uint32_t k_phase = 1u;
             bool ok = true;
             for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
                 const Block b = p.blocks[it / p.kv_heads];
                 const int kv_head = static_cast<int>(it % p.kv_heads);
                 const int n = (b.len + kTile - 1) / kTile;
-                ok = mbar_wait(kv_empty, kv_phase, abort_flag, p.status, 511);
+                ok = mbar_wait(k_empty, k_phase, abort_flag, p.status, 511);
                 if (!ok) break;
-                kv_phase ^= 1u;
-                mbar_expect_tx(kv_full, 2 * B::kTileBytes);
-                load_tile<kD>(k_tile, &map_k, kv_full, kv_head, b.start + b.index * kTile);
-                load_tile<kD>(v_tile, &map_v, kv_full, kv_head, b.start + b.index * kTile);
+                k_phase ^= 1u;
+                mbar_expect_tx(k_full, B::kTileBytes);
+                load_tile<kD>(k_tile, &map_k, k_full, kv_head, b.start + b.index * kTile);
                 for (int g = 0; ok && g < p.group; ++g) {
                     for (int i = b.index; ok && i < n; ++i) {
                         ok = mbar_wait(q_empty + 8 * q.stage, q.phase ^ 1u, abort_flag, p.status, 512);
@@ -781,14 +782,20 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         }
         __syncwarp();
     } else if (warp == 3) {
-        // do tiles with the rows' statistics
+        // v, and do tiles with the rows' statistics
         if (lane == 0) {
             Ring d;
+            uint32_t v_phase = 1u;
             bool ok = true;
             for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
                 const Block b = p.blocks[it / p.kv_heads];
                 const int kv_head = static_cast<int>(it % p.kv_heads);
                 const int n = (b.len + kTile - 1) / kTile;
+                ok = mbar_wait(v_empty, v_phase, abort_flag, p.status, 529);
+                if (!ok) break;
+                v_phase ^= 1u;
+                mbar_expect_tx(v_full, B::kTileBytes);
+                load_tile<kD>(v_tile, &map_v, v_full, kv_head, b.start + b.index * kTile);
                 for (int g = 0; ok && g < p.group; ++g) {
                     const int head = kv_head * p.group + g;
                     for (int i = b.index; ok && i < n; ++i) {
@@ -812,21 +819,22 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         const uint32_t idesc_s = make_idesc(kTile, kTile, false, false, p.ab_format);
         const uint32_t idesc_d = make_idesc(kTile, p.dim_steps * 16, false, true, p.ab_format);
         Ring q, d;
-        uint32_t kv_phase = 0, p_phase = 0;
+        uint32_t k_phase = 0, p_phase = 0;
         bool ok = true;
         for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
             const Block b = load_block(p.blocks + it / p.kv_heads);
             const int n = (b.len + kTile - 1) / kTile;
             const int per_head = n - b.index, steps = per_head * p.group;
-            ok = mbar_wait_warp(kv_full, kv_phase, abort_flag, p.status, 513);
+            ok = mbar_wait_warp(k_full, k_phase, abort_flag, p.status, 513);
             if (!ok) break;
-            kv_phase ^= 1u;
+            k_phase ^= 1u;
             ok = mbar_wait_warp(q_full + 8 * q.stage, q.phase, abort_flag, p.status, 514);
             if (!ok) break;
             tc_fence_after();
             if (elect_one()) {
                 mma_scores<kD>(tm_s, k_tile, q_ring + q.stage * B::kTileBytes, idesc_s, p.dim_steps);
                 umma_commit_cta1(s_full);
+                if (steps == 1) umma_commit_cta1(k_empty);
             }
             __syncwarp();
             q.next(B::kLong);
@@ -858,6 +866,7 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
                     if (more) {
                         mma_scores<kD>(tm_s, k_tile, next_q, idesc_s, p.dim_steps);
                         umma_commit_cta1(s_full);
+                        if (st + 2 == steps) umma_commit_cta1(k_empty);
                     } else {
                         umma_commit_cta1(done);
                     }
@@ -873,21 +882,22 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         const uint32_t idesc_s = make_idesc(kTile, kTile, false, false, p.ab_format);
         const uint32_t idesc_d = make_idesc(kTile, p.dim_steps * 16, false, true, p.ab_format);
         Ring q, d;
-        uint32_t kv_phase = 0, ds_phase = 0;
+        uint32_t v_phase = 0, ds_phase = 0;
         bool ok = true;
         for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
             const Block b = load_block(p.blocks + it / p.kv_heads);
             const int n = (b.len + kTile - 1) / kTile;
             const int per_head = n - b.index, steps = per_head * p.group;
-            ok = mbar_wait_warp(kv_full, kv_phase, abort_flag, p.status, 535);
+            ok = mbar_wait_warp(v_full, v_phase, abort_flag, p.status, 535);
             if (!ok) break;
-            kv_phase ^= 1u;
+            v_phase ^= 1u;
             ok = mbar_wait_warp(do_full + 8 * d.stage, d.phase, abort_flag, p.status, 536);
             if (!ok) break;
             tc_fence_after();
             if (elect_one()) {
                 mma_scores<kD>(tm_dp, v_tile, do_ring + d.stage * B::kTileBytes, idesc_s, p.dim_steps);
                 umma_commit_cta1(dp_full);
+                if (steps == 1) umma_commit_cta1(v_empty);
             }
             __syncwarp();
             int i = b.index;
@@ -923,9 +933,9 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
                     if (more) {
                         mma_scores<kD>(tm_dp, v_tile, next_do, idesc_s, p.dim_steps);
                         umma_commit_cta1(dp_full);
+                        if (st + 2 == steps) umma_commit_cta1(v_empty);
                     } else {
                         umma_commit_cta1(done);
-                        umma_commit_cta1(kv_empty);
                     }
                 }
                 __syncwarp();
@@ -1051,7 +1061,7 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
     const uint32_t q_tile = base, do_tile = base + B::kTileBytes, k_ring = base + B::kLongAt, v_ring = base + B::kShortAt;
     const uint32_t bars = base + B::kBars;
     const uint32_t k_full = bars, k_empty = bars + 24, v_full = bars + 48, v_empty = bars + 64, q_full = bars + 80, q_empty = bars + 88,
-                   s_full = bars + 96, s_free = bars + 112, dp_full = bars + 128, ds_ready = bars + 136, done = bars + 152;
+                   s_full = bars + 96, s_free = bars + 112, dp_full = bars + 128, ds_ready = bars + 136, done = bars + 152, do_full = bars + 168, do_empty = bars + 176;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + B::kBars + 160);
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + B::kBars + 164);
 
@@ -1070,6 +1080,8 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
         }
         mbar_init(q_full, 1);
         mbar_init(q_empty, 1);
+        mbar_init(do_full, 1);
+        mbar_init(do_empty, 1);
         mbar_init(dp_full, 1);
         mbar_init(done, 1);
         *abort_flag = 0;
@@ -1091,7 +1103,7 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
     const int64_t items = static_cast<int64_t>(warp_uniform(*p.num_blocks)) * p.heads;
 
     if (warp == 0) {
-        // q, do and the key tiles
+        // q and the key tiles
         if (lane == 0) {
             Ring k;
             uint32_t q_phase = 1u;
@@ -1102,9 +1114,8 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
                 ok = mbar_wait(q_empty, q_phase, abort_flag, p.status, 521);
                 if (!ok) break;
                 q_phase ^= 1u;
-                mbar_expect_tx(q_full, 2 * B::kTileBytes);
+                mbar_expect_tx(q_full, B::kTileBytes);
                 load_tile<kD>(q_tile, &map_q, q_full, head, b.start + b.index * kTile);
-                load_tile<kD>(do_tile, &map_do, q_full, head, b.start + b.index * kTile);
                 for (int j = 0; ok && j <= b.index; ++j) {
                     ok = mbar_wait(k_empty + 8 * k.stage, k.phase ^ 1u, abort_flag, p.status, 522);
                     if (!ok) break;
@@ -1116,13 +1127,19 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
         }
         __syncwarp();
     } else if (warp == 3) {
-        // value tiles
+        // do and the value tiles
         if (lane == 0) {
             Ring v;
+            uint32_t do_phase = 1u;
             bool ok = true;
             for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
                 const Block b = p.blocks[it / p.heads];
-                const int kv_head = static_cast<int>(it % p.heads) / p.group;
+                const int head = static_cast<int>(it % p.heads), kv_head = head / p.group;
+                ok = mbar_wait(do_empty, do_phase, abort_flag, p.status, 548);
+                if (!ok) break;
+                do_phase ^= 1u;
+                mbar_expect_tx(do_full, B::kTileBytes);
+                load_tile<kD>(do_tile, &map_do, do_full, head, b.start + b.index * kTile);
                 for (int j = 0; ok && j <= b.index; ++j) {
                     ok = mbar_wait(v_empty + 8 * v.stage, v.phase ^ 1u, abort_flag, p.status, 541);
                     if (!ok) break;
@@ -1152,6 +1169,7 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
                 if (elect_one()) {
                     mma_scores<kD>(tmem + buf.stage * kTile, q_tile, k_ring + k.stage * B::kTileBytes, idesc_s, p.dim_steps);
                     umma_commit_cta1(s_full + 8 * buf.stage);
+                    if (j == b.index) umma_commit_cta1(q_empty);
                 }
                 __syncwarp();
                 k.next(B::kLong);
@@ -1163,19 +1181,20 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
         const uint32_t idesc_s = make_idesc(kTile, kTile, false, false, p.ab_format);
         const uint32_t idesc_d = make_idesc(kTile, p.dim_steps * 16, false, true, p.ab_format);
         Ring k, v;
-        uint32_t q_phase = 0, ds_phase = 0;
+        uint32_t do_phase = 0, ds_phase = 0;
         bool ok = true;
         for (int64_t turn = 0, it; ok && (it = work_item(turn)) < items; ++turn) {
             const Block b = load_block(p.blocks + it / p.heads);
-            ok = mbar_wait_warp(q_full, q_phase, abort_flag, p.status, 543);
+            ok = mbar_wait_warp(do_full, do_phase, abort_flag, p.status, 543);
             if (ok) ok = mbar_wait_warp(v_full + 8 * v.stage, v.phase, abort_flag, p.status, 544);
             if (!ok) break;
-            q_phase ^= 1u;
+            do_phase ^= 1u;
             tc_fence_after();
             if (elect_one()) {
                 mma_scores<kD>(tm_dp, do_tile, v_ring + v.stage * B::kTileBytes, idesc_s, p.dim_steps);
                 umma_commit_cta1(dp_full);
                 umma_commit_cta1(v_empty + 8 * v.stage);
+                if (b.index == 0) umma_commit_cta1(do_empty);
             }
             __syncwarp();
             v.next(B::kShort);
@@ -1206,9 +1225,9 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
                         mma_scores<kD>(tm_dp, do_tile, v_ring + v.stage * B::kTileBytes, idesc_s, p.dim_steps);
                         umma_commit_cta1(dp_full);
                         umma_commit_cta1(v_empty + 8 * v.stage);
+                        if (j + 1 == b.index) umma_commit_cta1(do_empty);
                     } else {
                         umma_commit_cta1(done);
-                        umma_commit_cta1(q_empty);  // every s has been read: ds of the last one is here
                     }
                 }
                 __syncwarp();
