@@ -57,6 +57,7 @@ bool make_tmap(CUtensorMap* map, int dtype, const void* base, int rank, const ui
     for (int i = 0; i < rank - 1; ++i) gstrides[i] = strides_bytes[i];
     const CUtensorMapDataType dt = dtype == kDtypeBF16  ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                    : dtype == kDtypeF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                   : dtype == kDtypeU8  ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                                         : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
     const auto encode = [&] {
         return fn(map, dt, static_cast<cuuint32_t>(rank), const_cast<void*>(base), gdims, gstrides, gbox, estr,

@@ -24,6 +24,8 @@
 // Rows beyond a sequence's end inside a tile belong to other sequences: their scores are masked by
 // selection, and where a masked (zero) probability would multiply such a row, the row is zeroed in shared
 // memory first, so that not even a NaN crosses over. Every wait is bounded, as in the grouped GEMM.
+#include <cuda_fp8.h>
+
 #include <type_traits>
 
 #include "common.cuh"
@@ -61,6 +63,8 @@ struct Params {
     float scale, scale_log2;
     void* out;         // forward: o
     float* lse;        // [heads][pad_rows], log2 units; may be NULL in the forward pass
+    uint8_t* rest;     // [tokens, heads, rest_row]: what out's rounding took away; NULL when lse is
+    int64_t rest_row;  // dim, rounded up to 16
     const float* delta;
     void* dq;
     void* dk;
@@ -232,6 +236,12 @@ __device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t second
         umma_ts_cta1(d, a + (kk >> 2) * second + (kk & 3) * 8, b + row_step(kk), idesc, (accumulate || kk != 0) ? 1u : 0u);
 }
 
+// What rounding o to T takes away is kept in 8 bits (e5m2, times a power of two that puts the residue of values from
+// 2^-16 to 2^12 into its range; beyond it saturates or underflows). delta = o . do is subtracted for every key of a
+// row, so an error of o would not average out over the keys; two mantissa bits leave an eighth of it at most.
+template <typename T>
+constexpr float kRestScale = std::is_same<T, __half>::value ? 32768.f : 4096.f;
+
 // 16-byte pieces of one row of kD float32 values in tensor memory, scaled and rounded, to global memory.
 template <typename T, int kD>
 __device__ __forceinline__ void store_row(uint32_t taddr, T* dst, int dim, float scale, bool valid) {
@@ -252,6 +262,100 @@ __device__ __forceinline__ void store_row(uint32_t taddr, T* dst, int dim, float
                 *reinterpret_cast<uint4*>(dst + c * 32 + q * 8) = v;
             }
         }
+    }
+}
+
+// Byte `at` of a staging tile as a bulk store with 128-byte swizzle reads it (tile 1024-byte aligned).
+__device__ __forceinline__ uint32_t swizzled(uint32_t at) { return at ^ ((at >> 7 & 7u) << 4); }
+__device__ __forceinline__ void st_shared16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// What rounding took from eight values, one byte each.
+template <typename T>
+__device__ __forceinline__ uint2 rest8(const uint32_t* r, float scale) {
+    uint32_t two[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float a = __uint_as_float(r[2 * e]) * scale, b = __uint_as_float(r[2 * e + 1]) * scale;
+        const float2 f = unpack2<T>(pack2<T>(a, b));
+        two[e] = __nv_cvt_float2_to_fp8x2(make_float2((a - f.x) * kRestScale<T>, (b - f.y) * kRestScale<T>), __NV_SATFINITE, __NV_E5M2);
+    }
+    return make_uint2(two[0] | two[1] << 16, two[2] | two[3] << 16);
+}
+
+// The output rows of one warp (32 of a tile, one a lane) and, with `save`, what their rounding took away. Full
+// groups of rows leave through bulk tensor stores from the warp's 4 KB staging tile: 32 rows written 16 bytes a lane
+// straight from registers would take the load/store unit 32 cycles an instruction, some 4000 cycles a work item. Rows
+// at a sequence's end go that way, since a tile's store would run into the next sequence.
+template <typename T, int kD>
+__device__ __forceinline__ void store_output(uint32_t o_addr, uint32_t staging, const CUtensorMap* map_out, const CUtensorMap* map_rest,
+                                             T* out, uint8_t* rest, int64_t rest_row, int64_t token, int rows, int heads, int head,
+                                             int dim, float scale, int lane) {
+    if (rows <= 0) return;
+    if (rows < 32) {
+        const int64_t row = (token + lane) * heads + head;
+        store_row<T, kD>(o_addr, out + row * dim, dim, scale, lane < rows);
+        if (rest == nullptr) return;
+#pragma unroll 1
+        for (int c = 0; c < kD / 32; ++c) {
+            uint32_t r[32];
+            tmem_ld32(o_addr + c * 32, r);
+            tmem_ld_wait();
+            tmem_tie32(r);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (lane < rows && c * 32 + q * 8 < dim)
+                    *reinterpret_cast<uint2*>(rest + row * rest_row + c * 32 + q * 8) = rest8<T>(r + q * 8, scale);
+        }
+        return;
+    }
+#pragma unroll 1
+    for (int c = 0; c < kD / 32; ++c) {
+        uint32_t r[32];
+        tmem_ld32(o_addr + c * 32, r);
+        if ((c & 1) == 0) {
+            if (lane == 0) bulk_wait_read<0>();  // the store that used the tile last has read it
+            __syncwarp();
+        }
+        tmem_ld_wait();
+        tmem_tie32(r);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                w[e] = pack2<T>(__uint_as_float(r[q * 8 + 2 * e]) * scale, __uint_as_float(r[q * 8 + 2 * e + 1]) * scale);
+            st_shared16(staging + swizzled(lane * 128 + ((c & 1) * 4 + q) * 16), w[0], w[1], w[2], w[3]);
+        }
+        if (c & 1) {
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0 && (c - 1) * 32 < dim) {
+                tma_store_3d(map_out, staging, (c - 1) * 32, head, static_cast<int>(token));
+                bulk_commit();
+            }
+        }
+    }
+    if (rest == nullptr) return;
+    if (lane == 0) bulk_wait_read<0>();
+    __syncwarp();
+#pragma unroll 1
+    for (int c = 0; c < kD / 32; ++c) {
+        uint32_t r[32];
+        tmem_ld32(o_addr + c * 32, r);
+        tmem_ld_wait();
+        tmem_tie32(r);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint2 a = rest8<T>(r + h * 16, scale), b = rest8<T>(r + h * 16 + 8, scale);
+            st_shared16(staging + swizzled(lane * 128 + c * 32 + h * 16), a.x, a.y, b.x, b.y);
+        }
+    }
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) {
+        tma_store_3d(map_rest, staging, 0, head, static_cast<int>(token));
+        bulk_commit();
     }
 }
 
@@ -279,8 +383,10 @@ struct Ring {
 template <int kD>
 struct Forward {
     static constexpr uint32_t kTileBytes = kTile * kD * 2;
-    static constexpr int kStages = kD == 128 ? 5 : 8;
-    static constexpr uint32_t kSmem = 1024 + (2 + kStages) * kTileBytes + 256;
+    static constexpr int kStages = kD == 128 ? 4 : 8;
+    static constexpr uint32_t kStaging = 4096;  // of each compute warp
+    static constexpr uint32_t kSmem = 1024 + (2 + kStages) * kTileBytes + 8 * kStaging + 256;
+    static_assert(kSmem <= 227 * 1024, "shared memory");
     static constexpr uint32_t kO = 256;  // tensor memory: s of the two tiles at 0 and 128, o at 256 and 256 + kD
 };
 
@@ -288,13 +394,14 @@ struct Forward {
 template <typename T, int kD>
 __global__ void __launch_bounds__(kThreads, 1)
 forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-               const __grid_constant__ CUtensorMap map_v, const Params p) {
+               const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_out,
+               const __grid_constant__ CUtensorMap map_rest, const Params p) {
     using F = Forward<kD>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
     const uint32_t q_tile = base, ring = base + 2 * F::kTileBytes;
-    constexpr uint32_t kBars = (2 + F::kStages) * F::kTileBytes;
+    constexpr uint32_t kStagingAt = (2 + F::kStages) * F::kTileBytes, kBars = kStagingAt + 8 * F::kStaging;
     const uint32_t bars = base + kBars;
     const uint32_t full = bars, empty = bars + 64;
     const uint32_t q_full = bars + 128, q_empty = bars + 144, s_full = bars + 160, o_full = bars + 176;
@@ -536,14 +643,16 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             if (!ok) break;
             o_phase ^= 1u;
             tc_fence_after();
-            const int r = row0 + t * kTile + row;
+            const int r = row0 + t * kTile + row, first = r - lane;
             const bool valid = r < b.len;
-            T* dst = static_cast<T*>(p.out) + (static_cast<int64_t>(b.start + r) * p.heads + head) * p.dim;
-            store_row<T, kD>(o_addr, dst, p.dim, 1.f / l, valid);
+            store_output<T, kD>(o_addr, base + kStagingAt + (warp - 4) * F::kStaging, &map_out, &map_rest, static_cast<T*>(p.out),
+                                p.rest, p.rest_row, static_cast<int64_t>(b.start) + first, min(32, b.len - first), p.heads, head, p.dim,
+                                1.f / l, lane);
             if (p.lse != nullptr && valid) p.lse[head * p.pad_rows + b.pad + r] = m + lg2(l);
             tc_fence_before();
         }
     }
+    if (warp >= 4 && lane == 0) bulk_wait_read<0>();  // the staging tiles stay until the last stores have read them
     tc_fence_before();
     __syncthreads();
     if (warp == 1) {
@@ -572,75 +681,90 @@ __device__ __forceinline__ float ds_factor<__half>(const Params& p) {
     return exp2f(static_cast<float>(min(max(14 - ilogbf(bound), -100), 100)));
 }
 
-// delta_i = o_i . do_i for every owned row and head; for fp16 also max |do| and max |v| (over bit patterns, whose
-// order does not depend on that of the atomics). A CTA takes kDeltaRows rows at a time: it looks their sequences up
-// once, then groups of kD / 8 lanes take one head of one row each, 16 bytes a lane.
-constexpr int kDeltaRows = 16;
-template <typename T, int kD, typename IntT>
-__global__ void __launch_bounds__(256)
-delta_kernel(const T* __restrict__ o, const T* __restrict__ d_o, const T* __restrict__ v, int64_t v_token, int64_t v_head,
-             const IntT* __restrict__ cu, int64_t batch, int64_t total, float* __restrict__ delta, uint32_t* absmax, const Params p) {
+// delta_i = o_i . do_i for every row of every block and head, o with what its rounding took away; for fp16 also max |do| and max |v| (over bit
+// patterns, whose order does not depend on that of the atomics). A CTA takes kDeltaRows rows of a block of the plan;
+// groups of kD / 8 lanes take one head of one row each, 16 bytes a lane, four at a time.
+constexpr int kDeltaRows = 16, kDeltaThreads = 256;
+template <typename T, int kD>
+__global__ void __launch_bounds__(kDeltaThreads, 3)
+delta_kernel(const T* __restrict__ o, const uint8_t* __restrict__ rest, const T* __restrict__ d_o, const T* __restrict__ v, int64_t v_token, int64_t v_head,
+             float* __restrict__ delta, uint32_t* absmax, const Params p) {
     constexpr bool kHalf = std::is_same<T, __half>::value;
-    constexpr int kLanes = kD / 8;
-    __shared__ int at[kDeltaRows];  // entry in the row statistics, -1 for nobody's row
-    __shared__ uint32_t most[2];
-    if (threadIdx.x < 2) most[threadIdx.x] = 0;
+    constexpr int kLanes = kD / 8, kSlots = kDeltaThreads / kLanes, kBatch = 4;
+    constexpr int kParts = kTile / kDeltaRows;
+    if (static_cast<int>(blockIdx.x) / kParts >= *p.num_blocks) return;
+    const Block b = p.blocks[blockIdx.x / kParts];
+    const int first = b.index * kTile + static_cast<int>(blockIdx.x % kParts) * kDeltaRows;  // row of the sequence
+    const int rows = min(kDeltaRows, b.len - first);
+    if (rows <= 0) return;
     const int sub = threadIdx.x % kLanes, slot = threadIdx.x / kLanes;
     const bool in_head = sub * 8 < p.dim;
     uint32_t most_do = 0, most_v = 0;
-    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * kDeltaRows; row0 < total; row0 += static_cast<int64_t>(gridDim.x) * kDeltaRows) {
-        __syncthreads();
-        if (threadIdx.x < kDeltaRows) {
-            const int64_t row = row0 + threadIdx.x;
-            // last sequence that starts at or before the row
-            int64_t lo = 0, hi = batch - 1;
-            while (lo < hi) {
-                const int64_t mid = (lo + hi + 1) >> 1;
-                if (static_cast<int64_t>(cu[mid]) <= row) lo = mid; else hi = mid - 1;
-            }
-            int start, len;
-            sequence(cu, lo, total, &start, &len);
-            const bool owned = row >= start && row < static_cast<int64_t>(start) + len;
-            at[threadIdx.x] = owned ? pad_offset(start, lo) + static_cast<int>(row - start) : -1;
-        }
-        __syncthreads();
-        const int pairs = kDeltaRows * p.heads;
-#pragma unroll 4
-        for (int i = slot; i < pairs; i += 256 / kLanes) {  // whole warps stay together: a warp holds 32 / kLanes pairs
-            const int r = i / p.heads, h = i - r * p.heads;
-            const int where = at[r];
-            float sum = 0.f;
-            if (where >= 0 && in_head) {
-                const int64_t off = ((row0 + r) * p.heads + h) * p.dim + sub * 8;
-                const uint4 a = __ldg(reinterpret_cast<const uint4*>(o + off)), b = __ldg(reinterpret_cast<const uint4*>(d_o + off));
-                const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+    const int pairs = rows * p.heads;  // (row, head) pairs lie one after another in memory
+    const int64_t base = (static_cast<int64_t>(b.start) + first) * p.heads * p.dim + sub * 8;
+    const int64_t rest_base = (static_cast<int64_t>(b.start) + first) * p.heads * p.rest_row + sub * 8;
+    for (int i0 = slot; i0 - slot < pairs; i0 += kBatch * kSlots) {  // the same trips for every thread: whole warps shuffle
+        uint4 x[kBatch], y[kBatch];
+        uint2 z[kBatch];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const float2 x = unpack2<T>(aw[q]), y = unpack2<T>(bw[q]);
-                    sum += x.x * y.x + x.y * y.y;
-                    if (kHalf) most_do = max(most_do, __float_as_uint(fmaxf(fabsf(y.x), fabsf(y.y))));
-                }
+        for (int u = 0; u < kBatch; ++u) {
+            const int i = i0 + u * kSlots;
+            x[u] = y[u] = make_uint4(0, 0, 0, 0);
+            z[u] = make_uint2(0, 0);
+            if (i < pairs && in_head) {
+                z[u] = __ldg(reinterpret_cast<const uint2*>(rest + rest_base + static_cast<int64_t>(i) * p.rest_row));
+                x[u] = __ldg(reinterpret_cast<const uint4*>(o + base + static_cast<int64_t>(i) * p.dim));
+                y[u] = __ldg(reinterpret_cast<const uint4*>(d_o + base + static_cast<int64_t>(i) * p.dim));
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const uint32_t xw[4] = {x[u].x, x[u].y, x[u].z, x[u].w}, yw[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
+            float sum = 0.f;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float2 f = unpack2<T>(xw[q]), g = unpack2<T>(yw[q]);
+                const uint32_t two = (q < 2 ? z[u].x : z[u].y) >> ((q & 1) * 16);
+                const __half2_raw raw = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two & 0xffff), __NV_E5M2);
+                const float2 e = __half22float2(*reinterpret_cast<const __half2*>(&raw));
+                sum += fmaf(e.x, 1.f / kRestScale<T>, f.x) * g.x + fmaf(e.y, 1.f / kRestScale<T>, f.y) * g.y;
+                if (kHalf) most_do = max(most_do, __float_as_uint(fmaxf(fabsf(g.x), fabsf(g.y))));
             }
 #pragma unroll
             for (int w = kLanes / 2; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-            if (where >= 0 && sub == 0) delta[h * p.pad_rows + where] = sum;
-        }
-        if (kHalf) {
-            const int kv_pairs = kDeltaRows * p.kv_heads;
-            for (int i = slot; i < kv_pairs; i += 256 / kLanes) {
-                const int r = i / p.kv_heads, h = i - r * p.kv_heads;
-                if (at[r] < 0 || !in_head) continue;
-                const uint4 a = __ldg(reinterpret_cast<const uint4*>(v + (row0 + r) * v_token + h * v_head + sub * 8));
-                const uint32_t aw[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const float2 x = unpack2<T>(aw[q]);
-                    most_v = max(most_v, __float_as_uint(fmaxf(fabsf(x.x), fabsf(x.y))));
-                }
+            const int i = i0 + u * kSlots;
+            if (i < pairs && sub == 0) {
+                const int r = i / p.heads, h = i - r * p.heads;
+                delta[h * p.pad_rows + b.pad + first + r] = sum;
             }
         }
     }
     if (kHalf) {
+        const int kv_pairs = rows * p.kv_heads;
+        for (int i0 = slot; i0 < kv_pairs; i0 += kBatch * kSlots) {
+            uint4 x[kBatch];
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                const int i = i0 + u * kSlots;
+                x[u] = make_uint4(0, 0, 0, 0);
+                if (i < kv_pairs && in_head) {
+                    const int r = i / p.kv_heads, h = i - r * p.kv_heads;
+                    x[u] = __ldg(reinterpret_cast<const uint4*>(v + (static_cast<int64_t>(b.start) + first + r) * v_token + h * v_head + sub * 8));
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                const uint32_t xw[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float2 f = unpack2<T>(xw[q]);
+                    most_v = max(most_v, __float_as_uint(fmaxf(fabsf(f.x), fabsf(f.y))));
+                }
+            }
+        }
+        __shared__ uint32_t most[2];
+        if (threadIdx.x < 2) most[threadIdx.x] = 0;
+        __syncthreads();
         most_do = __reduce_max_sync(0xffffffffu, most_do);
         most_v = __reduce_max_sync(0xffffffffu, most_v);
         if ((threadIdx.x & 31) == 0) {
@@ -648,7 +772,9 @@ delta_kernel(const T* __restrict__ o, const T* __restrict__ d_o, const T* __rest
             atomicMax(&most[1], most_v);
         }
         __syncthreads();
-        if (threadIdx.x < 2) atomicMax(&absmax[threadIdx.x], most[threadIdx.x]);
+        // most CTAs find a larger value there already and leave the one address alone
+        if (threadIdx.x < 2 && *static_cast<volatile uint32_t*>(absmax + threadIdx.x) < most[threadIdx.x])
+            atomicMax(&absmax[threadIdx.x], most[threadIdx.x]);
     }
 }
 
@@ -1318,12 +1444,13 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
 // Host side
 // ---------------------------------------------------------------------------------------------
 
-// [tokens, heads, dim] with token and head strides in elements; boxes of 128 tokens x 64 columns of a head.
+// [tokens, heads, dim] with token and head strides in elements; boxes of `rows` tokens x `cols` columns of a head.
 static bool stream_map(CUtensorMap* map, int dtype, const void* base, int64_t total, int heads, int dim, int64_t token_stride,
-                       int64_t head_stride) {
+                       int64_t head_stride, int rows = kTile, int cols = 64) {
+    const uint64_t size = dtype == kDtypeU8 ? 1 : 2;
     const uint64_t dims[3] = {static_cast<uint64_t>(dim), static_cast<uint64_t>(heads), static_cast<uint64_t>(total)};
-    const uint64_t strides[2] = {static_cast<uint64_t>(head_stride) * 2, static_cast<uint64_t>(token_stride) * 2};
-    const uint32_t box[3] = {64, 1, static_cast<uint32_t>(kTile)};
+    const uint64_t strides[2] = {static_cast<uint64_t>(head_stride) * size, static_cast<uint64_t>(token_stride) * size};
+    const uint32_t box[3] = {static_cast<uint32_t>(cols), 1, static_cast<uint32_t>(rows)};
     return make_tmap(map, dtype, base, 3, dims, strides, box);
 }
 
@@ -1391,6 +1518,7 @@ static Params common_params(const Call& c) {
     Params p{};
     p.heads = c.heads, p.kv_heads = c.kv_heads, p.group = c.heads / c.kv_heads, p.dim = c.dim;
     p.dim_steps = static_cast<int>(ceil_div(c.dim, 16));
+    p.rest_row = ceil_div(c.dim, 16) * 16;
     p.pad_rows = (c.total / kTile + c.batch + 1) * kTile;
     p.scale = c.scale;
     p.scale_log2 = c.scale * 1.4426950408889634f;  // log2(e): exp(scale s) = 2^(scale_log2 s)
@@ -1405,7 +1533,7 @@ static unsigned grid_for(int64_t items) {
 }
 
 template <typename T, int kD>
-static int run_forward(const Call& c, void* out, float* lse) {
+static int run_forward(const Call& c, void* out, float* lse, uint8_t* rest) {
     CUtensorMap mq, mk, mv;
     if (!stream_map(&mq, c.dtype, c.q, c.total, c.heads, c.dim, c.q_token, c.q_head) ||
         !stream_map(&mk, c.dtype, c.k, c.total, c.kv_heads, c.dim, c.k_token, c.k_head) ||
@@ -1417,14 +1545,18 @@ static int run_forward(const Call& c, void* out, float* lse) {
     const int status = launch_plan(c.cu, c.cu_is_int64, c.batch, c.total, 2 * kTile, w, 1, zo, none, none, c.stream);
     if (status != XMA_OK) return status;
     Params p = common_params(c);
-    p.blocks = w.list0, p.num_blocks = w.counts, p.out = out, p.lse = lse;
+    p.blocks = w.list0, p.num_blocks = w.counts, p.out = out, p.lse = lse, p.rest = rest;
+    CUtensorMap mo, mr = mq;
+    if (!stream_map(&mo, c.dtype, out, c.total, c.heads, c.dim, static_cast<int64_t>(c.heads) * c.dim, c.dim, 32)) return XMA_ERR_DRIVER;
+    if (rest != nullptr && !stream_map(&mr, kDtypeU8, rest, c.total, c.heads, static_cast<int>(p.rest_row), c.heads * p.rest_row, p.rest_row, 32, 128))
+        return XMA_ERR_DRIVER;
     const unsigned grid = grid_for(list_capacity(c.total, c.batch, 2 * kTile) * c.heads);
-    forward_kernel<T, kD><<<grid, kThreads, Forward<kD>::kSmem, c.stream>>>(mq, mk, mv, p);
+    forward_kernel<T, kD><<<grid, kThreads, Forward<kD>::kSmem, c.stream>>>(mq, mk, mv, mo, mr, p);
     return launch_status();
 }
 
 template <typename T, int kD>
-static int run_backward(const Call& c, const void* out, const void* d_out, const float* lse, float* delta, void* dq, void* dk, void* dv) {
+static int run_backward(const Call& c, const void* out, const uint8_t* rest, const void* d_out, const float* lse, float* delta, void* dq, void* dk, void* dv) {
     CUtensorMap mq, mk, mv, mdo;
     const int64_t o_token = static_cast<int64_t>(c.heads) * c.dim;
     if (!stream_map(&mq, c.dtype, c.q, c.total, c.heads, c.dim, c.q_token, c.q_head) ||
@@ -1441,19 +1573,12 @@ static int run_backward(const Call& c, const void* out, const void* d_out, const
     if (status != XMA_OK || c.batch == 0) return status;
     Params p = common_params(c);
     p.lse = const_cast<float*>(lse), p.delta = delta, p.dq = dq, p.dk = dk, p.dv = dv, p.absmax = w.absmax;
-    const int64_t chunks = ceil_div(c.total, kDeltaRows), most = static_cast<int64_t>(sm_count()) * 8;
-    const unsigned grid = static_cast<unsigned>(chunks < most ? chunks : most);
-    if (c.cu_is_int64)
-        delta_kernel<T, kD, int64_t><<<grid, 256, 0, c.stream>>>(
-            static_cast<const T*>(out), static_cast<const T*>(d_out), static_cast<const T*>(c.v), c.v_token, c.v_head,
-            static_cast<const int64_t*>(c.cu), c.batch, c.total, delta, w.absmax, p);
-    else
-        delta_kernel<T, kD, int32_t><<<grid, 256, 0, c.stream>>>(
-            static_cast<const T*>(out), static_cast<const T*>(d_out), static_cast<const T*>(c.v), c.v_token, c.v_head,
-            static_cast<const int32_t*>(c.cu), c.batch, c.total, delta, w.absmax, p);
+    const int64_t blocks = list_capacity(c.total, c.batch, kTile);
+    p.blocks = w.list0, p.num_blocks = w.counts;
+    delta_kernel<T, kD><<<static_cast<unsigned>(blocks * (kTile / kDeltaRows)), kDeltaThreads, 0, c.stream>>>(
+        static_cast<const T*>(out), rest, static_cast<const T*>(d_out), static_cast<const T*>(c.v), c.v_token, c.v_head, delta, w.absmax, p);
     status = launch_status();
     if (status != XMA_OK) return status;
-    const int64_t blocks = list_capacity(c.total, c.batch, kTile);
     p.blocks = w.list1, p.num_blocks = w.counts + 1;
     dkdv_kernel<T, kD><<<grid_for(blocks * c.kv_heads), kThreads, Backward<kD>::kSmem, c.stream>>>(mq, mk, mv, mdo, p);
     status = launch_status();
@@ -1480,37 +1605,40 @@ int64_t xma_attention_stat_rows(int64_t total, int64_t batch) {
 int xma_attention_forward(const void* q, const void* k, const void* v, int64_t q_token, int64_t q_head, int64_t k_token,
                           int64_t k_head, int64_t v_token, int64_t v_head, int32_t dtype, const void* cu_seqlens,
                           int32_t cu_is_int64, int64_t batch, int64_t total, int32_t heads, int32_t kv_heads, int32_t dim,
-                          float scale, void* out, float* lse, void* workspace, int32_t* status, void* stream) {
+                          float scale, void* out, float* lse, void* out_rest, void* workspace, int32_t* status, void* stream) {
     using namespace xma;
     using namespace xma::attn;
     const Call c{q, k, v, q_token, q_head, k_token, k_head, v_token, v_head, dtype, cu_seqlens, cu_is_int64, batch, total,
                  heads, kv_heads, dim, scale, workspace, status, static_cast<cudaStream_t>(stream)};
     const int rc = check_call(c);
     if (rc != XMA_OK || total == 0) return rc;
-    if (!out || !aligned16(out)) return XMA_ERR_BAD_ARG;
-    if (dtype == kDtypeBF16) return dim <= 64 ? run_forward<__nv_bfloat16, 64>(c, out, lse) : run_forward<__nv_bfloat16, 128>(c, out, lse);
-    return dim <= 64 ? run_forward<__half, 64>(c, out, lse) : run_forward<__half, 128>(c, out, lse);
+    if (!out || !aligned16(out) || !aligned16(out_rest) || (lse == nullptr) != (out_rest == nullptr)) return XMA_ERR_BAD_ARG;
+    uint8_t* rest = static_cast<uint8_t*>(out_rest);
+    if (dtype == kDtypeBF16)
+        return dim <= 64 ? run_forward<__nv_bfloat16, 64>(c, out, lse, rest) : run_forward<__nv_bfloat16, 128>(c, out, lse, rest);
+    return dim <= 64 ? run_forward<__half, 64>(c, out, lse, rest) : run_forward<__half, 128>(c, out, lse, rest);
 }
 
 int xma_attention_backward(const void* q, const void* k, const void* v, int64_t q_token, int64_t q_head, int64_t k_token,
                            int64_t k_head, int64_t v_token, int64_t v_head, int32_t dtype, const void* cu_seqlens,
                            int32_t cu_is_int64, int64_t batch, int64_t total, int32_t heads, int32_t kv_heads, int32_t dim,
-                           float scale, const void* out, const void* d_out, const float* lse, float* delta, void* dq, void* dk,
-                           void* dv, void* workspace, int32_t* status, void* stream) {
+                           float scale, const void* out, const void* out_rest, const void* d_out, const float* lse, float* delta,
+                           void* dq, void* dk, void* dv, void* workspace, int32_t* status, void* stream) {
     using namespace xma;
     using namespace xma::attn;
     const Call c{q, k, v, q_token, q_head, k_token, k_head, v_token, v_head, dtype, cu_seqlens, cu_is_int64, batch, total,
                  heads, kv_heads, dim, scale, workspace, status, static_cast<cudaStream_t>(stream)};
     const int rc = check_call(c);
     if (rc != XMA_OK || total == 0) return rc;
-    const void* need[] = {out, d_out, lse, delta, dq, dk, dv};
-    for (int i = 0; i < 7; ++i)
+    const void* need[] = {out, out_rest, d_out, lse, delta, dq, dk, dv};
+    for (int i = 0; i < 8; ++i)
         if (need[i] == nullptr || !aligned16(need[i])) return XMA_ERR_BAD_ARG;
+    const uint8_t* rest = static_cast<const uint8_t*>(out_rest);
     if (dtype == kDtypeBF16)
-        return dim <= 64 ? run_backward<__nv_bfloat16, 64>(c, out, d_out, lse, delta, dq, dk, dv)
-                         : run_backward<__nv_bfloat16, 128>(c, out, d_out, lse, delta, dq, dk, dv);
-    return dim <= 64 ? run_backward<__half, 64>(c, out, d_out, lse, delta, dq, dk, dv)
-                     : run_backward<__half, 128>(c, out, d_out, lse, delta, dq, dk, dv);
+        return dim <= 64 ? run_backward<__nv_bfloat16, 64>(c, out, rest, d_out, lse, delta, dq, dk, dv)
+                         : run_backward<__nv_bfloat16, 128>(c, out, rest, d_out, lse, delta, dq, dk, dv);
+    return dim <= 64 ? run_backward<__half, 64>(c, out, rest, d_out, lse, delta, dq, dk, dv)
+                     : run_backward<__half, 128>(c, out, rest, d_out, lse, delta, dq, dk, dv);
 }
 
 }  // extern "C"

@@ -15,6 +15,7 @@ namespace xma {
 constexpr int kDtypeBF16 = 0;
 constexpr int kDtypeF16 = 1;
 constexpr int kDtypeF32 = 2;
+constexpr int kDtypeU8 = 3;  // tensor maps over bytes; no entry point takes it
 
 constexpr int kMaxExperts = 1024;
 

@@ -66,10 +66,10 @@ _SIGNATURES = {
     "xma_attention_stat_rows": (c_int64, [c_int64, c_int64]),
     "xma_attention_forward": (
         c_int32, [c_void_p] * 3 + [c_int64] * 6 + [c_int32, c_void_p, c_int32, c_int64, c_int64] + [c_int32] * 3
-        + [c_float] + [c_void_p] * 5),
+        + [c_float] + [c_void_p] * 6),
     "xma_attention_backward": (
         c_int32, [c_void_p] * 3 + [c_int64] * 6 + [c_int32, c_void_p, c_int32, c_int64, c_int64] + [c_int32] * 3
-        + [c_float] + [c_void_p] * 10),
+        + [c_float] + [c_void_p] * 11),
     "xma_ipc_get_handle": (c_int32, [c_void_p, ctypes.c_char_p]),
     "xma_ipc_open_handle": (c_int32, [ctypes.c_char_p, ctypes.POINTER(c_void_p)]),
     "xma_ipc_close_handle": (c_int32, [c_void_p]),

@@ -27,15 +27,16 @@ def _forward(q, k, v, cu_seqlens, softmax_scale: float, saving: bool):
     from ..ops import attention_packed_forward_cuda
 
     q, k, v, cu_seqlens = _tiled(q), _tiled(k), _tiled(v), cu_seqlens.contiguous()
-    total, heads, _ = q.shape
+    total, heads, dim = q.shape
     batch = cu_seqlens.numel() - 1
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = None
+    lse = out_rest = None
     if saving:
+        out_rest = torch.empty(total, heads, -(-dim // 16) * 16, dtype=torch.uint8, device=q.device)
         lse = torch.empty(heads, N.attention_stat_rows(total, batch), dtype=torch.float32, device=q.device)
     workspace = torch.empty(N.attention_workspace_bytes(total, batch), dtype=torch.uint8, device=q.device)
-    attention_packed_forward_cuda(q, k, v, cu_seqlens, softmax_scale, out, lse, workspace)
-    return out, (q, k, v, cu_seqlens, out, lse)
+    attention_packed_forward_cuda(q, k, v, cu_seqlens, softmax_scale, out, lse, out_rest, workspace)
+    return out, (q, k, v, cu_seqlens, out, out_rest, lse)
 
 
 class _AttentionPacked(torch.autograd.Function):
@@ -50,13 +51,13 @@ class _AttentionPacked(torch.autograd.Function):
     def backward(ctx, d_out):
         from ..ops import attention_packed_backward_cuda
 
-        q, k, v, cu_seqlens, out, lse = ctx.saved_tensors
+        q, k, v, cu_seqlens, out, out_rest, lse = ctx.saved_tensors
         opts = dict(dtype=q.dtype, device=q.device)
         dq, dk, dv = torch.empty(q.shape, **opts), torch.empty(k.shape, **opts), torch.empty(v.shape, **opts)
         delta = torch.empty_like(lse)
         workspace = torch.empty(N.attention_workspace_bytes(q.size(0), cu_seqlens.numel() - 1), dtype=torch.uint8, device=q.device)
         attention_packed_backward_cuda(
-            q, k, v, cu_seqlens, ctx.softmax_scale, out, d_out.contiguous(), lse, delta, dq, dk, dv, workspace)
+            q, k, v, cu_seqlens, ctx.softmax_scale, out, out_rest, d_out.contiguous(), lse, delta, dq, dk, dv, workspace)
         return dq, dk, dv, None, None
 
 
@@ -78,7 +79,8 @@ def attention_packed(
     the tokens `cu_seqlens[b] .. cu_seqlens[b + 1] - 1` (none, one or many). `softmax_scale` is positive and
     defaults to `1 / sqrt(head_dim)`.
 
-    Scores and sums are float32; probabilities are rounded to the inputs' dtype before they meet the values. Tokens
+    For a backward pass the call keeps its inputs, its output, a float32 per row and head and, so that gradients do
+    not suffer from the output's rounding, one byte per output element. Scores and sums are float32; probabilities are rounded to the inputs' dtype before they meet the values. Tokens
     that no sequence owns get zeros, in the output and in the gradients, and what they hold reaches nothing. Offsets are
     read on the device: values that are out of order or outside the stream give meaningless outputs, not an error."""
     require_cuda_backend(kernel_backend)

@@ -377,16 +377,16 @@ def _attention_args(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlen
             softmax_scale)
 
 
-@xma_op(mutates_args={"out", "lse", "workspace"})
+@xma_op(mutates_args={"out", "lse", "out_rest", "workspace"})
 def attention_packed_forward_cuda(
     q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, softmax_scale: float, out: torch.Tensor,
-    lse: torch.Tensor | None, workspace: torch.Tensor
+    lse: torch.Tensor | None, out_rest: torch.Tensor | None, workspace: torch.Tensor
 ) -> None:
     """Causal attention over a packed stream; see xma_attention_forward in include/xma_b200.h."""
     assert out.is_contiguous() and cu_seqlens.is_contiguous()
     q, k, v = _aligned(q), _aligned(k), _aligned(v)
     _launch("xma_attention_forward", q,
-        *_attention_args(q, k, v, cu_seqlens, softmax_scale), N.ptr(out), N.ptr(lse), N.ptr(workspace),
+        *_attention_args(q, k, v, cu_seqlens, softmax_scale), N.ptr(out), N.ptr(lse), N.ptr(out_rest), N.ptr(workspace),
         N.ptr(N.status_word(q.device)),
     )
 
@@ -394,13 +394,13 @@ def attention_packed_forward_cuda(
 @xma_op(mutates_args={"delta", "dq", "dk", "dv", "workspace"})
 def attention_packed_backward_cuda(
     q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, softmax_scale: float, out: torch.Tensor,
-    d_out: torch.Tensor, lse: torch.Tensor, delta: torch.Tensor, dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor,
+    out_rest: torch.Tensor, d_out: torch.Tensor, lse: torch.Tensor, delta: torch.Tensor, dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor,
     workspace: torch.Tensor
 ) -> None:
     """Gradients of attention_packed_forward_cuda; see xma_attention_backward in include/xma_b200.h."""
-    assert all(t.is_contiguous() for t in (out, d_out, lse, delta, dq, dk, dv, cu_seqlens))
+    assert all(t.is_contiguous() for t in (out, out_rest, d_out, lse, delta, dq, dk, dv, cu_seqlens))
     q, k, v, d_out = _aligned(q), _aligned(k), _aligned(v), _aligned(d_out)
     _launch("xma_attention_backward", q,
-        *_attention_args(q, k, v, cu_seqlens, softmax_scale), N.ptr(out), N.ptr(d_out), N.ptr(lse), N.ptr(delta), N.ptr(dq),
-        N.ptr(dk), N.ptr(dv), N.ptr(workspace), N.ptr(N.status_word(q.device)),
+        *_attention_args(q, k, v, cu_seqlens, softmax_scale), N.ptr(out), N.ptr(out_rest), N.ptr(d_out), N.ptr(lse), N.ptr(delta),
+        N.ptr(dq), N.ptr(dk), N.ptr(dv), N.ptr(workspace), N.ptr(N.status_word(q.device)),
     )

@@ -416,7 +416,9 @@ int xma_norm_backward(const void* dy, const void* d_stream, const void* stream_s
  *   h / (heads / kv_heads)), dim a multiple of 8 up to 128, scale positive.
  *   lse   float32 [heads, xma_attention_stat_rows(total, batch)], 16-byte aligned: the rows' log-sum-exp (base
  *         2), written by the forward pass for the backward pass; NULL when there is none
- *   delta float32, the same size, scratch of the backward pass
+ *   out_rest  bytes [total, heads, dim rounded up to 16], 16-byte aligned: what rounding took from out (e5m2,
+ *         scaled); written with lse and read by the backward pass; NULL when lse is
+ *   delta float32, the size of lse, scratch of the backward pass
  *   workspace  xma_attention_workspace_bytes(total, batch) bytes, 16-byte aligned, contents irrelevant
  * Tokens that no sequence owns (before cu_seqlens[0], from cu_seqlens[batch] on) get zeros in every output and
  * are read by nothing else. Entries of cu_seqlens outside [0, total] or out of order give meaningless values
@@ -427,12 +429,12 @@ int64_t xma_attention_stat_rows(int64_t total, int64_t batch);
 int xma_attention_forward(const void* q, const void* k, const void* v, int64_t q_token, int64_t q_head, int64_t k_token,
                           int64_t k_head, int64_t v_token, int64_t v_head, int32_t dtype, const void* cu_seqlens,
                           int32_t cu_is_int64, int64_t batch, int64_t total, int32_t heads, int32_t kv_heads, int32_t dim,
-                          float scale, void* out, float* lse, void* workspace, int32_t* status, void* stream);
+                          float scale, void* out, float* lse, void* out_rest, void* workspace, int32_t* status, void* stream);
 int xma_attention_backward(const void* q, const void* k, const void* v, int64_t q_token, int64_t q_head, int64_t k_token,
                            int64_t k_head, int64_t v_token, int64_t v_head, int32_t dtype, const void* cu_seqlens,
                            int32_t cu_is_int64, int64_t batch, int64_t total, int32_t heads, int32_t kv_heads, int32_t dim,
-                           float scale, const void* out, const void* d_out, const float* lse, float* delta, void* dq, void* dk,
-                           void* dv, void* workspace, int32_t* status, void* stream);
+                           float scale, const void* out, const void* out_rest, const void* d_out, const float* lse, float* delta,
+                           void* dq, void* dk, void* dv, void* workspace, int32_t* status, void* stream);
 
 /* Maps another process's device allocation into this process for the CURRENT device, with peer access
  * enabled: handle64 is that allocation's 64-byte cudaIpcMemHandle_t. Host-side call, no stream. */

@@ -350,3 +350,37 @@ def test_offsets_outside_the_stream_touch_nothing():
     torch.cuda.synchronize()
     assert_status_clean(q.device)
     assert (guard == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [8, 24, 64, 72, 80, 128])
+def test_what_rounding_took_is_kept(dtype, dim):
+    """The byte kept for every output element is its rounding, to the two mantissa bits of e5m2 (an eighth) and
+    float32: out plus it is that much nearer to the float32 result than half a step of out."""
+    from xma import _native as N
+    from xma.ops import attention_packed_forward_cuda
+
+    lengths = [300, 1, 31, 160]
+    q, k, v, do = make(lengths, 4, 2, dim, dtype, behind=9)
+    total, batch = q.size(0), len(lengths)
+    out = torch.empty_like(q)
+    lse = torch.empty(4, N.attention_stat_rows(total, batch), device="cuda")
+    row = -(-dim // 16) * 16
+    rest = torch.full((total, 4, row), 0x7F, dtype=torch.uint8, device="cuda")  # NaNs until they are written
+    workspace = torch.empty(N.attention_workspace_bytes(total, batch), dtype=torch.uint8, device="cuda")
+    scale = 2.0 ** (0 if dim == 8 else -3)
+    attention_packed_forward_cuda(q, k, v, offsets(lengths), scale, out, lse, rest, workspace)
+    kept = rest[..., :dim].view(torch.float8_e5m2).double() / (4096 if dtype == torch.bfloat16 else 32768)
+    owned = slice(0, sum(lengths))
+    assert kept[owned].isfinite().all()
+    taken = kept[owned].abs()
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps  # fp16 below 2^-14 steps by 2^-24, whatever the value
+    step = (2 * half_step(dtype) * out[owned].double().abs()).clamp_min(tiny)
+    assert (taken <= step * 1.13 / 2).all()  # never more than half a step (at a power of two, of the lower one)
+    assert (taken > 0.1 * step / 2).double().mean() > 0.5  # and spread over it
+    # A row with one key: p = 2^(s c - m) with m the rounded product s c, the exponent the exact one minus m, so p and
+    # with it the sum l are off 1 by 2^-24 |m| ln 2 and two steps of ex2; the output is v p / l with p rounded to 1.
+    # |m| <= 60 here, so what is taken is below 64 * 2^-24 |v|, far under the step of the type.
+    one = lengths[0]
+    value = v[one].repeat_interleave(2, 0)
+    assert torch.equal(out[one], value) and (kept[one].abs() <= 64 * F32 * value.double().abs()).all()

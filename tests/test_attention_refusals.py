@@ -50,14 +50,15 @@ def test_c_entry_refuses():
     from xma import _native as N
 
     lib, a = N.lib(), 1 << 20
-    def forward(q=a, k=a, v=a, strides=(128, 64) * 3, dt=0, cu=a, batch=1, total=4, heads=2, kv=2, dim=64, scale=0.1, out=a, ws=a):
-        return lib.xma_attention_forward(q, k, v, *strides, dt, cu, 0, batch, total, heads, kv, dim, scale, out, None, ws, None, None)
+    def forward(q=a, k=a, v=a, strides=(128, 64) * 3, dt=0, cu=a, batch=1, total=4, heads=2, kv=2, dim=64, scale=0.1, out=a, rest=None, ws=a):
+        return lib.xma_attention_forward(q, k, v, *strides, dt, cu, 0, batch, total, heads, kv, dim, scale, out, None, rest, ws, None, None)
 
     assert forward(total=0) == 0
     assert forward(q=None) == 1 and forward(out=None) == 1 and forward(ws=None) == 1 and forward(cu=None) == 1
     assert forward(q=a + 2) == 1 and forward(out=a + 8) == 1 and forward(batch=-1) == 1 and forward(total=-1) == 1
     assert forward(strides=(128, 64, 128, 60, 128, 64)) == 1 and forward(strides=(0, 64) * 3) == 1
     assert forward(scale=0.0) == 1 and forward(scale=float("nan")) == 1
+    assert forward(rest=a) == 1  # what the backward pass needs is written as a whole or not at all
     assert forward(dt=2) == 2 and forward(dim=20) == 2 and forward(dim=136) == 2 and forward(heads=3) == 2
     assert forward(batch=1 << 21) == 2 and forward(total=1 << 31) == 2
     for total, batch in ((0, 0), (1, 1), (127, 3), (128, 1), (100000, 77)):
