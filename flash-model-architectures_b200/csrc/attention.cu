@@ -703,6 +703,7 @@ delta_kernel(const T* __restrict__ o, const uint8_t* __restrict__ rest, const T*
     const int pairs = rows * p.heads;  // (row, head) pairs lie one after another in memory
     const int64_t base = (static_cast<int64_t>(b.start) + first) * p.heads * p.dim + sub * 8;
     const int64_t rest_base = (static_cast<int64_t>(b.start) + first) * p.heads * p.rest_row + sub * 8;
+    int r = slot / p.heads, h = slot - r * p.heads;  // pair i0, kept up without dividing
     for (int i0 = slot; i0 - slot < pairs; i0 += kBatch * kSlots) {  // the same trips for every thread: whole warps shuffle
         uint4 x[kBatch], y[kBatch];
         uint2 z[kBatch];
@@ -732,11 +733,8 @@ delta_kernel(const T* __restrict__ o, const uint8_t* __restrict__ rest, const T*
             }
 #pragma unroll
             for (int w = kLanes / 2; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-            const int i = i0 + u * kSlots;
-            if (i < pairs && sub == 0) {
-                const int r = i / p.heads, h = i - r * p.heads;
-                delta[h * p.pad_rows + b.pad + first + r] = sum;
-            }
+            if (r < rows && sub == 0) delta[h * p.pad_rows + b.pad + first + r] = sum;
+            for (h += kSlots; h >= p.heads; h -= p.heads) ++r;
         }
     }
     if (kHalf) {
@@ -748,7 +746,7 @@ delta_kernel(const T* __restrict__ o, const uint8_t* __restrict__ rest, const T*
                 const int i = i0 + u * kSlots;
                 x[u] = make_uint4(0, 0, 0, 0);
                 if (i < kv_pairs && in_head) {
-                    const int r = i / p.kv_heads, h = i - r * p.kv_heads;
+                    const int kr = i / p.kv_heads, kh = i - kr * p.kv_heads;
                     x[u] = __ldg(reinterpret_cast<const uint4*>(v + (static_cast<int64_t>(b.start) + first + r) * v_token + h * v_head + sub * 8));
                 }
             }
