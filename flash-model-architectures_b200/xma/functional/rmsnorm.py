@@ -14,21 +14,19 @@ _MAX_HIDDEN = 1 << 24
 
 
 def _forward(x, residual, weight, post_weight, gate, gate_mode: int, eps: float, multiplier: float, saving: bool):
-    """(y, stream or None, contiguous inputs, row statistics): the forward launch."""
+    """(y, stream or None, contiguous inputs, row statistics of both norms): the forward launch."""
     from ..ops import norm_forward_cuda
 
-    x, residual, weight, post_weight, gate = (
-        t if t is None or t.is_contiguous() else t.contiguous() for t in (x, residual, weight, post_weight, gate))
+    x = x.contiguous()
+    residual = None if residual is None else residual.contiguous()
+    weight = None if weight is None else weight.contiguous()
+    post_weight = None if post_weight is None else post_weight.contiguous()
+    gate = None if gate is None else gate.contiguous()
     y = torch.empty_like(x)
     stream = None if residual is None else torch.empty_like(residual)
-    rstd = rstd_post = None
-    if saving:
-        rows = x.numel() // x.size(-1)
-        rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
-        if post_weight is not None:
-            rstd_post = torch.empty(rows, dtype=torch.float32, device=x.device)
-    norm_forward_cuda(x, residual, weight, post_weight, gate, gate_mode, eps, multiplier, stream, y, rstd, rstd_post)
-    return y, stream, (x, weight, post_weight, gate), (rstd, rstd_post)
+    rstd = torch.empty(2, x.numel() // x.size(-1), dtype=torch.float32, device=x.device) if saving else None
+    norm_forward_cuda(x, residual, weight, post_weight, gate, gate_mode, eps, multiplier, stream, y, rstd)
+    return y, stream, (x, weight, post_weight, gate), rstd
 
 
 class _Norm(torch.autograd.Function):
@@ -36,10 +34,10 @@ class _Norm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, residual, weight, post_weight, gate, gate_mode: int, eps: float, multiplier: float):
-        y, stream, (x, weight, post_weight, gate), (rstd, rstd_post) = _forward(
+        y, stream, (x, weight, post_weight, gate), rstd = _forward(
             x, residual, weight, post_weight, gate, gate_mode, eps, multiplier, True)
         branch = x if post_weight is not None or gate is not None else None  # a plain residual add needs no input
-        ctx.save_for_backward(x if residual is None else stream, branch, weight, post_weight, gate, rstd, rstd_post)
+        ctx.save_for_backward(x if residual is None else stream, branch, weight, post_weight, gate, rstd)
         ctx.dtype, ctx.alone = x.dtype, residual is None
         ctx.gate_mode, ctx.multiplier = gate_mode, multiplier
         ctx.set_materialize_grads(False)
@@ -49,7 +47,7 @@ class _Norm(torch.autograd.Function):
     def backward(ctx, dy, d_stream=None):
         from ..ops import norm_backward_cuda
 
-        stream, x, weight, post_weight, gate, rstd, rstd_post = ctx.saved_tensors
+        stream, x, weight, post_weight, gate, rstd = ctx.saved_tensors
         dy = None if dy is None else dy.contiguous()
         d_stream = None if d_stream is None else d_stream.contiguous()
         want_x, want_residual, want_weight, want_post, want_gate = ctx.needs_input_grad[:5]
@@ -72,7 +70,7 @@ class _Norm(torch.autograd.Function):
             workspace = torch.empty(N.norm_workspace_floats(stream.numel() // hidden, hidden), dtype=torch.float32, device=stream.device)
             norm_backward_cuda(
                 dy, d_stream, stream, x, weight, post_weight, gate, ctx.gate_mode, ctx.dtype, ctx.multiplier, rstd,
-                rstd_post, dx, d_residual, d_gate, d_weight, d_post, workspace)
+                dx, d_residual, d_gate, d_weight, d_post, workspace)
         if ctx.alone:
             return d_residual, None, d_weight, None, None, None, None, None
         if shared:

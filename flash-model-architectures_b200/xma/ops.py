@@ -315,17 +315,26 @@ def pack_unpack_sequence_cuda(
 
 
 def _f32_params(weight: torch.Tensor | None, post_weight: torch.Tensor | None, gate: torch.Tensor | None) -> int:
-    return sum(bit for bit, t in ((1, weight), (2, post_weight), (4, gate)) if t is not None and t.dtype == torch.float32)
+    f32 = torch.float32
+    return ((weight is not None and weight.dtype is f32) + 2 * (post_weight is not None and post_weight.dtype is f32)
+            + 4 * (gate is not None and gate.dtype is f32))
 
 
-@xma_op(mutates_args={"stream_out", "y", "rstd", "rstd_post"})
+def _rstd_ptrs(rstd: torch.Tensor | None, post_weight: torch.Tensor | None, rows: int) -> tuple[int | None, int | None]:
+    if rstd is None:
+        return None, None
+    base = rstd.data_ptr()
+    return base, None if post_weight is None else base + 4 * rows
+
+
+@xma_op(mutates_args={"stream_out", "y", "rstd"})
 def norm_forward_cuda(
     x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor | None, post_weight: torch.Tensor | None,
     gate: torch.Tensor | None, gate_mode: int, eps: float, multiplier: float, stream_out: torch.Tensor | None,
-    y: torch.Tensor, rstd: torch.Tensor | None, rstd_post: torch.Tensor | None
+    y: torch.Tensor, rstd: torch.Tensor | None
 ) -> None:
-    """stream_out = residual + multiplier * gate * norm(x; post_weight), y = norm(stream_out; weight); see
-    xma_norm_forward in include/xma_b200.h."""
+    """stream_out = residual + multiplier * gate * norm(x; post_weight), y = norm(stream_out; weight); `rstd` [2, rows] takes
+    the reciprocals of both norms' roots; see xma_norm_forward in include/xma_b200.h."""
     _require_cuda(x)
     assert x.is_contiguous() and (residual is None or residual.is_contiguous())
     hidden = x.size(-1)
@@ -334,7 +343,7 @@ def norm_forward_cuda(
     _launch("xma_norm_forward", x,
         N.ptr(x), N.ptr(residual), N.ptr(weight), N.ptr(post_weight), N.ptr(gate), gate_mode, N.dtype_code(x.dtype),
         N.dtype_code(stream_dtype), _f32_params(weight, post_weight, gate), rows, hidden, eps, multiplier,
-        N.ptr(stream_out), N.ptr(y), N.ptr(rstd), N.ptr(rstd_post), N.ptr(N.status_word(x.device)),
+        N.ptr(stream_out), N.ptr(y), *_rstd_ptrs(rstd, post_weight, rows), N.ptr(N.status_word(x.device)),
     )
 
 
@@ -342,7 +351,7 @@ def norm_forward_cuda(
 def norm_backward_cuda(
     dy: torch.Tensor | None, d_stream: torch.Tensor | None, stream: torch.Tensor, x: torch.Tensor | None,
     weight: torch.Tensor | None, post_weight: torch.Tensor | None, gate: torch.Tensor | None, gate_mode: int,
-    dtype: torch.dtype, multiplier: float, rstd: torch.Tensor, rstd_post: torch.Tensor | None, dx: torch.Tensor | None,
+    dtype: torch.dtype, multiplier: float, rstd: torch.Tensor, dx: torch.Tensor | None,
     d_residual: torch.Tensor | None, d_gate: torch.Tensor | None, d_weight: torch.Tensor | None,
     d_post_weight: torch.Tensor | None, workspace: torch.Tensor
 ) -> None:
@@ -353,7 +362,7 @@ def norm_backward_cuda(
     _launch("xma_norm_backward", stream,
         N.ptr(dy), N.ptr(d_stream), N.ptr(stream), N.ptr(x), N.ptr(weight), N.ptr(post_weight), N.ptr(gate), gate_mode,
         N.dtype_code(dtype), N.dtype_code(stream.dtype), _f32_params(weight, post_weight, gate), rows, hidden,
-        multiplier, N.ptr(rstd), N.ptr(rstd_post), N.ptr(dx), N.ptr(d_residual), N.ptr(d_gate), N.ptr(d_weight),
+        multiplier, *_rstd_ptrs(rstd, post_weight, rows), N.ptr(dx), N.ptr(d_residual), N.ptr(d_gate), N.ptr(d_weight),
         N.ptr(d_post_weight), N.ptr(workspace), N.ptr(N.status_word(stream.device)),
     )
 
