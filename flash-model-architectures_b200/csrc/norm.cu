@@ -64,7 +64,8 @@ struct Params {
     void* dx;
     void* d_residual;
     void* d_gate;
-    float* partials;  // [3][kPartials][hidden]: weight, post weight, channel gate
+    float* partials;  // [3][partial_rows][hidden]: weight, post weight, channel gate
+    int partial_rows; // as many as there are rows, at most kPartials
     bool want_weight, want_post, want_gate;
     float* row_sums;  // two-kernel backward: [rows][4]
     int32_t* status;
@@ -856,7 +857,7 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
     for (int which = 0; which < 3; ++which) {
         if (!want[which]) continue;
         f32x2(&acc)[kVpt][4] = which == 0 ? acc_w : which == 1 ? acc_p : acc_g;
-        float* out = p.partials + (static_cast<int64_t>(which) * kPartials + blockIdx.x) * p.hidden;
+        float* out = p.partials + (static_cast<int64_t>(which) * p.partial_rows + blockIdx.x) * p.hidden;
         float* mine = lay.slots == 1 ? out : buf + slot * p.hidden;
 #pragma unroll
         for (int v = 0; v < kVpt; ++v) {
@@ -945,7 +946,7 @@ backward_elements_kernel(const Params p, int64_t rows_per_cta) {
         if (p.dx != nullptr) static_cast<T*>(p.dx)[base + c] = Elem<T>::from_float(b);
     }
     const int64_t at = static_cast<int64_t>(blockIdx.y) * p.hidden + c;
-    const int64_t plane = static_cast<int64_t>(kPartials) * p.hidden;
+    const int64_t plane = static_cast<int64_t>(p.partial_rows) * p.hidden;
     if (p.want_weight) p.partials[at] = acc_w;
     if (p.want_post) p.partials[plane + at] = acc_p;
     if (p.want_gate) p.partials[2 * plane + at] = acc_g;
@@ -961,7 +962,7 @@ sum_kernel(const Params p, int count, void* d_weight, void* d_post, void* d_gate
     if (out == nullptr) return;
     const bool f32 = which == 0 ? p.weight_f32 : which == 1 ? p.post_f32 : p.gate_f32;
     const int c = blockIdx.x * 32 + threadIdx.x;
-    const float* src = p.partials + static_cast<int64_t>(which) * kPartials * p.hidden + c;
+    const float* src = p.partials + static_cast<int64_t>(which) * p.partial_rows * p.hidden + c;
     float sum = 0.f;
     if (c < p.hidden)
         for (int i = threadIdx.y; i < count; i += 8) sum += src[static_cast<int64_t>(i) * p.hidden];
@@ -1132,7 +1133,8 @@ static bool size_ok(int64_t rows, int64_t hidden, int32_t gate_mode) {
 extern "C" {
 
 int64_t xma_norm_workspace_floats(int64_t rows, int64_t hidden) {
-    return rows < 0 || hidden < 0 ? 0 : 3 * static_cast<int64_t>(XMA_NORM_PARTIALS) * hidden + 4 * rows;
+    if (rows < 0 || hidden < 0) return 0;
+    return 3 * (rows < XMA_NORM_PARTIALS ? rows : XMA_NORM_PARTIALS) * hidden + 4 * rows;
 }
 
 int xma_norm_forward(const void* x, const void* residual, const void* weight, const void* post_weight, const void* gate,
@@ -1182,7 +1184,8 @@ int xma_norm_backward(const void* dy, const void* d_stream, const void* stream_s
     p.dy = dy, p.d_stream = d_stream, p.s = stream_saved, p.dx = dx, p.d_residual = d_residual;
     p.d_gate = gate_mode == kGateChannel ? nullptr : d_gate;
     p.partials = workspace;
-    p.row_sums = workspace + 3 * static_cast<int64_t>(kPartials) * hidden;
+    p.partial_rows = static_cast<int>(rows < kPartials ? rows : kPartials);
+    p.row_sums = workspace + 3 * static_cast<int64_t>(p.partial_rows) * hidden;
     void* d_gate_channel = gate_mode == kGateChannel ? d_gate : nullptr;
     p.want_weight = d_weight != nullptr, p.want_post = d_post_weight != nullptr, p.want_gate = d_gate_channel != nullptr;
     p.status = status;

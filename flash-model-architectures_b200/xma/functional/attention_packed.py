@@ -79,10 +79,16 @@ def attention_packed(
     the tokens `cu_seqlens[b] .. cu_seqlens[b + 1] - 1` (none, one or many). `softmax_scale` is positive and
     defaults to `1 / sqrt(head_dim)`.
 
-    For a backward pass the call keeps its inputs, its output, a float32 per row and head and, so that gradients do
-    not suffer from the output's rounding, one byte per output element. Scores and sums are float32; probabilities are rounded to the inputs' dtype before they meet the values. Tokens
-    that no sequence owns get zeros, in the output and in the gradients, and what they hold reaches nothing. Offsets are
-    read on the device: values that are out of order or outside the stream give meaningless outputs, not an error."""
+    Scores and sums are float32; probabilities are rounded to the inputs' dtype before they meet the values. For a
+    backward pass the call keeps its inputs, its output, a float32 per row and head and, so that gradients do not suffer
+    from the output's rounding, one byte per output element; gradients are summed in a fixed order. In float16 the
+    gradient of the scores is rounded with a power-of-two factor that the batch's largest upstream gradient and value
+    set, so small gradients keep their bits without loss scaling.
+
+    Tokens that no sequence owns get zeros, in the output and in the gradients, and what they hold reaches nothing. A
+    NaN or an infinity in a value also reaches rows before it in its own sequence, as in a product with probabilities
+    that are zero there. Offsets are read on the device: values that are out of order or outside the stream give
+    meaningless outputs, not an error."""
     require_cuda_backend(kernel_backend)
     dtype, device = q.dtype, q.device
     if dtype not in (torch.bfloat16, torch.float16):

@@ -21,10 +21,13 @@ def _kernels_per_call(name: str, args: tuple) -> int:
     launch up to the size the library reports (xma_moe_index_small_limit, at most 256 experts) and
     five launches beyond (csrc/routing.cu:launch_index_build)."""
     global _index_small_limit
-    if name in ("xma_attention_forward", "xma_norm_backward"):  # a plan and the kernel; the kernel and the sums of its partials
+    if name == "xma_attention_forward":  # the plan and the kernel
         return 2
     if name == "xma_attention_backward":  # plan, row sums, dk and dv, dq
         return 4
+    if name == "xma_norm_backward":  # the kernel (two for rows that no vector fits), the sums of parameters' partials
+        gate_mode, d_gate, d_weight, d_post_weight = args[7], args[18], args[19], args[20]
+        return 1 + (d_weight is not None or d_post_weight is not None or (gate_mode == 1 and d_gate is not None))
     if name == "xma_moe_index_build":
         if _index_small_limit is None:
             _index_small_limit = int(N.lib().xma_moe_index_small_limit())
