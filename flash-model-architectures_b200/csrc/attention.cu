@@ -746,8 +746,8 @@ delta_kernel(const T* __restrict__ o, const uint8_t* __restrict__ rest, const T*
                 const int i = i0 + u * kSlots;
                 x[u] = make_uint4(0, 0, 0, 0);
                 if (i < kv_pairs && in_head) {
-                    const int kr = i / p.kv_heads, kh = i - kr * p.kv_heads;
-                    x[u] = __ldg(reinterpret_cast<const uint4*>(v + (static_cast<int64_t>(b.start) + first + r) * v_token + h * v_head + sub * 8));
+                    const int vr = i / p.kv_heads, vh = i - vr * p.kv_heads;
+                    x[u] = __ldg(reinterpret_cast<const uint4*>(v + (static_cast<int64_t>(b.start) + first + vr) * v_token + vh * v_head + sub * 8));
                 }
             }
 #pragma unroll

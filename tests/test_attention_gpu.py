@@ -384,3 +384,24 @@ def test_what_rounding_took_is_kept(dtype, dim):
     one = lengths[0]
     value = v[one].repeat_interleave(2, 0)
     assert torch.equal(out[one], value) and (kept[one].abs() <= 64 * F32 * value.double().abs()).all()
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 64), (6, 2, 128), (5, 5, 40), (16, 1, 80)])
+def test_factor_of_small_gradients(heads, kv_heads, dim):
+    """fp16: the factor that ds is rounded with comes from the largest |do| and |v| of the sequences' rows, exactly."""
+    from xma import _native as N
+    from xma.ops import attention_packed_backward_cuda, attention_packed_forward_cuda
+
+    lengths = [127, 3, 300]
+    q, k, v, do = make(lengths, heads, kv_heads, dim, torch.float16, behind=20)
+    v[-20:], do[-20:] = 1e4, 1e4
+    total = q.size(0)
+    new = lambda t: torch.empty_like(t)
+    stats = lambda: torch.empty(heads, N.attention_stat_rows(total, 3), device="cuda")
+    out, lse, delta = new(q), stats(), stats()
+    rest = torch.empty(total, heads, -(-dim // 16) * 16, dtype=torch.uint8, device="cuda")
+    workspace = torch.full((N.attention_workspace_bytes(total, 3),), 0x3C, dtype=torch.uint8, device="cuda")
+    attention_packed_forward_cuda(q, k, v, offsets(lengths), 0.1, out, lse, rest, workspace)
+    attention_packed_backward_cuda(q, k, v, offsets(lengths), 0.1, out, rest, do, lse, delta, new(q), new(k), new(v), workspace)
+    most = workspace[8:16].view(torch.float32)
+    assert most.tolist() == [do[:-20].abs().max().item(), v[:-20].abs().max().item()]
