@@ -405,3 +405,10 @@ def test_factor_of_small_gradients(heads, kv_heads, dim):
     attention_packed_backward_cuda(q, k, v, offsets(lengths), 0.1, out, rest, do, lse, delta, new(q), new(k), new(v), workspace)
     most = workspace[8:16].view(torch.float32)
     assert most.tolist() == [do[:-20].abs().max().item(), v[:-20].abs().max().item()]
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, torch.float16), (128, torch.bfloat16), (48, torch.bfloat16), (80, torch.float16)])
+def test_many_work_items(dim, dtype):
+    """More work items than SMs, of one and of two query tiles in every order: each CTA goes through several."""
+    lengths = [(37 * n * n + 11 * n) % 700 + 1 for n in range(48)]
+    check(lengths, 12, 3, dim, dtype, behind=5)
