@@ -15,6 +15,9 @@
 // sum(b x) follows from three more sums over the row's inputs (ds is linear in a, s and d), so a row
 // takes ONE reduction: with c = post * gate * x,
 //   sum(c ds) = rs sum(c a) - rs^3 mean(a s) sum(c s) + sum(c d).
+// The backward pass recomputes s from the residual and x where it reads x anyway, so that the rounding of the
+// stream does not reach the gradients; for a plain residual add it reads the rounded stream, one tensor less.
+//
 // The mean of squares adds up (v / H) v, so that it overflows where the mean itself does and no sooner.
 // All of it is bound by HBM: every tensor is read and written once.
 #include "common.cuh"
@@ -60,7 +63,7 @@ struct Params {
     // backward
     const void* dy;
     const void* d_stream;
-    const void* s;
+    const void* s;    // the stream (x for the norm alone); the residual where x is there to compute the stream from
     void* dx;
     void* d_residual;
     void* d_gate;
@@ -726,13 +729,14 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
     int previous = -1;
     for (int64_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
         const int64_t row0 = chunk * per_chunk + slot * kRows;
-        float rs[kRows], rp[kRows], token[kRows];
+        float rs[kRows], rp[kRows], token[kRows], branch[kRows];
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
             const bool valid = row0 + r < p.rows;  // the same in the whole group
             rs[r] = valid ? p.rs[row0 + r] : 0.f;
             rp[r] = valid && kX && p.post != nullptr ? p.rp[row0 + r] : 1.f;
             token[r] = valid && kX ? token_gate<T>(p, row0 + r) : 1.f;
+            branch[r] = p.multiplier * token[r] * rp[r];
         }
         if (!mbar_wait(st.full + 8 * st.stage, st.phase, st.abort_flag, p.status, 402)) {
             st.drain(lay.stages);
@@ -750,8 +754,19 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
             for (int v = 0; v < kVpt; ++v) {
                 const int c = (v * group + t) * 8;
                 if (!kKnown && c >= p.hidden) continue;
-                f32x2 a[4], s8[4], f[4];
+                f32x2 a[4], s8[4], f[4], x8[4];
                 load8(reinterpret_cast<const R*>(stage + lay.s) + off + c, s8);
+                if (kX) {
+                    f32x2 g[4];
+                    load8(reinterpret_cast<const T*>(stage + lay.x) + off + c, x8);
+                    post8(c, f);
+                    gate8(reinterpret_cast<const T*>(stage + lay.gate) + off, c, g);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        x8[j] = mul_f32x2(x8[j], mul_f32x2(f[j], g[j]));
+                        s8[j] = fma_f32x2(x8[j], both(branch[r]), s8[j]);  // the stream, from the residual
+                    }
+                }
                 if (has_dy) {
                     load8(reinterpret_cast<const T*>(stage + lay.dy) + off + c, a);
                     weight8(c, f);
@@ -765,13 +780,8 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
                     for (int j = 0; j < 4; ++j) a[j] = both(0.f);
                 }
                 if (kX) {
-                    f32x2 x8[4], g[4];
-                    load8(reinterpret_cast<const T*>(stage + lay.x) + off + c, x8);
-                    post8(c, f);
-                    gate8(reinterpret_cast<const T*>(stage + lay.gate) + off, c, g);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        x8[j] = mul_f32x2(x8[j], mul_f32x2(f[j], g[j]));
                         sum[kSums > 1 ? 1 : 0] = fma_f32x2(x8[j], a[j], sum[kSums > 1 ? 1 : 0]);
                         sum[kSums > 1 ? 2 : 0] = fma_f32x2(x8[j], s8[j], sum[kSums > 1 ? 2 : 0]);
                     }
@@ -804,7 +814,19 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
             for (int v = 0; v < kVpt; ++v) {
                 const int c = (v * group + t) * 8;
                 if (!kKnown && c >= p.hidden) continue;
-                f32x2 ds[4], f[4];
+                f32x2 ds[4], f[4], s8[4], hat[4], u[4], g[4];
+                if (has_dy || kX) load8(reinterpret_cast<const R*>(stage + lay.s) + off + c, s8);
+                if (kX) {
+                    load8(reinterpret_cast<const T*>(stage + lay.x) + off + c, hat);
+                    post8(c, f);
+                    gate8(reinterpret_cast<const T*>(stage + lay.gate) + off, c, g);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        hat[j] = mul_f32x2(hat[j], both(k.rp));
+                        u[j] = mul_f32x2(hat[j], f[j]);
+                        s8[j] = fma_f32x2(mul_f32x2(u[j], g[j]), both(k.m), s8[j]);
+                    }
+                }
                 if (has_d_stream) {
                     load8(reinterpret_cast<const R*>(stage + lay.d_stream) + off + c, ds);
                 } else {
@@ -812,14 +834,13 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
                     for (int j = 0; j < 4; ++j) ds[j] = both(0.f);
                 }
                 if (has_dy) {
-                    f32x2 d8[4], s8[4];
-                    load8(reinterpret_cast<const R*>(stage + lay.s) + off + c, s8);
+                    f32x2 d8[4], w8[4];
                     load8(reinterpret_cast<const T*>(stage + lay.dy) + off + c, d8);
-                    weight8(c, f);
+                    weight8(c, w8);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         acc_w[v][j] = fma_f32x2(d8[j], mul_f32x2(s8[j], both(k.rs)), acc_w[v][j]);
-                        ds[j] = fma_f32x2(mul_f32x2(d8[j], f[j]), both(k.rs), fma_f32x2(s8[j], both(-k.rs * k.k_s), ds[j]));
+                        ds[j] = fma_f32x2(mul_f32x2(d8[j], w8[j]), both(k.rs), fma_f32x2(s8[j], both(-k.rs * k.k_s), ds[j]));
                     }
                 }
                 if (has_d_residual) store8(static_cast<R*>(p.d_residual) + base + c, ds);
@@ -827,22 +848,15 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) b[j] = mul_f32x2(ds[j], both(k.m));  // gradient of the gated branch, token gate in it
                 if (kX) {
-                    f32x2 hat[4], g[4];
-                    load8(reinterpret_cast<const T*>(stage + lay.x) + off + c, hat);
-                    post8(c, f);
-                    gate8(reinterpret_cast<const T*>(stage + lay.gate) + off, c, g);
-                    f32x2 dg[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        hat[j] = mul_f32x2(hat[j], both(k.rp));
-                        const f32x2 u = mul_f32x2(hat[j], f[j]);
-                        if (kFull) dg[j] = mul_f32x2(b[j], u);
-                        else acc_g[v][j] = fma_f32x2(b[j], u, acc_g[v][j]);
+                        if (kFull) u[j] = mul_f32x2(b[j], u[j]);
+                        else acc_g[v][j] = fma_f32x2(b[j], u[j], acc_g[v][j]);
                         b[j] = mul_f32x2(b[j], g[j]);
                         acc_p[v][j] = fma_f32x2(b[j], hat[j], acc_p[v][j]);
                         b[j] = fma_f32x2(mul_f32x2(b[j], f[j]), both(k.rp), mul_f32x2(hat[j], both(-k.rp * k.k_x)));
                     }
-                    if (kFull && p.d_gate != nullptr) store8(static_cast<T*>(p.d_gate) + base + c, dg);
+                    if (kFull && p.d_gate != nullptr) store8(static_cast<T*>(p.d_gate) + base + c, u);
                 }
                 if (has_dx) store8(static_cast<T*>(p.dx) + base + c, b);
             }
@@ -879,7 +893,8 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
 template <typename T, typename R>
 struct Element {
     float dy, s, d, x, w, post, gate;
-    __device__ __forceinline__ Element(const Params& p, int64_t base, int c) {
+    // branch: multiplier * token gate * rp of the row
+    __device__ __forceinline__ Element(const Params& p, int64_t base, int c, float branch) {
         dy = p.dy != nullptr ? Elem<T>::to_float(static_cast<const T*>(p.dy)[base + c]) : 0.f;
         s = Elem<R>::to_float(static_cast<const R*>(p.s)[base + c]);
         d = p.d_stream != nullptr ? Elem<R>::to_float(static_cast<const R*>(p.d_stream)[base + c]) : 0.f;
@@ -889,6 +904,7 @@ struct Element {
         gate = p.gate_mode == kGateFull      ? Elem<T>::to_float(static_cast<const T*>(p.gate)[base + c])
                : p.gate_mode == kGateChannel ? param_at<T>(p.gate, p.gate_f32, c)
                                              : 1.f;
+        if (p.x != nullptr) s = fmaf(x * post * gate, branch, s);  // the stream, from the residual
     }
 };
 
@@ -901,8 +917,9 @@ backward_sums_kernel(const Params p) {
     const int64_t row = blockIdx.x;
     const int64_t base = row * p.hidden;
     float sums[4] = {0.f, 0.f, 0.f, 0.f};
+    const float branch = p.multiplier * token_gate<T>(p, row) * (p.post != nullptr ? p.rp[row] : 1.f);
     for (int c = threadIdx.x; c < p.hidden; c += blockDim.x) {
-        const Element<T, R> e(p, base, c);
+        const Element<T, R> e(p, base, c, branch);
         const float a = e.dy * e.w, q = e.x * e.post * e.gate;
         sums[0] += a * e.s;
         sums[1] += q * a;
@@ -923,11 +940,12 @@ backward_elements_kernel(const Params p, int64_t rows_per_cta) {
     if (c >= p.hidden) return;
     for (int64_t row = first; row < last; ++row) {
         const int64_t base = row * p.hidden;
-        const Element<T, R> e(p, base, c);
+        const float rp = p.post != nullptr ? p.rp[row] : 1.f, token = token_gate<T>(p, row);
+        const Element<T, R> e(p, base, c, p.multiplier * token * rp);
         float sums[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) sums[i] = p.row_sums[row * 4 + i];
-        const RowScale k = row_scale(p, sums, p.rs[row], p.post != nullptr ? p.rp[row] : 1.f, token_gate<T>(p, row));
+        const RowScale k = row_scale(p, sums, p.rs[row], rp, token);
         if (p.gate_mode == kGateToken && p.d_gate != nullptr && c == 0)
             static_cast<T*>(p.d_gate)[row] = Elem<T>::from_float(k.d_token_gate);
         acc_w += e.dy * (e.s * k.rs);
@@ -1162,7 +1180,7 @@ int xma_norm_forward(const void* x, const void* residual, const void* weight, co
     return XMA_ERR_UNSUPPORTED;
 }
 
-int xma_norm_backward(const void* dy, const void* d_stream, const void* stream_saved, const void* x, const void* weight,
+int xma_norm_backward(const void* dy, const void* d_stream, const void* stream_or_residual, const void* x, const void* weight,
                       const void* post_weight, const void* gate, int32_t gate_mode, int32_t dtype, int32_t stream_dtype,
                       int32_t f32_params, int64_t rows, int64_t hidden, float multiplier, const float* rstd,
                       const float* rstd_post, void* dx, void* d_residual, void* d_gate, void* d_weight, void* d_post_weight,
@@ -1171,7 +1189,7 @@ int xma_norm_backward(const void* dy, const void* d_stream, const void* stream_s
     using namespace xma::norm;
     if (!size_ok(rows, hidden, gate_mode)) return XMA_ERR_BAD_ARG;
     if (rows == 0) return XMA_OK;
-    if (!stream_saved || !rstd || !workspace || !aligned16(workspace)) return XMA_ERR_BAD_ARG;
+    if (!stream_or_residual || !rstd || !workspace || !aligned16(workspace)) return XMA_ERR_BAD_ARG;
     if ((gate_mode != kGateNone) != (gate != nullptr) || ((post_weight || gate) && !x) || (post_weight && !rstd_post))
         return XMA_ERR_BAD_ARG;
     if ((d_weight && !weight) || (d_post_weight && !post_weight) || (d_gate && !gate)) return XMA_ERR_BAD_ARG;
@@ -1181,7 +1199,7 @@ int xma_norm_backward(const void* dy, const void* d_stream, const void* stream_s
     p.weight_f32 = f32_params & 1, p.post_f32 = f32_params & 2, p.gate_f32 = f32_params & 4;
     p.rows = rows, p.hidden = static_cast<int>(hidden), p.multiplier = multiplier;
     p.rs = const_cast<float*>(rstd), p.rp = const_cast<float*>(rstd_post);
-    p.dy = dy, p.d_stream = d_stream, p.s = stream_saved, p.dx = dx, p.d_residual = d_residual;
+    p.dy = dy, p.d_stream = d_stream, p.s = stream_or_residual, p.dx = dx, p.d_residual = d_residual;
     p.d_gate = gate_mode == kGateChannel ? nullptr : d_gate;
     p.partials = workspace;
     p.partial_rows = static_cast<int>(rows < kPartials ? rows : kPartials);

@@ -26,7 +26,7 @@ def _forward(x, residual, weight, post_weight, gate, gate_mode: int, eps: float,
     stream = None if residual is None else torch.empty_like(residual)
     rstd = torch.empty(2, x.numel() // x.size(-1), dtype=torch.float32, device=x.device) if saving else None
     norm_forward_cuda(x, residual, weight, post_weight, gate, gate_mode, eps, multiplier, stream, y, rstd)
-    return y, stream, (x, weight, post_weight, gate), rstd
+    return y, stream, (x, residual, weight, post_weight, gate), rstd
 
 
 class _Norm(torch.autograd.Function):
@@ -34,10 +34,15 @@ class _Norm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, residual, weight, post_weight, gate, gate_mode: int, eps: float, multiplier: float):
-        y, stream, (x, weight, post_weight, gate), rstd = _forward(
+        y, stream, (x, residual, weight, post_weight, gate), rstd = _forward(
             x, residual, weight, post_weight, gate, gate_mode, eps, multiplier, True)
-        branch = x if post_weight is not None or gate is not None else None  # a plain residual add needs no input
-        ctx.save_for_backward(x if residual is None else stream, branch, weight, post_weight, gate, rstd)
+        if residual is None:
+            base, branch = x, None
+        elif post_weight is None and gate is None:
+            base, branch = stream, None  # a plain residual add: the stream alone will do
+        else:
+            base, branch = residual, x  # the stream is computed from them again, before its rounding
+        ctx.save_for_backward(base, branch, weight, post_weight, gate, rstd)
         ctx.dtype, ctx.alone = x.dtype, residual is None
         ctx.gate_mode, ctx.multiplier = gate_mode, multiplier
         ctx.set_materialize_grads(False)
@@ -47,29 +52,29 @@ class _Norm(torch.autograd.Function):
     def backward(ctx, dy, d_stream=None):
         from ..ops import norm_backward_cuda
 
-        stream, x, weight, post_weight, gate, rstd = ctx.saved_tensors
+        base, x, weight, post_weight, gate, rstd = ctx.saved_tensors
         dy = None if dy is None else dy.contiguous()
         d_stream = None if d_stream is None else d_stream.contiguous()
         want_x, want_residual, want_weight, want_post, want_gate = ctx.needs_input_grad[:5]
-        empty = stream.numel() == 0
+        empty = base.numel() == 0
 
         # The norm alone differentiates with respect to its "stream", x. A plain residual add in one type
         # gives x and the residual the same gradient: one tensor.
-        shared = not ctx.alone and x is None and ctx.multiplier == 1.0 and stream.dtype == ctx.dtype
+        shared = not ctx.alone and x is None and ctx.multiplier == 1.0 and base.dtype == ctx.dtype
         want_stream = want_x if ctx.alone else want_residual or (shared and want_x)
-        d_residual = torch.empty_like(stream) if want_stream else None
+        d_residual = torch.empty_like(base) if want_stream else None
         dx = None
         if want_x and not ctx.alone and not shared:
-            dx = torch.empty_like(stream, dtype=ctx.dtype)
+            dx = torch.empty_like(base, dtype=ctx.dtype)
         new = torch.zeros_like if empty else torch.empty_like
         d_weight = new(weight) if want_weight and weight is not None else None
         d_post = new(post_weight) if want_post and post_weight is not None else None
         d_gate = new(gate) if want_gate and gate is not None else None
         if not empty:
-            hidden = stream.size(-1)
-            workspace = torch.empty(N.norm_workspace_floats(stream.numel() // hidden, hidden), dtype=torch.float32, device=stream.device)
+            hidden = base.size(-1)
+            workspace = torch.empty(N.norm_workspace_floats(base.numel() // hidden, hidden), dtype=torch.float32, device=base.device)
             norm_backward_cuda(
-                dy, d_stream, stream, x, weight, post_weight, gate, ctx.gate_mode, ctx.dtype, ctx.multiplier, rstd,
+                dy, d_stream, base, x, weight, post_weight, gate, ctx.gate_mode, ctx.dtype, ctx.multiplier, rstd,
                 dx, d_residual, d_gate, d_weight, d_post, workspace)
         if ctx.alone:
             return d_residual, None, d_weight, None, None, None, None, None

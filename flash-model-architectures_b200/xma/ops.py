@@ -352,21 +352,22 @@ def norm_forward_cuda(
 
 @xma_op(mutates_args={"dx", "d_residual", "d_gate", "d_weight", "d_post_weight", "workspace"})
 def norm_backward_cuda(
-    dy: torch.Tensor | None, d_stream: torch.Tensor | None, stream: torch.Tensor, x: torch.Tensor | None,
+    dy: torch.Tensor | None, d_stream: torch.Tensor | None, stream_or_residual: torch.Tensor, x: torch.Tensor | None,
     weight: torch.Tensor | None, post_weight: torch.Tensor | None, gate: torch.Tensor | None, gate_mode: int,
     dtype: torch.dtype, multiplier: float, rstd: torch.Tensor, dx: torch.Tensor | None,
     d_residual: torch.Tensor | None, d_gate: torch.Tensor | None, d_weight: torch.Tensor | None,
     d_post_weight: torch.Tensor | None, workspace: torch.Tensor
 ) -> None:
-    """Gradients of norm_forward_cuda's inputs; see xma_norm_backward in include/xma_b200.h."""
-    assert stream.is_contiguous() and all(t is None or t.is_contiguous() for t in (dy, d_stream, x, gate))
-    hidden = stream.size(-1)
-    rows = stream.numel() // hidden
-    _launch("xma_norm_backward", stream,
-        N.ptr(dy), N.ptr(d_stream), N.ptr(stream), N.ptr(x), N.ptr(weight), N.ptr(post_weight), N.ptr(gate), gate_mode,
-        N.dtype_code(dtype), N.dtype_code(stream.dtype), _f32_params(weight, post_weight, gate), rows, hidden,
+    """Gradients of norm_forward_cuda's inputs, from the stream or (with a post norm or a gate) from the residual and x;
+    see xma_norm_backward in include/xma_b200.h."""
+    assert stream_or_residual.is_contiguous() and all(t is None or t.is_contiguous() for t in (dy, d_stream, x, gate))
+    hidden = stream_or_residual.size(-1)
+    rows = stream_or_residual.numel() // hidden
+    _launch("xma_norm_backward", stream_or_residual,
+        N.ptr(dy), N.ptr(d_stream), N.ptr(stream_or_residual), N.ptr(x), N.ptr(weight), N.ptr(post_weight), N.ptr(gate), gate_mode,
+        N.dtype_code(dtype), N.dtype_code(stream_or_residual.dtype), _f32_params(weight, post_weight, gate), rows, hidden,
         multiplier, *_rstd_ptrs(rstd, post_weight, rows), N.ptr(dx), N.ptr(d_residual), N.ptr(d_gate), N.ptr(d_weight),
-        N.ptr(d_post_weight), N.ptr(workspace), N.ptr(N.status_word(stream.device)),
+        N.ptr(d_post_weight), N.ptr(workspace), N.ptr(N.status_word(stream_or_residual.device)),
     )
 
 

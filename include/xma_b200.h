@@ -388,9 +388,9 @@ int xma_unpack_sequence(const void* x, const void* cu_seqlens, int32_t cu_is_int
  * aligned bases take wide accesses.
  *
  * xma_norm_backward: from dy (gradient of y) and d_stream (gradient of stream_out), either of which may be
- * NULL (zero), to d_residual, dx, d_gate, d_weight, d_post_weight; each output may be NULL. stream_saved is
- * stream_out (x for the norm alone, whose gradient is then d_residual); x is needed with a post norm or a
- * gate only. Gradients of parameters have the parameters' types and are summed over the rows in a fixed
+ * NULL (zero), to d_residual, dx, d_gate, d_weight, d_post_weight; each output may be NULL. With a post norm or a
+ * gate, stream_or_residual is the residual and x is needed; without them it is stream_out (x for the norm alone,
+ * whose gradient is then d_residual). Gradients of parameters have the parameters' types and are summed over the rows in a fixed
  * order through `workspace`: xma_norm_workspace_floats(rows, hidden) floats, 16-byte aligned, contents
  * irrelevant before and after. rows == 0 writes nothing. Code 402 or 403 goes to *status when a wait for a
  * kernel's own copies runs out.
@@ -401,7 +401,7 @@ int xma_norm_forward(const void* x, const void* residual, const void* weight, co
                      int32_t gate_mode, int32_t dtype, int32_t stream_dtype, int32_t f32_params, int64_t rows, int64_t hidden,
                      float eps, float multiplier, void* stream_out, void* y, float* rstd, float* rstd_post, int32_t* status,
                      void* stream);
-int xma_norm_backward(const void* dy, const void* d_stream, const void* stream_saved, const void* x, const void* weight,
+int xma_norm_backward(const void* dy, const void* d_stream, const void* stream_or_residual, const void* x, const void* weight,
                       const void* post_weight, const void* gate, int32_t gate_mode, int32_t dtype, int32_t stream_dtype,
                       int32_t f32_params, int64_t rows, int64_t hidden, float multiplier, const float* rstd,
                       const float* rstd_post, void* dx, void* d_residual, void* d_gate, void* d_weight, void* d_post_weight,

@@ -16,7 +16,7 @@ def half_step(dtype: torch.dtype) -> float:
 
 def norm_reference(x, residual, weight, post, gate, eps, m, dy=None, dd=None, stream_rounded=None):
     """dict name -> (value, magnitude) in float64. All inputs 2-D rows (gate broadcastable) or [H]; gradients use
-    `stream_rounded` (the stream as it was returned) where the backward pass reads it."""
+    `stream_rounded` (the stream as it was returned), if it is given, where the backward pass reads it (a plain residual add)."""
     f = lambda t: None if t is None else t.detach().double()
     x, residual, weight, post, gate, dy, dd = map(f, (x, residual, weight, post, gate, dy, dd))
     H = x.size(-1)

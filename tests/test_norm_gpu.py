@@ -50,7 +50,7 @@ def check(t, m, use=("y", "stream"), eps=EPS):
     pairs = [(out[k], d) for k, d in (("y", dy), ("stream", dd)) if k in out and d is not None]
     grads = torch.autograd.grad([o for o, _ in pairs], list(leaves.values()), [d for _, d in pairs], allow_unused=True)
     ref = norm_reference(t["x"], t.get("residual"), t["weight"], t.get("post_weight"), t.get("gate"), eps, m, dy, dd,
-                         out.get("stream"))
+                         None if t.get("post_weight") is not None or t.get("gate") is not None else out.get("stream"))
     got = {**out, **{"d_" + k: v for k, v in zip(leaves, grads)}}
     for name, value in got.items():
         if value is None:
