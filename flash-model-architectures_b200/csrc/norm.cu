@@ -70,7 +70,7 @@ struct Params {
     float* partials;  // [3][partial_rows][hidden]: weight, post weight, channel gate
     int partial_rows; // as many as there are rows, at most kPartials
     bool want_weight, want_post, want_gate;
-    float* row_sums;  // two-kernel backward: [rows][4]
+    float* row_sums;  // two-kernel backward: [rows][8], what a row's elements need
     int32_t* status;
 };
 
@@ -908,8 +908,9 @@ struct Element {
     }
 };
 
-// Any row length and alignment, in two kernels: the row sums, then the elements (a block of columns
-// times a share of the rows per CTA, so that the parameters' gradients are sums in registers).
+// Any row length and alignment, in two kernels: the row sums, from which what a row's elements need is worked out
+// once, then the elements (a block of columns times a share of the rows per CTA, so that the parameters' gradients
+// are sums in registers; four rows at a time, for loads in flight).
 template <typename T, typename R>
 __global__ void __launch_bounds__(256)
 backward_sums_kernel(const Params p) {
@@ -917,7 +918,8 @@ backward_sums_kernel(const Params p) {
     const int64_t row = blockIdx.x;
     const int64_t base = row * p.hidden;
     float sums[4] = {0.f, 0.f, 0.f, 0.f};
-    const float branch = p.multiplier * token_gate<T>(p, row) * (p.post != nullptr ? p.rp[row] : 1.f);
+    const float rp = p.post != nullptr ? p.rp[row] : 1.f, token = token_gate<T>(p, row);
+    const float branch = p.multiplier * token * rp;
     for (int c = threadIdx.x; c < p.hidden; c += blockDim.x) {
         const Element<T, R> e(p, base, c, branch);
         const float a = e.dy * e.w, q = e.x * e.post * e.gate;
@@ -927,41 +929,61 @@ backward_sums_kernel(const Params p) {
         sums[3] += q * e.d;
     }
     group_sum<4>(sums, scratch, threadIdx.x, blockDim.x, 1);
-    if (threadIdx.x < 4) p.row_sums[row * 4 + threadIdx.x] = sums[threadIdx.x];
+    if (threadIdx.x == 0) {
+        const RowScale k = row_scale(p, sums, p.rs[row], rp, token);
+        float4* out = reinterpret_cast<float4*>(p.row_sums) + row * 2;
+        out[0] = make_float4(k.rs, k.rs * k.k_s, k.rp, k.rp * k.k_x);
+        out[1] = make_float4(k.m, branch, 0.f, 0.f);
+        if (p.gate_mode == kGateToken && p.d_gate != nullptr) static_cast<T*>(p.d_gate)[row] = Elem<T>::from_float(k.d_token_gate);
+    }
 }
 
 template <typename T, typename R>
 __global__ void __launch_bounds__(256)
 backward_elements_kernel(const Params p, int64_t rows_per_cta) {
+    constexpr int kBatch = 4;
     const int c = blockIdx.x * blockDim.x + threadIdx.x;
     const int64_t first = static_cast<int64_t>(blockIdx.y) * rows_per_cta;
     const int64_t last = min(first + rows_per_cta, p.rows);
     float acc_w = 0.f, acc_p = 0.f, acc_g = 0.f;
     if (c >= p.hidden) return;
-    for (int64_t row = first; row < last; ++row) {
-        const int64_t base = row * p.hidden;
-        const float rp = p.post != nullptr ? p.rp[row] : 1.f, token = token_gate<T>(p, row);
-        const Element<T, R> e(p, base, c, p.multiplier * token * rp);
-        float sums[4];
+    const float w = param_at<T>(p.weight, p.weight_f32, c), post = param_at<T>(p.post, p.post_f32, c);
+    const float gate = p.gate_mode == kGateChannel ? param_at<T>(p.gate, p.gate_f32, c) : 1.f;
+    for (int64_t row0 = first; row0 < last; row0 += kBatch) {
+        float dy[kBatch], s[kBatch], d[kBatch], x[kBatch], g[kBatch];
+        float4 k[kBatch], k2[kBatch];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sums[i] = p.row_sums[row * 4 + i];
-        const RowScale k = row_scale(p, sums, p.rs[row], rp, token);
-        if (p.gate_mode == kGateToken && p.d_gate != nullptr && c == 0)
-            static_cast<T*>(p.d_gate)[row] = Elem<T>::from_float(k.d_token_gate);
-        acc_w += e.dy * (e.s * k.rs);
-        const float ds = k.rs * (e.dy * e.w - e.s * k.k_s) + e.d;
-        if (p.d_residual != nullptr) static_cast<R*>(p.d_residual)[base + c] = Elem<R>::from_float(ds);
-        float b = k.m * ds;
-        const float hat = e.x * k.rp;
-        const float dg = b * hat * e.post;
-        if (p.gate_mode == kGateFull && p.d_gate != nullptr) static_cast<T*>(p.d_gate)[base + c] = Elem<T>::from_float(dg);
-        acc_g += dg;
-        b *= e.gate;
-        if (p.post != nullptr) {
-            acc_p += b * hat;
-            b = k.rp * (b * e.post - hat * k.k_x);
+        for (int u = 0; u < kBatch; ++u) {
+            const int64_t row = min(row0 + u, last - 1), at = row * p.hidden + c;  // the last row again where there is none
+            dy[u] = p.dy != nullptr ? Elem<T>::to_float(static_cast<const T*>(p.dy)[at]) : 0.f;
+            s[u] = Elem<R>::to_float(static_cast<const R*>(p.s)[at]);
+            d[u] = p.d_stream != nullptr ? Elem<R>::to_float(static_cast<const R*>(p.d_stream)[at]) : 0.f;
+            x[u] = p.x != nullptr ? Elem<T>::to_float(static_cast<const T*>(p.x)[at]) : 0.f;
+            g[u] = p.gate_mode == kGateFull ? Elem<T>::to_float(static_cast<const T*>(p.gate)[at]) : gate;
+            k[u] = reinterpret_cast<const float4*>(p.row_sums)[row * 2];
+            k2[u] = reinterpret_cast<const float4*>(p.row_sums)[row * 2 + 1];
         }
-        if (p.dx != nullptr) static_cast<T*>(p.dx)[base + c] = Elem<T>::from_float(b);
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            if (row0 + u >= last) break;
+            const int64_t at = (row0 + u) * p.hidden + c;
+            const float rs = k[u].x, rs_ks = k[u].y, rp = k[u].z, rp_kx = k[u].w, m = k2[u].x, branch = k2[u].y;
+            if (p.x != nullptr) s[u] = fmaf(x[u] * post * g[u], branch, s[u]);
+            acc_w += dy[u] * (s[u] * rs);
+            const float ds = rs * (dy[u] * w) - s[u] * rs_ks + d[u];
+            if (p.d_residual != nullptr) static_cast<R*>(p.d_residual)[at] = Elem<R>::from_float(ds);
+            float b = m * ds;
+            const float hat = x[u] * rp;
+            const float dg = b * hat * post;
+            if (p.gate_mode == kGateFull && p.d_gate != nullptr) static_cast<T*>(p.d_gate)[at] = Elem<T>::from_float(dg);
+            acc_g += dg;
+            b *= g[u];
+            if (p.post != nullptr) {
+                acc_p += b * hat;
+                b = b * post * rp - hat * rp_kx;
+            }
+            if (p.dx != nullptr) static_cast<T*>(p.dx)[at] = Elem<T>::from_float(b);
+        }
     }
     const int64_t at = static_cast<int64_t>(blockIdx.y) * p.hidden + c;
     const int64_t plane = static_cast<int64_t>(p.partial_rows) * p.hidden;
@@ -1152,7 +1174,7 @@ extern "C" {
 
 int64_t xma_norm_workspace_floats(int64_t rows, int64_t hidden) {
     if (rows < 0 || hidden < 0) return 0;
-    return 3 * (rows < XMA_NORM_PARTIALS ? rows : XMA_NORM_PARTIALS) * hidden + 4 * rows;
+    return 3 * (rows < XMA_NORM_PARTIALS ? rows : XMA_NORM_PARTIALS) * hidden + 8 * rows;
 }
 
 int xma_norm_forward(const void* x, const void* residual, const void* weight, const void* post_weight, const void* gate,
@@ -1201,9 +1223,9 @@ int xma_norm_backward(const void* dy, const void* d_stream, const void* stream_o
     p.rs = const_cast<float*>(rstd), p.rp = const_cast<float*>(rstd_post);
     p.dy = dy, p.d_stream = d_stream, p.s = stream_or_residual, p.dx = dx, p.d_residual = d_residual;
     p.d_gate = gate_mode == kGateChannel ? nullptr : d_gate;
-    p.partials = workspace;
     p.partial_rows = static_cast<int>(rows < kPartials ? rows : kPartials);
-    p.row_sums = workspace + 3 * static_cast<int64_t>(p.partial_rows) * hidden;
+    p.row_sums = workspace;
+    p.partials = workspace + 8 * rows;
     void* d_gate_channel = gate_mode == kGateChannel ? d_gate : nullptr;
     p.want_weight = d_weight != nullptr, p.want_post = d_post_weight != nullptr, p.want_gate = d_gate_channel != nullptr;
     p.status = status;

@@ -167,7 +167,7 @@ def index_workspace_elems(n: int, num_experts: int) -> int:
 def norm_workspace_floats(rows: int, hidden: int) -> int:
     """float32 elements of workspace xma_norm_backward needs (xma_norm_workspace_floats, kept in Python for
     the same reason as index_workspace_elems)."""
-    return 3 * min(rows, NORM_PARTIALS) * hidden + 4 * rows
+    return 3 * min(rows, NORM_PARTIALS) * hidden + 8 * rows
 
 
 def attention_workspace_bytes(total: int, batch: int) -> int:
