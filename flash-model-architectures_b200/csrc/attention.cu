@@ -21,6 +21,12 @@
 // dk, dv and dq are each summed by one CTA in a fixed order: no atomics, the same bits every time. That
 // costs two of seven products (s and dp are computed twice).
 //
+// What bounds it: long sequences run into the board's power limit (16384 tokens, 32 heads on 8 of 128, bf16:
+// forward 1.62 ms, 1350 TFLOP/s; dkdv 3.2 ms, 1360 TFLOP/s, both at 1.6 GHz; dq 2.6-2.9 ms, 1140-1270
+// TFLOP/s), short ones and narrow heads the chain scores -> softmax -> product of a query tile (8192 tokens of
+// ragged prompts, 16 heads on 4 of 64, fp16: 80 us, 550 TFLOP/s), since one tile's softmax takes about 1700
+// cycles of which 1024 are the ex2 unit's, and tensor memory holds no third tile of width 128.
+//
 // Rows beyond a sequence's end inside a tile belong to other sequences: their scores are masked by
 // selection, and where a masked (zero) probability would multiply such a row, the row is zeroed in shared
 // memory first, so that not even a NaN crosses over. Every wait is bounded, as in the grouped GEMM.
@@ -391,6 +397,10 @@ struct Forward {
 };
 
 // Work item: 256 query rows (two tiles) of one head. Tile t's last key tile is its diagonal.
+// One MMA warp serves both tiles in turn: that keeps their softmaxes half a period apart, where two MMA warps, or
+// scores issued further ahead, let them fall into step and wait for the same unit (measured 520 and 441 us against
+// 427 and 409 for 8192 tokens). Its operands are computed warp-uniformly: issued from a branch on the lane number
+// every product took 100 cycles to issue and 577 us were needed.
 template <typename T, int kD>
 __global__ void __launch_bounds__(kThreads, 1)
 forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -681,9 +691,11 @@ __device__ __forceinline__ float ds_factor<__half>(const Params& p) {
     return exp2f(static_cast<float>(min(max(14 - ilogbf(bound), -100), 100)));
 }
 
-// delta_i = o_i . do_i for every row of every block and head, o with what its rounding took away; for fp16 also max |do| and max |v| (over bit
-// patterns, whose order does not depend on that of the atomics). A CTA takes kDeltaRows rows of a block of the plan;
-// groups of kD / 8 lanes take one head of one row each, 16 bytes a lane, four at a time.
+// delta_i = o_i . do_i for every row of every block and head, o with what its rounding took away; for fp16 also
+// max |do| and max |v| (over bit patterns, whose order does not depend on that of the atomics). A CTA takes
+// kDeltaRows rows of a block of the plan; groups of kD / 8 lanes take one head of one row each, 16 bytes a lane, four at
+// a time. Bound by HBM: 77 us for 16384 tokens x 32 heads of 128 (335 MB, 4.4 TB/s; smaller batches at more occupancy
+// gain 5 us there and lose as much on short sequences).
 constexpr int kDeltaRows = 16, kDeltaThreads = 256;
 template <typename T, int kD>
 __global__ void __launch_bounds__(kDeltaThreads, 3)
@@ -821,7 +833,9 @@ __device__ __forceinline__ void mma_rows_part(int part, uint32_t d, uint32_t a, 
 // Tensor memory: s^T at 0, dp^T at 128, dv at 256, dk at 256 + kD. Each group of four compute warps takes 64
 // of the 128 query columns; p^T (and ds^T) of a half lies at the start of that half's columns. One MMA warp
 // issues dv += p^T do and the next s^T, the other dk += ds^T q and the next dp^T: each pair shares a region of
-// tensor memory, and while one warp waits for the compute warps the other's products run.
+// tensor memory, and while one warp waits for the compute warps the other's products run. Query tiles are
+// operands of a step's first and last product, so they need three buffers: with two, a step waited 1400 cycles for
+// its tile. 16384 tokens, 32 heads on 8 of 128: 3734 us with two buffers and one MMA warp, 3260 us so.
 template <typename T, int kD>
 __global__ void __launch_bounds__(kThreads, 1)
 dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -1172,7 +1186,8 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
 
 // Work item: 128 query rows of one head over their key tiles. Tensor memory: s at 0 and 128 (two buffers),
 // dp (then ds) at 256, dq at 384. The compute groups take 64 key columns each. One MMA warp issues s ahead, the
-// other dq += ds k and the next dp.
+// other dq += ds k and the next dp. Bound by the compute warps' chain (exponentials, then ds) beside three products
+// of 512 cycles: some 2600 cycles a tile.
 template <typename T, int kD>
 __global__ void __launch_bounds__(kThreads, 1)
 dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,

@@ -228,7 +228,9 @@ __device__ __forceinline__ float token_gate(const Params& p, int64_t row) {
 // Forward
 // ---------------------------------------------------------------------------------------------
 
-// `group` threads per row hold it in registers (kVpt vectors of eight each); several short rows share a CTA.
+// `group` threads per row hold it in registers (kVpt vectors of eight each); several short rows share a CTA. For few
+// rows (4 x 4096: 3.6 us) and rows of up to 2048 elements (8191 x 2048 bf16 with a float32 stream, post norm and
+// channel gate: 37 us, 5.4 TB/s); one vector a thread or four are slower (48 and 46 us).
 template <typename T, typename R, int kVpt, bool kVec>
 __global__ void __launch_bounds__(1024)
 forward_kernel(const Params p, int group) {
@@ -367,7 +369,10 @@ forward_long_kernel(const Params p) {
 // `slots` groups of `group` threads share a CTA; a thread keeps its columns (kVpt vectors of eight) and takes
 // kRows rows of every chunk of slots * kRows rows. Chunks are copied whole (bulk copies, one per tensor) into a
 // ring of stages, so what is in flight does not depend on registers and every row can be read twice. The
-// CTA's barriers, which a row sum needs anyway, also say when a stage is free: thread 0 refills it.
+// CTA's barriers, which a row sum needs anyway, also say when a stage is free: thread 0 refills it. What a chunk costs
+// whatever its size (sums over the CTA, waits, addresses) is some 200 instructions a thread, so a thread takes as
+// many rows at once as registers and the ring allow. 16384 x 4096 bf16 with post norm and channel gate: forward 89 us
+// (6.1 TB/s, two rows a thread 109), backward 170 us (4.7 TB/s, issue slots half used).
 struct RingLayout {
     int slots, group, stages;
     uint32_t stage_bytes;
@@ -910,7 +915,8 @@ struct Element {
 
 // Any row length and alignment, in two kernels: the row sums, from which what a row's elements need is worked out
 // once, then the elements (a block of columns times a share of the rows per CTA, so that the parameters' gradients
-// are sums in registers; four rows at a time, for loads in flight).
+// are sums in registers; four rows at a time, for loads in flight). Every tensor is read twice, two or four bytes a
+// lane: 5001 x 1001 float32, whose 20 MB tensors stay in L2, 19 + 19 us; 8000 x 3001 bf16 with everything 91 + 119 us.
 template <typename T, typename R>
 __global__ void __launch_bounds__(256)
 backward_sums_kernel(const Params p) {
