@@ -6,9 +6,11 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _native as N
 from ..accelerator import KernelBackend, require_cuda_backend
+from ..ops import attention_packed_backward_cuda, attention_packed_forward_cuda
 
 MAX_HEAD_DIM = 128
 _MAX_TOKENS = 1 << 30
@@ -24,8 +26,6 @@ def _tiled(t: torch.Tensor) -> torch.Tensor:
 
 
 def _forward(q, k, v, cu_seqlens, softmax_scale: float, saving: bool):
-    from ..ops import attention_packed_forward_cuda
-
     q, k, v, cu_seqlens = _tiled(q), _tiled(k), _tiled(v), cu_seqlens.contiguous()
     total, heads, dim = q.shape
     batch = cu_seqlens.numel() - 1
@@ -48,9 +48,8 @@ class _AttentionPacked(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_out):
-        from ..ops import attention_packed_backward_cuda
-
         q, k, v, cu_seqlens, out, out_rest, lse = ctx.saved_tensors
         opts = dict(dtype=q.dtype, device=q.device)
         dq, dk, dv = torch.empty(q.shape, **opts), torch.empty(k.shape, **opts), torch.empty(v.shape, **opts)

@@ -5,9 +5,11 @@ its residual add; one kernel forward and one (plus a small sum) backward."""
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _native as N
 from ..accelerator import KernelBackend, require_cuda_backend
+from ..ops import norm_backward_cuda, norm_forward_cuda
 
 GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_FULL = 0, 1, 2, 3
 _MAX_HIDDEN = 1 << 24
@@ -15,8 +17,6 @@ _MAX_HIDDEN = 1 << 24
 
 def _forward(x, residual, weight, post_weight, gate, gate_mode: int, eps: float, multiplier: float, saving: bool):
     """(y, stream or None, contiguous inputs, row statistics of both norms): the forward launch."""
-    from ..ops import norm_forward_cuda
-
     x = x.contiguous()
     residual = None if residual is None else residual.contiguous()
     weight = None if weight is None else weight.contiguous()
@@ -49,9 +49,8 @@ class _Norm(torch.autograd.Function):
         return y if residual is None else (y, stream)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, d_stream=None):
-        from ..ops import norm_backward_cuda
-
         base, x, weight, post_weight, gate, rstd = ctx.saved_tensors
         dy = None if dy is None else dy.contiguous()
         d_stream = None if d_stream is None else d_stream.contiguous()

@@ -133,3 +133,40 @@ def test_block_captured():
     for a, b in zip(captured, step()):
         assert torch.equal(a, b)
     assert_status_clean(tokens.device)
+
+
+def test_second_derivatives_are_refused():
+    x = torch.randn(4, 64, device="cuda", requires_grad=True)
+    (dx,) = torch.autograd.grad(xma.rmsnorm(x, None, EPS).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dx.sum(), x)
+    q = torch.randn(9, 2, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    cu = torch.tensor([0, 9], dtype=torch.int32, device="cuda")
+    (dq,) = torch.autograd.grad(xma.attention_packed(q, q, q, cu).sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dq.sum(), q)
+
+
+def test_compiled_for_any_length():
+    """One compiled graph for all lengths, with and without gradients; checkpointing computes the same again."""
+    from torch.utils.checkpoint import checkpoint
+
+    attention = torch.compile(lambda q, k, v, cu: xma.attention_packed(q, k, v, cu), fullgraph=True, dynamic=True)
+    norm = torch.compile(lambda x, r, w: xma.fused_residual_add_rmsnorm(x, r, w, EPS, M, gate=w), fullgraph=True, dynamic=True)
+    for lengths in ([100, 28], [300], [77, 1, 9, 200]):
+        total = sum(lengths)
+        q, k, v, up = (torch.randn(total, h, D, device="cuda", dtype=torch.bfloat16) for h in (4, 2, 2, 4))
+        cu = torch.tensor([0] + lengths, device="cuda").cumsum(0).to(torch.int32)
+        leaves = [t.requires_grad_() for t in (q, k, v)]
+        want = xma.attention_packed(*leaves, cu)
+        grads = torch.autograd.grad(want, leaves, up, retain_graph=True)
+        for call in (lambda: attention(*leaves, cu), lambda: checkpoint(lambda *a: xma.attention_packed(*a, cu), *leaves, use_reentrant=False)):
+            got = call()
+            assert torch.equal(got, want)
+            for a, b in zip(torch.autograd.grad(got, leaves, up), grads):
+                assert torch.equal(a, b)
+        with torch.no_grad():
+            assert torch.equal(attention(q, k, v, cu), want)
+            x, w = torch.randn(total, 8 * len(lengths), device="cuda"), torch.randn(8 * len(lengths), device="cuda")
+            for a, b in zip(norm(x, x, w), xma.fused_residual_add_rmsnorm(x, x, w, EPS, M, gate=w)):
+                assert torch.equal(a, b)
