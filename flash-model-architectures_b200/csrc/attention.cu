@@ -112,11 +112,13 @@ struct ZeroRows {
 
 // Block 0 (and 1, for the second list) writes a list; the others zero the rows before the first and after
 // the last sequence. A list holds every block of `block_rows` rows of every sequence, by falling work:
-// kFromEnd = false: a block's index (keys before it), true: the number of blocks after it.
+// kFromEnd = false: a block's index (keys before it), true: the number of blocks after it. Offsets out of order are no
+// valid cu_seqlens: sequences would overlap and could be more than a list holds, or than its counters count. They get an
+// empty list; in order, the blocks are at most total / block_rows + batch.
 template <typename IntT>
 __global__ void __launch_bounds__(kPlanThreads)
-plan_kernel(const IntT* __restrict__ cu, int64_t batch, int64_t total, int block_rows, int64_t capacity, Block* list0, int32_t* count0,
-            Block* list1, int32_t* count1, uint32_t* absmax, ZeroRows z0, ZeroRows z1, ZeroRows z2, int num_lists) {
+plan_kernel(const IntT* __restrict__ cu, int64_t batch, int64_t total, int block_rows, Block* list0, int32_t* count0, Block* list1,
+            int32_t* count1, uint32_t* absmax, ZeroRows z0, ZeroRows z1, ZeroRows z2, int num_lists) {
     if (static_cast<int>(blockIdx.x) >= num_lists) {
         const int64_t first = min(max(static_cast<int64_t>(cu[0]), int64_t(0)), total);
         const int64_t last = min(max(static_cast<int64_t>(cu[batch]), first), total);
@@ -142,7 +144,13 @@ plan_kernel(const IntT* __restrict__ cu, int64_t batch, int64_t total, int block
     __shared__ int warp_sum[32];
     for (int i = threadIdx.x; i < kPlanBuckets; i += blockDim.x) bucket[i] = 0;
     if (threadIdx.x < 2 && absmax != nullptr && !from_end) absmax[threadIdx.x] = 0;
-    __syncthreads();
+    int32_t* count = from_end ? count1 : count0;
+    bool falls = false;
+    for (int64_t b = threadIdx.x; b < batch; b += kPlanThreads) falls = falls || cu[b + 1] < cu[b];
+    if (__syncthreads_or(falls)) {
+        if (threadIdx.x == 0) *count = 0;
+        return;
+    }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int64_t b = warp; b < batch; b += kPlanThreads / 32) {
         int start, len;
@@ -173,8 +181,7 @@ plan_kernel(const IntT* __restrict__ cu, int64_t batch, int64_t total, int block
     }
     __syncthreads();
     bucket[mine] = incl - value + (warp > 0 ? warp_sum[warp - 1] : 0);
-    // Sequences that overlap (not a valid cu_seqlens) could be more than the list holds: the rest is dropped.
-    if (threadIdx.x == 0) *(from_end ? count1 : count0) = static_cast<int>(min(static_cast<int64_t>(warp_sum[31]), capacity));
+    if (threadIdx.x == 0) *count = warp_sum[31];
     __syncthreads();
     for (int64_t b = warp; b < batch; b += kPlanThreads / 32) {
         int start, len;
@@ -183,7 +190,7 @@ plan_kernel(const IntT* __restrict__ cu, int64_t batch, int64_t total, int block
         for (int i = lane; i < n; i += 32) {
             // the order inside a bucket is not fixed; it decides who computes a block, not what
             const int at = atomicAdd(&bucket[min(from_end ? n - 1 - i : i, kPlanBuckets - 1)], 1);
-            if (at < capacity) list[at] = Block{start, len, i, pad_offset(start, b)};
+            list[at] = Block{start, len, i, pad_offset(start, b)};
         }
     }
 }
@@ -1487,14 +1494,13 @@ static Workspace split_workspace(void* base, int64_t total, int64_t batch) {
 static int launch_plan(const void* cu, int cu_is_int64, int64_t batch, int64_t total, int block_rows, const Workspace& w, int lists,
                        ZeroRows z0, ZeroRows z1, ZeroRows z2, cudaStream_t stream) {
     constexpr int kZeroBlocks = 32;
-    const int64_t capacity = list_capacity(total, batch, block_rows);
     uint32_t* absmax = lists == 2 ? w.absmax : nullptr;
     if (cu_is_int64)
         plan_kernel<int64_t><<<lists + kZeroBlocks, kPlanThreads, 0, stream>>>(
-            static_cast<const int64_t*>(cu), batch, total, block_rows, capacity, w.list0, w.counts, w.list1, w.counts + 1, absmax, z0, z1, z2, lists);
+            static_cast<const int64_t*>(cu), batch, total, block_rows, w.list0, w.counts, w.list1, w.counts + 1, absmax, z0, z1, z2, lists);
     else
         plan_kernel<int32_t><<<lists + kZeroBlocks, kPlanThreads, 0, stream>>>(
-            static_cast<const int32_t*>(cu), batch, total, block_rows, capacity, w.list0, w.counts, w.list1, w.counts + 1, absmax, z0, z1, z2, lists);
+            static_cast<const int32_t*>(cu), batch, total, block_rows, w.list0, w.counts, w.list1, w.counts + 1, absmax, z0, z1, z2, lists);
     return launch_status();
 }
 

@@ -86,8 +86,8 @@ def attention_packed(
 
     Tokens that no sequence owns get zeros, in the output and in the gradients, and what they hold reaches nothing. A
     NaN or an infinity in a value also reaches rows before it in its own sequence, as in a product with probabilities
-    that are zero there. Offsets are read on the device: values that are out of order or outside the stream give
-    meaningless outputs, not an error."""
+    that are zero there, and one in a key their gradients. Offsets are read on the device: values that are out of order
+    or outside the stream give meaningless outputs, not an error."""
     require_cuda_backend(kernel_backend)
     dtype, device = q.dtype, q.device
     if dtype not in (torch.bfloat16, torch.float16):

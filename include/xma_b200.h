@@ -421,8 +421,8 @@ int xma_norm_backward(const void* dy, const void* d_stream, const void* stream_o
  *   delta float32, the size of lse, scratch of the backward pass
  *   workspace  xma_attention_workspace_bytes(total, batch) bytes, 16-byte aligned, contents irrelevant
  * Tokens that no sequence owns (before cu_seqlens[0], from cu_seqlens[batch] on) get zeros in every output and
- * are read by nothing else. Entries of cu_seqlens outside [0, total] or out of order give meaningless values
- * but touch no memory outside the operands. A code 501-548 goes to *status when a device-side wait runs out.
+ * are read by nothing else. Entries of cu_seqlens outside [0, total] are clamped to it; out of order, nothing is
+ * computed and the sequences' rows are left unwritten. A code 501-548 goes to *status when a device-side wait runs out.
  */
 int64_t xma_attention_workspace_bytes(int64_t total, int64_t batch);
 int64_t xma_attention_stat_rows(int64_t total, int64_t batch);

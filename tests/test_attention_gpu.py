@@ -412,3 +412,26 @@ def test_many_work_items(dim, dtype):
     """More work items than SMs, of one and of two query tiles in every order: each CTA goes through several."""
     lengths = [(37 * n * n + 11 * n) % 700 + 1 for n in range(48)]
     check(lengths, 12, 3, dim, dtype, behind=5)
+
+
+@pytest.mark.parametrize("int_type", [torch.int32, torch.int64])
+def test_offsets_out_of_order_are_no_work(int_type):
+    """Overlapping sequences of 2^32 row blocks together, more than the plan's counters hold: the rows are left as they were
+    and later calls are not touched."""
+    from xma import _native as N
+    from xma.ops import attention_packed_backward_cuda, attention_packed_forward_cuda
+
+    total, batch = 1 << 22, (1 << 18) + 1
+    cu = torch.zeros(batch + 1, dtype=int_type, device="cuda")
+    cu[1::2] = total
+    q, k, v, do = make([total], 1, 1, 8, torch.bfloat16)
+    workspace = torch.empty(N.attention_workspace_bytes(total, batch), dtype=torch.uint8, device="cuda")
+    out, dq, dk, dv = (torch.full_like(q, 7.0) for _ in range(4))
+    lse, delta = (torch.empty(1, N.attention_stat_rows(total, batch), device="cuda") for _ in range(2))
+    rest = torch.zeros(total, 1, 16, dtype=torch.uint8, device="cuda")
+    attention_packed_forward_cuda(q, k, v, cu, 0.3, out, lse, rest, workspace)
+    attention_packed_backward_cuda(q, k, v, cu, 0.3, out, rest, do, lse, delta, dq, dk, dv, workspace)
+    torch.cuda.synchronize()
+    assert_status_clean(q.device)
+    assert all((t == 7.0).all() for t in (out, dq, dk, dv))
+    check([130, 1, 300], 2, 1, 64, torch.bfloat16)
