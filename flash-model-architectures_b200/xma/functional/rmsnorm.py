@@ -172,7 +172,8 @@ def fused_residual_add_rmsnorm(
             gate_mode = GATE_TOKEN
         else:
             raise ValueError(
-                f"gate should have shape {tuple(x.shape[-1:])}, {tuple(x.shape[:-1]) + (1,)} or {tuple(x.shape)}, got {tuple(gate.shape)}")
+                f"gate should have shape {tuple(x.shape[-1:])}, {tuple(x.shape[:-1]) + (1,)} or, in {x.dtype}, {tuple(x.shape)}, "
+                f"got {tuple(gate.shape)} {gate.dtype}")
         if gate_mode != GATE_CHANNEL and gate.dtype != x.dtype:
             raise ValueError(f"a gate of every token should be {x.dtype}, got {gate.dtype}")
         if gate.device != x.device:

@@ -25,7 +25,7 @@ def _kernels_per_call(name: str, args: tuple) -> int:
         return 2
     if name == "xma_attention_backward":  # plan, row sums, dk and dv, dq
         return 4
-    if name == "xma_norm_backward":  # the kernel (two for rows that no vector fits), the sums of parameters' partials
+    if name == "xma_norm_backward":  # the kernel (counted as one, also where rows fit no ring and take two), the parameters' sums
         gate_mode, d_gate, d_weight, d_post_weight = args[7], args[18], args[19], args[20]
         return 1 + (d_weight is not None or d_post_weight is not None or (gate_mode == 1 and d_gate is not None))
     if name == "xma_moe_index_build":
