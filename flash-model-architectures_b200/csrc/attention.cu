@@ -71,7 +71,7 @@ struct Params {
     float* lse;        // [heads][pad_rows], log2 units; may be NULL in the forward pass
     uint8_t* rest;     // [tokens, heads, rest_row]: what out's rounding took away; NULL when lse is
     int64_t rest_row;  // dim, rounded up to 16
-    const float* delta;
+    const float* delta;      // negated
     void* dq;
     void* dk;
     void* dv;
@@ -698,7 +698,8 @@ __device__ __forceinline__ float ds_factor<__half>(const Params& p) {
     return exp2f(static_cast<float>(min(max(14 - ilogbf(bound), -100), 100)));
 }
 
-// delta_i = o_i . do_i for every row of every block and head, o with what its rounding took away; for fp16 also
+// -delta_i = -o_i . do_i for every row of every block and head (negated: the backward kernels add it two at a
+// time), o with what its rounding took away; for fp16 also
 // max |do| and max |v| (over bit patterns, whose order does not depend on that of the atomics). A CTA takes
 // kDeltaRows rows of a block of the plan; groups of kD / 8 lanes take one head of one row each, 16 bytes a lane, four at
 // a time. Bound by HBM: 77 us for 16384 tokens x 32 heads of 128 (335 MB, 4.4 TB/s; smaller batches at more occupancy
@@ -752,7 +753,7 @@ delta_kernel(const T* __restrict__ o, const uint8_t* __restrict__ rest, const T*
             }
 #pragma unroll
             for (int w = kLanes / 2; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-            if (r < rows && sub == 0) delta[h * p.pad_rows + b.pad + first + r] = sum;
+            if (r < rows && sub == 0) delta[h * p.pad_rows + b.pad + first + r] = -sum;
             for (h += kSlots; h >= p.heads; h -= p.heads) ++r;
         }
     }
@@ -819,11 +820,40 @@ __device__ __forceinline__ bool base_is_aligned(uint32_t base, int32_t* status) 
 
 // p (or ds) of 32 neighbouring columns to tensor memory, as 16 packed columns.
 template <typename T>
-__device__ __forceinline__ void store_packed32(uint32_t taddr, const float* v) {
+__device__ __forceinline__ void store_packed32(uint32_t taddr, const f32x2* v) {
     uint32_t packed[16];
 #pragma unroll
-    for (int c = 0; c < 16; ++c) packed[c] = pack2<T>(v[2 * c], v[2 * c + 1]);
+    for (int c = 0; c < 16; ++c) {
+        float lo, hi;
+        split_f32x2(v[c], lo, hi);
+        packed[c] = pack2<T>(lo, hi);
+    }
     tmem_st16(taddr, packed);
+}
+__device__ __forceinline__ f32x2 pair(const uint32_t* r) { return make_f32x2(__uint_as_float(r[0]), __uint_as_float(r[1])); }
+// 2^-x
+__device__ __forceinline__ f32x2 ex2_neg2(f32x2 x) {
+    float lo, hi;
+    split_f32x2(x, lo, hi);
+    return make_f32x2(ex2(-lo), ex2(-hi));
+}
+// ds = p (dp - delta), with the factor that fp16 is rounded with
+template <typename T>
+__device__ __forceinline__ f32x2 ds_pair(f32x2 p, f32x2 dp, f32x2 neg_delta, f32x2 factor) {
+    f32x2 d = add_f32x2(dp, neg_delta);
+    if (std::is_same<T, __half>::value) d = mul_f32x2(d, factor);  // 1 for bf16
+    return mul_f32x2(p, d);
+}
+// Of 32 columns those before `from` and from `last` on become zeros, whatever they held.
+__device__ __forceinline__ void clear_outside(f32x2* v, int from, int last) {
+#pragma unroll
+    for (int c = 0; c < 16; ++c) {
+        float lo, hi;
+        split_f32x2(v[c], lo, hi);
+        if (2 * c < from || 2 * c >= last) lo = 0.f;
+        if (2 * c + 1 < from || 2 * c + 1 >= last) hi = 0.f;
+        v[c] = make_f32x2(lo, hi);
+    }
 }
 // Half `part` of the product over 128 rows of B whose A operand store_packed32 wrote: columns 32 part .. 32
 // part + 31 of each compute group's 64.
@@ -1093,6 +1123,7 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_addr = tm_s + lanes + half * 64, dp_addr = tm_dp + lanes + half * 64;
         const float factor = ds_factor<T>(p);
+        const f32x2 factor2 = make_f32x2(factor, factor), neg_scale2 = make_f32x2(-p.scale_log2, -p.scale_log2);
         Ring d;
         uint32_t s_phase = 0, dp_phase = 0, done_phase = 0;
         bool ok = true;
@@ -1105,7 +1136,7 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
                     ok = mbar_wait(do_full + 8 * d.stage, d.phase, abort_flag, p.status, 517);
                     if (!ok) break;
                     const float4* lse = reinterpret_cast<const float4*>(gen + B::kStatsAt + d.stage * B::kStats + half * 256);
-                    const float4* delta = lse + kTile / 4;
+                    const float4* neg_delta = lse + kTile / 4;
                     ok = mbar_wait(s_full, s_phase, abort_flag, p.status, 518);
                     if (!ok) break;
                     s_phase ^= 1u;
@@ -1113,7 +1144,8 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
                     const int last = b.len - i * kTile - half * 64;        // columns from here on are no queries
                     const int from = i == b.index ? row - half * 64 : 0;   // columns before are not causal
                     const bool edge = last < 64 || i == b.index;
-                    float pr[64];
+                    // probabilities, two at a time; x = lse - scale s, so that no sign takes an instruction
+                    f32x2 pr[32];
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         uint32_t s[32];
@@ -1123,17 +1155,11 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             const float4 f = lse[c * 8 + e];
-                            pr[c * 32 + e * 4] = ex2(fmaf(__uint_as_float(s[e * 4]), p.scale_log2, -f.x));
-                            pr[c * 32 + e * 4 + 1] = ex2(fmaf(__uint_as_float(s[e * 4 + 1]), p.scale_log2, -f.y));
-                            pr[c * 32 + e * 4 + 2] = ex2(fmaf(__uint_as_float(s[e * 4 + 2]), p.scale_log2, -f.z));
-                            pr[c * 32 + e * 4 + 3] = ex2(fmaf(__uint_as_float(s[e * 4 + 3]), p.scale_log2, -f.w));
+                            pr[c * 16 + e * 2] = ex2_neg2(fma_f32x2(pair(s + e * 4), neg_scale2, make_f32x2(f.x, f.y)));
+                            pr[c * 16 + e * 2 + 1] = ex2_neg2(fma_f32x2(pair(s + e * 4 + 2), neg_scale2, make_f32x2(f.z, f.w)));
                         }
-                        if (edge) {
-#pragma unroll
-                            for (int e = 0; e < 32; ++e)
-                                if (c * 32 + e < from || c * 32 + e >= last) pr[c * 32 + e] = 0.f;
-                        }
-                        store_packed32<T>(s_addr + c * 16, pr + c * 32);
+                        if (edge) clear_outside(pr + c * 16, from - c * 32, last - c * 32);
+                        store_packed32<T>(s_addr + c * 16, pr + c * 16);
                         tmem_st_wait();
                         tc_fence_before();
                         __syncwarp();
@@ -1152,17 +1178,12 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
                         tmem_tie32(dp);
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
-                            const float4 f = delta[c * 8 + e];
-                            const float sub[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) pr[c * 32 + e * 4 + q] *= (__uint_as_float(dp[e * 4 + q]) - sub[q]) * factor;
+                            const float4 f = neg_delta[c * 8 + e];
+                            pr[c * 16 + e * 2] = ds_pair<T>(pr[c * 16 + e * 2], pair(dp + e * 4), make_f32x2(f.x, f.y), factor2);
+                            pr[c * 16 + e * 2 + 1] = ds_pair<T>(pr[c * 16 + e * 2 + 1], pair(dp + e * 4 + 2), make_f32x2(f.z, f.w), factor2);
                         }
-                        if (edge) {
-#pragma unroll
-                            for (int e = 0; e < 32; ++e)  // delta of such a column is no number to rely on
-                                if (c * 32 + e < from || c * 32 + e >= last) pr[c * 32 + e] = 0.f;
-                        }
-                        store_packed32<T>(dp_addr + c * 16, pr + c * 32);
+                        if (edge) clear_outside(pr + c * 16, from - c * 32, last - c * 32);  // delta of such a column is no number to rely on
+                        store_packed32<T>(dp_addr + c * 16, pr + c * 16);
                         tmem_st_wait();
                         tc_fence_before();
                         __syncwarp();
@@ -1387,6 +1408,7 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t dp_addr = tm_dp + lanes + half * 64;
         const float factor = ds_factor<T>(p);
+        const f32x2 factor2 = make_f32x2(factor, factor), neg_scale2 = make_f32x2(-p.scale_log2, -p.scale_log2);
         Ring buf;
         uint32_t dp_phase = 0, done_phase = 0;
         bool ok = true;
@@ -1396,8 +1418,8 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
             const int query = b.index * kTile + row;
             const bool valid = query < b.len;
             const int64_t stat = head * p.pad_rows + b.pad + query;
-            const float neg_lse = valid ? -p.lse[stat] : 0.f;
-            const float delta = valid ? p.delta[stat] : 0.f;
+            const float lse = valid ? p.lse[stat] : 0.f, minus = valid ? p.delta[stat] : 0.f;
+            const f32x2 lse2 = make_f32x2(lse, lse), neg_delta = make_f32x2(minus, minus);
             for (int j = 0; j <= b.index; ++j) {
                 ok = mbar_wait(s_full + 8 * buf.stage, buf.phase, abort_flag, p.status, 526);
                 if (!ok) break;
@@ -1413,9 +1435,9 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
                 __syncwarp();
                 if (lane == 0) mbar_arrive(s_free + 8 * buf.stage);
                 buf.next(2);
-                float pr[64];
+                f32x2 pr[32];
 #pragma unroll
-                for (int c = 0; c < 64; ++c) pr[c] = ex2(fmaf(__uint_as_float(s[c >> 5][c & 31]), p.scale_log2, neg_lse));
+                for (int c = 0; c < 32; ++c) pr[c] = ex2_neg2(fma_f32x2(pair(s[c >> 4] + (c & 15) * 2), neg_scale2, lse2));
                 ok = mbar_wait(dp_full, dp_phase, abort_flag, p.status, 527);
                 if (!ok) break;
                 dp_phase ^= 1u;
@@ -1427,13 +1449,9 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
                     tmem_ld_wait();
                     tmem_tie32(dp);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) pr[c * 32 + i] *= (__uint_as_float(dp[i]) - delta) * factor;
-                    if (j == b.index) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (half * 64 + c * 32 + i > row) pr[c * 32 + i] = 0.f;
-                    }
-                    store_packed32<T>(dp_addr + c * 16, pr + c * 32);
+                    for (int i = 0; i < 16; ++i) pr[c * 16 + i] = ds_pair<T>(pr[c * 16 + i], pair(dp + i * 2), neg_delta, factor2);
+                    if (j == b.index) clear_outside(pr + c * 16, 0, row + 1 - half * 64 - c * 32);
+                    store_packed32<T>(dp_addr + c * 16, pr + c * 16);
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
