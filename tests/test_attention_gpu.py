@@ -435,3 +435,26 @@ def test_offsets_out_of_order_are_no_work(int_type):
     assert_status_clean(q.device)
     assert all((t == 7.0).all() for t in (out, dq, dk, dv))
     check([130, 1, 300], 2, 1, 64, torch.bfloat16)
+
+
+def test_most_heads():
+    check([130], 4096, 1, 8, torch.bfloat16)
+
+
+def test_one_input_learns():
+    """Gradients that nobody asked for are not handed out, and the others do not change; one tensor may be all three inputs."""
+    lengths = [200, 3, 140]
+    q, k, v, do = make(lengths, 4, 4, 64, torch.bfloat16)
+    cu = offsets(lengths)
+    want = run(q, k, v, do, cu)
+    for i, name in enumerate(("dq", "dk", "dv")):
+        leaves = [t.detach().requires_grad_(i == j) for j, t in enumerate((q, k, v))]
+        xma.attention_packed(*leaves, cu).backward(do)
+        assert [t.grad is not None for t in leaves] == [i == j for j in range(3)]
+        assert torch.equal(leaves[i].grad, want[name])
+    one = q.detach().requires_grad_()
+    xma.attention_packed(one, one, one, cu).backward(do)
+    parts = run(q, q, q, do, cu)
+    total = sum(parts[n].double() for n in ("dq", "dk", "dv"))
+    magnitude = sum(parts[n].double().abs() for n in ("dq", "dk", "dv"))
+    assert ((one.grad.double() - total).abs() <= 2 * half_step(torch.bfloat16) * magnitude * (1 + 2 ** -7)).all()  # two additions in bf16

@@ -257,3 +257,39 @@ def test_many_rows(rows, hidden):
         check(make(rows, hidden, types[0], None, "none", False), 1.0)
     check(make(rows, hidden, torch.bfloat16, torch.bfloat16, "token", True, param_dtype=torch.float32), 0.5)
     check(make(rows, hidden, torch.bfloat16, torch.float32, "none", False), 1.0)
+
+
+@pytest.mark.parametrize("post", [False, True])
+def test_stream_and_branch_are_one_tensor(post):
+    """x as its own residual gets the sum of both gradients; gradients of two tensors share no memory."""
+    t = make(37, 264, torch.bfloat16, torch.bfloat16, "none", post)
+    t["residual"] = t["x"].detach().clone().requires_grad_()
+    torch.autograd.backward(list(run(t, None).values()), [t["dy"], t["dd"]])
+    dx, dr = t["x"].grad, t["residual"].grad
+    assert dx.data_ptr() != dr.data_ptr()
+    one = t["x"].detach().requires_grad_()
+    y, s = xma.fused_residual_add_rmsnorm(one, one, t["weight"], EPS, post_weight=t["post_weight"])
+    got, = torch.autograd.grad([y, s], [one], [t["dy"], t["dd"]])
+    assert torch.equal(got, dx + dr)
+
+
+@pytest.mark.parametrize("rows,hidden", [(5000, 4096), (1500, 6144), (3000, 520), (500, 1001)])
+def test_non_finite_rows_stay_alone_in_large_batches(rows, hidden):
+    """A row of NaNs or infinities changes no other row, whatever kernel the size picks."""
+    t = make(rows, hidden, torch.bfloat16, torch.bfloat16, "token", True)
+    pick = [0, 1, rows // 2, rows - 1]
+    keep = torch.ones(rows, dtype=torch.bool, device="cuda")
+    keep[pick] = False
+
+    def rows_of(t):
+        out = run(t, 0.5)
+        return {**out, **dict(zip(("dx", "dr", "dg"), torch.autograd.grad(list(out.values()), [t["x"], t["residual"], t["gate"]], [t["dy"], t["dd"]])))}
+
+    want = rows_of(t)
+    with torch.no_grad():
+        for i, (name, value) in zip(pick, (("x", float("nan")), ("residual", float("inf")), ("dy", float("nan")), ("gate", float("inf")))):
+            t[name][i] = value
+    got = rows_of(t)
+    for name in want:
+        assert torch.equal(got[name][keep], want[name][keep])
+    assert got["y"][0].isnan().all() and got["dx"][rows // 2].isnan().all()
