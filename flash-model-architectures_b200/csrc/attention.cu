@@ -22,7 +22,7 @@
 // costs two of seven products (s and dp are computed twice).
 //
 // What bounds it: long sequences run into the board's power limit (16384 tokens, 32 heads on 8 of 128, bf16:
-// forward 1.62 ms, 1350 TFLOP/s; dkdv 3.2 ms, 1360 TFLOP/s, both at 1.6 GHz; dq 2.6-2.9 ms, 1140-1270
+// forward 1.62 ms, 1350 TFLOP/s; dkdv 3.1-3.2 ms, 1400 TFLOP/s, both at 1.6 GHz; dq 2.6-2.9 ms, 1140-1270
 // TFLOP/s), short ones and narrow heads the chain scores -> softmax -> product of a query tile (8192 tokens of
 // ragged prompts, 16 heads on 4 of 64, fp16: 80 us, 550 TFLOP/s), since one tile's softmax takes about 1700
 // cycles of which 1024 are the ex2 unit's, and tensor memory holds no third tile of width 128.
@@ -872,7 +872,8 @@ __device__ __forceinline__ void mma_rows_part(int part, uint32_t d, uint32_t a, 
 // issues dv += p^T do and the next s^T, the other dk += ds^T q and the next dp^T: each pair shares a region of
 // tensor memory, and while one warp waits for the compute warps the other's products run. Query tiles are
 // operands of a step's first and last product, so they need three buffers: with two, a step waited 1400 cycles for
-// its tile. 16384 tokens, 32 heads on 8 of 128: 3734 us with two buffers and one MMA warp, 3260 us so.
+// its tile. 16384 tokens, 32 heads on 8 of 128: 3734 us with two buffers and one MMA warp, 3300 us so
+// and 3110 us with probabilities and ds computed two elements an instruction.
 template <typename T, int kD>
 __global__ void __launch_bounds__(kThreads, 1)
 dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -1215,7 +1216,8 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
 // Work item: 128 query rows of one head over their key tiles. Tensor memory: s at 0 and 128 (two buffers),
 // dp (then ds) at 256, dq at 384. The compute groups take 64 key columns each. One MMA warp issues s ahead, the
 // other dq += ds k and the next dp. Bound by the compute warps' chain (exponentials, then ds) beside three products
-// of 512 cycles: some 2600 cycles a tile.
+// of 512 cycles: some 2500 cycles a tile (2970 -> 2800 us at 16384 tokens with two elements an instruction). The groups
+// a tile apart, three buffers between them, are no faster: the key tiles that fit, which stay from s to dq, run out.
 template <typename T, int kD>
 __global__ void __launch_bounds__(kThreads, 1)
 dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
