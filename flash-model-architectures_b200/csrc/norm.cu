@@ -36,13 +36,15 @@ constexpr int kGateFull = 3;     // [rows, H]
 constexpr int kForwardThreads = 256;       // plain forward: threads of a CTA with short rows
 constexpr int kForwardMaxHidden = 16384;   // plain forward: longer rows are read once per pass
 constexpr int kRingThreads = 512;          // ring kernels: threads of a CTA, at most
-constexpr int kRingMaxHidden = 8192;
+constexpr int kRingMaxHidden = 8192, kRingMaxHiddenAny = 4096;  // rows of whole vectors; others take one vector a thread
 constexpr uint32_t kRingSmem = 220 * 1024;
 constexpr int kMaxStages = 6;
 // Forward: the ring pays for rows of more than 2048 elements (16384 x 4096 bf16 with a post norm and a gate: 94 us
 // against 130 us in the plain kernel, whose CTA-wide sums stall more the more warps share a row; 8191 x 2048 with a
-// float32 stream: 43 us against 37 us), with a few chunks for every CTA.
-constexpr int kRingMinHidden = 2049, kRingMinChunks = 3;
+// float32 stream: 43 us against 37 us), with a few chunks for every CTA. Rows that no vector fits load two or four bytes a
+// lane, from shared memory sooner than from HBM: 8000 x 3001 bf16 with both 93 us against 126, 16000 x 1111 float32 with a
+// residual 58 against 89; 5001 x 1001 float32 (L2, four chunks a CTA) 13 against 11.
+constexpr int kRingMinHidden = 2049, kRingMinHiddenAny = 512, kRingMinChunks = 3, kRingMinChunksAny = 8;
 constexpr int kPartials = XMA_NORM_PARTIALS;
 
 struct Params {
@@ -177,19 +179,6 @@ __device__ __forceinline__ void load_param(const void* p, bool f32, int v, int t
         load_cols<kVec>(static_cast<const float*>(p), v, t, group, hidden, f);
     } else {
         load_cols<kVec>(static_cast<const T*>(p), v, t, group, hidden, f);
-    }
-}
-
-// Eight neighbours of a parameter (ones where there is none).
-template <typename T>
-__device__ __forceinline__ void param8(const void* p, bool f32, int c, f32x2 (&f)[4]) {
-    if (p == nullptr) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] = both(1.f);
-    } else if (f32) {
-        load8(static_cast<const float*>(p) + c, f);
-    } else {
-        load8(static_cast<const T*>(p) + c, f);
     }
 }
 
@@ -439,11 +428,74 @@ __device__ __forceinline__ void ring_sum(float (&v)[kCount], RingState& st, int 
     for (int i = 0; i < kCount; ++i) v[i] = __shfl_sync(0xffffffffu, sum, i);
 }
 
-// One tensor's share of a chunk.
+// One tensor's share of a chunk, bytes [at, at + bytes), where rows are whole vectors.
 __device__ __forceinline__ void ring_copy(uint32_t dst, const void* src, int64_t at, int64_t bytes, uint32_t bar) {
     if (src != nullptr) bulk_load(dst, static_cast<const uint8_t*>(src) + at, static_cast<uint32_t>(bytes), bar);
 }
 __device__ __forceinline__ int64_t ring_bytes(const void* src, int64_t bytes) { return src != nullptr ? bytes : 0; }
+
+// The same for rows of any length, of a tensor of `total` bytes. Bulk copies take whole pieces of 16 bytes: they start with
+// the piece that holds the first byte, so rows lie at & 15 into the tensor's place, and what follows the tensor's last
+// whole piece, some elements of two bytes, is copied by the thread itself, before its arrival releases it.
+struct RingSpan {
+    const uint8_t* src;
+    int64_t at, end, from;
+    uint32_t bytes;  // of the bulk copy, from `from` on
+    __device__ __forceinline__ RingSpan(const void* tensor, int64_t at_, int64_t size, int64_t total)
+        : src(static_cast<const uint8_t*>(tensor)), at(at_), end(at_ + size), from(at_ & ~int64_t(15)) {
+        bytes = src != nullptr ? static_cast<uint32_t>(max(min((end + 15) & ~int64_t(15), total & ~int64_t(15)) - from, int64_t(0))) : 0u;
+    }
+    __device__ __forceinline__ void copy_rest(uint8_t* dst) const {
+        if (src == nullptr) return;
+#pragma unroll 1
+        for (int64_t b = max(at, from + bytes); b < end; b += 2)
+            *reinterpret_cast<uint16_t*>(dst + (b - from)) = *reinterpret_cast<const uint16_t*>(src + b);
+    }
+    __device__ __forceinline__ void copy(uint32_t dst, uint32_t bar) const {
+        if (bytes > 0) bulk_load(dst, src + from, bytes, bar);
+    }
+};
+// A thread's eight elements of vector v of a row (see `column`); those past the end are zeros where rows have any length,
+// and where a vector fits, the caller has seen to it that it lies inside.
+template <bool kVec, typename T>
+__device__ __forceinline__ void load_cols(const T* row, int v, int t, int group, int hidden, f32x2 (&f)[4]) {
+    if (kVec) {
+        load8(row + column<true>(v, t, group, 0), f);
+    } else {
+        float e[8];
+        load_cols<false>(row, v, t, group, hidden, e);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = make_f32x2(e[2 * j], e[2 * j + 1]);
+    }
+}
+// The same from a tensor's place in a stage: `row` is the row's offset in the chunk, `start` the chunk's first element.
+template <bool kVec, typename T>
+__device__ __forceinline__ void ring_load(const uint8_t* place, int64_t start, int row, int v, int t, int group, int hidden, f32x2 (&f)[4]) {
+    if constexpr (kVec) load8(reinterpret_cast<const T*>(place) + (row + column<true>(v, t, group, 0)), f);
+    else load_cols<false>(reinterpret_cast<const T*>(place + ((start * sizeof(T)) & 15)) + row, v, t, group, hidden, f);
+}
+template <bool kVec, typename T>
+__device__ __forceinline__ void store_cols(T* row, int v, int t, int group, int hidden, const f32x2 (&f)[4]) {
+    if (kVec) {
+        store8(row + column<true>(v, t, group, 0), f);
+    } else {
+        float e[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split_f32x2(f[j], e[2 * j], e[2 * j + 1]);
+        store_cols<false>(row, v, t, group, hidden, e);
+    }
+}
+template <bool kVec, typename T>
+__device__ __forceinline__ void load_param(const void* p, bool f32, int v, int t, int group, int hidden, f32x2 (&f)[4]) {
+    if (p == nullptr) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = both(1.f);
+    } else if (f32) {
+        load_cols<kVec>(static_cast<const float*>(p), v, t, group, hidden, f);
+    } else {
+        load_cols<kVec>(static_cast<const T*>(p), v, t, group, hidden, f);
+    }
+}
 
 // The parameters' copies in shared memory, in their own types.
 template <typename T>
@@ -455,8 +507,10 @@ __device__ __forceinline__ void copy_param(uint8_t* dst, const void* p, bool f32
     }
 }
 
-// kDense: every thread's vectors lie inside the row.
-template <typename T, typename R, int kVpt, int kRows, bool kDense>
+// kDense: every thread's vectors lie inside the row. kVec: rows of whole 16-byte vectors; others take two rows of one vector
+// a thread, since the assembler of CUDA 12.9 fails on four rows of 16 bits, which were 10 us faster at 8000 x 3001, and on
+// two vectors.
+template <typename T, typename R, int kVpt, int kRows, bool kDense, bool kVec>
 __global__ void __launch_bounds__(kRingThreads, 1)
 forward_ring_kernel(const Params p, const RingLayout lay) {
     extern __shared__ __align__(128) uint8_t smem[];
@@ -477,12 +531,25 @@ forward_ring_kernel(const Params p, const RingLayout lay) {
         if (chunk >= chunks) return;
         const int64_t row0 = chunk * per_chunk;
         const int64_t count = min(static_cast<int64_t>(per_chunk), p.rows - row0) * p.hidden;
-        const uint32_t bar = st.full + 8 * stage, dst = smem_u32(smem) + lay.ring + stage * lay.stage_bytes;
+        const uint32_t bar = st.full + 8 * stage, place = lay.ring + stage * lay.stage_bytes, dst = smem_u32(smem) + place;
         const int64_t at = row0 * p.hidden, bt = count * static_cast<int64_t>(sizeof(T)), br = count * static_cast<int64_t>(sizeof(R));
-        mbar_expect_tx(bar, static_cast<uint32_t>(bt + ring_bytes(p.residual, br) + ring_bytes(gate_rows, bt)));
-        ring_copy(dst + lay.x, p.x, at * sizeof(T), bt, bar);
-        ring_copy(dst + lay.residual, p.residual, at * sizeof(R), br, bar);
-        ring_copy(dst + lay.gate, gate_rows, at * sizeof(T), bt, bar);
+        if constexpr (kVec) {
+            mbar_expect_tx(bar, static_cast<uint32_t>(bt + ring_bytes(p.residual, br) + ring_bytes(gate_rows, bt)));
+            ring_copy(dst + lay.x, p.x, at * sizeof(T), bt, bar);
+            ring_copy(dst + lay.residual, p.residual, at * sizeof(R), br, bar);
+            ring_copy(dst + lay.gate, gate_rows, at * sizeof(T), bt, bar);
+        } else {
+            const int64_t all = p.rows * p.hidden;
+            const RingSpan x(p.x, at * sizeof(T), bt, all * sizeof(T)), residual(p.residual, at * sizeof(R), br, all * sizeof(R)),
+                gate(gate_rows, at * sizeof(T), bt, all * sizeof(T));
+            x.copy_rest(smem + place + lay.x);
+            residual.copy_rest(smem + place + lay.residual);
+            gate.copy_rest(smem + place + lay.gate);
+            mbar_expect_tx(bar, x.bytes + residual.bytes + gate.bytes);
+            x.copy(dst + lay.x, bar);
+            residual.copy(dst + lay.residual, bar);
+            gate.copy(dst + lay.gate, bar);
+        }
     };
     if (threadIdx.x == 0) {
         for (int i = 0; i < lay.stages; ++i) mbar_init(st.full + 8 * i, 1);
@@ -493,13 +560,12 @@ forward_ring_kernel(const Params p, const RingLayout lay) {
     // What a column is multiplied with: in registers for one vector a thread, else in shared memory.
     f32x2 w_reg[4], c_reg[4];
     if (kVpt == 1) {
-        const int c = t * 8;
-        if (c < p.hidden) {
-            param8<T>(p.weight, p.weight_f32, c, w_reg);
-            param8<T>(p.post, p.post_f32, c, c_reg);
+        if (!kVec || t * 8 < p.hidden) {
+            load_param<kVec, T>(p.weight, p.weight_f32, 0, t, group, p.hidden, w_reg);
+            load_param<kVec, T>(p.post, p.post_f32, 0, t, group, p.hidden, c_reg);
             if (channel_gate) {
                 f32x2 g[4];
-                param8<T>(p.gate, p.gate_f32, c, g);
+                load_param<kVec, T>(p.gate, p.gate_f32, 0, t, group, p.hidden, g);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) c_reg[j] = mul_f32x2(c_reg[j], g[j]);
             }
@@ -518,19 +584,19 @@ forward_ring_kernel(const Params p, const RingLayout lay) {
             break;
         }
         const uint8_t* stage = smem + lay.ring + st.stage * lay.stage_bytes;
+        const int64_t start = chunk * per_chunk * p.hidden;  // the chunk's first element
+        const auto inside = [&](int v) { return kDense || !kVec || (v * group + t) * 8 < p.hidden; };
         f32x2 s[kRows][kVpt][4];
         float sums[kRows], scale[kRows];
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
-            const T* x = reinterpret_cast<const T*>(stage + lay.x) + (slot * kRows + r) * p.hidden;
             f32x2 sum = both(0.f);
 #pragma unroll
             for (int v = 0; v < kVpt; ++v) {
-                const int c = (v * group + t) * 8;
-                if (kDense || c < p.hidden) load8(x + c, s[r][v]);
+                if (inside(v)) ring_load<kVec, T>(stage + lay.x, start, (slot * kRows + r) * p.hidden, v, t, group, p.hidden, s[r][v]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    if (!kDense && c >= p.hidden) s[r][v][j] = both(0.f);
+                    if (!inside(v)) s[r][v][j] = both(0.f);
                     sum = fma_f32x2(mul_f32x2(s[r][v][j], both(inv_h)), s[r][v][j], sum);
                 }
             }
@@ -549,26 +615,25 @@ forward_ring_kernel(const Params p, const RingLayout lay) {
             }
 #pragma unroll
             for (int v = 0; v < kVpt; ++v) {
-                const int c = (v * group + t) * 8;
                 f32x2 f[4];
-                if (kVpt > 1 && (kDense || c < p.hidden)) {
-                    param8<T>(p.post ? smem + lay.post : nullptr, p.post_f32, c, f);
+                if (kVpt > 1 && inside(v)) {
+                    load_param<kVec, T>(p.post ? smem + lay.post : nullptr, p.post_f32, v, t, group, p.hidden, f);
                     if (channel_gate) {
                         f32x2 g[4];
-                        param8<T>(smem + lay.channel_gate, p.gate_f32, c, g);
+                        load_param<kVec, T>(smem + lay.channel_gate, p.gate_f32, v, t, group, p.hidden, g);
 #pragma unroll
                         for (int j = 0; j < 4; ++j) f[j] = mul_f32x2(f[j], g[j]);
                     }
                 }
 #pragma unroll
                 for (int r = 0; r < kRows; ++r) {
-                    if (!kDense && c >= p.hidden) continue;
-                    const int off = (slot * kRows + r) * p.hidden + c;
+                    if (!inside(v)) continue;
+                    const int off = (slot * kRows + r) * p.hidden;
                     f32x2 res[4];
-                    load8(reinterpret_cast<const R*>(stage + lay.residual) + off, res);
+                    ring_load<kVec, R>(stage + lay.residual, start, off, v, t, group, p.hidden, res);
                     if (full_gate) {
                         f32x2 g[4];
-                        load8(reinterpret_cast<const T*>(stage + lay.gate) + off, g);
+                        ring_load<kVec, T>(stage + lay.gate, start, off, v, t, group, p.hidden, g);
 #pragma unroll
                         for (int j = 0; j < 4; ++j) s[r][v][j] = mul_f32x2(s[r][v][j], g[j]);
                     }
@@ -599,14 +664,13 @@ forward_ring_kernel(const Params p, const RingLayout lay) {
             const int64_t base = (row0 + r) * p.hidden;
 #pragma unroll
             for (int v = 0; v < kVpt; ++v) {
-                const int c = (v * group + t) * 8;
-                if (!kDense && c >= p.hidden) continue;
-                if (p.residual != nullptr) store8(static_cast<R*>(p.s_out) + base + c, s[r][v]);
+                if (!inside(v)) continue;
+                if (p.residual != nullptr) store_cols<kVec>(static_cast<R*>(p.s_out) + base, v, t, group, p.hidden, s[r][v]);
                 f32x2 f[4];
-                if (kVpt > 1) param8<T>(p.weight ? smem + lay.weight : nullptr, p.weight_f32, c, f);
+                if (kVpt > 1) load_param<kVec, T>(p.weight ? smem + lay.weight : nullptr, p.weight_f32, v, t, group, p.hidden, f);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) f[j] = mul_f32x2(mul_f32x2(s[r][v][j], both(rs)), kVpt > 1 ? f[j] : w_reg[j]);
-                store8(static_cast<T*>(p.y) + base + c, f);
+                store_cols<kVec>(static_cast<T*>(p.y) + base, v, t, group, p.hidden, f);
             }
         }
     }
@@ -643,7 +707,7 @@ __device__ __forceinline__ RowScale row_scale(const Params& p, const float (&sum
 // read; kFull: the gate has the shape of x. kCall: what the call is known to have (kCallAny: nothing); a branch per
 // vector costs a sixth of the time (16384 x 4096 bf16 with post norm and channel gate: 192 us with them, 159 without).
 constexpr int kCallAny = 0, kCallAll = 1, kCallAlone = 2, kCallShared = 3;
-template <typename T, typename R, int kVpt, int kRows, bool kX, bool kFull, int kCall>
+template <typename T, typename R, int kVpt, int kRows, bool kX, bool kFull, int kCall, bool kVec>
 __global__ void __launch_bounds__(kRingThreads, 1)
 backward_ring_kernel(const Params p, const RingLayout lay) {
     constexpr int kSums = kX ? 4 : 1;
@@ -668,15 +732,33 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
         if (chunk >= chunks) return;
         const int64_t row0 = chunk * per_chunk;
         const int64_t count = min(static_cast<int64_t>(per_chunk), p.rows - row0) * p.hidden;
-        const uint32_t bar = st.full + 8 * stage, dst = smem_u32(smem) + lay.ring + stage * lay.stage_bytes;
+        const uint32_t bar = st.full + 8 * stage, place = lay.ring + stage * lay.stage_bytes, dst = smem_u32(smem) + place;
         const int64_t at = row0 * p.hidden, bt = count * static_cast<int64_t>(sizeof(T)), br = count * static_cast<int64_t>(sizeof(R));
-        mbar_expect_tx(bar, static_cast<uint32_t>(br + ring_bytes(p.dy, bt) + ring_bytes(p.d_stream, br) + ring_bytes(p.x, bt) +
-                                                  ring_bytes(gate_rows, bt)));
-        ring_copy(dst + lay.s, p.s, at * sizeof(R), br, bar);
-        ring_copy(dst + lay.dy, p.dy, at * sizeof(T), bt, bar);
-        ring_copy(dst + lay.d_stream, p.d_stream, at * sizeof(R), br, bar);
-        ring_copy(dst + lay.x, p.x, at * sizeof(T), bt, bar);
-        ring_copy(dst + lay.gate, gate_rows, at * sizeof(T), bt, bar);
+        if constexpr (kVec) {
+            mbar_expect_tx(bar, static_cast<uint32_t>(br + ring_bytes(p.dy, bt) + ring_bytes(p.d_stream, br) + ring_bytes(p.x, bt) +
+                                                      ring_bytes(gate_rows, bt)));
+            ring_copy(dst + lay.s, p.s, at * sizeof(R), br, bar);
+            ring_copy(dst + lay.dy, p.dy, at * sizeof(T), bt, bar);
+            ring_copy(dst + lay.d_stream, p.d_stream, at * sizeof(R), br, bar);
+            ring_copy(dst + lay.x, p.x, at * sizeof(T), bt, bar);
+            ring_copy(dst + lay.gate, gate_rows, at * sizeof(T), bt, bar);
+        } else {
+            const int64_t all = p.rows * p.hidden;
+            const RingSpan s(p.s, at * sizeof(R), br, all * sizeof(R)), dy(p.dy, at * sizeof(T), bt, all * sizeof(T)),
+                d_stream(p.d_stream, at * sizeof(R), br, all * sizeof(R)), x(p.x, at * sizeof(T), bt, all * sizeof(T)),
+                gate(gate_rows, at * sizeof(T), bt, all * sizeof(T));
+            s.copy_rest(smem + place + lay.s);
+            dy.copy_rest(smem + place + lay.dy);
+            d_stream.copy_rest(smem + place + lay.d_stream);
+            x.copy_rest(smem + place + lay.x);
+            gate.copy_rest(smem + place + lay.gate);
+            mbar_expect_tx(bar, s.bytes + dy.bytes + d_stream.bytes + x.bytes + gate.bytes);
+            s.copy(dst + lay.s, bar);
+            dy.copy(dst + lay.dy, bar);
+            d_stream.copy(dst + lay.d_stream, bar);
+            x.copy(dst + lay.x, bar);
+            gate.copy(dst + lay.gate, bar);
+        }
     };
     if (threadIdx.x == 0) {
         for (int i = 0; i < lay.stages; ++i) mbar_init(st.full + 8 * i, 1);
@@ -687,38 +769,37 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
     // Parameters: in registers for one vector a thread, else in shared memory.
     f32x2 w_reg[4], post_reg[4], gate_reg[4];
     if (kVpt == 1) {
-        const int c = t * 8;
-        if (c < p.hidden) {
-            param8<T>(p.weight, p.weight_f32, c, w_reg);
-            if (kX) param8<T>(p.post, p.post_f32, c, post_reg);
-            if (kX && !kFull) param8<T>(channel_gate ? p.gate : nullptr, p.gate_f32, c, gate_reg);
+        if (!kVec || t * 8 < p.hidden) {
+            load_param<kVec, T>(p.weight, p.weight_f32, 0, t, group, p.hidden, w_reg);
+            if (kX) load_param<kVec, T>(p.post, p.post_f32, 0, t, group, p.hidden, post_reg);
+            if (kX && !kFull) load_param<kVec, T>(channel_gate ? p.gate : nullptr, p.gate_f32, 0, t, group, p.hidden, gate_reg);
         }
     } else {
         copy_param<T>(smem + lay.weight, p.weight, p.weight_f32, p.hidden);
         copy_param<T>(smem + lay.post, p.post, p.post_f32, p.hidden);
         if (channel_gate) copy_param<T>(smem + lay.channel_gate, p.gate, p.gate_f32, p.hidden);
     }
-    const auto weight8 = [&](int c, f32x2 (&f)[4]) {
+    const auto weight8 = [&](int v, f32x2 (&f)[4]) {
         if (kVpt > 1) {
-            param8<T>(p.weight ? smem + lay.weight : nullptr, p.weight_f32, c, f);
+            load_param<kVec, T>(p.weight ? smem + lay.weight : nullptr, p.weight_f32, v, t, group, p.hidden, f);
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j) f[j] = w_reg[j];
         }
     };
-    const auto post8 = [&](int c, f32x2 (&f)[4]) {
+    const auto post8 = [&](int v, f32x2 (&f)[4]) {
         if (kVpt > 1) {
-            param8<T>(p.post ? smem + lay.post : nullptr, p.post_f32, c, f);
+            load_param<kVec, T>(p.post ? smem + lay.post : nullptr, p.post_f32, v, t, group, p.hidden, f);
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j) f[j] = post_reg[j];
         }
     };
-    const auto gate8 = [&](const T* gate_row, int c, f32x2 (&f)[4]) {
+    const auto gate8 = [&](const uint8_t* place, int64_t start, int row, int v, f32x2 (&f)[4]) {
         if (kFull) {
-            load8(gate_row + c, f);
+            ring_load<kVec, T>(place, start, row, v, t, group, p.hidden, f);
         } else if (kVpt > 1) {
-            param8<T>(channel_gate ? smem + lay.channel_gate : nullptr, p.gate_f32, c, f);
+            load_param<kVec, T>(channel_gate ? smem + lay.channel_gate : nullptr, p.gate_f32, v, t, group, p.hidden, f);
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j) f[j] = gate_reg[j];
@@ -748,6 +829,14 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
             break;
         }
         const uint8_t* stage = smem + lay.ring + st.stage * lay.stage_bytes;
+        const int64_t start = chunk * per_chunk * p.hidden;  // the chunk's first element
+        const auto outside = [&](int v) { return !kKnown && kVec && (v * group + t) * 8 >= p.hidden; };
+        const auto load_t = [&](uint32_t tensor, int row, int v, f32x2 (&f)[4]) {
+            ring_load<kVec, T>(stage + tensor, start, row, v, t, group, p.hidden, f);
+        };
+        const auto load_r = [&](uint32_t tensor, int row, int v, f32x2 (&f)[4]) {
+            ring_load<kVec, R>(stage + tensor, start, row, v, t, group, p.hidden, f);
+        };
         float sums[kRows * kSums];
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
@@ -757,15 +846,14 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
             for (int i = 0; i < kSums; ++i) sum[i] = both(0.f);
 #pragma unroll
             for (int v = 0; v < kVpt; ++v) {
-                const int c = (v * group + t) * 8;
-                if (!kKnown && c >= p.hidden) continue;
+                if (outside(v)) continue;
                 f32x2 a[4], s8[4], f[4], x8[4];
-                load8(reinterpret_cast<const R*>(stage + lay.s) + off + c, s8);
+                load_r(lay.s, off, v, s8);
                 if (kX) {
                     f32x2 g[4];
-                    load8(reinterpret_cast<const T*>(stage + lay.x) + off + c, x8);
-                    post8(c, f);
-                    gate8(reinterpret_cast<const T*>(stage + lay.gate) + off, c, g);
+                    load_t(lay.x, off, v, x8);
+                    post8(v, f);
+                    gate8(stage + lay.gate, start, off, v, g);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         x8[j] = mul_f32x2(x8[j], mul_f32x2(f[j], g[j]));
@@ -773,8 +861,8 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
                     }
                 }
                 if (has_dy) {
-                    load8(reinterpret_cast<const T*>(stage + lay.dy) + off + c, a);
-                    weight8(c, f);
+                    load_t(lay.dy, off, v, a);
+                    weight8(v, f);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         a[j] = mul_f32x2(a[j], f[j]);
@@ -791,7 +879,7 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
                         sum[kSums > 1 ? 2 : 0] = fma_f32x2(x8[j], s8[j], sum[kSums > 1 ? 2 : 0]);
                     }
                     if (has_d_stream) {
-                        load8(reinterpret_cast<const R*>(stage + lay.d_stream) + off + c, f);
+                        load_r(lay.d_stream, off, v, f);
 #pragma unroll
                         for (int j = 0; j < 4; ++j) sum[kSums > 1 ? 3 : 0] = fma_f32x2(x8[j], f[j], sum[kSums > 1 ? 3 : 0]);
                     }
@@ -817,14 +905,13 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
                 static_cast<T*>(p.d_gate)[row0 + r] = Elem<T>::from_float(k.d_token_gate);
 #pragma unroll
             for (int v = 0; v < kVpt; ++v) {
-                const int c = (v * group + t) * 8;
-                if (!kKnown && c >= p.hidden) continue;
+                if (outside(v)) continue;
                 f32x2 ds[4], f[4], s8[4], hat[4], u[4], g[4];
-                if (has_dy || kX) load8(reinterpret_cast<const R*>(stage + lay.s) + off + c, s8);
+                if (has_dy || kX) load_r(lay.s, off, v, s8);
                 if (kX) {
-                    load8(reinterpret_cast<const T*>(stage + lay.x) + off + c, hat);
-                    post8(c, f);
-                    gate8(reinterpret_cast<const T*>(stage + lay.gate) + off, c, g);
+                    load_t(lay.x, off, v, hat);
+                    post8(v, f);
+                    gate8(stage + lay.gate, start, off, v, g);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         hat[j] = mul_f32x2(hat[j], both(k.rp));
@@ -833,22 +920,22 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
                     }
                 }
                 if (has_d_stream) {
-                    load8(reinterpret_cast<const R*>(stage + lay.d_stream) + off + c, ds);
+                    load_r(lay.d_stream, off, v, ds);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) ds[j] = both(0.f);
                 }
                 if (has_dy) {
                     f32x2 d8[4], w8[4];
-                    load8(reinterpret_cast<const T*>(stage + lay.dy) + off + c, d8);
-                    weight8(c, w8);
+                    load_t(lay.dy, off, v, d8);
+                    weight8(v, w8);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         acc_w[v][j] = fma_f32x2(d8[j], mul_f32x2(s8[j], both(k.rs)), acc_w[v][j]);
                         ds[j] = fma_f32x2(mul_f32x2(d8[j], w8[j]), both(k.rs), fma_f32x2(s8[j], both(-k.rs * k.k_s), ds[j]));
                     }
                 }
-                if (has_d_residual) store8(static_cast<R*>(p.d_residual) + base + c, ds);
+                if (has_d_residual) store_cols<kVec>(static_cast<R*>(p.d_residual) + base, v, t, group, p.hidden, ds);
                 f32x2 b[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) b[j] = mul_f32x2(ds[j], both(k.m));  // gradient of the gated branch, token gate in it
@@ -861,9 +948,9 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
                         acc_p[v][j] = fma_f32x2(b[j], hat[j], acc_p[v][j]);
                         b[j] = fma_f32x2(mul_f32x2(b[j], f[j]), both(k.rp), mul_f32x2(hat[j], both(-k.rp * k.k_x)));
                     }
-                    if (kFull && p.d_gate != nullptr) store8(static_cast<T*>(p.d_gate) + base + c, u);
+                    if (kFull && p.d_gate != nullptr) store_cols<kVec>(static_cast<T*>(p.d_gate) + base, v, t, group, p.hidden, u);
                 }
-                if (has_dx) store8(static_cast<T*>(p.dx) + base + c, b);
+                if (has_dx) store_cols<kVec>(static_cast<T*>(p.dx) + base, v, t, group, p.hidden, b);
             }
         }
     }
@@ -880,8 +967,7 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
         float* mine = lay.slots == 1 ? out : buf + slot * p.hidden;
 #pragma unroll
         for (int v = 0; v < kVpt; ++v) {
-            const int c = (v * group + t) * 8;
-            if (kKnown || c < p.hidden) store8(mine + c, acc[v]);
+            if (kKnown || !kVec || (v * group + t) * 8 < p.hidden) store_cols<kVec>(mine, v, t, group, p.hidden, acc[v]);
         }
         if (lay.slots == 1) continue;
         __syncthreads();
@@ -913,10 +999,11 @@ struct Element {
     }
 };
 
-// Any row length and alignment, in two kernels: the row sums, from which what a row's elements need is worked out
-// once, then the elements (a block of columns times a share of the rows per CTA, so that the parameters' gradients
-// are sums in registers; four rows at a time, for loads in flight). Every tensor is read twice, two or four bytes a
-// lane: 5001 x 1001 float32, whose 20 MB tensors stay in L2, 19 + 19 us; 8000 x 3001 bf16 with everything 91 + 119 us.
+// What the ring does not take (longer rows, tensors off a 16-byte boundary), in two kernels: the row sums, from which
+// what a row's elements need is worked out once, then the elements (a block of columns times a share of the rows per CTA,
+// so that the parameters' gradients are sums in registers; four rows at a time, for loads in flight). Every tensor is
+// read twice, two or four bytes a lane: 9000 x 4999 bf16 alone 119 + 152 us; 8000 x 3001 bf16 with everything took
+// 91 + 119 us here and takes 115 in the ring, 5001 x 1001 float32 19 + 19 and 14.5.
 template <typename T, typename R>
 __global__ void __launch_bounds__(256)
 backward_sums_kernel(const Params p) {
@@ -1028,7 +1115,7 @@ sum_kernel(const Params p, int count, void* d_weight, void* d_post, void* d_gate
 
 // Threads, stages and offsets of a ring kernel; false when not `min_stages` stages of a chunk fit.
 template <typename T, typename R>
-static bool ring_layout(const Params& p, bool backward, int vpt, int rows, int min_stages, RingLayout* lay) {
+static bool ring_layout(const Params& p, bool vec, bool backward, int vpt, int rows, int min_stages, RingLayout* lay) {
     const uint32_t h = static_cast<uint32_t>(p.hidden);
     lay->group = static_cast<int>(ceil_div(ceil_div(h, 8 * vpt), 32) * 32);
     if (lay->group > kRingThreads) return false;
@@ -1036,7 +1123,7 @@ static bool ring_layout(const Params& p, bool backward, int vpt, int rows, int m
     uint32_t at = kRingHeader;
     const auto param = [&](bool there, bool f32) {
         const uint32_t here = at;
-        if (vpt > 1 && there) at += h * (f32 ? 4u : static_cast<uint32_t>(sizeof(T)));
+        if (vpt > 1 && there) at += (h * (f32 ? 4u : static_cast<uint32_t>(sizeof(T))) + 15u) & ~15u;
         return here;
     };
     lay->weight = param(p.weight != nullptr, p.weight_f32);
@@ -1049,7 +1136,7 @@ static bool ring_layout(const Params& p, bool backward, int vpt, int rows, int m
         uint32_t off = 0;
         const auto tensor = [&](bool there, uint32_t row) {
             const uint32_t here = off;
-            off += there ? n * row : 0;
+            off += !there ? 0 : vec ? n * row : ((n * row + 15u) & ~15u) + 32u;  // see RingSpan
             return here;
         };
         lay->s = tensor(backward, row_r);
@@ -1086,18 +1173,30 @@ static int launch_ring(const Params& p, const RingLayout& lay, int rows, int* co
 // Whether the group's vectors fill a row exactly.
 static bool dense(const Params& p, const RingLayout& lay, int vpt) { return p.hidden == lay.group * vpt * 8; }
 
+// Whether rows are whole 16-byte vectors, or at least start on such a boundary with the first one.
+struct Layout {
+    bool vec, wide;
+};
+
+template <typename T, typename R, int kVpt, int kRows>
+static int run_forward_ring(const Params& p, const RingLayout& lay, cudaStream_t stream) {
+    int count = 0;
+    if (dense(p, lay, kVpt)) return launch_ring<forward_ring_kernel<T, R, kVpt, kRows, true, true>>(p, lay, kRows, &count, stream);
+    return launch_ring<forward_ring_kernel<T, R, kVpt, kRows, false, true>>(p, lay, kRows, &count, stream);
+}
+
 template <typename T, typename R>
-static int run_forward(const Params& p, bool vec, cudaStream_t stream) {
-    if (vec && p.hidden >= kRingMinHidden && p.hidden <= kRingMaxHidden) {
-        const int ring_vpt = p.hidden > 4096 ? 2 : 1, rows = ring_vpt == 1 ? 4 : 2;
+static int run_forward(const Params& p, Layout rows_are, cudaStream_t stream) {
+    const bool vec = rows_are.vec;
+    if (rows_are.wide && p.hidden >= (vec ? kRingMinHidden : kRingMinHiddenAny) && p.hidden <= (vec ? kRingMaxHidden : kRingMaxHiddenAny)) {
+        const int ring_vpt = p.hidden > 4096 ? 2 : 1, rows = vec && ring_vpt == 1 ? 4 : 2;
         RingLayout lay;
         int count = 0;
-        if (ring_layout<T, R>(p, false, ring_vpt, rows, 2, &lay) &&
-            p.rows >= static_cast<int64_t>(kRingMinChunks) * sm_count() * lay.slots * rows)
-            return ring_vpt == 1 ? (dense(p, lay, 1) ? launch_ring<forward_ring_kernel<T, R, 1, 4, true>>(p, lay, rows, &count, stream)
-                                                     : launch_ring<forward_ring_kernel<T, R, 1, 4, false>>(p, lay, rows, &count, stream))
-                                 : (dense(p, lay, 2) ? launch_ring<forward_ring_kernel<T, R, 2, 2, true>>(p, lay, rows, &count, stream)
-                                                     : launch_ring<forward_ring_kernel<T, R, 2, 2, false>>(p, lay, rows, &count, stream));
+        if (ring_layout<T, R>(p, vec, false, ring_vpt, rows, 2, &lay) &&
+            p.rows >= static_cast<int64_t>(vec ? kRingMinChunks : kRingMinChunksAny) * sm_count() * lay.slots * rows) {
+            if (!vec) return launch_ring<forward_ring_kernel<T, R, 1, 2, false, false>>(p, lay, rows, &count, stream);
+            return ring_vpt == 1 ? run_forward_ring<T, R, 1, 4>(p, lay, stream) : run_forward_ring<T, R, 2, 2>(p, lay, stream);
+        }
     }
     if (p.hidden > kForwardMaxHidden) {
         forward_long_kernel<T, R><<<static_cast<unsigned>(p.rows), 1024, 0, stream>>>(p);
@@ -1118,32 +1217,44 @@ static int run_forward(const Params& p, bool vec, cudaStream_t stream) {
     return launch_status();
 }
 
+template <typename T, typename R, int kVpt, int kRows, bool kX, bool kFull, int kCall, bool kVec = true>
+static int launch_backward_ring(const Params& p, const RingLayout& lay, int* count, cudaStream_t stream) {
+    return launch_ring<backward_ring_kernel<T, R, kVpt, kRows, kX, kFull, kCall, kVec>>(p, lay, kRows, count, stream);
+}
+
 template <typename T, typename R, int kVpt, int kRows>
-static int run_backward_ring(const Params& p, const RingLayout& lay, int* count, cudaStream_t stream) {
+static int run_backward_ring(const Params& p, const RingLayout& lay, bool vec, int* count, cudaStream_t stream) {
+    if constexpr (kVpt == 1) {
+        if (!vec && p.x == nullptr) return launch_backward_ring<T, R, kVpt, kRows, false, false, kCallAny, false>(p, lay, count, stream);
+        if (!vec)
+            return p.gate_mode == kGateFull ? launch_backward_ring<T, R, kVpt, kRows, true, true, kCallAny, false>(p, lay, count, stream)
+                                            : launch_backward_ring<T, R, kVpt, kRows, true, false, kCallAny, false>(p, lay, count, stream);
+    }
     const bool known = dense(p, lay, kVpt) && p.dy != nullptr && p.d_residual != nullptr;
     const bool all = known && p.d_stream != nullptr && p.dx != nullptr;
     if (p.x == nullptr) {
-        if (all) return launch_ring<backward_ring_kernel<T, R, kVpt, kRows, false, false, kCallAll>>(p, lay, kRows, count, stream);
+        if (all) return launch_backward_ring<T, R, kVpt, kRows, false, false, kCallAll>(p, lay, count, stream);
         if (known && p.d_stream == nullptr && p.dx == nullptr)
-            return launch_ring<backward_ring_kernel<T, R, kVpt, kRows, false, false, kCallAlone>>(p, lay, kRows, count, stream);
+            return launch_backward_ring<T, R, kVpt, kRows, false, false, kCallAlone>(p, lay, count, stream);
         if (known && p.d_stream != nullptr)
-            return launch_ring<backward_ring_kernel<T, R, kVpt, kRows, false, false, kCallShared>>(p, lay, kRows, count, stream);
-        return launch_ring<backward_ring_kernel<T, R, kVpt, kRows, false, false, kCallAny>>(p, lay, kRows, count, stream);
+            return launch_backward_ring<T, R, kVpt, kRows, false, false, kCallShared>(p, lay, count, stream);
+        return launch_backward_ring<T, R, kVpt, kRows, false, false, kCallAny>(p, lay, count, stream);
     }
     if (p.gate_mode == kGateFull)
-        return all ? launch_ring<backward_ring_kernel<T, R, kVpt, kRows, true, true, kCallAll>>(p, lay, kRows, count, stream)
-                   : launch_ring<backward_ring_kernel<T, R, kVpt, kRows, true, true, kCallAny>>(p, lay, kRows, count, stream);
-    return all ? launch_ring<backward_ring_kernel<T, R, kVpt, kRows, true, false, kCallAll>>(p, lay, kRows, count, stream)
-               : launch_ring<backward_ring_kernel<T, R, kVpt, kRows, true, false, kCallAny>>(p, lay, kRows, count, stream);
+        return all ? launch_backward_ring<T, R, kVpt, kRows, true, true, kCallAll>(p, lay, count, stream)
+                   : launch_backward_ring<T, R, kVpt, kRows, true, true, kCallAny>(p, lay, count, stream);
+    return all ? launch_backward_ring<T, R, kVpt, kRows, true, false, kCallAll>(p, lay, count, stream)
+               : launch_backward_ring<T, R, kVpt, kRows, true, false, kCallAny>(p, lay, count, stream);
 }
 
 template <typename T, typename R>
-static int run_backward(const Params& p, bool vec, void* d_weight, void* d_post, void* d_gate_channel, cudaStream_t stream) {
+static int run_backward(const Params& p, Layout rows_are, void* d_weight, void* d_post, void* d_gate_channel, cudaStream_t stream) {
     int count = 0, status = XMA_OK;
     const int vpt = p.hidden > 4096 ? 2 : 1, rows = vpt == 1 ? 2 : 1;
     RingLayout lay;
-    if (vec && p.hidden <= kRingMaxHidden && ring_layout<T, R>(p, true, vpt, rows, 2, &lay)) {
-        status = vpt == 1 ? run_backward_ring<T, R, 1, 2>(p, lay, &count, stream) : run_backward_ring<T, R, 2, 1>(p, lay, &count, stream);
+    const bool vec = rows_are.vec;
+    if (rows_are.wide && p.hidden <= (vec ? kRingMaxHidden : kRingMaxHiddenAny) && ring_layout<T, R>(p, vec, true, vpt, rows, 2, &lay)) {
+        status = vpt == 1 ? run_backward_ring<T, R, 1, 2>(p, lay, vec, &count, stream) : run_backward_ring<T, R, 2, 1>(p, lay, vec, &count, stream);
     } else {
         backward_sums_kernel<T, R><<<static_cast<unsigned>(p.rows), 256, 0, stream>>>(p);
         status = launch_status();
@@ -1160,13 +1271,13 @@ static int run_backward(const Params& p, bool vec, void* d_weight, void* d_post,
     return launch_status();
 }
 
-static bool all_aligned(const Params& p) {
+static Layout layout_of(const Params& p) {
     const void* ptrs[] = {p.x, p.residual, p.weight, p.post, p.gate, p.s_out, p.y, p.dy, p.d_stream, p.s, p.dx, p.d_residual, p.d_gate};
     for (int i = 0; i < static_cast<int>(sizeof(ptrs) / sizeof(ptrs[0])); ++i) {
         const bool token = p.gate_mode == kGateToken && (ptrs[i] == p.gate || ptrs[i] == p.d_gate);
-        if (!token && !aligned16(ptrs[i])) return false;
+        if (!token && !aligned16(ptrs[i])) return Layout{false, false};
     }
-    return p.hidden % 8 == 0;
+    return Layout{p.hidden % 8 == 0, true};
 }
 
 static bool size_ok(int64_t rows, int64_t hidden, int32_t gate_mode) {
@@ -1198,13 +1309,13 @@ int xma_norm_forward(const void* x, const void* residual, const void* weight, co
     p.weight_f32 = f32_params & 1, p.post_f32 = f32_params & 2, p.gate_f32 = f32_params & 4;
     p.rows = rows, p.hidden = static_cast<int>(hidden), p.eps = eps, p.multiplier = multiplier;
     p.s_out = stream_out, p.y = y, p.rs = rstd, p.rp = rstd_post, p.status = status;
-    const bool vec = all_aligned(p);
+    const Layout lay = layout_of(p);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == kDtypeBF16 && stream_dtype == kDtypeBF16) return run_forward<__nv_bfloat16, __nv_bfloat16>(p, vec, st);
-    if (dtype == kDtypeBF16 && stream_dtype == kDtypeF32) return run_forward<__nv_bfloat16, float>(p, vec, st);
-    if (dtype == kDtypeF16 && stream_dtype == kDtypeF16) return run_forward<__half, __half>(p, vec, st);
-    if (dtype == kDtypeF16 && stream_dtype == kDtypeF32) return run_forward<__half, float>(p, vec, st);
-    if (dtype == kDtypeF32 && stream_dtype == kDtypeF32) return run_forward<float, float>(p, vec, st);
+    if (dtype == kDtypeBF16 && stream_dtype == kDtypeBF16) return run_forward<__nv_bfloat16, __nv_bfloat16>(p, lay, st);
+    if (dtype == kDtypeBF16 && stream_dtype == kDtypeF32) return run_forward<__nv_bfloat16, float>(p, lay, st);
+    if (dtype == kDtypeF16 && stream_dtype == kDtypeF16) return run_forward<__half, __half>(p, lay, st);
+    if (dtype == kDtypeF16 && stream_dtype == kDtypeF32) return run_forward<__half, float>(p, lay, st);
+    if (dtype == kDtypeF32 && stream_dtype == kDtypeF32) return run_forward<float, float>(p, lay, st);
     return XMA_ERR_UNSUPPORTED;
 }
 
@@ -1235,18 +1346,18 @@ int xma_norm_backward(const void* dy, const void* d_stream, const void* stream_o
     void* d_gate_channel = gate_mode == kGateChannel ? d_gate : nullptr;
     p.want_weight = d_weight != nullptr, p.want_post = d_post_weight != nullptr, p.want_gate = d_gate_channel != nullptr;
     p.status = status;
-    const bool vec = all_aligned(p);
+    const Layout lay = layout_of(p);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == kDtypeBF16 && stream_dtype == kDtypeBF16)
-        return run_backward<__nv_bfloat16, __nv_bfloat16>(p, vec, d_weight, d_post_weight, d_gate_channel, st);
+        return run_backward<__nv_bfloat16, __nv_bfloat16>(p, lay, d_weight, d_post_weight, d_gate_channel, st);
     if (dtype == kDtypeBF16 && stream_dtype == kDtypeF32)
-        return run_backward<__nv_bfloat16, float>(p, vec, d_weight, d_post_weight, d_gate_channel, st);
+        return run_backward<__nv_bfloat16, float>(p, lay, d_weight, d_post_weight, d_gate_channel, st);
     if (dtype == kDtypeF16 && stream_dtype == kDtypeF16)
-        return run_backward<__half, __half>(p, vec, d_weight, d_post_weight, d_gate_channel, st);
+        return run_backward<__half, __half>(p, lay, d_weight, d_post_weight, d_gate_channel, st);
     if (dtype == kDtypeF16 && stream_dtype == kDtypeF32)
-        return run_backward<__half, float>(p, vec, d_weight, d_post_weight, d_gate_channel, st);
+        return run_backward<__half, float>(p, lay, d_weight, d_post_weight, d_gate_channel, st);
     if (dtype == kDtypeF32 && stream_dtype == kDtypeF32)
-        return run_backward<float, float>(p, vec, d_weight, d_post_weight, d_gate_channel, st);
+        return run_backward<float, float>(p, lay, d_weight, d_post_weight, d_gate_channel, st);
     return XMA_ERR_UNSUPPORTED;
 }
 

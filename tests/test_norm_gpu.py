@@ -293,3 +293,13 @@ def test_non_finite_rows_stay_alone_in_large_batches(rows, hidden):
     for name in want:
         assert torch.equal(got[name][keep], want[name][keep])
     assert got["y"][0].isnan().all() and got["dx"][rows // 2].isnan().all()
+
+
+@pytest.mark.parametrize("rows,hidden", [(9601, 777), (2401, 4095), (18945, 515), (9473, 1002)])
+@pytest.mark.parametrize("types", range(len(TYPES)))
+def test_many_rows_of_no_whole_vectors(rows, hidden, types):
+    """Rows that start anywhere in a 16-byte piece, the tensors' last bytes outside a whole one."""
+    dtype, stream_dtype = TYPES[types]
+    assert hidden % 8 and rows * hidden % 8
+    check(make(rows, hidden, dtype, stream_dtype, GATES[types % 4], types % 2 == 0), 0.3)
+    check(make(rows, hidden, dtype, None, None, False), 1.0)
