@@ -458,3 +458,18 @@ def test_one_input_learns():
     total = sum(parts[n].double() for n in ("dq", "dk", "dv"))
     magnitude = sum(parts[n].double().abs() for n in ("dq", "dk", "dv"))
     assert ((one.grad.double() - total).abs() <= 2 * half_step(torch.bfloat16) * magnitude * (1 + 2 ** -7)).all()  # two additions in bf16
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 96])
+def test_one_key_has_no_gradient(dtype, dim):
+    """A softmax over one key is 1 whatever the score: the first rows' dq, and dk of sequences of one token, are zeros."""
+    lengths = [1, 1, 0, 1, 300, 1, 128, 2]
+    got = check(lengths, 4, 2, dim, dtype, behind=3)
+    at = 0
+    for n in lengths:
+        if n:
+            assert (got["dq"][at] == 0).all()
+        if n == 1:
+            assert (got["dk"][at] == 0).all()
+        at += n
