@@ -1183,7 +1183,9 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
                             pr[c * 16 + e * 2] = ds_pair<T>(pr[c * 16 + e * 2], pair(dp + e * 4), make_f32x2(f.x, f.y), factor2);
                             pr[c * 16 + e * 2 + 1] = ds_pair<T>(pr[c * 16 + e * 2 + 1], pair(dp + e * 4 + 2), make_f32x2(f.z, f.w), factor2);
                         }
-                        if (edge) clear_outside(pr + c * 16, from - c * 32, last - c * 32);  // delta of such a column is no number to rely on
+                        // delta of a column outside is no number to rely on; a sequence's first query has one key, whose
+                        // score has no gradient: dp - delta would leave a rounding there
+                        if (edge) clear_outside(pr + c * 16, (i == 0 && half == 0 ? max(from, 1) : from) - c * 32, last - c * 32);
                         store_packed32<T>(dp_addr + c * 16, pr + c * 16);
                         tmem_st_wait();
                         tc_fence_before();
@@ -1452,7 +1454,8 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
                     tmem_tie32(dp);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) pr[c * 16 + i] = ds_pair<T>(pr[c * 16 + i], pair(dp + i * 2), neg_delta, factor2);
-                    if (j == b.index) clear_outside(pr + c * 16, 0, row + 1 - half * 64 - c * 32);
+                    // a sequence's first query has one key, whose score has no gradient
+                    if (j == b.index) clear_outside(pr + c * 16, 0, (query == 0 ? 0 : row + 1) - half * 64 - c * 32);
                     store_packed32<T>(dp_addr + c * 16, pr + c * 16);
                     tmem_st_wait();
                     tc_fence_before();
