@@ -45,7 +45,15 @@ using namespace ptx;
 constexpr int kTile = 128;            // query or key rows of a tile
 constexpr int kThreads = 384;         // load warp, MMA warp, two idle, two groups of four compute warps
 constexpr int kTmemCols = 512;
-constexpr float kRescaleLog2 = 8.f;   // the accumulator is rescaled when a row's maximum grew by more than 2^8
+// The accumulator is rescaled when a row's maximum grew by more than 2^kRescaleLog2, and p carries 2^kShiftLog2: together
+// they leave a factor of two under fp16's largest number, and p of a key that others outweigh keeps its bits down to 2^-23
+// beside the row's largest and has some down to 2^-33 (without the shift 2^-14 and 2^-25, which thousands of such keys
+// show). 2^4 and 2^11 cost rescaled tiles: 8192 tokens, 32 heads on 8 of 128, 465 us against 441; 2^6 costs nothing. bf16
+// has float32's range and needs no shift.
+template <typename T>
+constexpr float kRescaleLog2 = std::is_same<T, __half>::value ? 6.f : 8.f;
+template <typename T>
+constexpr float kShiftLog2 = std::is_same<T, __half>::value ? 9.f : 0.f;
 constexpr int kControlRegs = 88;      // registers of the load and MMA warps' group and of the compute groups:
 constexpr int kComputeRegs = 208;     // 128 * 88 + 256 * 208 = 384 * 168
 constexpr int kPlanThreads = 1024;
@@ -579,7 +587,7 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             const int row0 = b.index * 2 * kTile;
             if (t == 1 && b.len <= row0 + kTile) continue;
             const int count = b.index * 2 + 1 + t;
-            float m = -INFINITY, l = 0.f;  // running maximum (log2 units) that p refers to, and sum of p
+            float m = -INFINITY, l = 0.f;  // running maximum (log2 units) that p refers to, and sum of p, shift and all
             for (int j = 0; j < count; ++j) {
                 ok = mbar_wait(s_full + 8 * t, s_phase, abort_flag, p.status, 508);
                 if (!ok) break;
@@ -610,8 +618,8 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                     m = tile_max;
                 } else {
                     // The sum stays exact whatever m is, as long as p does not overflow: the accumulator is
-                    // touched only when a maximum grew by 2^8, which after the first tiles hardly happens.
-                    const bool grow = tile_max - m > kRescaleLog2;
+                    // touched only when a maximum grew by so much, which after the first tiles hardly happens.
+                    const bool grow = tile_max - m > kRescaleLog2<T>;
                     if (__any_sync(0xffffffffu, grow)) {
                         const float factor = grow ? ex2(m - tile_max) : 1.f;
                         if (grow) m = tile_max;
@@ -628,7 +636,7 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                         }
                     }
                 }
-                const float neg_m = m == -INFINITY ? 0.f : -m;  // a row with no finite score so far
+                const float neg_m = m == -INFINITY ? 0.f : kShiftLog2<T> - m;  // a row with no finite score so far
                 const f32x2 scale2 = make_f32x2(p.scale_log2, p.scale_log2), neg_m2 = make_f32x2(neg_m, neg_m);
                 f32x2 sum[2] = {make_f32x2(0.f, 0.f), make_f32x2(0.f, 0.f)};
 #pragma unroll
@@ -665,7 +673,7 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             store_output<T, kD>(o_addr, base + kStagingAt + (warp - 4) * F::kStaging, &map_out, &map_rest, static_cast<T*>(p.out),
                                 p.rest, p.rest_row, static_cast<int64_t>(b.start) + first, min(32, b.len - first), p.heads, head, p.dim,
                                 1.f / l, lane);
-            if (p.lse != nullptr && valid) p.lse[head * p.pad_rows + b.pad + r] = m + lg2(l);
+            if (p.lse != nullptr && valid) p.lse[head * p.pad_rows + b.pad + r] = m + (lg2(l) - kShiftLog2<T>);
             tc_fence_before();
         }
     }

@@ -78,8 +78,8 @@ def attention_packed(
     the tokens `cu_seqlens[b] .. cu_seqlens[b + 1] - 1` (none, one or many). `softmax_scale` is positive and
     defaults to `1 / sqrt(head_dim)`.
 
-    Scores and sums are float32; probabilities are rounded to the inputs' dtype before they meet the values. For a
-    backward pass the call keeps its inputs, its output, a float32 per row and head and, so that gradients do not suffer
+    Scores and sums are float32; probabilities are rounded to the inputs' dtype before they meet the values (in float16
+    times a power of two, so that keys which others outweigh keep their share). For a backward pass the call keeps its inputs, its output, a float32 per row and head and, so that gradients do not suffer
     from the output's rounding, one byte per output element; gradients are summed in a fixed order. In float16 the
     gradient of the scores is rounded with a power-of-two factor that the batch's largest upstream gradient and value
     set, so small gradients keep their bits without loss scaling.

@@ -473,3 +473,58 @@ def test_one_key_has_no_gradient(dtype, dim):
         if n == 1:
             assert (got["dk"][at] == 0).all()
         at += n
+
+
+def reference_fp16(q, k, v, do, lengths, scale=None):
+    """`reference` with what fp16 adds where numbers fall under its smallest normal one, steps there being 2^-24: half a
+    step for every p of a row, which carries 2^9 (in units of its row's largest p) on its way to o and 2^14 on its way to
+    dv, and for every ds, which carries the power of two that puts 2 dim max|do| max|v| between 2^14 and 2^15."""
+    ref = reference(q, k, v, do, lengths, scale=scale)
+    G, D = q.size(1) // k.size(1), q.size(2)
+    e = 2 * D * do.double().abs().max() * v.double().abs().max() * 2.0 ** -14 * 2.0 ** -25 * (scale or 1 / math.sqrt(D))
+    at = 0
+    for L in lengths:
+        r = slice(at, at + L)
+        at += L
+        before = lambda t: t[r].double().abs().cumsum(0).repeat_interleave(G, 1)
+        behind = lambda t: t[r].double().abs().flip(0).cumsum(0).flip(0).unflatten(1, (-1, G)).sum(2)
+        for name, term in (("o", 2.0 ** -34 * before(v)), ("dv", 2.0 ** -39 * behind(do)), ("dq", e * before(k)), ("dk", e * behind(q))):
+            ref[name][1][r] += term * (1 + 2.0 ** -10)
+    return ref
+
+
+def outweighed(gap):
+    """One key beside which each of the others weighs exp(-gap), with values and upstream gradients of one sign."""
+    L, D = 4000, 64
+    q, k, v, do = make([L], 1, 1, D, torch.float16)
+    q.zero_(), k.zero_()
+    q[..., 0], k[0, :, 0] = 8.0, gap
+    v[0], v[1:] = 0.0, v[1:].abs() * 8
+    return q, k, v, (do.abs() * 100 + 8).to(torch.float16), [L]
+
+
+def sharp(q_scale):
+    lengths = [1200, 1, 340]
+    q, k, v, do = make(lengths, 4, 2, 64, torch.float16, q_scale=q_scale)
+    return q, k, v, (do * 400).to(torch.float16), lengths
+
+
+def growing(top):
+    """Scores that rise along the keys, by as much as leaves the accumulator alone from tile to tile and by more."""
+    q, k, v, do = make([900], 2, 2, 64, torch.float16)
+    q[..., 0], k[..., 0] = 8.0, torch.linspace(0, top, 900, device="cuda")[:, None].to(torch.float16)
+    return q, k, v, do, [900]
+
+
+SMALL_WEIGHTS = ([(outweighed, gap) for gap in (12.0, 18.0, 22.0)] + [(sharp, s) for s in (0.0, 1e-3, 3.0, 20.0)]
+                 + [(growing, top) for top in (2.0, 6.0, 11.0, 20.0, 60.0)])
+
+
+@pytest.mark.parametrize("make_inputs,value", SMALL_WEIGHTS)
+def test_small_weights_fp16(make_inputs, value):
+    """Keys too small for fp16 beside their row's largest, each alone; thousands of them are not."""
+    q, k, v, do, lengths = make_inputs(value)
+    ref = reference_fp16(q, k, v, do, lengths)
+    with torch.no_grad():
+        assert_within("o", xma.attention_packed(q, k, v, offsets(lengths)), *ref["o"])
+    assert_status_clean(q.device)
