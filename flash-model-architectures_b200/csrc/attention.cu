@@ -54,6 +54,12 @@ template <typename T>
 constexpr float kRescaleLog2 = std::is_same<T, __half>::value ? 6.f : 8.f;
 template <typename T>
 constexpr float kShiftLog2 = std::is_same<T, __half>::value ? 9.f : 0.f;
+// The same in the backward pass, where p is at most 1: it carries 2^kProbLog2, which the row statistics are kept less of
+// and dv and ds are divided by; a factor of four under the largest number is for what the exponent is off by.
+template <typename T>
+constexpr int kProbLog2 = std::is_same<T, __half>::value ? 14 : 0;
+template <typename T>
+constexpr float kProbInverse = 1.f / static_cast<float>(1 << kProbLog2<T>);
 constexpr int kControlRegs = 88;      // registers of the load and MMA warps' group and of the compute groups:
 constexpr int kComputeRegs = 208;     // 128 * 88 + 256 * 208 = 384 * 168
 constexpr int kPlanThreads = 1024;
@@ -76,7 +82,7 @@ struct Params {
     int64_t pad_rows;  // entries of the padded row statistics per head
     float scale, scale_log2;
     void* out;         // forward: o
-    float* lse;        // [heads][pad_rows], log2 units; may be NULL in the forward pass
+    float* lse;        // [heads][pad_rows], log2 units, less kProbLog2; may be NULL in the forward pass
     uint8_t* rest;     // [tokens, heads, rest_row]: what out's rounding took away; NULL when lse is
     int64_t rest_row;  // dim, rounded up to 16
     const float* delta;      // negated
@@ -673,7 +679,7 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             store_output<T, kD>(o_addr, base + kStagingAt + (warp - 4) * F::kStaging, &map_out, &map_rest, static_cast<T*>(p.out),
                                 p.rest, p.rest_row, static_cast<int64_t>(b.start) + first, min(32, b.len - first), p.heads, head, p.dim,
                                 1.f / l, lane);
-            if (p.lse != nullptr && valid) p.lse[head * p.pad_rows + b.pad + r] = m + (lg2(l) - kShiftLog2<T>);
+            if (p.lse != nullptr && valid) p.lse[head * p.pad_rows + b.pad + r] = m + (lg2(l) - (kShiftLog2<T> + kProbLog2<T>));
             tc_fence_before();
         }
     }
@@ -845,7 +851,7 @@ __device__ __forceinline__ f32x2 ex2_neg2(f32x2 x) {
     split_f32x2(x, lo, hi);
     return make_f32x2(ex2(-lo), ex2(-hi));
 }
-// ds = p (dp - delta), with the factor that fp16 is rounded with
+// ds = p (dp - delta), with the factor that fp16 is rounded with (and without the one that p has)
 template <typename T>
 __device__ __forceinline__ f32x2 ds_pair(f32x2 p, f32x2 dp, f32x2 neg_delta, f32x2 factor) {
     f32x2 d = add_f32x2(dp, neg_delta);
@@ -1132,7 +1138,7 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_addr = tm_s + lanes + half * 64, dp_addr = tm_dp + lanes + half * 64;
         const float factor = ds_factor<T>(p);
-        const f32x2 factor2 = make_f32x2(factor, factor), neg_scale2 = make_f32x2(-p.scale_log2, -p.scale_log2);
+        const f32x2 factor2 = make_f32x2(factor * kProbInverse<T>, factor * kProbInverse<T>), neg_scale2 = make_f32x2(-p.scale_log2, -p.scale_log2);
         Ring d;
         uint32_t s_phase = 0, dp_phase = 0, done_phase = 0;
         bool ok = true;
@@ -1210,7 +1216,7 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
             tc_fence_after();
             const int key = b.index * kTile + row;
             const int64_t at = (static_cast<int64_t>(b.start + key) * p.kv_heads + kv_head) * p.dim;
-            if (half == 0) store_row<T, kD>(tm_dv + lanes, static_cast<T*>(p.dv) + at, p.dim, 1.f, key < b.len);
+            if (half == 0) store_row<T, kD>(tm_dv + lanes, static_cast<T*>(p.dv) + at, p.dim, kProbInverse<T>, key < b.len);
             else store_row<T, kD>(tm_dk + lanes, static_cast<T*>(p.dk) + at, p.dim, p.scale / factor, key < b.len);
             tc_fence_before();
         }
@@ -1420,7 +1426,7 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t dp_addr = tm_dp + lanes + half * 64;
         const float factor = ds_factor<T>(p);
-        const f32x2 factor2 = make_f32x2(factor, factor), neg_scale2 = make_f32x2(-p.scale_log2, -p.scale_log2);
+        const f32x2 factor2 = make_f32x2(factor * kProbInverse<T>, factor * kProbInverse<T>), neg_scale2 = make_f32x2(-p.scale_log2, -p.scale_log2);
         Ring buf;
         uint32_t dp_phase = 0, done_phase = 0;
         bool ok = true;

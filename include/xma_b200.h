@@ -415,7 +415,7 @@ int xma_norm_backward(const void* dy, const void* d_stream, const void* stream_o
  *   [total, kv_heads, dim] are contiguous. heads is a multiple of kv_heads (query head h reads kv head
  *   h / (heads / kv_heads)), dim a multiple of 8 up to 128, scale positive.
  *   lse   float32 [heads, xma_attention_stat_rows(total, batch)], 16-byte aligned: the rows' log-sum-exp (base
- *         2), written by the forward pass for the backward pass; NULL when there is none
+ *         2; in fp16 less 14), written by the forward pass for the backward pass; NULL when there is none
  *   out_rest  bytes [total, heads, dim rounded up to 16], 16-byte aligned: what rounding took from out (e5m2,
  *         scaled); written with lse and read by the backward pass; NULL when lse is
  *   delta float32, the size of lse, scratch of the backward pass

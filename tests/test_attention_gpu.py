@@ -478,19 +478,38 @@ def test_one_key_has_no_gradient(dtype, dim):
 def reference_fp16(q, k, v, do, lengths, scale=None):
     """`reference` with what fp16 adds where numbers fall under its smallest normal one, steps there being 2^-24: half a
     step for every p of a row, which carries 2^9 (in units of its row's largest p) on its way to o and 2^14 on its way to
-    dv, and for every ds, which carries the power of two that puts 2 dim max|do| max|v| between 2^14 and 2^15."""
+    dv, and for every ds, which carries the power of two that puts 2 dim max|do| max|v| between 2^14 and 2^15. What o is
+    off by is in delta = o . do too, and with it in every ds of the row, times p. Largest finite number: 65504; from 65520
+    on the nearest one is infinity."""
     ref = reference(q, k, v, do, lengths, scale=scale)
-    G, D = q.size(1) // k.size(1), q.size(2)
-    e = 2 * D * do.double().abs().max() * v.double().abs().max() * 2.0 ** -14 * 2.0 ** -25 * (scale or 1 / math.sqrt(D))
+    H, D = q.shape[1:]
+    G, scale = H // k.size(1), scale or 1 / math.sqrt(D)
+    e_ds = 2 * D * do.double().abs().max() * v.double().abs().max() * 2.0 ** -14 * 2.0 ** -25
+    more = 1 + 2.0 ** -10  # products of two errors, the results' own rounding
     at = 0
     for L in lengths:
         r = slice(at, at + L)
         at += L
-        before = lambda t: t[r].double().abs().cumsum(0).repeat_interleave(G, 1)
-        behind = lambda t: t[r].double().abs().flip(0).cumsum(0).flip(0).unflatten(1, (-1, G)).sum(2)
-        for name, term in (("o", 2.0 ** -34 * before(v)), ("dv", 2.0 ** -39 * behind(do)), ("dq", e * before(k)), ("dk", e * behind(q))):
-            ref[name][1][r] += term * (1 + 2.0 ** -10)
+        for h in range(H):
+            qq, kk, vv, dd = (t.double() for t in (q[r, h], k[r, h // G], v[r, h // G], do[r, h]))
+            seen = torch.ones(L, L, dtype=torch.float64, device=q.device).tril()
+            p = torch.softmax((qq @ kk.t() * scale).masked_fill(seen == 0, -math.inf), -1)
+            e_o = 2.0 ** -34 * (seen @ vv.abs())
+            e = seen * e_ds + p * (e_o * dd.abs()).sum(-1, keepdim=True)
+            for name, head, term in (("o", h, e_o), ("dv", h // G, 2.0 ** -39 * (seen.t() @ dd.abs())),
+                                     ("dq", h, scale * (e @ kk.abs())), ("dk", h // G, scale * (e.t() @ qq.abs()))):
+                ref[name][1][r, head] += term * more
+    for name, (want, bound) in ref.items():
+        over = want.abs() - bound >= 65520
+        want[over], bound[over] = want[over].sign() * math.inf, 0.0
     return ref
+
+
+def assert_within_fp16(name, got, want, bound):
+    """assert_within for values of which some are too large for fp16."""
+    over = want.isinf()
+    assert torch.equal(got[over].double(), want[over]), name
+    assert_within(name, got.masked_fill(over, 0), want.masked_fill(over, 0), bound)
 
 
 def outweighed(gap):
@@ -527,4 +546,14 @@ def test_small_weights_fp16(make_inputs, value):
     ref = reference_fp16(q, k, v, do, lengths)
     with torch.no_grad():
         assert_within("o", xma.attention_packed(q, k, v, offsets(lengths)), *ref["o"])
+    assert_status_clean(q.device)
+
+
+@pytest.mark.parametrize("make_inputs,value", SMALL_WEIGHTS)
+def test_gradients_of_small_weights_fp16(make_inputs, value):
+    """The same backward: dv of keys that each row hardly looks at is a sum over all the rows."""
+    q, k, v, do, lengths = make_inputs(value)
+    got, ref = run(q, k, v, do, offsets(lengths)), reference_fp16(q, k, v, do, lengths)
+    for name in ("dq", "dk", "dv"):
+        assert_within_fp16(name, got[name], *ref[name])
     assert_status_clean(q.device)
