@@ -89,7 +89,7 @@ struct Params {
     void* dq;
     void* dk;
     void* dv;
-    const uint32_t* absmax;  // backward, fp16: bit patterns of max |do| and max |v|
+    const uint32_t* absmax;  // backward, fp16: bit patterns of the largest finite |do| and |v|
     int32_t* status;
     int ab_format;
 };
@@ -696,9 +696,25 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 // Backward
 // ---------------------------------------------------------------------------------------------
 
-__device__ __forceinline__ float absmax_value(uint32_t bits) {
-    const float v = __uint_as_float(bits);
-    return v <= 65504.f ? v : 65504.f;  // also when it is infinite or NaN
+// Largest finite |x| of eight. A row that holds an infinity or a NaN is lost whatever its factor, and must not take the
+// bits of other sequences' gradients with it.
+template <typename T>
+__device__ __forceinline__ float largest_finite(const uint32_t (&words)[4]) {
+    float top = 0.f;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const float2 f = unpack2<T>(words[q]);
+        top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));  // passes NaNs by
+    }
+    if (top < INFINITY) return top;
+    top = 0.f;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const float2 f = unpack2<T>(words[q]);
+        if (fabsf(f.x) < INFINITY) top = fmaxf(top, fabsf(f.x));
+        if (fabsf(f.y) < INFINITY) top = fmaxf(top, fabsf(f.y));
+    }
+    return top;
 }
 // Factor (a power of two) that ds carries while it is rounded to T. bf16 has float32's range: 1. fp16 has
 // not: |ds| is at most 2 dim max|do| max|v|, and that bound is put at 2^15, just below the largest fp16, so
@@ -707,14 +723,14 @@ template <typename T>
 __device__ __forceinline__ float ds_factor(const Params& p) { return 1.f; }
 template <>
 __device__ __forceinline__ float ds_factor<__half>(const Params& p) {
-    const float bound = 2.f * static_cast<float>(p.dim) * absmax_value(p.absmax[0]) * absmax_value(p.absmax[1]);
+    const float bound = 2.f * static_cast<float>(p.dim) * __uint_as_float(p.absmax[0]) * __uint_as_float(p.absmax[1]);
     if (!(bound > 0.f)) return 1.f;
     return exp2f(static_cast<float>(min(max(14 - ilogbf(bound), -100), 100)));
 }
 
 // -delta_i = -o_i . do_i for every row of every block and head (negated: the backward kernels add it two at a
 // time), o with what its rounding took away; for fp16 also
-// max |do| and max |v| (over bit patterns, whose order does not depend on that of the atomics). A CTA takes
+// max |do| and max |v| of the finite ones (over bit patterns, whose order does not depend on that of the atomics). A CTA takes
 // kDeltaRows rows of a block of the plan; groups of kD / 8 lanes take one head of one row each, 16 bytes a lane, four at
 // a time. Bound by HBM: 77 us for 16384 tokens x 32 heads of 128 (335 MB, 4.4 TB/s; smaller batches at more occupancy
 // gain 5 us there and lose as much on short sequences).
@@ -733,7 +749,7 @@ delta_kernel(const T* __restrict__ o, const uint8_t* __restrict__ rest, const T*
     if (rows <= 0) return;
     const int sub = threadIdx.x % kLanes, slot = threadIdx.x / kLanes;
     const bool in_head = sub * 8 < p.dim;
-    uint32_t most_do = 0, most_v = 0;
+    float most_do = 0.f, most_v = 0.f;
     const int pairs = rows * p.heads;  // (row, head) pairs lie one after another in memory
     const int64_t base = (static_cast<int64_t>(b.start) + first) * p.heads * p.dim + sub * 8;
     const int64_t rest_base = (static_cast<int64_t>(b.start) + first) * p.heads * p.rest_row + sub * 8;
@@ -763,8 +779,8 @@ delta_kernel(const T* __restrict__ o, const uint8_t* __restrict__ rest, const T*
                 const __half2_raw raw = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two & 0xffff), __NV_E5M2);
                 const float2 e = __half22float2(*reinterpret_cast<const __half2*>(&raw));
                 sum += fmaf(e.x, 1.f / kRestScale<T>, f.x) * g.x + fmaf(e.y, 1.f / kRestScale<T>, f.y) * g.y;
-                if (kHalf) most_do = max(most_do, __float_as_uint(fmaxf(fabsf(g.x), fabsf(g.y))));
             }
+            if (kHalf) most_do = fmaxf(most_do, largest_finite<T>(yw));
 #pragma unroll
             for (int w = kLanes / 2; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
             if (r < rows && sub == 0) delta[h * p.pad_rows + b.pad + first + r] = -sum;
@@ -787,21 +803,17 @@ delta_kernel(const T* __restrict__ o, const uint8_t* __restrict__ rest, const T*
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) {
                 const uint32_t xw[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const float2 f = unpack2<T>(xw[q]);
-                    most_v = max(most_v, __float_as_uint(fmaxf(fabsf(f.x), fabsf(f.y))));
-                }
+                most_v = fmaxf(most_v, largest_finite<T>(xw));
             }
         }
         __shared__ uint32_t most[2];
         if (threadIdx.x < 2) most[threadIdx.x] = 0;
         __syncthreads();
-        most_do = __reduce_max_sync(0xffffffffu, most_do);
-        most_v = __reduce_max_sync(0xffffffffu, most_v);
+        const uint32_t warp_do = __reduce_max_sync(0xffffffffu, __float_as_uint(most_do));
+        const uint32_t warp_v = __reduce_max_sync(0xffffffffu, __float_as_uint(most_v));
         if ((threadIdx.x & 31) == 0) {
-            atomicMax(&most[0], most_do);
-            atomicMax(&most[1], most_v);
+            atomicMax(&most[0], warp_do);
+            atomicMax(&most[1], warp_v);
         }
         __syncthreads();
         // most CTAs find a larger value there already and leave the one address alone

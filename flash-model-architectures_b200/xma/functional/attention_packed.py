@@ -79,10 +79,11 @@ def attention_packed(
     defaults to `1 / sqrt(head_dim)`.
 
     Scores and sums are float32; probabilities are rounded to the inputs' dtype before they meet the values (in float16
-    times a power of two, so that keys which others outweigh keep their share). For a backward pass the call keeps its inputs, its output, a float32 per row and head and, so that gradients do not suffer
-    from the output's rounding, one byte per output element; gradients are summed in a fixed order. In float16
-    probabilities and the gradient of the scores are rounded with powers of two, the latter one that the batch's largest
-    upstream gradient and value set, so small gradients keep their bits without loss scaling.
+    times a power of two, so that keys which others outweigh keep their share). For a backward pass the call keeps its
+    inputs, its output, a float32 per row and head and, so that gradients do not suffer from the output's rounding, one
+    byte per output element; gradients are summed in a fixed order. In float16 probabilities and the gradient of the
+    scores are rounded with powers of two, the latter one that the batch's largest finite upstream gradient and value
+    set, so small gradients keep their bits without loss scaling.
 
     Tokens that no sequence owns get zeros, in the output and in the gradients, and what they hold reaches nothing. A
     NaN or an infinity in a value also reaches rows before it in its own sequence, as in a product with probabilities

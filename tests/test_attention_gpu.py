@@ -557,3 +557,17 @@ def test_gradients_of_small_weights_fp16(make_inputs, value):
     for name in ("dq", "dk", "dv"):
         assert_within_fp16(name, got[name], *ref[name])
     assert_status_clean(q.device)
+
+
+@pytest.mark.parametrize("what", [math.inf, -math.inf, math.nan])
+def test_non_finite_values_leave_the_factor_alone(what):
+    """A sequence whose upstream gradient or values are not finite takes no bit from its neighbours' small gradients."""
+    lengths = [100, 60, 300]
+    q, k, v, do = make(lengths, 4, 2, 64, torch.float16)
+    do = (do * 2.0 ** -8).to(torch.float16)
+    do[100:160], v[100:160] = 0.0, 0.0
+    clean = run(q, k, v, do, offsets(lengths))
+    do[107, 1, 5], v[111, 0, 9], do[120, 2, 8] = what, what, what
+    got = run(q, k, v, do, offsets(lengths))
+    for name in got:
+        assert torch.equal(got[name][:100], clean[name][:100]) and torch.equal(got[name][160:], clean[name][160:])
