@@ -269,8 +269,28 @@ __device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t second
 template <typename T>
 constexpr float kRestScale = std::is_same<T, __half>::value ? 32768.f : 4096.f;
 
+// 32 values of o, divided by their row's sum. The sum adds p as it was, the product p as it was rounded (2^-11 off at most),
+// so a mean of values next to fp16's largest number could round to infinity; no mean is above the largest value.
+template <typename T>
+__device__ __forceinline__ void scale_output(uint32_t (&r)[32], float scale) {
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        const float v = __uint_as_float(r[i]) * scale;
+        r[i] = __float_as_uint(v);
+        if (std::is_same<T, __half>::value) top = fmaxf(top, fabsf(v));
+    }
+    if (std::is_same<T, __half>::value && __any_sync(0xffffffffu, top > 65504.f)) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const float v = __uint_as_float(r[i]);
+            if (fabsf(v) < 65600.f) r[i] = __float_as_uint(fminf(fmaxf(v, -65504.f), 65504.f));  // an infinity stays one
+        }
+    }
+}
+
 // 16-byte pieces of one row of kD float32 values in tensor memory, scaled and rounded, to global memory.
-template <typename T, int kD>
+template <typename T, int kD, bool kOutput = false>
 __device__ __forceinline__ void store_row(uint32_t taddr, T* dst, int dim, float scale, bool valid) {
 #pragma unroll
     for (int c = 0; c < kD / 32; ++c) {
@@ -278,14 +298,20 @@ __device__ __forceinline__ void store_row(uint32_t taddr, T* dst, int dim, float
         tmem_ld32(taddr + c * 32, r);
         tmem_ld_wait();
         tmem_tie32(r);
+        if (kOutput) {
+            scale_output<T>(r, scale);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * scale);
+        }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             if (valid && c * 32 + q * 8 < dim) {
                 uint4 v;
-                v.x = pack2<T>(__uint_as_float(r[q * 8]) * scale, __uint_as_float(r[q * 8 + 1]) * scale);
-                v.y = pack2<T>(__uint_as_float(r[q * 8 + 2]) * scale, __uint_as_float(r[q * 8 + 3]) * scale);
-                v.z = pack2<T>(__uint_as_float(r[q * 8 + 4]) * scale, __uint_as_float(r[q * 8 + 5]) * scale);
-                v.w = pack2<T>(__uint_as_float(r[q * 8 + 6]) * scale, __uint_as_float(r[q * 8 + 7]) * scale);
+                v.x = pack2<T>(__uint_as_float(r[q * 8]), __uint_as_float(r[q * 8 + 1]));
+                v.y = pack2<T>(__uint_as_float(r[q * 8 + 2]), __uint_as_float(r[q * 8 + 3]));
+                v.z = pack2<T>(__uint_as_float(r[q * 8 + 4]), __uint_as_float(r[q * 8 + 5]));
+                v.w = pack2<T>(__uint_as_float(r[q * 8 + 6]), __uint_as_float(r[q * 8 + 7]));
                 *reinterpret_cast<uint4*>(dst + c * 32 + q * 8) = v;
             }
         }
@@ -299,11 +325,11 @@ __device__ __forceinline__ void st_shared16(uint32_t at, uint32_t a, uint32_t b,
 }
 // What rounding took from eight values, one byte each.
 template <typename T>
-__device__ __forceinline__ uint2 rest8(const uint32_t* r, float scale) {
+__device__ __forceinline__ uint2 rest8(const uint32_t* r) {
     uint32_t two[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const float a = __uint_as_float(r[2 * e]) * scale, b = __uint_as_float(r[2 * e + 1]) * scale;
+        const float a = __uint_as_float(r[2 * e]), b = __uint_as_float(r[2 * e + 1]);
         const float2 f = unpack2<T>(pack2<T>(a, b));
         two[e] = __nv_cvt_float2_to_fp8x2(make_float2((a - f.x) * kRestScale<T>, (b - f.y) * kRestScale<T>), __NV_SATFINITE, __NV_E5M2);
     }
@@ -321,7 +347,7 @@ __device__ __forceinline__ void store_output(uint32_t o_addr, uint32_t staging, 
     if (rows <= 0) return;
     if (rows < 32) {
         const int64_t row = (token + lane) * heads + head;
-        store_row<T, kD>(o_addr, out + row * dim, dim, scale, lane < rows);
+        store_row<T, kD, true>(o_addr, out + row * dim, dim, scale, lane < rows);
         if (rest == nullptr) return;
 #pragma unroll 1
         for (int c = 0; c < kD / 32; ++c) {
@@ -329,10 +355,11 @@ __device__ __forceinline__ void store_output(uint32_t o_addr, uint32_t staging, 
             tmem_ld32(o_addr + c * 32, r);
             tmem_ld_wait();
             tmem_tie32(r);
+            scale_output<T>(r, scale);
 #pragma unroll
             for (int q = 0; q < 4; ++q)
                 if (lane < rows && c * 32 + q * 8 < dim)
-                    *reinterpret_cast<uint2*>(rest + row * rest_row + c * 32 + q * 8) = rest8<T>(r + q * 8, scale);
+                    *reinterpret_cast<uint2*>(rest + row * rest_row + c * 32 + q * 8) = rest8<T>(r + q * 8);
         }
         return;
     }
@@ -346,12 +373,13 @@ __device__ __forceinline__ void store_output(uint32_t o_addr, uint32_t staging, 
         }
         tmem_ld_wait();
         tmem_tie32(r);
+        scale_output<T>(r, scale);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                w[e] = pack2<T>(__uint_as_float(r[q * 8 + 2 * e]) * scale, __uint_as_float(r[q * 8 + 2 * e + 1]) * scale);
+                w[e] = pack2<T>(__uint_as_float(r[q * 8 + 2 * e]), __uint_as_float(r[q * 8 + 2 * e + 1]));
             st_shared16(staging + swizzled(lane * 128 + ((c & 1) * 4 + q) * 16), w[0], w[1], w[2], w[3]);
         }
         if (c & 1) {
@@ -372,9 +400,10 @@ __device__ __forceinline__ void store_output(uint32_t o_addr, uint32_t staging, 
         tmem_ld32(o_addr + c * 32, r);
         tmem_ld_wait();
         tmem_tie32(r);
+        scale_output<T>(r, scale);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint2 a = rest8<T>(r + h * 16, scale), b = rest8<T>(r + h * 16 + 8, scale);
+            const uint2 a = rest8<T>(r + h * 16), b = rest8<T>(r + h * 16 + 8);
             st_shared16(staging + swizzled(lane * 128 + c * 32 + h * 16), a.x, a.y, b.x, b.y);
         }
     }

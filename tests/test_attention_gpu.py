@@ -571,3 +571,26 @@ def test_non_finite_values_leave_the_factor_alone(what):
     got = run(q, k, v, do, offsets(lengths))
     for name in got:
         assert torch.equal(got[name][:100], clean[name][:100]) and torch.equal(got[name][160:], clean[name][160:])
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_largest_values_fp16(dim):
+    """Means of fp16's largest number are that number, whatever rounding does to the weights; an infinity stays one. Beside
+    the first key of weight 1 (scores of 0) all others weigh exp(-scale), just above the middle of two steps of fp16."""
+    lengths = [700, 33]
+    q, k, v, do = make(lengths, 4, 2, dim, torch.float16)
+    q.zero_(), k.zero_()
+    q[..., 0], k[..., 0] = 1.0, -1.0
+    k[0, :, 0], k[700, :, 0] = 0.0, 0.0
+    v[..., ::3], v[..., 1::3] = 65504.0, -65504.0
+    scale = -math.log(0.5 * (1 + 0.51 * 2.0 ** -10))
+    cu = offsets(lengths)
+    want, bound = reference(q, k, v, do, lengths, scale=scale)["o"]
+    with torch.no_grad():
+        o = xma.attention_packed(q, k, v, cu, softmax_scale=scale)
+    assert_within("o", o, want, bound)
+    got = run(q, k, v, (do * 2.0 ** -10).to(torch.float16), cu, scale)
+    assert torch.equal(got["o"], o) and all(t.isfinite().all() for t in got.values())
+    v[3, :, 0] = math.inf
+    with torch.no_grad():
+        assert xma.attention_packed(q, k, v, cu, softmax_scale=scale)[3:700, :, 0].isposinf().all()
