@@ -29,7 +29,8 @@
 //
 // Rows beyond a sequence's end inside a tile belong to other sequences: their scores are masked by
 // selection, and where a masked (zero) probability would multiply such a row, the row is zeroed in shared
-// memory first, so that not even a NaN crosses over. Every wait is bounded, as in the grouped GEMM.
+// memory first, so that not even a NaN crosses over. Every wait is bounded, as in the grouped GEMM; after one that
+// ran out a CTA still waits for its copies and products in flight before it ends.
 #include <cuda_fp8.h>
 
 #include <type_traits>
@@ -273,14 +274,15 @@ constexpr float kRestScale = std::is_same<T, __half>::value ? 32768.f : 4096.f;
 // so a mean of values next to fp16's largest number could round to infinity; no mean is above the largest value.
 template <typename T>
 __device__ __forceinline__ void scale_output(uint32_t (&r)[32], float scale) {
-    float top = 0.f;
+    float top[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
         const float v = __uint_as_float(r[i]) * scale;
         r[i] = __float_as_uint(v);
-        if (std::is_same<T, __half>::value) top = fmaxf(top, fabsf(v));
+        if (std::is_same<T, __half>::value) top[i & 3] = fmaxf(top[i & 3], fabsf(v));
     }
-    if (std::is_same<T, __half>::value && __any_sync(0xffffffffu, top > 65504.f)) {
+    if (std::is_same<T, __half>::value &&
+        __any_sync(0xffffffffu, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > 65504.f)) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
             const float v = __uint_as_float(r[i]);
@@ -421,16 +423,28 @@ __device__ __forceinline__ int64_t work_item(int64_t turn) {
     return turn * gridDim.x + ((turn & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
 }
 
-struct Ring {
-    int stage = 0;
-    uint32_t phase = 0;
-    __device__ __forceinline__ void next(int stages) {
-        if (++stage == stages) {
-            stage = 0;
-            phase ^= 1u;
-        }
-    }
-};
+// After a wait that ran out, a CTA waits once more, for what it has in flight (bounded too): copies write shared memory
+// and products read it and write tensor memory, all of which another CTA gets next. A load role leaves where its ring
+// and its resident tiles stand (the parity of the last turn, 1 if there was none); MMA warps' products are asked for. At
+// the end of every CTA instead, without the branch, the loops above came out 2 % slower.
+__device__ __forceinline__ uint32_t pack_in_flight(const Ring& ring, uint32_t resident0, uint32_t resident1) {
+    return static_cast<uint32_t>(ring.stage) | ring.phase << 8 | resident0 << 9 | resident1 << 10;
+}
+__device__ __forceinline__ void settle_copies(uint32_t packed, uint32_t full, int stages, uint32_t resident0, uint32_t resident1) {
+    Ring ring;
+    ring.stage = static_cast<int>(packed & 0xffu);
+    ring.phase = packed >> 8 & 1u;
+    const uint64_t now = global_timer_ns();
+    ring.settle(full, stages, now);
+    mbar_settle(resident0, packed >> 9 & 1u, now);
+    mbar_settle(resident1, packed >> 10 & 1u, now);
+}
+__device__ __forceinline__ void settle_products(uint32_t bar) {
+    if (elect_one()) umma_commit_cta1(bar);
+    __syncwarp();
+    mbar_settle(bar, 0, global_timer_ns());
+    __syncwarp();
+}
 
 // ---------------------------------------------------------------------------------------------
 // Forward
@@ -468,6 +482,8 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     const uint32_t p_ready = bars + 192;  // [tile][half of the keys]
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + kBars + 224);
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + kBars + 228);
+    const uint32_t settled = bars + 232;
+    volatile uint32_t* in_flight = reinterpret_cast<volatile uint32_t*>(gen + kBars + 240);
 
     const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -483,6 +499,7 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             mbar_init(p_ready + 16 * t + 8, 4);
             mbar_init(o_full + 8 * t, 1);
         }
+        mbar_init(settled, 1);
         *abort_flag = 0;
         fence_barrier_init();
         prefetch_tmap(&map_q);
@@ -527,6 +544,7 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                     kv.next(F::kStages);
                 }
             }
+            *in_flight = pack_in_flight(kv, q_phase[0], q_phase[1]);
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -715,6 +733,11 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     if (warp >= 4 && lane == 0) bulk_wait_read<0>();  // the staging tiles stay until the last stores have read them
     tc_fence_before();
     __syncthreads();
+    if (*abort_flag != 0) {
+        if (threadIdx.x == 0) settle_copies(*in_flight, full, F::kStages, q_full, q_full + 8);
+        if (warp == 1) settle_products(settled);
+        __syncthreads();
+    }
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, kTmemCols);
@@ -944,6 +967,8 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
                    s_full = bars + 96, dp_full = bars + 104, p_ready = bars + 112, ds_ready = bars + 128, done = bars + 144, v_full = bars + 168, v_empty = bars + 176;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + B::kBars + 160);
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + B::kBars + 164);
+    const uint32_t settled = bars + 184;  // of each MMA warp
+    volatile uint32_t* in_flight = reinterpret_cast<volatile uint32_t*>(gen + B::kBars + 200);  // of each load warp
 
     const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -966,6 +991,7 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
             mbar_init(ds_ready + 8 * h, 8);
         }
         mbar_init(done, 2);
+        for (int i = 0; i < 2; ++i) mbar_init(settled + 8 * i, 1);
         *abort_flag = 0;
         fence_barrier_init();
         prefetch_tmap(&map_q);
@@ -1010,6 +1036,7 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
                     }
                 }
             }
+            in_flight[0] = pack_in_flight(q, k_phase, k_phase);
         }
         __syncwarp();
     } else if (warp == 3) {
@@ -1043,6 +1070,7 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
                     }
                 }
             }
+            in_flight[1] = pack_in_flight(d, v_phase, v_phase);
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -1264,6 +1292,12 @@ dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
     }
     tc_fence_before();
     __syncthreads();
+    if (*abort_flag != 0) {
+        if (threadIdx.x == 0) settle_copies(in_flight[0], q_full, B::kLong, k_full, k_full);
+        if (threadIdx.x == 96) settle_copies(in_flight[1], do_full, B::kShort, v_full, v_full);
+        if (warp == 1 || warp == 2) settle_products(settled + 8 * (warp - 1));
+        __syncthreads();
+    }
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, kTmemCols);
@@ -1290,6 +1324,8 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
                    s_full = bars + 96, s_free = bars + 112, dp_full = bars + 128, ds_ready = bars + 136, done = bars + 152, do_full = bars + 168, do_empty = bars + 176;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + B::kBars + 160);
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + B::kBars + 164);
+    const uint32_t settled = bars + 184;  // of each MMA warp
+    volatile uint32_t* in_flight = reinterpret_cast<volatile uint32_t*>(gen + B::kBars + 200);  // of each load warp
 
     const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -1310,6 +1346,7 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
         mbar_init(do_empty, 1);
         mbar_init(dp_full, 1);
         mbar_init(done, 1);
+        for (int i = 0; i < 2; ++i) mbar_init(settled + 8 * i, 1);
         *abort_flag = 0;
         fence_barrier_init();
         prefetch_tmap(&map_q);
@@ -1350,6 +1387,7 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
                     k.next(B::kLong);
                 }
             }
+            in_flight[0] = pack_in_flight(k, q_phase, q_phase);
         }
         __syncwarp();
     } else if (warp == 3) {
@@ -1374,6 +1412,7 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
                     v.next(B::kShort);
                 }
             }
+            in_flight[1] = pack_in_flight(v, do_phase, do_phase);
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -1532,10 +1571,42 @@ dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
     }
     tc_fence_before();
     __syncthreads();
+    if (*abort_flag != 0) {
+        if (threadIdx.x == 0) settle_copies(in_flight[0], k_full, B::kLong, q_full, q_full);
+        if (threadIdx.x == 96) settle_copies(in_flight[1], v_full, B::kShort, do_full, do_full);
+        if (warp == 1 || warp == 2) settle_products(settled + 8 * (warp - 1));
+        __syncthreads();
+    }
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, kTmemCols);
     }
+}
+
+// A load role that gives up: copies go through a ring and nobody reads them; what is in flight is settled by the ring's own
+// arithmetic. result[0] says that it landed, result[1] that a copy which never started did not (after limit_ns).
+constexpr int kSelfTestStages = 3, kSelfTestBytes = 8192;
+__global__ void __launch_bounds__(256) settle_selftest_kernel(const uint8_t* src, int fills, uint8_t* dst, int32_t* result, uint64_t limit_ns) {
+    __shared__ __align__(128) uint8_t tiles[kSelfTestStages * kSelfTestBytes];
+    __shared__ __align__(8) uint64_t bars[kSelfTestStages + 1];
+    const uint32_t full = smem_u32(bars);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i <= kSelfTestStages; ++i) mbar_init(full + 8 * i, 1);
+        fence_barrier_init();
+        Ring ring;
+        for (int i = 0; i < fills; ++i) {
+            const uint32_t bar = full + 8 * ring.stage;
+            if (!mbar_settle(bar, ring.phase ^ 1u, global_timer_ns(), limit_ns)) break;  // the stage's last copy, in the place of a reader
+            mbar_expect_tx(bar, kSelfTestBytes);
+            bulk_load(smem_u32(tiles) + ring.stage * kSelfTestBytes, src + static_cast<int64_t>(i) * kSelfTestBytes, kSelfTestBytes, bar);
+            ring.next(kSelfTestStages);
+        }
+        result[0] = ring.settle(full, kSelfTestStages, global_timer_ns(), limit_ns);
+        result[1] = mbar_settle(full + 8 * kSelfTestStages, 0, global_timer_ns(), limit_ns);
+    }
+    __syncthreads();
+    const int bytes = min(fills, kSelfTestStages) * kSelfTestBytes;
+    for (int i = threadIdx.x; i < bytes; i += blockDim.x) dst[i] = tiles[i];
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -1697,6 +1768,14 @@ int64_t xma_attention_workspace_bytes(int64_t total, int64_t batch) {
 
 int64_t xma_attention_stat_rows(int64_t total, int64_t batch) {
     return total < 0 || batch < 0 ? 0 : (total / xma::attn::kTile + batch + 1) * xma::attn::kTile;
+}
+
+int xma_selftest_settle(const void* src, int32_t fills, void* dst, int32_t* result, int64_t limit_ns, void* stream) {
+    if (!src || !xma::aligned16(src) || !dst || !result || fills < 0 || fills > 64) return XMA_ERR_BAD_ARG;
+    if (limit_ns <= 0 || limit_ns > 1000000000ll) return XMA_ERR_BAD_ARG;
+    xma::attn::settle_selftest_kernel<<<1, 256, 0, static_cast<cudaStream_t>(stream)>>>(
+        static_cast<const uint8_t*>(src), fills, static_cast<uint8_t*>(dst), result, static_cast<uint64_t>(limit_ns));
+    return xma::launch_status();
 }
 
 int xma_attention_forward(const void* q, const void* k, const void* v, int64_t q_token, int64_t q_head, int64_t k_token,

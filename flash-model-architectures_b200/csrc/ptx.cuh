@@ -69,6 +69,32 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     return true;
 }
 
+// Waits for what a thread has in flight before its CTA ends, whatever the other roles gave up on: copies that still write
+// shared memory, products that still read it. Bounded as well, and from `start` on for all that a thread waits for.
+__device__ __forceinline__ bool mbar_settle(uint32_t bar, uint32_t parity, uint64_t start, uint64_t limit_ns = kWaitLimitNs) {
+    while (!mbar_try_wait(bar, parity))
+        if (global_timer_ns() - start > limit_ns) return false;
+    return true;
+}
+
+// Stages of a ring of barriers, 8 bytes each: `stage` is the next one to fill (or to read), `phase` the parity of that turn.
+struct Ring {
+    int stage = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void next(int stages) {
+        if (++stage == stages) {
+            stage = 0;
+            phase ^= 1u;
+        }
+    }
+    // For the thread that fills the ring: every stage filled so far has landed (a stage that never was counts as such).
+    __device__ __forceinline__ bool settle(uint32_t full, int stages, uint64_t start, uint64_t limit_ns = kWaitLimitNs) const {
+        bool ok = true;
+        for (int i = 0; i < stages; ++i) ok = mbar_settle(full + 8 * i, i < stage ? phase : phase ^ 1u, start, limit_ns) && ok;
+        return ok;
+    }
+};
+
 __device__ __forceinline__ void fence_barrier_init() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }

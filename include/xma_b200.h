@@ -257,6 +257,15 @@ int xma_sum_partials(const float* partials, int32_t splits, int64_t count, int32
 int xma_selftest_bounded_wait(int32_t* status, int64_t limit_ns, void* stream);
 
 /*
+ * Self-test of what a load role of the attention kernels does before its CTA ends, also after it gave up: `fills`
+ * (0 to 64) copies of 8192 bytes from src go through a ring of three stages and are settled without a reader.
+ * result[0] = 1: all of them landed; result[1] = 0: the same wait on a copy that was never started ran out (limit_ns, at
+ * most 1 s). dst takes the stages, min(fills, 3) x 8192 bytes; stage i holds the last copy j with j % 3 = i. src is
+ * 16-byte aligned, fills x 8192 bytes. No reference counterpart.
+ */
+int xma_selftest_settle(const void* src, int32_t fills, void* dst, int32_t* result, int64_t limit_ns, void* stream);
+
+/*
  * Per-expert weight gradient: dw[e, m, n] = sum_{r in expert e} x[r, m] * y[r, n], zeros for an expert
  * without rows. Replaces group_bwd_W and the zeros_like fill
  * (xma/layers/moe/triton_implementation/group_backward_kernel.py:13-125,

@@ -594,3 +594,22 @@ def test_largest_values_fp16(dim):
     v[3, :, 0] = math.inf
     with torch.no_grad():
         assert xma.attention_packed(q, k, v, cu, softmax_scale=scale)[3:700, :, 0].isposinf().all()
+
+
+@pytest.mark.parametrize("fills", [0, 1, 2, 3, 4, 5, 6, 7, 64])
+def test_copies_in_flight_are_waited_for(fills):
+    """What a load warp does before its CTA ends, also when another role gave up: the copies that nobody reads any more have
+    landed, at every turn of their ring; a copy that never started does not hold it beyond the limit (1 ms)."""
+    from xma import _native as N
+
+    size = 8192
+    src = torch.randint(0, 256, (max(fills, 1) * size,), dtype=torch.uint8, device="cuda")
+    dst = torch.zeros(3, size, dtype=torch.uint8, device="cuda")
+    result = torch.full((2,), -1, dtype=torch.int32, device="cuda")
+    N.check(N.lib().xma_selftest_settle(src.data_ptr(), fills, dst.data_ptr(), result.data_ptr(), 1_000_000,
+                                        torch.cuda.current_stream().cuda_stream), "xma_selftest_settle")
+    assert result.tolist() == [1, 0]
+    for stage in range(3):
+        turns = [j for j in range(fills) if j % 3 == stage]
+        want = src[turns[-1] * size: (turns[-1] + 1) * size] if turns else torch.zeros_like(dst[0])
+        assert torch.equal(dst[stage], want)

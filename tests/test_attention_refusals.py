@@ -64,3 +64,12 @@ def test_c_entry_refuses():
     for total, batch in ((0, 0), (1, 1), (127, 3), (128, 1), (100000, 77)):
         assert lib.xma_attention_workspace_bytes(total, batch) == N.attention_workspace_bytes(total, batch)
         assert lib.xma_attention_stat_rows(total, batch) == N.attention_stat_rows(total, batch)
+
+
+def test_settle_selftest_refuses():
+    from xma import _native as N
+
+    f, a = N.lib().xma_selftest_settle, 1 << 20
+    assert f(None, 1, a, a, 1000, None) == 1 and f(a + 8, 1, a, a, 1000, None) == 1 and f(a, 1, None, a, 1000, None) == 1
+    assert f(a, 65, a, a, 1000, None) == 1 and f(a, -1, a, a, 1000, None) == 1 and f(a, 1, a, a, 0, None) == 1
+    assert f(a, 1, a, a, 2_000_000_000, None) == 1 and f(a, 1, a, None, 1000, None) == 1
