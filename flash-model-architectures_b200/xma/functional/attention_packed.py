@@ -11,6 +11,7 @@ from torch.autograd.function import once_differentiable
 from .. import _native as N
 from ..accelerator import KernelBackend, require_cuda_backend
 from ..ops import attention_packed_backward_cuda, attention_packed_forward_cuda
+from ._forward_mode import refuse_tangents
 
 MAX_HEAD_DIM = 128
 _MAX_TOKENS = 1 << 30
@@ -50,6 +51,7 @@ class _AttentionPacked(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, d_out):
+        refuse_tangents("attention_packed", d_out)
         q, k, v, cu_seqlens, out, out_rest, lse = ctx.saved_tensors
         opts = dict(dtype=q.dtype, device=q.device)
         dq, dk, dv = torch.empty(q.shape, **opts), torch.empty(k.shape, **opts), torch.empty(v.shape, **opts)
@@ -88,7 +90,7 @@ def attention_packed(
     Tokens that no sequence owns get zeros, in the output and in the gradients, and what they hold reaches nothing. A
     NaN or an infinity in a value also reaches rows before it in its own sequence, as in a product with probabilities
     that are zero there, and one in a key their gradients. Offsets are read on the device: values that are out of order
-    or outside the stream give meaningless outputs, not an error."""
+    or outside the stream give meaningless outputs, not an error. Forward-mode differentiation is refused."""
     require_cuda_backend(kernel_backend)
     dtype, device = q.dtype, q.device
     if dtype not in (torch.bfloat16, torch.float16):
@@ -119,6 +121,7 @@ def attention_packed(
     scale = 1.0 / math.sqrt(dim) if softmax_scale is None else float(softmax_scale)
     if not 0.0 < scale < 1e30:
         raise ValueError(f"softmax_scale should be positive and finite, got {scale}")
+    refuse_tangents("attention_packed", q, k, v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _AttentionPacked.apply(q, k, v, cu_seqlens, scale)
     return _forward(q, k, v, cu_seqlens, scale, False)[0]

@@ -10,6 +10,7 @@ from torch.autograd.function import once_differentiable
 from .. import _native as N
 from ..accelerator import KernelBackend, require_cuda_backend
 from ..ops import norm_backward_cuda, norm_forward_cuda
+from ._forward_mode import refuse_tangents
 
 GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_FULL = 0, 1, 2, 3
 _MAX_HIDDEN = 1 << 24
@@ -51,6 +52,7 @@ class _Norm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, d_stream=None):
+        refuse_tangents("rmsnorm" if ctx.alone else "fused_residual_add_rmsnorm", dy, d_stream)
         base, x, weight, post_weight, gate, rstd = ctx.saved_tensors
         dy = None if dy is None else dy.contiguous()
         d_stream = None if d_stream is None else d_stream.contiguous()
@@ -84,6 +86,7 @@ class _Norm(torch.autograd.Function):
 
 
 def _norm(x, residual, weight, post_weight, gate, gate_mode: int, eps: float, multiplier: float):
+    refuse_tangents("rmsnorm" if residual is None else "fused_residual_add_rmsnorm", x, residual, weight, post_weight, gate)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight, post_weight, gate)):
         return _Norm.apply(x, residual, weight, post_weight, gate, gate_mode, eps, multiplier)
     y, stream, _, _ = _forward(x, residual, weight, post_weight, gate, gate_mode, eps, multiplier, False)
@@ -121,7 +124,7 @@ def rmsnorm(
     """`weight * x / sqrt(mean(x^2, -1) + eps)`, computed in float32 and rounded once to the dtype of `x`.
 
     `weight` is `[H]` in the dtype of `x` or in float32, or None (ones). `eps=None` takes the machine epsilon of
-    the dtype of `x`."""
+    the dtype of `x`. Forward-mode differentiation is refused."""
     require_cuda_backend(kernel_backend)
     _check_rows(x)
     _check_parameter("weight", weight, x)
@@ -150,7 +153,8 @@ def fused_residual_add_rmsnorm(
     `residual` (and with it `stream`) has the shape of `x` and its dtype or float32. `gate` is `[H]` (a
     parameter), one factor per token (the shape of `x` with a last dimension of 1) or has the shape of `x`; a
     gate that is not `[H]` has the dtype of `x`, the parameters that or float32. `weight=None` norms without a
-    weight, `multiplier=None` is 1, `eps=None` the machine epsilon of the dtype of `x`."""
+    weight, `multiplier=None` is 1, `eps=None` the machine epsilon of the dtype of `x`. Forward-mode differentiation is
+    refused."""
     require_cuda_backend(kernel_backend)
     _check_rows(x)
     if residual.shape != x.shape:

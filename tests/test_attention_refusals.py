@@ -73,3 +73,17 @@ def test_settle_selftest_refuses():
     assert f(None, 1, a, a, 1000, None) == 1 and f(a + 8, 1, a, a, 1000, None) == 1 and f(a, 1, None, a, 1000, None) == 1
     assert f(a, 65, a, a, 1000, None) == 1 and f(a, -1, a, a, 1000, None) == 1 and f(a, 1, a, a, 0, None) == 1
     assert f(a, 1, a, a, 2_000_000_000, None) == 1 and f(a, 1, a, None, 1000, None) == 1
+
+
+@pytest.mark.parametrize("which", range(3))
+def test_forward_mode_is_refused(which):
+    """A dual tensor has no requires_grad; its tangent is not dropped in silence."""
+    from torch.autograd import forward_ad
+
+    inputs = [t(4, 2, 64), t(4, 2, 64), t(4, 2, 64)]
+    with forward_ad.dual_level():
+        inputs[which] = forward_ad.make_dual(inputs[which], torch.ones_like(inputs[which]))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            xma.attention_packed(*inputs, CU)
+        with pytest.raises(RuntimeError, match="no CPU path"):  # a level that is open is no reason
+            xma.attention_packed(t(4, 2, 64), t(4, 2, 64), t(4, 2, 64), CU)

@@ -170,3 +170,27 @@ def test_compiled_for_any_length():
             x, w = torch.randn(total, 8 * len(lengths), device="cuda"), torch.randn(8 * len(lengths), device="cuda")
             for a, b in zip(norm(x, x, w), xma.fused_residual_add_rmsnorm(x, x, w, EPS, M, gate=w)):
                 assert torch.equal(a, b)
+
+
+def test_forward_mode_is_refused():
+    """A directional derivative through the operators, or through their backward passes, is refused, not wrong."""
+    from torch.autograd import forward_ad
+
+    x = torch.randn(9, 64, device="cuda")
+    q = torch.randn(9, 2, 64, device="cuda", dtype=torch.bfloat16)
+    cu = torch.tensor([0, 9], dtype=torch.int32, device="cuda")
+    calls = [(x, lambda t: xma.rmsnorm(t, None, EPS)), (x, lambda t: xma.fused_residual_add_rmsnorm(t, x, None, EPS)[0]),
+             (q, lambda t: xma.attention_packed(t, q, q, cu))]
+    with forward_ad.dual_level():
+        for t, call in calls:
+            for leaf in (t, t.clone().requires_grad_()):
+                with pytest.raises(NotImplementedError):
+                    call(forward_ad.make_dual(leaf, torch.ones_like(leaf)))
+            leaf = t.clone().requires_grad_()
+            out = call(leaf)
+            upstream = forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
+            with pytest.raises(NotImplementedError):
+                torch.autograd.grad(out, leaf, upstream)
+    want = calls[0][1](x)
+    with forward_ad.dual_level():
+        assert torch.equal(calls[0][1](x), want)

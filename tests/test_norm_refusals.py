@@ -53,3 +53,20 @@ def test_c_entry_refuses():
     assert forward(post=1 << 20) == 1 and forward(sdt=2) == 1  # a post norm or another stream type without a residual
     assert forward(res=1 << 20, out=1 << 20, dt=0, sdt=1) == 2 and forward(dt=3, sdt=3) == 2
     assert lib.xma_norm_workspace_floats(3, 5) == N.norm_workspace_floats(3, 5)
+
+
+@pytest.mark.parametrize("which", ["x", "residual", "weight", "post_weight", "gate"])
+def test_forward_mode_is_refused(which):
+    """A dual tensor has no requires_grad; its tangent is not dropped in silence."""
+    from torch.autograd import forward_ad
+
+    t = {"x": x(2, 8), "residual": x(2, 8), "weight": x(8), "post_weight": x(8), "gate": x(2, 1)}
+    with forward_ad.dual_level():
+        t[which] = forward_ad.make_dual(t[which], torch.ones_like(t[which]))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            xma.fused_residual_add_rmsnorm(t["x"], t["residual"], t["weight"], post_weight=t["post_weight"], gate=t["gate"])
+        if which in ("x", "weight"):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                xma.rmsnorm(t["x"], t["weight"])
+        with pytest.raises(RuntimeError, match="no CPU path"):  # a level that is open is no reason
+            xma.rmsnorm(x(2, 8), x(8))
