@@ -18,7 +18,10 @@
 // The backward pass recomputes s from the residual and x where it reads x anyway, so that the rounding of the
 // stream does not reach the gradients; for a plain residual add it reads the rounded stream, one tensor less.
 //
-// The mean of squares adds up (v / H) v, so that it overflows where the mean itself does and no sooner.
+// The mean of squares adds up (v / H) v, so that it overflows where the mean itself does and no sooner. Below 2^-78 what
+// terms lose under float32's smallest normal number begins to show; where eps does not cover that (eps is below 2^-78
+// too), such a row's mean is added up again from its values times 2^100, by kernels of their own (kSmallEps: the test alone
+// cost the others 1-2 %).
 // All of it is bound by HBM: every tensor is read and written once.
 #include "common.cuh"
 #include "ptx.cuh"
@@ -47,6 +50,7 @@ constexpr int kMaxStages = 6;
 // residual 58 against 89; 5001 x 1001 float32 (L2, four chunks a CTA) 13 against 11.
 constexpr int kRingMinHidden = 2049, kRingMinHiddenAny = 512, kRingMinChunks = 3, kRingMinChunksAny = 8;
 constexpr int kPartials = XMA_NORM_PARTIALS;
+constexpr float kSmallMean = 0x1p-78f, kSmallScale = 0x1p100f;
 
 struct Params {
     const void* x;
@@ -209,6 +213,12 @@ __device__ __forceinline__ void group_sum(float (&v)[kCount], float* scratch, in
         for (int i = 0; i < kCount; ++i) v[i] += scratch[w * kCount + i];
 }
 
+// 1 / sqrt(mean + eps) of a row whose mean was added up again from its values times kSmallScale.
+__device__ __forceinline__ float small_rsqrt(float scaled_mean, float eps) {
+    return rsqrtf(scaled_mean + eps * kSmallScale * kSmallScale) * kSmallScale;
+}
+__device__ __forceinline__ bool is_small(float mean, float eps) { return eps < kSmallMean && mean < kSmallMean; }
+
 template <typename T>
 __device__ __forceinline__ float token_gate(const Params& p, int64_t row) {
     return p.gate_mode == kGateToken ? Elem<T>::to_float(static_cast<const T*>(p.gate)[row]) : 1.f;
@@ -221,20 +231,40 @@ __device__ __forceinline__ float token_gate(const Params& p, int64_t row) {
 // `group` threads per row hold it in registers (kVpt vectors of eight each); several short rows share a CTA. For few
 // rows (4 x 4096: 3.6 us) and rows of up to 2048 elements (8191 x 2048 bf16 with a float32 stream, post norm and
 // channel gate: 37 us, 5.4 TB/s); one vector a thread or four are slower (48 and 46 us).
-template <typename T, typename R, int kVpt, bool kVec>
+template <typename T, typename R, int kVpt, bool kVec, bool kSmallEps>
 __global__ void __launch_bounds__(1024)
 forward_kernel(const Params p, int group) {
-    __shared__ float scratch[2][32];
+    __shared__ float scratch[kSmallEps ? 4 : 2][32];
     const int slot = threadIdx.x / group, t = threadIdx.x - slot * group;
     const int slots = blockDim.x / group;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * slots + slot;
     if (row >= p.rows) return;  // the whole group leaves: its barrier is its own
     const int64_t base = row * p.hidden;
-    float* my_scratch[2] = {&scratch[0][slot * (group >> 5)], &scratch[1][slot * (group >> 5)]};
-    const int barrier = 1 + slot;
+    const int barrier = 1 + slot, my_warps = slot * (group >> 5);
     const float inv_h = 1.f / static_cast<float>(p.hidden);
 
     float s[kVpt][8];
+    // 1 / sqrt(mean(s^2) + eps); `which`: 0 the post norm's, 1 the stream's
+    const auto reciprocal_root = [&](int which) {
+        float sum[1] = {0.f};
+#pragma unroll
+        for (int v = 0; v < kVpt; ++v)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum[0] = fmaf(s[v][j] * inv_h, s[v][j], sum[0]);
+        group_sum<1>(sum, &scratch[which][my_warps], t, group, barrier);
+        if constexpr (kSmallEps) {
+            if (is_small(sum[0], p.eps)) {
+                sum[0] = 0.f;
+#pragma unroll
+                for (int v = 0; v < kVpt; ++v)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) sum[0] = fmaf(s[v][j] * kSmallScale * inv_h, s[v][j] * kSmallScale, sum[0]);
+                group_sum<1>(sum, &scratch[2 + which][my_warps], t, group, barrier);
+                return small_rsqrt(sum[0], p.eps);
+            }
+        }
+        return rsqrtf(sum[0] + p.eps);
+    };
 #pragma unroll
     for (int v = 0; v < kVpt; ++v) load_cols<kVec>(static_cast<const T*>(p.x) + base, v, t, group, p.hidden, s[v]);
     if (p.residual != nullptr) {
@@ -244,13 +274,7 @@ forward_kernel(const Params p, int group) {
             load_cols<kVec>(static_cast<const R*>(p.residual) + base, v, t, group, p.hidden, r[v]);
         float scale = p.multiplier * token_gate<T>(p, row);
         if (p.post != nullptr) {
-            float sum[1] = {0.f};
-#pragma unroll
-            for (int v = 0; v < kVpt; ++v)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) sum[0] = fmaf(s[v][j] * inv_h, s[v][j], sum[0]);
-            group_sum<1>(sum, my_scratch[0], t, group, barrier);
-            const float rp = rsqrtf(sum[0] + p.eps);
+            const float rp = reciprocal_root(0);
             if (t == 0 && p.rp != nullptr) p.rp[row] = rp;
             scale *= rp;
 #pragma unroll
@@ -280,13 +304,7 @@ forward_kernel(const Params p, int group) {
             store_cols<kVec>(static_cast<R*>(p.s_out) + base, v, t, group, p.hidden, s[v]);
         }
     }
-    float sum[1] = {0.f};
-#pragma unroll
-    for (int v = 0; v < kVpt; ++v)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sum[0] = fmaf(s[v][j] * inv_h, s[v][j], sum[0]);
-    group_sum<1>(sum, my_scratch[1], t, group, barrier);
-    const float rs = rsqrtf(sum[0] + p.eps);
+    const float rs = reciprocal_root(1);
     if (t == 0 && p.rs != nullptr) p.rs[row] = rs;
 #pragma unroll
     for (int v = 0; v < kVpt; ++v) {
@@ -320,30 +338,34 @@ __device__ __forceinline__ float stream_at(const Params& p, int64_t base, int c,
 template <typename T, typename R>
 __global__ void __launch_bounds__(1024)
 forward_long_kernel(const Params p) {
-    __shared__ float scratch[2][32];
+    __shared__ float scratch[4][32];
     const int64_t row = blockIdx.x;
     const int64_t base = row * p.hidden;
     const int t = threadIdx.x, group = blockDim.x;
     const float inv_h = 1.f / static_cast<float>(p.hidden);
-    float scale = p.multiplier * token_gate<T>(p, row);
-    if (p.residual != nullptr && p.post != nullptr) {
+    const auto reciprocal_root = [&](int which, const auto& at) {
         float sum[1] = {0.f};
         for (int c = t; c < p.hidden; c += group) {
-            const float v = Elem<T>::to_float(static_cast<const T*>(p.x)[base + c]);
+            const float v = at(c);
             sum[0] = fmaf(v * inv_h, v, sum[0]);
         }
-        group_sum<1>(sum, scratch[0], t, group, 1);
-        const float rp = rsqrtf(sum[0] + p.eps);
+        group_sum<1>(sum, scratch[which], t, group, 1);
+        if (!is_small(sum[0], p.eps)) return rsqrtf(sum[0] + p.eps);
+        sum[0] = 0.f;
+        for (int c = t; c < p.hidden; c += group) {
+            const float v = at(c) * kSmallScale;
+            sum[0] = fmaf(v * inv_h, v, sum[0]);
+        }
+        group_sum<1>(sum, scratch[2 + which], t, group, 1);
+        return small_rsqrt(sum[0], p.eps);
+    };
+    float scale = p.multiplier * token_gate<T>(p, row);
+    if (p.residual != nullptr && p.post != nullptr) {
+        const float rp = reciprocal_root(0, [&](int c) { return Elem<T>::to_float(static_cast<const T*>(p.x)[base + c]); });
         if (t == 0 && p.rp != nullptr) p.rp[row] = rp;
         scale *= rp;
     }
-    float sum[1] = {0.f};
-    for (int c = t; c < p.hidden; c += group) {
-        const float s = stream_at<T, R>(p, base, c, scale);
-        sum[0] = fmaf(s * inv_h, s, sum[0]);
-    }
-    group_sum<1>(sum, scratch[1], t, group, 1);
-    const float rs = rsqrtf(sum[0] + p.eps);
+    const float rs = reciprocal_root(1, [&](int c) { return stream_at<T, R>(p, base, c, scale); });
     if (t == 0 && p.rs != nullptr) p.rs[row] = rs;
     for (int c = t; c < p.hidden; c += group) {
         const float s = stream_at<T, R>(p, base, c, scale);
@@ -511,7 +533,7 @@ __device__ __forceinline__ void copy_param(uint8_t* dst, const void* p, bool f32
 // kDense: every thread's vectors lie inside the row. kVec: rows of whole 16-byte vectors; others take two rows of one vector
 // a thread, since the assembler of CUDA 12.9 fails on four rows of 16 bits, which were 10 us faster at 8000 x 3001, and on
 // two vectors.
-template <typename T, typename R, int kVpt, int kRows, bool kDense, bool kVec>
+template <typename T, typename R, int kVpt, int kRows, bool kDense, bool kVec, bool kSmallEps>
 __global__ void __launch_bounds__(kRingThreads, 1)
 forward_ring_kernel(const Params p, const RingLayout lay) {
     extern __shared__ __align__(128) uint8_t smem[];
@@ -589,6 +611,31 @@ forward_ring_kernel(const Params p, const RingLayout lay) {
         const auto inside = [&](int v) { return kDense || !kVec || (v * group + t) * 8 < p.hidden; };
         f32x2 s[kRows][kVpt][4];
         float sums[kRows], scale[kRows];
+        // kSmallEps: the rows' means become 1 / sqrt(mean + eps); the whole CTA takes the second sum if a row needs it
+        const auto small_roots = [&] {
+            bool small[kRows], any = false;
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) any = (small[r] = is_small(sums[r], p.eps)) || any;
+            float again[kRows];
+            if (__syncthreads_or(any)) {
+#pragma unroll
+                for (int r = 0; r < kRows; ++r) {
+                    f32x2 sum = both(0.f);
+#pragma unroll
+                    for (int v = 0; v < kVpt; ++v)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const f32x2 up = mul_f32x2(s[r][v][j], both(kSmallScale));
+                            sum = fma_f32x2(mul_f32x2(up, both(inv_h)), up, sum);
+                        }
+                    again[r] = total(sum);
+                }
+                ring_sum<kRows>(again, st, first_warp, warps);
+            }
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) sums[r] = small[r] ? small_rsqrt(again[r], p.eps) : rsqrtf(sums[r] + p.eps);
+        };
+        const auto reciprocal_root = [&](int r) { return kSmallEps ? sums[r] : rsqrtf(sums[r] + p.eps); };
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
             f32x2 sum = both(0.f);
@@ -607,9 +654,10 @@ forward_ring_kernel(const Params p, const RingLayout lay) {
         if (p.residual != nullptr) {
             if (p.post != nullptr) {
                 ring_sum<kRows>(sums, st, first_warp, warps);
+                if constexpr (kSmallEps) small_roots();
 #pragma unroll
                 for (int r = 0; r < kRows; ++r) {
-                    const float rp = rsqrtf(sums[r] + p.eps);
+                    const float rp = reciprocal_root(r);
                     scale[r] *= rp;
                     if (t == 0 && p.rp != nullptr && row0 + r < p.rows) p.rp[row0 + r] = rp;
                 }
@@ -657,10 +705,11 @@ forward_ring_kernel(const Params p, const RingLayout lay) {
         // every thread has read the stage: it can take the chunk after the ones in flight
         if (threadIdx.x == 0) load(chunk + static_cast<int64_t>(lay.stages) * gridDim.x, st.stage);
         st.next(lay.stages);
+        if constexpr (kSmallEps) small_roots();
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
             if (row0 + r >= p.rows) continue;
-            const float rs = rsqrtf(sums[r] + p.eps);
+            const float rs = reciprocal_root(r);
             if (t == 0 && p.rs != nullptr) p.rs[row0 + r] = rs;
             const int64_t base = (row0 + r) * p.hidden;
 #pragma unroll
@@ -1179,15 +1228,15 @@ struct Layout {
     bool vec, wide;
 };
 
-template <typename T, typename R, int kVpt, int kRows>
+template <typename T, typename R, int kVpt, int kRows, bool kSmallEps>
 static int run_forward_ring(const Params& p, const RingLayout& lay, cudaStream_t stream) {
     int count = 0;
-    if (dense(p, lay, kVpt)) return launch_ring<forward_ring_kernel<T, R, kVpt, kRows, true, true>>(p, lay, kRows, &count, stream);
-    return launch_ring<forward_ring_kernel<T, R, kVpt, kRows, false, true>>(p, lay, kRows, &count, stream);
+    if (dense(p, lay, kVpt)) return launch_ring<forward_ring_kernel<T, R, kVpt, kRows, true, true, kSmallEps>>(p, lay, kRows, &count, stream);
+    return launch_ring<forward_ring_kernel<T, R, kVpt, kRows, false, true, kSmallEps>>(p, lay, kRows, &count, stream);
 }
 
-template <typename T, typename R>
-static int run_forward(const Params& p, Layout rows_are, cudaStream_t stream) {
+template <typename T, typename R, bool kSmallEps>
+static int run_forward_of(const Params& p, Layout rows_are, cudaStream_t stream) {
     const bool vec = rows_are.vec;
     if (rows_are.wide && p.hidden >= (vec ? kRingMinHidden : kRingMinHiddenAny) && p.hidden <= (vec ? kRingMaxHidden : kRingMaxHiddenAny)) {
         const int ring_vpt = p.hidden > 4096 ? 2 : 1, rows = vec && ring_vpt == 1 ? 4 : 2;
@@ -1195,8 +1244,8 @@ static int run_forward(const Params& p, Layout rows_are, cudaStream_t stream) {
         int count = 0;
         if (ring_layout<T, R>(p, vec, false, ring_vpt, rows, 2, &lay) &&
             p.rows >= static_cast<int64_t>(vec ? kRingMinChunks : kRingMinChunksAny) * sm_count() * lay.slots * rows) {
-            if (!vec) return launch_ring<forward_ring_kernel<T, R, 1, 2, false, false>>(p, lay, rows, &count, stream);
-            return ring_vpt == 1 ? run_forward_ring<T, R, 1, 4>(p, lay, stream) : run_forward_ring<T, R, 2, 2>(p, lay, stream);
+            if (!vec) return launch_ring<forward_ring_kernel<T, R, 1, 2, false, false, kSmallEps>>(p, lay, rows, &count, stream);
+            return ring_vpt == 1 ? run_forward_ring<T, R, 1, 4, kSmallEps>(p, lay, stream) : run_forward_ring<T, R, 2, 2, kSmallEps>(p, lay, stream);
         }
     }
     if (p.hidden > kForwardMaxHidden) {
@@ -1209,13 +1258,18 @@ static int run_forward(const Params& p, Layout rows_are, cudaStream_t stream) {
     const unsigned grid = static_cast<unsigned>(ceil_div(p.rows, slots));
     const unsigned threads = static_cast<unsigned>(group * slots);
     if (vpt == 1) {
-        if (vec) forward_kernel<T, R, 1, true><<<grid, threads, 0, stream>>>(p, group);
-        else forward_kernel<T, R, 1, false><<<grid, threads, 0, stream>>>(p, group);
+        if (vec) forward_kernel<T, R, 1, true, kSmallEps><<<grid, threads, 0, stream>>>(p, group);
+        else forward_kernel<T, R, 1, false, kSmallEps><<<grid, threads, 0, stream>>>(p, group);
     } else {
-        if (vec) forward_kernel<T, R, 2, true><<<grid, threads, 0, stream>>>(p, group);
-        else forward_kernel<T, R, 2, false><<<grid, threads, 0, stream>>>(p, group);
+        if (vec) forward_kernel<T, R, 2, true, kSmallEps><<<grid, threads, 0, stream>>>(p, group);
+        else forward_kernel<T, R, 2, false, kSmallEps><<<grid, threads, 0, stream>>>(p, group);
     }
     return launch_status();
+}
+
+template <typename T, typename R>
+static int run_forward(const Params& p, Layout rows_are, cudaStream_t stream) {
+    return p.eps < kSmallMean ? run_forward_of<T, R, true>(p, rows_are, stream) : run_forward_of<T, R, false>(p, rows_are, stream);
 }
 
 template <typename T, typename R, int kVpt, int kRows, bool kX, bool kFull, int kCall, bool kVec = true>

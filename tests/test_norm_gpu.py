@@ -303,3 +303,52 @@ def test_many_rows_of_no_whole_vectors(rows, hidden, types):
     assert hidden % 8 and rows * hidden % 8
     check(make(rows, hidden, dtype, stream_dtype, GATES[types % 4], types % 2 == 0), 0.3)
     check(make(rows, hidden, dtype, None, None, False), 1.0)
+
+
+SMALL = [1.0, 1e-9, 1e-12, 1e-17, 1e-20, 1e-23, 1e-27]
+SMALL_SHAPES = [(8, 64), (9, 4096), (7, 1001), (2000, 4096), (4800, 1001), (1400, 6144), (7, 16384), (7, 20001)]
+
+
+def small_rows(rows, hidden, dtype, stream_dtype, gate, post, names):
+    """Rows of which each is scaled by another of SMALL, in the tensors `names`."""
+    t = make(rows, hidden, dtype, stream_dtype, gate, post)
+    scale = torch.tensor(SMALL, device="cuda")[torch.arange(rows, device="cuda") % len(SMALL)][:, None]
+    with torch.no_grad():
+        for n in names:
+            t[n].mul_(scale)
+    return t
+
+
+SMALL_CALLS = [(torch.float32, None, "none", False, ("x",)), (torch.bfloat16, None, "none", False, ("x",)),
+               (torch.float32, torch.float32, "none", True, ("x",)), (torch.bfloat16, torch.bfloat16, "none", False, ("x", "residual")),
+               (torch.bfloat16, torch.float32, "channel", True, ("x", "residual")), (torch.float32, torch.float32, "token", True, ("x", "residual")),
+               (torch.bfloat16, torch.bfloat16, "full", False, ("x", "residual")), (torch.float32, torch.float32, "full", True, ("x", "residual"))]
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-30])
+@pytest.mark.parametrize("rows,hidden", SMALL_SHAPES)
+def test_small_rows_and_a_small_eps(rows, hidden, eps):
+    """Root mean squares whose square is no float32 number, beside ordinary rows."""
+    for dtype, stream_dtype, gate, post, names in SMALL_CALLS:
+        t = small_rows(rows, hidden, dtype, stream_dtype, gate, post, names)
+        with torch.no_grad():
+            got = run(t, 0.5, eps)
+        ref = norm_reference(t["x"], t.get("residual"), t["weight"], t.get("post_weight"), t.get("gate"), eps, 0.5)
+        for name, value in got.items():
+            want, magnitude = ref[name]
+            tiny = torch.finfo(value.dtype).smallest_normal * torch.finfo(value.dtype).eps
+            assert_within(name, value, want, half_step(value.dtype) * want.abs() * (1 + 2 ** -7) + (hidden / 256 + 80) * F32 * magnitude + tiny)
+    assert_status_clean(t["x"].device)
+
+
+def test_rows_of_zeros_without_eps():
+    """0 / 0, as the formula says; the rows beside them are what they are alone."""
+    for hidden in (64, 4096, 20001):
+        x = torch.randn(2500 if hidden == 4096 else 9, hidden, device="cuda")
+        clean = xma.rmsnorm(x, None, 0.0)
+        x[3], x[5] = 0.0, 1e-25
+        y = xma.rmsnorm(x, None, 0.0)
+        assert y[3].isnan().all() and (y[5] - 1.0).abs().max() <= 8 * F32
+        keep = torch.ones(len(x), dtype=torch.bool, device="cuda")
+        keep[[3, 5]] = False
+        assert torch.equal(y[keep], clean[keep])
