@@ -8,13 +8,15 @@
 // Without a residual s = x and only y is written. Backward, with a = weight * dy and the gradient
 // d of the stream output:
 //
-//   ds = rs (a - s rs^2 mean(a s)) + d            d_residual = ds
-//   d_gate = m ds u,   b = m ds gate post,        dx = rp (b - x rp^2 mean(b x))
-//   d_weight = sum_rows dy s rs,                  d_post = sum_rows m ds gate x rp
+//   ds = rs (a - h mean(a h)) + d,  h = s rs      d_residual = ds
+//   d_gate = m ds u,   b = m ds gate post,        dx = rp (b - g mean(b g)),  g = x rp
+//   d_weight = sum_rows dy h,                     d_post = sum_rows m ds gate g
 //
-// sum(b x) follows from three more sums over the row's inputs (ds is linear in a, s and d), so a row
-// takes ONE reduction: with c = post * gate * x,
-//   sum(c ds) = rs sum(c a) - rs^3 mean(a s) sum(c s) + sum(c d).
+// sum(b g) follows from three more sums over the row's inputs (ds is linear in a, s and d), so a row
+// takes ONE reduction: with c = post * gate * g,
+//   sum(c ds) = rs (sum(c a) - mean(a h) rs sum(c s)) + sum(c d).
+// No product of two rs, rp or of s and x is formed: of a row of 1e-20 (with an eps that allows it) they are not in
+// float32's range, though every h, g and gradient is.
 // The backward pass recomputes s from the residual and x where it reads x anyway, so that the rounding of the
 // stream does not reach the gradients; for a plain residual add it reads the rounded stream, one tensor less.
 //
@@ -733,22 +735,22 @@ forward_ring_kernel(const Params p, const RingLayout lay) {
 // What the elements of a row need beside their inputs.
 struct RowScale {
     float rs, rp;
-    float k_s;   // rs^2 mean(a s)
-    float k_x;   // rp mean(b x), with the multiplier and the token gate in it
+    float k_s;   // mean(a h), h = rs s
+    float k_x;   // mean(b g), g = rp x, with the multiplier and the token gate in it
     float m;     // multiplier * token gate
     float d_token_gate;
 };
-// sums: (a s), (c a), (c s), (c d)
+// sums: (a s), (c a), (c s), (c d); c = post * gate * g
 __device__ __forceinline__ RowScale row_scale(const Params& p, const float (&sums)[4], float rs, float rp, float token) {
     RowScale r;
     const float inv_h = 1.f / static_cast<float>(p.hidden);
     r.rs = rs;
     r.rp = rp;
-    r.k_s = rs * rs * sums[0] * inv_h;
-    const float c_ds = rs * sums[1] - rs * r.k_s * sums[2] + sums[3];
+    r.k_s = rs * sums[0] * inv_h;
+    const float c_ds = rs * (sums[1] - r.k_s * (rs * sums[2])) + sums[3];
     r.m = p.multiplier * token;
-    r.k_x = p.post != nullptr ? r.m * rp * c_ds * inv_h : 0.f;
-    r.d_token_gate = p.multiplier * rp * c_ds;
+    r.k_x = p.post != nullptr ? r.m * c_ds * inv_h : 0.f;
+    r.d_token_gate = p.multiplier * c_ds;
     return r;
 }
 
@@ -865,14 +867,13 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
     int previous = -1;
     for (int64_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
         const int64_t row0 = chunk * per_chunk + slot * kRows;
-        float rs[kRows], rp[kRows], token[kRows], branch[kRows];
+        float rs[kRows], rp[kRows], token[kRows];
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
             const bool valid = row0 + r < p.rows;  // the same in the whole group
             rs[r] = valid ? p.rs[row0 + r] : 0.f;
             rp[r] = valid && kX && p.post != nullptr ? p.rp[row0 + r] : 1.f;
             token[r] = valid && kX ? token_gate<T>(p, row0 + r) : 1.f;
-            branch[r] = p.multiplier * token[r] * rp[r];
         }
         if (!mbar_wait(st.full + 8 * st.stage, st.phase, st.abort_flag, p.status, 402)) {
             st.drain(lay.stages);
@@ -906,8 +907,8 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
                     gate8(stage + lay.gate, start, off, v, g);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        x8[j] = mul_f32x2(x8[j], mul_f32x2(f[j], g[j]));
-                        s8[j] = fma_f32x2(x8[j], both(branch[r]), s8[j]);  // the stream, from the residual
+                        x8[j] = mul_f32x2(mul_f32x2(x8[j], both(rp[r])), mul_f32x2(f[j], g[j]));
+                        s8[j] = fma_f32x2(x8[j], both(p.multiplier * token[r]), s8[j]);  // the stream, from the residual
                     }
                 }
                 if (has_dy) {
@@ -981,8 +982,9 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
                     weight8(v, w8);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        acc_w[v][j] = fma_f32x2(d8[j], mul_f32x2(s8[j], both(k.rs)), acc_w[v][j]);
-                        ds[j] = fma_f32x2(mul_f32x2(d8[j], w8[j]), both(k.rs), fma_f32x2(s8[j], both(-k.rs * k.k_s), ds[j]));
+                        s8[j] = mul_f32x2(s8[j], both(k.rs));
+                        acc_w[v][j] = fma_f32x2(d8[j], s8[j], acc_w[v][j]);
+                        ds[j] = fma_f32x2(fma_f32x2(s8[j], both(-k.k_s), mul_f32x2(d8[j], w8[j])), both(k.rs), ds[j]);
                     }
                 }
                 if (has_d_residual) store_cols<kVec>(static_cast<R*>(p.d_residual) + base, v, t, group, p.hidden, ds);
@@ -996,7 +998,7 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
                         else acc_g[v][j] = fma_f32x2(b[j], u[j], acc_g[v][j]);
                         b[j] = mul_f32x2(b[j], g[j]);
                         acc_p[v][j] = fma_f32x2(b[j], hat[j], acc_p[v][j]);
-                        b[j] = fma_f32x2(mul_f32x2(b[j], f[j]), both(k.rp), mul_f32x2(hat[j], both(-k.rp * k.k_x)));
+                        b[j] = mul_f32x2(fma_f32x2(hat[j], both(-k.k_x), mul_f32x2(b[j], f[j])), both(k.rp));
                     }
                     if (kFull && p.d_gate != nullptr) store_cols<kVec>(static_cast<T*>(p.d_gate) + base, v, t, group, p.hidden, u);
                 }
@@ -1033,19 +1035,19 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
 // The elements of one position, from global memory (two-kernel backward).
 template <typename T, typename R>
 struct Element {
-    float dy, s, d, x, w, post, gate;
-    // branch: multiplier * token gate * rp of the row
-    __device__ __forceinline__ Element(const Params& p, int64_t base, int c, float branch) {
+    float dy, s, d, x, w, post, gate;  // x: times the row's rp
+    // m: multiplier * token gate of the row
+    __device__ __forceinline__ Element(const Params& p, int64_t base, int c, float m, float rp) {
         dy = p.dy != nullptr ? Elem<T>::to_float(static_cast<const T*>(p.dy)[base + c]) : 0.f;
         s = Elem<R>::to_float(static_cast<const R*>(p.s)[base + c]);
         d = p.d_stream != nullptr ? Elem<R>::to_float(static_cast<const R*>(p.d_stream)[base + c]) : 0.f;
-        x = p.x != nullptr ? Elem<T>::to_float(static_cast<const T*>(p.x)[base + c]) : 0.f;
+        x = p.x != nullptr ? Elem<T>::to_float(static_cast<const T*>(p.x)[base + c]) * rp : 0.f;
         w = param_at<T>(p.weight, p.weight_f32, c);
         post = param_at<T>(p.post, p.post_f32, c);
         gate = p.gate_mode == kGateFull      ? Elem<T>::to_float(static_cast<const T*>(p.gate)[base + c])
                : p.gate_mode == kGateChannel ? param_at<T>(p.gate, p.gate_f32, c)
                                              : 1.f;
-        if (p.x != nullptr) s = fmaf(x * post * gate, branch, s);  // the stream, from the residual
+        if (p.x != nullptr) s = fmaf(x * post * gate, m, s);  // the stream, from the residual
     }
 };
 
@@ -1062,9 +1064,9 @@ backward_sums_kernel(const Params p) {
     const int64_t base = row * p.hidden;
     float sums[4] = {0.f, 0.f, 0.f, 0.f};
     const float rp = p.post != nullptr ? p.rp[row] : 1.f, token = token_gate<T>(p, row);
-    const float branch = p.multiplier * token * rp;
+    const float m = p.multiplier * token;
     for (int c = threadIdx.x; c < p.hidden; c += blockDim.x) {
-        const Element<T, R> e(p, base, c, branch);
+        const Element<T, R> e(p, base, c, m, rp);
         const float a = e.dy * e.w, q = e.x * e.post * e.gate;
         sums[0] += a * e.s;
         sums[1] += q * a;
@@ -1075,8 +1077,8 @@ backward_sums_kernel(const Params p) {
     if (threadIdx.x == 0) {
         const RowScale k = row_scale(p, sums, p.rs[row], rp, token);
         float4* out = reinterpret_cast<float4*>(p.row_sums) + row * 2;
-        out[0] = make_float4(k.rs, k.rs * k.k_s, k.rp, k.rp * k.k_x);
-        out[1] = make_float4(k.m, branch, 0.f, 0.f);
+        out[0] = make_float4(k.rs, k.k_s, k.rp, k.k_x);
+        out[1] = make_float4(k.m, 0.f, 0.f, 0.f);
         if (p.gate_mode == kGateToken && p.d_gate != nullptr) static_cast<T*>(p.d_gate)[row] = Elem<T>::from_float(k.d_token_gate);
     }
 }
@@ -1094,7 +1096,8 @@ backward_elements_kernel(const Params p, int64_t rows_per_cta) {
     const float gate = p.gate_mode == kGateChannel ? param_at<T>(p.gate, p.gate_f32, c) : 1.f;
     for (int64_t row0 = first; row0 < last; row0 += kBatch) {
         float dy[kBatch], s[kBatch], d[kBatch], x[kBatch], g[kBatch];
-        float4 k[kBatch], k2[kBatch];
+        float4 k[kBatch];
+        float m[kBatch];
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
             const int64_t row = min(row0 + u, last - 1), at = row * p.hidden + c;  // the last row again where there is none
@@ -1104,26 +1107,27 @@ backward_elements_kernel(const Params p, int64_t rows_per_cta) {
             x[u] = p.x != nullptr ? Elem<T>::to_float(static_cast<const T*>(p.x)[at]) : 0.f;
             g[u] = p.gate_mode == kGateFull ? Elem<T>::to_float(static_cast<const T*>(p.gate)[at]) : gate;
             k[u] = reinterpret_cast<const float4*>(p.row_sums)[row * 2];
-            k2[u] = reinterpret_cast<const float4*>(p.row_sums)[row * 2 + 1];
+            m[u] = p.row_sums[row * 8 + 4];
         }
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
             if (row0 + u >= last) break;
             const int64_t at = (row0 + u) * p.hidden + c;
-            const float rs = k[u].x, rs_ks = k[u].y, rp = k[u].z, rp_kx = k[u].w, m = k2[u].x, branch = k2[u].y;
-            if (p.x != nullptr) s[u] = fmaf(x[u] * post * g[u], branch, s[u]);
-            acc_w += dy[u] * (s[u] * rs);
-            const float ds = rs * (dy[u] * w) - s[u] * rs_ks + d[u];
+            const float rs = k[u].x, k_s = k[u].y, rp = k[u].z, k_x = k[u].w;
+            const float g_x = x[u] * rp;
+            if (p.x != nullptr) s[u] = fmaf(g_x * post * g[u], m[u], s[u]);
+            const float h = s[u] * rs;
+            acc_w += dy[u] * h;
+            const float ds = fmaf(rs, dy[u] * w - h * k_s, d[u]);
             if (p.d_residual != nullptr) static_cast<R*>(p.d_residual)[at] = Elem<R>::from_float(ds);
-            float b = m * ds;
-            const float hat = x[u] * rp;
-            const float dg = b * hat * post;
+            float b = m[u] * ds;
+            const float dg = b * g_x * post;
             if (p.gate_mode == kGateFull && p.d_gate != nullptr) static_cast<T*>(p.d_gate)[at] = Elem<T>::from_float(dg);
             acc_g += dg;
             b *= g[u];
             if (p.post != nullptr) {
-                acc_p += b * hat;
-                b = b * post * rp - hat * rp_kx;
+                acc_p += b * g_x;
+                b = rp * (b * post - g_x * k_x);
             }
             if (p.dx != nullptr) static_cast<T*>(p.dx)[at] = Elem<T>::from_float(b);
         }

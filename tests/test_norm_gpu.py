@@ -352,3 +352,11 @@ def test_rows_of_zeros_without_eps():
         keep = torch.ones(len(x), dtype=torch.bool, device="cuda")
         keep[[3, 5]] = False
         assert torch.equal(y[keep], clean[keep])
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-30])
+@pytest.mark.parametrize("rows,hidden", SMALL_SHAPES)
+def test_gradients_of_small_rows(rows, hidden, eps):
+    """Where the square of a root mean square, or of its reciprocal, is no float32 number, the gradients are."""
+    for dtype, stream_dtype, gate, post, names in SMALL_CALLS:
+        check(small_rows(rows, hidden, dtype, stream_dtype, gate, post, names), 0.5, eps=eps)
