@@ -613,3 +613,35 @@ def test_copies_in_flight_are_waited_for(fills):
         turns = [j for j in range(fills) if j % 3 == stage]
         want = src[turns[-1] * size: (turns[-1] + 1) * size] if turns else torch.zeros_like(dst[0])
         assert torch.equal(dst[stage], want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_bad_offsets_write_nothing_else(dtype):
+    """Outputs, statistics, lists: whatever the offsets hold, what lies around them keeps its bytes."""
+    from xma import _native as N
+    from xma.ops import attention_packed_backward_cuda, attention_packed_forward_cuda
+
+    T, H, K, D, edge = 300, 4, 2, 40, 4096
+    q, k, v, do = make([T], H, K, D, dtype)
+    for int_type in (torch.int32, torch.int64):
+        for values in ([0, 300], [0, 10 ** 6], [-50, 100, 300], [200, 100, 300], [0, 300, 0, 300, 0, 300], [-7, -7], [400, 500],
+                       [0, 0, 0, 129, 129, 300], [301, 300, 0], [-2 ** 31, 2 ** 31 - 1]):
+            cu = torch.tensor(values, dtype=int_type, device="cuda")
+            B = len(values) - 1
+            buffers = []
+
+            def inside(shape, to):
+                size = math.prod(shape) * torch.empty(0, dtype=to).element_size()
+                raw = torch.full((size + 2 * edge,), 0x5A, dtype=torch.uint8, device="cuda")
+                buffers.append((raw, size))
+                return raw[edge: edge + size].view(to).view(shape)
+
+            rows = N.attention_stat_rows(T, B)
+            workspace = lambda: inside((N.attention_workspace_bytes(T, B),), torch.uint8)
+            out, dq, dk, dv = (inside(tuple(t.shape), dtype) for t in (q, q, k, v))
+            lse, delta, rest = inside((H, rows), torch.float32), inside((H, rows), torch.float32), inside((T, H, 48), torch.uint8)
+            attention_packed_forward_cuda(q, k, v, cu, 0.2, out, lse, rest, workspace())
+            attention_packed_backward_cuda(q, k, v, cu, 0.2, out, rest, do, lse, delta, dq, dk, dv, workspace())
+            assert_status_clean(q.device)
+            for raw, size in buffers:
+                assert (raw[:edge] == 0x5A).all() and (raw[edge + size:] == 0x5A).all()
