@@ -360,3 +360,28 @@ def test_gradients_of_small_rows(rows, hidden, eps):
     """Where the square of a root mean square, or of its reciprocal, is no float32 number, the gradients are."""
     for dtype, stream_dtype, gate, post, names in SMALL_CALLS:
         check(small_rows(rows, hidden, dtype, stream_dtype, gate, post, names), 0.5, eps=eps)
+
+
+@pytest.mark.parametrize("dtype,stream", TYPES)
+@pytest.mark.parametrize("rows,hidden", [(900, 1024), (40, 1001), (3000, 4096)])
+def test_residual_add_against_its_definition(rows, hidden, dtype, stream):
+    """The backward pass of a plain residual add reads the stream as it was rounded (h, half a step of its type, of each
+    element); against the gradients of the exact one that is h sum |dy s rs| in the weight's, and in the rows' once h in
+    the stream itself and once in its mean with a."""
+    t = make(rows, hidden, dtype, stream, "none", False)
+    with torch.no_grad():
+        t["residual"].mul_(torch.exp(torch.randn(hidden, device="cuda", generator=torch.Generator(device="cuda").manual_seed(4))))
+    leaves = [t["x"], t["residual"], t["weight"]]
+    grads = torch.autograd.grad(list(run(t, 0.5).values()), leaves, [t["dy"], t["dd"]])
+    ref = norm_reference(t["x"], t["residual"], t["weight"], None, None, EPS, 0.5, t["dy"], t["dd"])
+    s, dy, w = ref["stream"][0], t["dy"].double(), t["weight"].detach().double()
+    rs = torch.rsqrt(s.pow(2).mean(-1, keepdim=True) + EPS)
+    h = half_step(stream)
+    row = h * (2 + h) * rs.pow(3) * s.abs() * (w * dy * s).abs().mean(-1, keepdim=True)
+    extra = {"d_weight": h * (dy * s * rs).abs().sum(0), "d_residual": row, "d_x": 0.5 * row}
+    for name, value in zip(("d_x", "d_residual", "d_weight"), grads):
+        want, magnitude = ref[name]
+        steps = hidden / 256 + 80 + (rows / 148 + 64 if name == "d_weight" else 0)
+        u = half_step(value.dtype)
+        assert_within(name, value, want, u * want.abs() * (1 + 2 ** -7) + (1 + u) * extra[name] + steps * F32 * magnitude + torch.finfo(value.dtype).tiny)
+    assert_status_clean(t["x"].device)
