@@ -1672,7 +1672,7 @@ static int check_call(const Call& c) {
     if (c.batch < 0 || c.total < 0 || c.heads <= 0 || c.kv_heads <= 0 || c.dim <= 0) return XMA_ERR_BAD_ARG;
     if (c.dim % 8 != 0 || c.dim > 128 || c.heads % c.kv_heads != 0 || c.heads > kMaxHeads) return XMA_ERR_UNSUPPORTED;
     if (c.total > (int64_t(1) << 30) || c.batch > (int64_t(1) << 20)) return XMA_ERR_UNSUPPORTED;
-    if (!(c.scale > 0.f) || !(c.scale <= 3.4e38f)) return XMA_ERR_BAD_ARG;
+    if (!(c.scale > 0.f) || !(c.scale <= 2.3e38f)) return XMA_ERR_BAD_ARG;  // its product with log2(e) is a number too
     if (c.total == 0) return XMA_OK;
     if (!c.q || !c.k || !c.v || !c.cu || !c.workspace) return XMA_ERR_BAD_ARG;
     if (!aligned16(c.q) || !aligned16(c.k) || !aligned16(c.v) || !aligned16(c.workspace)) return XMA_ERR_BAD_ARG;

@@ -16,6 +16,7 @@ from ._forward_mode import refuse_tangents
 MAX_HEAD_DIM = 128
 _MAX_TOKENS = 1 << 30
 _MAX_SEQUENCES = 1 << 20
+_MIN_SCALE = 2.0 ** -149  # float32's smallest number
 
 
 def _tiled(t: torch.Tensor) -> torch.Tensor:
@@ -77,8 +78,8 @@ def attention_packed(
     float16; `heads` is a multiple of `kv_heads` (query head `h` reads head `h // (heads // kv_heads)`), `head_dim` a
     multiple of 8 up to 128. Any strides are taken; slices along the head dimension of one projection are read in
     place. `cu_seqlens` (`[sequences + 1]`, int32 or int64, on the same device) holds ascending offsets: sequence `b` is
-    the tokens `cu_seqlens[b] .. cu_seqlens[b + 1] - 1` (none, one or many). `softmax_scale` is positive and
-    defaults to `1 / sqrt(head_dim)`.
+    the tokens `cu_seqlens[b] .. cu_seqlens[b + 1] - 1` (none, one or many). `softmax_scale` is positive (a
+    float32 number below 1e30) and defaults to `1 / sqrt(head_dim)`.
 
     Scores and sums are float32; probabilities are rounded to the inputs' dtype before they meet the values (in float16
     times a power of two, so that keys which others outweigh keep their share). For a backward pass the call keeps its
@@ -119,8 +120,8 @@ def attention_packed(
     if total > _MAX_TOKENS or cu_seqlens.numel() > _MAX_SEQUENCES:
         raise ValueError(f"at most {_MAX_TOKENS} tokens and {_MAX_SEQUENCES - 1} sequences are supported")
     scale = 1.0 / math.sqrt(dim) if softmax_scale is None else float(softmax_scale)
-    if not 0.0 < scale < 1e30:
-        raise ValueError(f"softmax_scale should be positive and finite, got {scale}")
+    if not _MIN_SCALE <= scale < 1e30:
+        raise ValueError(f"softmax_scale should be a positive float32 number below 1e30, got {scale}")
     refuse_tangents("attention_packed", q, k, v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _AttentionPacked.apply(q, k, v, cu_seqlens, scale)

@@ -422,7 +422,7 @@ int xma_norm_backward(const void* dy, const void* d_stream, const void* stream_o
  *   q [total, heads, dim], k, v [total, kv_heads, dim] of `dtype` (bf16 or fp16); *_token and *_head are their
  *   strides in elements (multiples of 8, bases 16-byte aligned); out, d_out, dq [total, heads, dim] and dk, dv
  *   [total, kv_heads, dim] are contiguous. heads is a multiple of kv_heads (query head h reads kv head
- *   h / (heads / kv_heads)), dim a multiple of 8 up to 128, scale positive.
+ *   h / (heads / kv_heads)), dim a multiple of 8 up to 128, scale positive, up to 2.3e38.
  *   lse   float32 [heads, xma_attention_stat_rows(total, batch)], 16-byte aligned: the rows' log-sum-exp (base
  *         2; in fp16 less 14), written by the forward pass for the backward pass; NULL when there is none
  *   out_rest  bytes [total, heads, dim rounded up to 16], 16-byte aligned: what rounding took from out (e5m2,

@@ -87,3 +87,13 @@ def test_forward_mode_is_refused(which):
             xma.attention_packed(*inputs, CU)
         with pytest.raises(RuntimeError, match="no CPU path"):  # a level that is open is no reason
             xma.attention_packed(t(4, 2, 64), t(4, 2, 64), t(4, 2, 64), CU)
+
+
+@pytest.mark.parametrize("scale", [1e-50, 3e38, 1e39, float("nan"), float("-inf")])
+def test_scales_that_float32_cannot_work_with(scale):
+    from xma import _native as N
+
+    with pytest.raises(ValueError, match="softmax_scale"):
+        xma.attention_packed(t(4, 2, 64), t(4, 2, 64), t(4, 2, 64), CU, softmax_scale=scale)
+    a = 1 << 20
+    assert N.lib().xma_attention_forward(a, a, a, *(128, 64) * 3, 0, a, 0, 1, 0, 2, 2, 64, scale, a, None, None, a, None, None) == 1
