@@ -14,6 +14,20 @@ def pytest_configure(config):
 
 
 @pytest.fixture(scope="session", autouse=True)
+def _library_products_are_summed_in_float32():
+    """The products that tests compare with, and the router's gate where it is a library product, are rounded once. By default
+    the library may add up 16-bit partial sums where it splits the reduction, and whether it does differs from machine to
+    machine (7 tokens, 6 experts, H=2048: 25 of 42 logits off the rounded product on one, by up to a step)."""
+    import torch
+
+    matmul = torch.backends.cuda.matmul
+    before = matmul.allow_bf16_reduced_precision_reduction, matmul.allow_fp16_reduced_precision_reduction
+    matmul.allow_bf16_reduced_precision_reduction = matmul.allow_fp16_reduced_precision_reduction = False
+    yield
+    matmul.allow_bf16_reduced_precision_reduction, matmul.allow_fp16_reduced_precision_reduction = before
+
+
+@pytest.fixture(scope="session", autouse=True)
 def _native_library_is_built():
     """The shared library is built once per session (nvcc cross-compiles without a GPU)."""
     sys.path.insert(0, os.path.join(_ROOT, "flash-model-architectures_b200"))
