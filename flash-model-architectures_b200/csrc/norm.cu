@@ -16,7 +16,8 @@
 // takes ONE reduction: with c = post * gate * g,
 //   sum(c ds) = rs (sum(c a) - mean(a h) rs sum(c s)) + sum(c d).
 // No product of two rs, rp or of s and x is formed: of a row of 1e-20 (with an eps that allows it) they are not in
-// float32's range, though every h, g and gradient is.
+// float32's range, though every h, g and gradient is. Without a post norm g is x, and the sums take it times the power
+// of two under rs.
 // The backward pass recomputes s from the residual and x where it reads x anyway, so that the rounding of the
 // stream does not reach the gradients; for a plain residual add it reads the rounded stream, one tensor less.
 //
@@ -740,14 +741,21 @@ struct RowScale {
     float m;     // multiplier * token gate
     float d_token_gate;
 };
-// sums: (a s), (c a), (c s), (c d); c = post * gate * g
-__device__ __forceinline__ RowScale row_scale(const Params& p, const float (&sums)[4], float rs, float rp, float token) {
+// What x is multiplied with in the sums: rp, or the power of two under rs where there is no post norm.
+__device__ __forceinline__ float sum_scale(const Params& p, float rs, float rp) {
+    return p.post != nullptr ? rp : __uint_as_float(__float_as_uint(rs) & 0x7f800000u);
+}
+// That back: g = x rp is `sum_scale` times x times this.
+__device__ __forceinline__ float sum_unscale(const Params& p, float scale) { return p.post != nullptr ? 1.f : 1.f / scale; }
+
+// sums: (a s), (c a), (c s), (c d); c = post * gate * x * sum_scale
+__device__ __forceinline__ RowScale row_scale(const Params& p, const float (&sums)[4], float rs, float rp, float token, float unscale) {
     RowScale r;
     const float inv_h = 1.f / static_cast<float>(p.hidden);
     r.rs = rs;
     r.rp = rp;
     r.k_s = rs * sums[0] * inv_h;
-    const float c_ds = rs * (sums[1] - r.k_s * (rs * sums[2])) + sums[3];
+    const float c_ds = (rs * (sums[1] - r.k_s * (rs * sums[2])) + sums[3]) * unscale;
     r.m = p.multiplier * token;
     r.k_x = p.post != nullptr ? r.m * c_ds * inv_h : 0.f;
     r.d_token_gate = p.multiplier * c_ds;
@@ -867,13 +875,15 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
     int previous = -1;
     for (int64_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
         const int64_t row0 = chunk * per_chunk + slot * kRows;
-        float rs[kRows], rp[kRows], token[kRows];
+        float rs[kRows], rp[kRows], token[kRows], scale[kRows], unscale[kRows];
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
             const bool valid = row0 + r < p.rows;  // the same in the whole group
             rs[r] = valid ? p.rs[row0 + r] : 0.f;
             rp[r] = valid && kX && p.post != nullptr ? p.rp[row0 + r] : 1.f;
             token[r] = valid && kX ? token_gate<T>(p, row0 + r) : 1.f;
+            scale[r] = kX ? sum_scale(p, rs[r], rp[r]) : 1.f;
+            unscale[r] = kX ? sum_unscale(p, scale[r]) : 1.f;
         }
         if (!mbar_wait(st.full + 8 * st.stage, st.phase, st.abort_flag, p.status, 402)) {
             st.drain(lay.stages);
@@ -907,8 +917,8 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
                     gate8(stage + lay.gate, start, off, v, g);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        x8[j] = mul_f32x2(mul_f32x2(x8[j], both(rp[r])), mul_f32x2(f[j], g[j]));
-                        s8[j] = fma_f32x2(x8[j], both(p.multiplier * token[r]), s8[j]);  // the stream, from the residual
+                        x8[j] = mul_f32x2(mul_f32x2(x8[j], both(scale[r])), mul_f32x2(f[j], g[j]));
+                        s8[j] = fma_f32x2(x8[j], both(p.multiplier * token[r] * unscale[r]), s8[j]);  // the stream, from the residual
                     }
                 }
                 if (has_dy) {
@@ -949,7 +959,7 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
             if (row0 + r >= p.rows) continue;
             float four[4] = {sums[r * kSums], 0.f, 0.f, 0.f};
             if (kX) four[1] = sums[r * kSums + kSums - 3], four[2] = sums[r * kSums + kSums - 2], four[3] = sums[r * kSums + kSums - 1];
-            const RowScale k = row_scale(p, four, rs[r], rp[r], token[r]);
+            const RowScale k = row_scale(p, four, rs[r], rp[r], token[r], unscale[r]);
             const int64_t base = (row0 + r) * p.hidden;
             const int off = (slot * kRows + r) * p.hidden;
             if (kX && !kFull && p.gate_mode == kGateToken && p.d_gate != nullptr && t == 0)
@@ -1035,13 +1045,13 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
 // The elements of one position, from global memory (two-kernel backward).
 template <typename T, typename R>
 struct Element {
-    float dy, s, d, x, w, post, gate;  // x: times the row's rp
-    // m: multiplier * token gate of the row
-    __device__ __forceinline__ Element(const Params& p, int64_t base, int c, float m, float rp) {
+    float dy, s, d, x, w, post, gate;  // x: times the row's `scale`
+    // m: multiplier * token gate of the row, times what undoes `scale`
+    __device__ __forceinline__ Element(const Params& p, int64_t base, int c, float m, float scale) {
         dy = p.dy != nullptr ? Elem<T>::to_float(static_cast<const T*>(p.dy)[base + c]) : 0.f;
         s = Elem<R>::to_float(static_cast<const R*>(p.s)[base + c]);
         d = p.d_stream != nullptr ? Elem<R>::to_float(static_cast<const R*>(p.d_stream)[base + c]) : 0.f;
-        x = p.x != nullptr ? Elem<T>::to_float(static_cast<const T*>(p.x)[base + c]) * rp : 0.f;
+        x = p.x != nullptr ? Elem<T>::to_float(static_cast<const T*>(p.x)[base + c]) * scale : 0.f;
         w = param_at<T>(p.weight, p.weight_f32, c);
         post = param_at<T>(p.post, p.post_f32, c);
         gate = p.gate_mode == kGateFull      ? Elem<T>::to_float(static_cast<const T*>(p.gate)[base + c])
@@ -1064,9 +1074,10 @@ backward_sums_kernel(const Params p) {
     const int64_t base = row * p.hidden;
     float sums[4] = {0.f, 0.f, 0.f, 0.f};
     const float rp = p.post != nullptr ? p.rp[row] : 1.f, token = token_gate<T>(p, row);
-    const float m = p.multiplier * token;
+    const float scale = sum_scale(p, p.rs[row], rp), unscale = sum_unscale(p, scale);
+    const float m = p.multiplier * token * unscale;
     for (int c = threadIdx.x; c < p.hidden; c += blockDim.x) {
-        const Element<T, R> e(p, base, c, m, rp);
+        const Element<T, R> e(p, base, c, m, scale);
         const float a = e.dy * e.w, q = e.x * e.post * e.gate;
         sums[0] += a * e.s;
         sums[1] += q * a;
@@ -1075,7 +1086,7 @@ backward_sums_kernel(const Params p) {
     }
     group_sum<4>(sums, scratch, threadIdx.x, blockDim.x, 1);
     if (threadIdx.x == 0) {
-        const RowScale k = row_scale(p, sums, p.rs[row], rp, token);
+        const RowScale k = row_scale(p, sums, p.rs[row], rp, token, unscale);
         float4* out = reinterpret_cast<float4*>(p.row_sums) + row * 2;
         out[0] = make_float4(k.rs, k.k_s, k.rp, k.k_x);
         out[1] = make_float4(k.m, 0.f, 0.f, 0.f);

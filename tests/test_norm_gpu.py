@@ -385,3 +385,12 @@ def test_residual_add_against_its_definition(rows, hidden, dtype, stream):
         u = half_step(value.dtype)
         assert_within(name, value, want, u * want.abs() * (1 + 2 ** -7) + (1 + u) * extra[name] + steps * F32 * magnitude + torch.finfo(value.dtype).tiny)
     assert_status_clean(t["x"].device)
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-30])
+@pytest.mark.parametrize("rows,hidden", SMALL_SHAPES)
+def test_token_gates_of_small_rows(rows, hidden, eps):
+    """A token's gate without a post norm: its gradient is a sum over products of a small row with itself."""
+    for dtype, stream_dtype in ((torch.float32, torch.float32), (torch.bfloat16, torch.float32), (torch.bfloat16, torch.bfloat16)):
+        check(small_rows(rows, hidden, dtype, stream_dtype, "token", False, ("x", "residual")), 0.5, eps=eps)
+        check(small_rows(rows, hidden, dtype, stream_dtype, "token", False, ("x",)), -1.5, eps=eps)
