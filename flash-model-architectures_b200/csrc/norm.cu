@@ -743,10 +743,12 @@ struct RowScale {
 };
 // What x is multiplied with in the sums: rp, or the power of two under rs where there is no post norm.
 __device__ __forceinline__ float sum_scale(const Params& p, float rs, float rp) {
-    return p.post != nullptr ? rp : __uint_as_float(__float_as_uint(rs) & 0x7f800000u);
+    return p.post != nullptr ? rp : __uint_as_float(min(__float_as_uint(rs) & 0x7f800000u, 0x7e800000u));
 }
-// That back: g = x rp is `sum_scale` times x times this.
-__device__ __forceinline__ float sum_unscale(const Params& p, float scale) { return p.post != nullptr ? 1.f : 1.f / scale; }
+// That back: g = x rp is `sum_scale` times x times this, 1 or the reciprocal of a power of two.
+__device__ __forceinline__ float sum_unscale(const Params& p, float scale) {
+    return p.post != nullptr ? 1.f : __uint_as_float(0x7f000000u - __float_as_uint(scale));
+}
 
 // sums: (a s), (c a), (c s), (c d); c = post * gate * x * sum_scale
 __device__ __forceinline__ RowScale row_scale(const Params& p, const float (&sums)[4], float rs, float rp, float token, float unscale) {
@@ -875,15 +877,13 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
     int previous = -1;
     for (int64_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
         const int64_t row0 = chunk * per_chunk + slot * kRows;
-        float rs[kRows], rp[kRows], token[kRows], scale[kRows], unscale[kRows];
+        float rs[kRows], scale[kRows], token[kRows];  // scale: rp, where there is a post norm
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
             const bool valid = row0 + r < p.rows;  // the same in the whole group
             rs[r] = valid ? p.rs[row0 + r] : 0.f;
-            rp[r] = valid && kX && p.post != nullptr ? p.rp[row0 + r] : 1.f;
+            scale[r] = kX ? sum_scale(p, rs[r], valid && p.post != nullptr ? p.rp[row0 + r] : 1.f) : 1.f;
             token[r] = valid && kX ? token_gate<T>(p, row0 + r) : 1.f;
-            scale[r] = kX ? sum_scale(p, rs[r], rp[r]) : 1.f;
-            unscale[r] = kX ? sum_unscale(p, scale[r]) : 1.f;
         }
         if (!mbar_wait(st.full + 8 * st.stage, st.phase, st.abort_flag, p.status, 402)) {
             st.drain(lay.stages);
@@ -902,6 +902,7 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
             const int off = (slot * kRows + r) * p.hidden;
+            const float m = kX ? p.multiplier * token[r] * sum_unscale(p, scale[r]) : 1.f;
             f32x2 sum[kSums];
 #pragma unroll
             for (int i = 0; i < kSums; ++i) sum[i] = both(0.f);
@@ -918,7 +919,7 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         x8[j] = mul_f32x2(mul_f32x2(x8[j], both(scale[r])), mul_f32x2(f[j], g[j]));
-                        s8[j] = fma_f32x2(x8[j], both(p.multiplier * token[r] * unscale[r]), s8[j]);  // the stream, from the residual
+                        s8[j] = fma_f32x2(x8[j], both(m), s8[j]);  // the stream, from the residual
                     }
                 }
                 if (has_dy) {
@@ -959,7 +960,7 @@ backward_ring_kernel(const Params p, const RingLayout lay) {
             if (row0 + r >= p.rows) continue;
             float four[4] = {sums[r * kSums], 0.f, 0.f, 0.f};
             if (kX) four[1] = sums[r * kSums + kSums - 3], four[2] = sums[r * kSums + kSums - 2], four[3] = sums[r * kSums + kSums - 1];
-            const RowScale k = row_scale(p, four, rs[r], rp[r], token[r], unscale[r]);
+            const RowScale k = row_scale(p, four, rs[r], kX && p.post != nullptr ? scale[r] : 1.f, token[r], kX ? sum_unscale(p, scale[r]) : 1.f);
             const int64_t base = (row0 + r) * p.hidden;
             const int off = (slot * kRows + r) * p.hidden;
             if (kX && !kFull && p.gate_mode == kGateToken && p.d_gate != nullptr && t == 0)
