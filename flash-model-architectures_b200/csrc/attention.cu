@@ -24,8 +24,10 @@
 // What bounds it: long sequences run into the board's power limit (16384 tokens, 32 heads on 8 of 128, bf16:
 // forward 1.62 ms, 1350 TFLOP/s; dkdv 3.1-3.2 ms, 1400 TFLOP/s, both at 1.6 GHz; dq 2.6-2.9 ms, 1140-1270
 // TFLOP/s), short ones and narrow heads the chain scores -> softmax -> product of a query tile (8192 tokens of
-// ragged prompts, 16 heads on 4 of 64, fp16: 80 us, 550 TFLOP/s), since one tile's softmax takes about 1700
-// cycles of which 1024 are the ex2 unit's, and tensor memory holds no third tile of width 128.
+// ragged prompts, 16 heads on 4 of 64, fp16: 83 us, 530 TFLOP/s), since one tile's softmax takes about 1700
+// cycles of which 1024 are the ex2 unit's, and tensor memory holds no third tile of width 128. Work items are not split
+// where they are few: with 4 heads on 1 at 8192 tokens dkdv has 64 for 148 SMs, each of up to 256 steps, and takes 380
+// us where balanced work would take about 85 (forward: 128 items, 115 us where it would take 50).
 //
 // Rows beyond a sequence's end inside a tile belong to other sequences: their scores are masked by
 // selection, and where a masked (zero) probability would multiply such a row, the row is zeroed in shared

@@ -24,8 +24,9 @@
 // The mean of squares adds up (v / H) v, so that it overflows where the mean itself does and no sooner. Below 2^-78 what
 // terms lose under float32's smallest normal number begins to show; where eps does not cover that (eps is below 2^-78
 // too), such a row's mean is added up again from its values times 2^100, by kernels of their own (kSmallEps: the test alone
-// cost the others 1-2 %).
-// All of it is bound by HBM: every tensor is read and written once.
+// cost the others 1-2 %; 16384 x 4096 with post norm and gate 99 us so, 90 without).
+// The ring kernels and the plain forward kernel read and write every tensor once; forward they are bound by HBM, backward
+// by issue slots. Rows that the ring does not take are read twice backward, forward above kForwardMaxHidden up to three times.
 #include "common.cuh"
 #include "ptx.cuh"
 
@@ -620,7 +621,7 @@ forward_ring_kernel(const Params p, const RingLayout lay) {
 #pragma unroll
             for (int r = 0; r < kRows; ++r) any = (small[r] = is_small(sums[r], p.eps)) || any;
             float again[kRows];
-            if (__syncthreads_or(any)) {
+            if (lay.slots == 1 ? any : __syncthreads_or(any) != 0) {  // one row group a CTA knows it without asking
 #pragma unroll
                 for (int r = 0; r < kRows; ++r) {
                     f32x2 sum = both(0.f);
@@ -1065,8 +1066,9 @@ struct Element {
 // What the ring does not take (longer rows, tensors off a 16-byte boundary), in two kernels: the row sums, from which
 // what a row's elements need is worked out once, then the elements (a block of columns times a share of the rows per CTA,
 // so that the parameters' gradients are sums in registers; four rows at a time, for loads in flight). Every tensor is
-// read twice, two or four bytes a lane: 9000 x 4999 bf16 alone 119 + 152 us; 8000 x 3001 bf16 with everything took
-// 91 + 119 us here and takes 115 in the ring, 5001 x 1001 float32 19 + 19 and 14.5.
+// read twice, two or four bytes a lane, whole vectors or not: 9000 x 4999 bf16 alone 121 + 131 us; 8000 x 3001 bf16 with
+// everything took 91 + 119 us here and takes 117 in the ring, 5001 x 1001 float32 19 + 19 and 14. It also takes calls of
+// which two stages of two rows a thread do not fit (16384 x 4096 float32 with a post norm: 206 + 269 us, floor 187).
 template <typename T, typename R>
 __global__ void __launch_bounds__(256)
 backward_sums_kernel(const Params p) {

@@ -393,8 +393,11 @@ int xma_unpack_sequence(const void* x, const void* cu_seqlens, int32_t cu_is_int
  *   gate_mode     0 none, 1 [hidden] (a parameter), 2 [rows], 3 [rows, hidden]
  *   f32_params    bit 0 weight, bit 1 post_weight, bit 2 a [hidden] gate is float32 (else `dtype`)
  *   rstd, rstd_post   float32 [rows], 1 / rms of the stream and of x, kept for the backward pass; may be NULL
- * Any row length up to 2^24 and any element alignment; rows of a multiple of 8 elements with 16-byte
- * aligned bases take wide accesses.
+ * Up to 2^31 - 1 rows of any length up to 2^24, any element alignment. Rows of a multiple of 8 elements with
+ * 16-byte aligned bases take wide accesses forward up to 16384 elements and backward up to 8192 where two stages of a
+ * CTA's rows fit shared memory; other calls load an element a lane.
+ * eps may be 0: a row whose mean square is below float32's normal range is scaled up for its sum. A row of zeros is
+ * 0 / 0 then.
  *
  * xma_norm_backward: from dy (gradient of y) and d_stream (gradient of stream_out), either of which may be
  * NULL (zero), to d_residual, dx, d_gate, d_weight, d_post_weight; each output may be NULL. With a post norm or a
