@@ -266,6 +266,85 @@ __device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t second
         umma_ts_cta1(d, a + (kk >> 2) * second + (kk & 3) * 8, b + row_step(kk), idesc, (accumulate || kk != 0) ? 1u : 0u);
 }
 
+// p in two operands, for sequences of one key tile: rounded down, and what that took. Few keys do not average p's rounding
+// out, and the backward pass meets it again in delta: with one operand o was 1.04 to 1.14 and dq 1.46 to 1.52 times a
+// single rounding off on sequences of 120 to 2 tokens, with two 1.0 and 1.42. Longer sequences (700 tokens: 1.23 and 1.47)
+// gain less and would pay a product more. The second operand is positive where p is, so that an infinite value makes an
+// infinity, as in one product, and no NaN.
+template <typename T>
+constexpr float kLeast = std::is_same<T, __half>::value ? 0x1p-24f : 0x1p-100f;
+template <typename T>
+__device__ __forceinline__ uint32_t pack2_down(float a, float b) {
+    uint32_t r;
+    if (std::is_same<T, __half>::value) asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    else asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+// 32 columns of scores, of which `row` sees `seen`: p times 2^kShiftLog2 beside the row's maximum, as packed operands; the sum
+// of p is returned. `neg_m` is the shift less the maximum.
+template <typename T>
+__device__ __forceinline__ float two_operands(const uint32_t (&s)[32], int seen, float scale_log2, float neg_m, uint32_t* high, uint32_t* low) {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float a = 2 * i < seen ? ex2(fmaf(__uint_as_float(s[2 * i]), scale_log2, neg_m)) : 0.f;
+        const float b = 2 * i + 1 < seen ? ex2(fmaf(__uint_as_float(s[2 * i + 1]), scale_log2, neg_m)) : 0.f;
+        sum += a + b;
+        high[i] = pack2_down<T>(a, b);
+        const float2 f = unpack2<T>(high[i]);
+        low[i] = pack2<T>(fmaxf(a - f.x, fminf(a, kLeast<T>)), fmaxf(b - f.y, fminf(b, kLeast<T>)));
+    }
+    return sum;
+}
+
+// The softmax of such a tile, a row a thread: scores at taddr to operands, the first of 64 keys at columns 64 h .. 64 h + 31,
+// the second at the 32 after them; `ready` are the halves' barriers. Returns the row's maximum (log2 units) and sum. A call
+// of its own: inlined it costs the long sequences' loops registers.
+template <typename T>
+__device__ __noinline__ float2 one_tile_probabilities(uint32_t taddr, int row, float scale_log2, uint32_t ready) {
+    float m = -INFINITY, l = 0.f;
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+        uint32_t s[32];
+        tmem_ld32(taddr + c * 32, s);
+        tmem_ld_wait();
+        tmem_tie32(s);
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (c * 32 + i <= row) m = fmaxf(m, __uint_as_float(s[i]));
+    }
+    m *= scale_log2;
+    const float neg_m = m == -INFINITY ? 0.f : kShiftLog2<T> - m;
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {
+        uint32_t s[2][32], high[32], low[32];
+        tmem_ld32(taddr + h * 64, s[0]);
+        tmem_ld32(taddr + h * 64 + 32, s[1]);
+        tmem_ld_wait();
+        tmem_tie32(s[0]);
+        tmem_tie32(s[1]);
+        l += two_operands<T>(s[0], row + 1 - h * 64, scale_log2, neg_m, high, low);
+        l += two_operands<T>(s[1], row + 1 - h * 64 - 32, scale_log2, neg_m, high + 16, low + 16);
+        tmem_st32(taddr + h * 64, high);
+        tmem_st32(taddr + h * 64 + 32, low);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(ready + 8 * h);
+    }
+    return make_float2(m, l);
+}
+// The products of half h of such a tile. Rolled up: with the loops written out the kernel's other loops lost 4 % (8192
+// tokens 446 us against 426), to the instruction cache as it seems.
+__device__ __forceinline__ void one_tile_products(uint32_t d, uint32_t a, uint32_t b_tile, uint32_t idesc, int h) {
+    const uint64_t b = desc_row_major(b_tile);
+#pragma unroll 1
+    for (int part = 0; part < 2; ++part)
+#pragma unroll 1
+        for (int kk = 0; kk < 4; ++kk)
+            umma_ts_cta1(d, a + h * 64 + part * 32 + kk * 8, b + row_step(h * 4 + kk), idesc, (h != 0 || part != 0 || kk != 0) ? 1u : 0u);
+}
+
 // What rounding o to T takes away is kept in 8 bits (e5m2, times a power of two that puts the residue of values from
 // 2^-16 to 2^12 into its range; beyond it saturates or underflows). delta = o . do is subtracted for every key of a
 // row, so an error of o would not average out over the keys; two mantissa bits leave an eighth of it at most.
@@ -578,6 +657,32 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             if (!ok) break;
             if (elect_one()) umma_commit_cta1(empty + 8 * kv.stage);
             kv.next(F::kStages);
+            if (b.len <= kTile) {  // p comes in two operands
+                const uint32_t v_tile = ring + kv.stage * F::kTileBytes;
+                ok = mbar_wait_warp(full + 8 * kv.stage, kv.phase, abort_flag, p.status, 505);
+                if (!ok) break;
+                if (b.len < kTile) {
+                    zero_tile_rows<kD>(v_tile, b.len, lane);
+                    fence_proxy_async();
+                    __syncwarp();
+                }
+                for (int h = 0; ok && h < 2; ++h) {
+                    ok = mbar_wait_warp(p_ready + 8 * h, p_phase[0], abort_flag, p.status, h == 0 ? 507 : 510);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        one_tile_products(tmem + F::kO, tmem, v_tile, idesc_o, h);
+                        if (h == 1) {
+                            umma_commit_cta1(o_full);
+                            umma_commit_cta1(empty + 8 * kv.stage);
+                        }
+                    }
+                    __syncwarp();
+                }
+                p_phase[0] ^= 1u;
+                kv.next(F::kStages);
+                continue;
+            }
             for (int j = 0; ok && j < n; ++j) {
                 const uint32_t v_tile = ring + kv.stage * F::kTileBytes;
                 const uint32_t v_empty = empty + 8 * kv.stage;
@@ -643,7 +748,17 @@ forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             if (t == 1 && b.len <= row0 + kTile) continue;
             const int count = b.index * 2 + 1 + t;
             float m = -INFINITY, l = 0.f;  // running maximum (log2 units) that p refers to, and sum of p, shift and all
-            for (int j = 0; j < count; ++j) {
+            const bool one_tile = b.len <= kTile;  // p in two operands
+            if (one_tile) {
+                ok = mbar_wait(s_full + 8 * t, s_phase, abort_flag, p.status, 508);
+                if (!ok) break;
+                s_phase ^= 1u;
+                tc_fence_after();
+                const float2 found = one_tile_probabilities<T>(s_addr, row, p.scale_log2, p_ready + 16 * t);
+                m = found.x;
+                l = found.y;
+            }
+            for (int j = one_tile ? count : 0; j < count; ++j) {
                 ok = mbar_wait(s_full + 8 * t, s_phase, abort_flag, p.status, 508);
                 if (!ok) break;
                 s_phase ^= 1u;

@@ -645,3 +645,43 @@ def test_bad_offsets_write_nothing_else(dtype):
             assert_status_clean(q.device)
             for raw, size in buffers:
                 assert (raw[:edge] == 0x5A).all() and (raw[edge + size:] == 0x5A).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [24, 64, 128])
+def test_short_sequences_keep_what_rounding_takes_from_weights(dtype, dim):
+    """Sequences of up to 128 tokens: o is off by its own rounding and by float32's, not by that of the probabilities, which
+    go into the product as two numbers: the first cut off (2u), the second rounded (u of that) and at least a step of 2^-24
+    in fp16, where a row's largest is 2^9."""
+    lengths = [128, 1, 2, 7, 300, 96, 127]
+    q, k, v, do = make(lengths, 4, 2, dim, dtype)
+    with torch.no_grad():
+        o = xma.attention_packed(q, k, v, offsets(lengths))
+    u, at, scale = half_step(dtype), 0, 1 / math.sqrt(dim)
+    for L in lengths:
+        r = slice(at, at + L)
+        at += L
+        for h in range(4 if L <= 128 else 0):
+            qq, kk, vv = (t.double() for t in (q[r, h], k[r, h // 2], v[r, h // 2]))
+            seen = torch.ones(L, L, dtype=torch.float64, device="cuda").tril()
+            p = torch.softmax((qq @ kk.t() * scale).masked_fill(seen == 0, -math.inf), -1)
+            es = (dim + 8) * F32 * (qq.abs() @ kk.abs().t()) * scale * seen  # as in `reference`
+            ep = es + es.max(-1, keepdim=True).values + 2.0 ** -16 + 80 * F32
+            want = p @ vv
+            bound = u * want.abs() * (1 + 2 ** -7) + (p * (ep + 2 * u * u)) @ vv.abs() + 2.0 ** -33 * (seen @ vv.abs()) + 64 * F32 * (p @ vv.abs())
+            assert_within("o", o[r, h], want, bound)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("what", [math.inf, -math.inf])
+def test_infinite_values_make_infinities(dtype, what):
+    """Rows that see an infinite value with a weight above zero get that infinity, in the first tile and behind it."""
+    lengths = [60, 400]
+    q, k, v, do = make(lengths, 4, 2, 64, dtype, q_scale=0.5)
+    clean = xma.attention_packed(q, k, v, offsets(lengths))
+    v[5, 0, 3], v[70, 1, 9], v[300, 0, 0] = what, what, what
+    o = xma.attention_packed(q, k, v, offsets(lengths))
+    assert (o[5:60, :2, 3] == what).all() and (o[70:, 2:, 9] == what).all() and (o[300:, :2, 0] == what).all()
+    other = torch.ones_like(o, dtype=torch.bool)
+    other[:60, :2, 3], other[60:, 2:, 9], other[60:, :2, 0] = False, False, False
+    assert torch.equal(o[other], clean[other])
