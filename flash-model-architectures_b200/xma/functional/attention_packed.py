@@ -82,7 +82,8 @@ def attention_packed(
     float32 number below 1e30) and defaults to `1 / sqrt(head_dim)`.
 
     Scores and sums are float32; probabilities are rounded to the inputs' dtype before they meet the values (in float16
-    times a power of two, so that keys which others outweigh keep their share). For a backward pass the call keeps its
+    times a power of two, so that keys which others outweigh keep their share; in sequences of up to 128 tokens as two
+    numbers, so that nothing is lost). For a backward pass the call keeps its
     inputs, its output, a float32 per row and head and, so that gradients do not suffer from the output's rounding, one
     byte per output element; gradients are summed in a fixed order. In float16 probabilities and the gradient of the
     scores are rounded with powers of two, the latter one that the batch's largest finite upstream gradient and value
