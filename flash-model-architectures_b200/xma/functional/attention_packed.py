@@ -83,11 +83,11 @@ def attention_packed(
 
     Scores and sums are float32; probabilities are rounded to the inputs' dtype before they meet the values (in float16
     times a power of two, so that keys which others outweigh keep their share; in sequences of up to 128 tokens as two
-    numbers, so that nothing is lost). For a backward pass the call keeps its
-    inputs, its output, a float32 per row and head and, so that gradients do not suffer from the output's rounding, one
-    byte per output element; gradients are summed in a fixed order. In float16 probabilities and the gradient of the
-    scores are rounded with powers of two, the latter one that the batch's largest finite upstream gradient and value
-    set, so small gradients keep their bits without loss scaling.
+    numbers, so that nothing is lost). For a backward pass the call keeps its inputs, its output, a float32 per row and
+    head and, so that gradients do not suffer from the output's rounding, one byte per output element; gradients are
+    summed in a fixed order. In float16 probabilities and the gradient of the scores are rounded with powers of two, the
+    latter one that the batch's largest finite upstream gradient and value set, so small gradients keep their bits
+    without loss scaling.
 
     Tokens that no sequence owns get zeros, in the output and in the gradients, and what they hold reaches nothing. A
     NaN or an infinity in a value also reaches rows before it in its own sequence, as in a product with probabilities
